@@ -48,6 +48,10 @@ extern "C" {
 #define WL_EINVAL_SCOPE -12    /* wl_moe_fork_begin with a scope open on the device; wl_moe_fork_end without one on
                                   this stream */
 
+#define WL_EINVAL_CACHE -13    /* cache type, head_dim or page_tokens outside what the kernels run */
+#define WL_EINVAL_PAGES -14    /* wl_kv_copy: a page out of range, two copies into one page, or a page both read and
+                                  written */
+
 #define WL_MAX_TOPK 16
 #define WL_MAX_BATCH_EXPERTS 64 /* experts per wl_gemv_batch / wl_gemv_combine call */
 
@@ -256,6 +260,99 @@ const char* wl_moe_stage_name(int stage);
  * No counterpart in the reference (whose MoE layer allocates per call); it is for callers that cannot allocate. */
 int wl_moe_layer_noalloc(const WlMoeLayer* layer, const float* x, int64_t tokens, float* y, int32_t* ids,
                          float* weights, void* stream);
+
+/* ---- The attention half: rotary positions, a paged 8-bit key/value cache and attention over it -------------------
+ * The layers beside the MoE half of the decoder (engines/base.py:328-367 is the reference's Engine.attention, whose
+ * cache is a bf16 tensor per layer that grows in blocks of 256 positions, :213-216,348-358). Activations are bf16. */
+
+#define WL_KV_INT8 0
+#define WL_KV_E4M3 1 /* OCP fp8, 4 exponent and 3 mantissa bits, largest value 448 */
+
+/* A key/value cache: `pages` pages in each of `layers` layers; a page holds page_tokens consecutive tokens of one
+ * sequence. A value is its byte times the scale of its block, the page's tokens of one kv head (K and V apart).
+ * V is stored with the tokens innermost: the order in which the matrix core takes it. */
+typedef struct WlKvCache {
+    void* k;            /* [layers][pages][kv_heads][page_tokens][head_dim] bytes of `type`, 16-byte aligned */
+    void* v;            /* [layers][pages][kv_heads][head_dim][page_tokens] bytes of `type`, 16-byte aligned */
+    float* k_scale;     /* [layers][pages][kv_heads] */
+    float* v_scale;     /* [layers][pages][kv_heads] */
+    int64_t pages;      /* 1 .. 2^31 - 1 */
+    int32_t layers;
+    int32_t kv_heads;   /* 1 .. 4096 */
+    int32_t head_dim;   /* 64, 128 or 256 */
+    int32_t page_tokens; /* a multiple of 16, 16 .. 1024 */
+    int32_t type;       /* WL_KV_* */
+    int32_t reserved;   /* 0 */
+} WlKvCache;
+
+/* The sequences of one call. Their tokens lie packed in rows [cu[b], cu[b + 1]) of the call's arrays, of which `tokens`
+ * rows exist; rows behind cu[seqs] are neither read nor written. Page numbers are read on the device: an entry outside
+ * [0, pages) stands for a page that is not there (its tokens are not written, and attended by nobody), as does a
+ * position behind table_width pages. cu is taken as if cut to [0, tokens], and a sequence's rows to max_count. */
+typedef struct WlKvBatch {
+    const int32_t* table; /* [seqs][table_width] page numbers, rows table_stride entries apart */
+    const int32_t* cu;    /* [seqs + 1] */
+    int64_t table_stride;
+    int64_t tokens;
+    int32_t seqs;         /* 1 .. 65535 */
+    int32_t table_width;  /* 1 .. 2^20 */
+    int32_t max_count;    /* the most rows that any sequence has: 1 .. tokens */
+    int32_t reserved;     /* 0 */
+} WlKvBatch;
+
+/* Checks a cache description without touching device memory; 0 or a WL_E* code. */
+int wl_kv_check(const WlKvCache* cache);
+
+/* Writes new keys and values (bf16 [tokens][kv_heads][head_dim], element strides given, head_dim contiguous) of one layer
+ * into the cache: sequence b's rows become its positions start[b], start[b] + 1, ... A page that this call begins (its
+ * first token is among the rows) gets the scale s = the smallest bf16 value with M * s >= max |x| of its rows (M = 127 or
+ * 448), and every byte is x / s rounded to nearest even: the same bits whatever the sums' precision, since x and s have 8
+ * significant bits each. A page that holds older tokens keeps s, or takes s * 2^n with the smallest n that covers the new
+ * rows; its older bytes are then divided by 2^n and rounded again (so an older value is off by less than one step of the
+ * final scale). Bytes behind the new rows stay as they are. A NaN or an infinity among a block's rows makes its scale NaN.
+ * Pages that a call writes must be distinct over its sequences. */
+int wl_kv_append(const WlKvCache* cache, int layer, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                 const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const WlKvBatch* batch,
+                 const int32_t* start, void* stream);
+
+/* Bytes of device workspace wl_kv_attend needs (0 on invalid arguments or when it needs none). */
+size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length);
+
+/* Grouped-query attention over one layer of the cache: q bf16 [tokens][q_heads][head_dim] (element strides given, head_dim
+ * contiguous), out bf16 [tokens][q_heads][head_dim], dense. Query head i reads kv head i / (q_heads / kv_heads). length[b]
+ * counts sequence b's tokens in the cache, its rows of this call included: row i of its n stands at position
+ * length[b] - n + i. out = sum_j softmax_j(scale * q . k_j) v_j over the positions j < length[b] and, with causal != 0,
+ * j <= the row's own position; a row that sees no token is 0. Softmax statistics and sums are fp32; the weights are rounded
+ * to bf16 for the matrix core, which adds up in fp32.
+ * max_length: a bound of length[], from which the work's split is chosen (results hold whatever it says).
+ * No counterpart in the reference, whose attention reads a bf16 cache (engines/base.py:348-366). */
+int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                 int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,
+                 uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Copies pages src_host[i] to dst_host[i], i < n, of every layer (bytes and scales). HOST arrays, passed by value to the
+ * kernels. Refused: a page out of range, a page written twice, a page both read and written. */
+int wl_kv_copy(const WlKvCache* cache, const int32_t* src_host, const int32_t* dst_host, int64_t n, void* stream);
+
+#define WL_MAX_ROPE_AXES 4
+/* One tensor to rotate: [tokens][heads][head_dim], element strides given (head_dim contiguous). out may be in. */
+typedef struct WlRopeTensor {
+    const void* in;
+    void* out;
+    int64_t in_token_stride, in_head_stride, out_token_stride, out_head_stride;
+    int32_t heads;
+    int32_t reserved; /* 0 */
+} WlRopeTensor;
+
+/* Rotary positions with up to WL_MAX_ROPE_AXES axes, on the first rotary_dim values of each head, pairs (j, j +
+ * rotary_dim / 2): (a, b) -> (a c - b s, b c + a s) with c = scale cos(angle), s = scale sin(angle), angle =
+ * positions[axis(j)][token] * inv_freq[j] taken in 64 bits. sections_host[i] frequencies belong to axis i (they add up to
+ * rotary_dim / 2): interleaved == 0: one axis after the other; interleaved != 0: axis i > 0 has the frequencies j = i +
+ * axes * n, n < sections[i], axis 0 the others. The rest of each head is copied. q and k (k may be NULL) of one dtype, in
+ * one launch. */
+int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
+            const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
+            const int32_t* sections_host, int interleaved, float scale, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,308 @@
+// Writing into the paged 8-bit cache (wl_kv_append) and moving its pages (wl_kv_copy).
+#include <algorithm>
+#include <vector>
+
+#include "wl_kv.h"
+
+namespace wl {
+namespace {
+
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+
+constexpr int kAppendThreads = 256;
+
+template <int TYPE>
+constexpr float kLargest = TYPE == WL_KV_INT8 ? 127.0f : 448.0f;
+
+// x (a value already divided by its scale, |x| <= kLargest) as a byte, rounded to nearest even.
+template <int TYPE>
+__device__ __forceinline__ uint32_t to_byte(float x) {
+    if constexpr (TYPE == WL_KV_INT8)
+        return static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x))) & 0xFFu;
+    else
+        return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false)) & 0xFFu;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float from_byte(uint32_t b) {
+    if constexpr (TYPE == WL_KV_INT8)
+        return static_cast<float>(static_cast<int8_t>(b));
+    else
+        return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(b), 0);
+}
+
+__device__ __forceinline__ float bf16_to_float(uint32_t bits) { return __builtin_bit_cast(float, bits << 16); }
+
+// The smallest bf16 value not below x (x >= 0, finite).
+__device__ __forceinline__ float round_up_bf16(float x) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) + 0xFFFFu) & 0xFFFF0000u);
+}
+
+// The scale of a block whose new rows reach `top`, and the power of two by which its older bytes shrink. `held`: it has
+// older tokens, `old` their scale. Exact: top and old have 8 significant bits, so 127 old and 448 old fit fp32, and the
+// quotient top / 127 is a bf16 value or at least 2^-16 (relative) away from one, so its rounding up is not moved by fp32's.
+template <int TYPE>
+__device__ __forceinline__ float block_scale(float top, bool held, float old, int& shrink) {
+    shrink = 0;
+    if (!held || old == 0.0f) {
+        const float s = round_up_bf16(top / kLargest<TYPE>);
+        if (held && s > 0.0f) shrink = 32;  // older values are 0: so are their bytes from here on
+        return s;
+    }
+    const float reach = old * kLargest<TYPE>;
+    if (!(top > reach)) return old;  // a NaN scale stays
+    int n = max(0, ilogbf(top) - ilogbf(reach));
+    if (ldexpf(reach, n) < top) n++;
+    shrink = n;
+    return ldexpf(old, n);
+}
+
+// One workgroup writes one block: a page of a sequence, one kv head, K or V (blockIdx.y's low bit), so the block's scale
+// and its older bytes have one writer. Two passes over the block's new rows: their largest magnitude, then the bytes; the
+// second finds them in the caches. K's bytes lie as the rows do, 16 values of a token to a thread. V's lie with the
+// tokens innermost: a thread takes two neighbouring values of 16 tokens, its loads run along the rows over the lanes, and
+// it writes 16 bytes for each value; where those 16 tokens are not all new, the bytes there are read first.
+// Bound by its reads and writes for prompts (6 bytes a value), by the launch and one round trip for single tokens.
+template <int TYPE, int D, bool WIDE>
+__global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs s, const int32_t* __restrict__ start,
+                                                              const uint16_t* __restrict__ kx, int64_t k_ts, int64_t k_hs,
+                                                              const uint16_t* __restrict__ vx, int64_t v_ts,
+                                                              int64_t v_hs) {
+    __shared__ uint32_t tops[kAppendThreads / 64];
+    const int b = blockIdx.z, head = blockIdx.y >> 1;
+    const bool is_v = blockIdx.y & 1;
+    const int at = s.first(b), n = s.count(b, at);
+    const int64_t from = max(start[b], 0), end = from + n;
+    const int P = c.page_tokens;
+    const int64_t col = c.column(static_cast<int>(from)) + static_cast<int64_t>(blockIdx.x), page0 = col * P;
+    if (page0 >= end) return;
+    const int page = col < s.table_width ? s.page(b, static_cast<int>(col), c.pages) : -1;
+    if (page < 0) return;
+    const int held = static_cast<int>(max(from - page0, int64_t{0}));
+    const int stop = static_cast<int>(min(end - page0, static_cast<int64_t>(P)));  // tokens [held, stop) are new
+    const int64_t ts = is_v ? v_ts : k_ts;
+    // row of token t (in the page): at + (page0 + t - from)
+    const uint16_t* __restrict__ x =
+        (is_v ? vx + head * v_hs : kx + head * k_hs) + (at + (page0 - from)) * ts;
+    const int64_t block = c.block(page, head);
+    uint8_t* __restrict__ out = (is_v ? c.v : c.k) + block * P * D;
+    float* scale = (is_v ? c.v_scale : c.k_scale) + block;
+
+    // the largest magnitude, as bits (bf16 magnitudes order as their bits do; infinities and NaN come out largest)
+    uint32_t top = 0;
+    if constexpr (WIDE) {
+        for (int i = threadIdx.x; i < (stop - held) * (D / 8); i += kAppendThreads) {
+            const uint4 w = *reinterpret_cast<const uint4*>(x + (held + i / (D / 8)) * ts + i % (D / 8) * 8);
+            for (uint32_t u : {w.x, w.y, w.z, w.w}) top = max(top, max(u & 0x7FFFu, (u >> 16) & 0x7FFFu));
+        }
+    } else {
+        for (int i = threadIdx.x; i < (stop - held) * D; i += kAppendThreads)
+            top = max(top, x[(held + i / D) * ts + i % D] & 0x7FFFu);
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = max(top, __shfl_xor(top, d));
+    if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+    const float old = *scale;
+    __syncthreads();
+    top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+
+    int shrink = 0;
+    float now = top < 0x7F80u ? block_scale<TYPE>(bf16_to_float(top), held > 0, old, shrink)
+                              : __builtin_nanf("");
+    const bool dead = !(now > 0.0f);  // nothing but zeros, or a NaN scale: the bytes are 0
+    const float per = dead ? 1.0f : now;
+    auto quantize = [&](uint32_t bits) { return dead ? 0u : to_byte<TYPE>(bf16_to_float(bits) / per); };
+    auto older = [&](uint32_t byte) { return to_byte<TYPE>(ldexpf(from_byte<TYPE>(byte), -shrink)); };
+    if (threadIdx.x == 0) *scale = now;
+
+    if (!is_v) {
+        for (int i = threadIdx.x; i < (stop - held) * (D / 16); i += kAppendThreads) {
+            const int t = held + i / (D / 16), d = i % (D / 16) * 16;
+            const uint16_t* row = x + t * ts + d;
+            uint32_t in[8], w[4];
+            if constexpr (WIDE) {
+                const uint4 lo = *reinterpret_cast<const uint4*>(row), hi = *reinterpret_cast<const uint4*>(row + 8);
+                in[0] = lo.x, in[1] = lo.y, in[2] = lo.z, in[3] = lo.w;
+                in[4] = hi.x, in[5] = hi.y, in[6] = hi.z, in[7] = hi.w;
+            } else {
+                for (int j = 0; j < 8; j++) in[j] = row[2 * j] | static_cast<uint32_t>(row[2 * j + 1]) << 16;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                w[j] = quantize(in[2 * j] & 0xFFFFu) | quantize(in[2 * j] >> 16) << 8 |
+                       quantize(in[2 * j + 1] & 0xFFFFu) << 16 | quantize(in[2 * j + 1] >> 16) << 24;
+            *reinterpret_cast<uint4*>(out + t * D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+        if (shrink)
+            for (int i = threadIdx.x; i < held * (D / 4); i += kAppendThreads) {
+                const uint32_t w = reinterpret_cast<uint32_t*>(out)[i];
+                reinterpret_cast<uint32_t*>(out)[i] = older(w & 0xFFu) | older(w >> 8 & 0xFFu) << 8 |
+                                                      older(w >> 16 & 0xFFu) << 16 | older(w >> 24) << 24;
+            }
+        return;
+    }
+    const int g0 = shrink ? 0 : held / 16, g1 = (stop + 15) / 16;  // the groups of 16 tokens that change
+    for (int i = threadIdx.x; i < (g1 - g0) * (D / 2); i += kAppendThreads) {
+        const int t0 = (g0 + i / (D / 2)) * 16, d = i % (D / 2) * 2;
+        uint32_t w[2][4] = {};
+        uint4* to[2] = {reinterpret_cast<uint4*>(out + d * P + t0), reinterpret_cast<uint4*>(out + (d + 1) * P + t0)};
+        if (t0 < held || t0 + 16 > stop) {
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                const uint4 was = *to[e];
+                w[e][0] = was.x, w[e][1] = was.y, w[e][2] = was.z, w[e][3] = was.w;
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = t0 + j;
+            const uint32_t sh = 8 * (j % 4);
+            if (t >= stop) continue;
+            if (t >= held) {
+                uint32_t two;
+                if constexpr (WIDE)
+                    two = *reinterpret_cast<const uint32_t*>(x + t * ts + d);
+                else
+                    two = x[t * ts + d] | static_cast<uint32_t>(x[t * ts + d + 1]) << 16;
+                w[0][j / 4] = (w[0][j / 4] & ~(0xFFu << sh)) | quantize(two & 0xFFFFu) << sh;
+                w[1][j / 4] = (w[1][j / 4] & ~(0xFFu << sh)) | quantize(two >> 16) << sh;
+            } else if (shrink) {
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    w[e][j / 4] = (w[e][j / 4] & ~(0xFFu << sh)) | older(w[e][j / 4] >> sh & 0xFFu) << sh;
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 2; e++) *to[e] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+    }
+}
+
+template <int TYPE, int D>
+void launch_append(bool wide, dim3 grid, hipStream_t stream, const KvLayer& c, const KvSeqs& s, const int32_t* start,
+                   const uint16_t* k, int64_t k_ts, int64_t k_hs, const uint16_t* v, int64_t v_ts, int64_t v_hs) {
+    if (wide)
+        k_kv_append<TYPE, D, true><<<grid, kAppendThreads, 0, stream>>>(c, s, start, k, k_ts, k_hs, v, v_ts, v_hs);
+    else
+        k_kv_append<TYPE, D, false><<<grid, kAppendThreads, 0, stream>>>(c, s, start, k, k_ts, k_hs, v, v_ts, v_hs);
+}
+
+// Page copies: the pairs of one launch travel in its arguments, so nothing is uploaded and a graph keeps them.
+constexpr int kCopyPairs = 256;
+constexpr int kCopyThreads = 256;
+constexpr int kCopyChunk = kCopyThreads * 16 * 4;  // bytes of one workgroup: four 16-byte loads a thread in flight
+
+struct CopyPairs {
+    int32_t src[kCopyPairs], dst[kCopyPairs];
+};
+
+// blockIdx: (chunk of the page's K then V bytes, pair, layer).
+__global__ __launch_bounds__(kCopyThreads) void k_kv_copy(uint8_t* k, uint8_t* v, float* k_scale, float* v_scale,
+                                                          int64_t pages, int kv_heads, int64_t page_bytes, int chunks,
+                                                          CopyPairs pairs) {
+    const int64_t layer = blockIdx.z, src = layer * pages + pairs.src[blockIdx.y],
+                  dst = layer * pages + pairs.dst[blockIdx.y];
+    const bool is_v = static_cast<int>(blockIdx.x) >= chunks;
+    const int64_t at = static_cast<int64_t>(blockIdx.x - (is_v ? chunks : 0)) * kCopyChunk + threadIdx.x * 16;
+    constexpr int kStep = kCopyThreads * 16;
+    const uint8_t* from = (is_v ? v : k) + src * page_bytes + at;
+    uint8_t* to = (is_v ? v : k) + dst * page_bytes + at;
+    if (at + 3 * kStep < page_bytes) {
+        u32x4 w[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) w[i] = *reinterpret_cast<const u32x4*>(from + i * kStep);
+#pragma unroll
+        for (int i = 0; i < 4; i++) *reinterpret_cast<u32x4*>(to + i * kStep) = w[i];
+    } else {
+        for (int i = 0; at + i * kStep < page_bytes; i++)
+            *reinterpret_cast<u32x4*>(to + i * kStep) = *reinterpret_cast<const u32x4*>(from + i * kStep);
+    }
+    if (blockIdx.x == 0)
+        for (int h = threadIdx.x; h < kv_heads; h += kCopyThreads) {
+            k_scale[dst * kv_heads + h] = k_scale[src * kv_heads + h];
+            v_scale[dst * kv_heads + h] = v_scale[src * kv_heads + h];
+        }
+}
+
+int check_copies(const WlKvCache* cache, const int32_t* src, const int32_t* dst, int64_t n) {
+    for (int64_t i = 0; i < n; i++)
+        if (src[i] < 0 || src[i] >= cache->pages || dst[i] < 0 || dst[i] >= cache->pages) return WL_EINVAL_PAGES;
+    std::vector<int32_t> to(dst, dst + n);
+    std::sort(to.begin(), to.end());
+    if (std::adjacent_find(to.begin(), to.end()) != to.end()) return WL_EINVAL_PAGES;
+    for (int64_t i = 0; i < n; i++)
+        if (std::binary_search(to.begin(), to.end(), src[i])) return WL_EINVAL_PAGES;
+    return WL_OK;
+}
+
+}  // namespace
+}  // namespace wl
+
+using namespace wl;
+
+extern "C" {
+
+int wl_kv_check(const WlKvCache* cache) { return check_cache(cache); }
+
+int wl_kv_append(const WlKvCache* cache, int layer, const uint16_t* k, int64_t k_token_stride, int64_t k_head_stride,
+                 const uint16_t* v, int64_t v_token_stride, int64_t v_head_stride, const WlKvBatch* batch,
+                 const int32_t* start, void* stream) {
+    if (const int rc = check_cache(cache)) return rc;
+    if (const int rc = check_batch(batch)) return rc;
+    if (!k || !v || !start) return WL_EINVAL_NULL;
+    if (layer < 0 || layer >= cache->layers) return WL_EINVAL_SHAPE;
+    const auto kb = reinterpret_cast<uintptr_t>(k), vb = reinterpret_cast<uintptr_t>(v);
+    if (kb % 2 || vb % 2 || reinterpret_cast<uintptr_t>(start) % 4) return WL_EINVAL_ALIGN;
+    // 16-byte loads of whole rows, where every row starts on 16 bytes; else one value at a time
+    const bool wide = kb % 16 == 0 && vb % 16 == 0 && k_token_stride % 8 == 0 && k_head_stride % 8 == 0 &&
+                      v_token_stride % 8 == 0 && v_head_stride % 8 == 0;
+    const int P = cache->page_tokens;
+    // a sequence's rows touch at most this many pages: one more than fill, where they begin inside one
+    const dim3 grid((batch->max_count + P - 2) / P + 1, 2 * cache->kv_heads, batch->seqs);
+    const KvLayer c = layer_of(cache, layer);
+    const KvSeqs s = seqs_of(batch);
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    auto run = [&](auto type, auto dim) {
+        launch_append<decltype(type)::value, decltype(dim)::value>(wide, grid, st, c, s, start, k, k_token_stride,
+                                                                   k_head_stride, v, v_token_stride, v_head_stride);
+    };
+    auto with_dim = [&](auto type) {
+        if (cache->head_dim == 64)
+            run(type, std::integral_constant<int, 64>());
+        else if (cache->head_dim == 128)
+            run(type, std::integral_constant<int, 128>());
+        else
+            run(type, std::integral_constant<int, 256>());
+    };
+    if (cache->type == WL_KV_INT8)
+        with_dim(std::integral_constant<int, WL_KV_INT8>());
+    else
+        with_dim(std::integral_constant<int, WL_KV_E4M3>());
+    return launch_status();
+}
+
+int wl_kv_copy(const WlKvCache* cache, const int32_t* src_host, const int32_t* dst_host, int64_t n, void* stream) {
+    if (const int rc = check_cache(cache)) return rc;
+    if (n < 0 || n > cache->pages) return WL_EINVAL_SHAPE;
+    if (n == 0) return WL_OK;
+    if (!src_host || !dst_host) return WL_EINVAL_NULL;
+    try {
+        if (const int rc = check_copies(cache, src_host, dst_host, n)) return rc;
+    } catch (...) {
+        return static_cast<int>(hipErrorOutOfMemory);
+    }
+    const int64_t page_bytes = static_cast<int64_t>(cache->kv_heads) * cache->page_tokens * cache->head_dim;
+    const int chunks = static_cast<int>((page_bytes + kCopyChunk - 1) / kCopyChunk);
+    for (int64_t i = 0; i < n; i += kCopyPairs) {
+        const int m = static_cast<int>(std::min<int64_t>(kCopyPairs, n - i));
+        CopyPairs pairs;
+        std::copy(src_host + i, src_host + i + m, pairs.src);
+        std::copy(dst_host + i, dst_host + i + m, pairs.dst);
+        k_kv_copy<<<dim3(2 * chunks, m, cache->layers), kCopyThreads, 0, static_cast<hipStream_t>(stream)>>>(
+            static_cast<uint8_t*>(cache->k), static_cast<uint8_t*>(cache->v), cache->k_scale, cache->v_scale,
+            cache->pages, cache->kv_heads, page_bytes, chunks, pairs);
+        if (const int rc = launch_status()) return rc;
+    }
+    return WL_OK;
+}
+
+}  // extern "C"

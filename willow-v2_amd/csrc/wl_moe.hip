@@ -1751,6 +1751,11 @@ const char* wl_error_string(int code) {
         case WL_EINVAL_SCOPE:
             return "fork scope: wl_moe_fork_begin with a scope already open on this device, or wl_moe_fork_end "
                    "without one open on this stream";
+        case WL_EINVAL_CACHE:
+            return "cache: type must be WL_KV_INT8 or WL_KV_E4M3, head_dim 64, 128 or 256, page_tokens a multiple of 16 "
+                   "in 16..1024";
+        case WL_EINVAL_PAGES:
+            return "page copies: a page is out of range, written twice, or both read and written";
         case WL_EINVAL_SCRATCH:
             return "the call needs more workspace than wl_moe_layer_noalloc's scratch holds "
                    "(WL_NOALLOC_SCRATCH_BYTES): use wl_moe_layer with a workspace";
@@ -1760,7 +1765,7 @@ const char* wl_error_string(int code) {
     return "unknown error";
 }
 
-int wl_abi_version(void) { return (1 << 16) | 3; }  // 1.3: min_expert_weight (was reserved2, 0); 1.2: next, noalloc
+int wl_abi_version(void) { return (1 << 16) | 4; }  // 1.4: rope, cache; 1.3: min_expert_weight (was reserved2, 0); 1.2: next, noalloc
 
 int wl_moe_check(const WlMoeLayer* layer) { return check_layer(layer); }
 

@@ -1,0 +1,171 @@
+// Rotary positions with several axes (wl_rope).
+#include "wl_host.h"
+
+namespace wl {
+namespace {
+
+constexpr int kRopeThreads = 256;
+
+struct RopeArgs {
+    WlRopeTensor q, k;
+    const int64_t* positions;
+    int64_t positions_stride;
+    const double* inv_freq;
+    int32_t sections[WL_MAX_ROPE_AXES];
+    int32_t tokens, head_dim, half, axes, interleaved;
+    float scale;
+};
+
+// The axis that frequency j belongs to.
+__device__ __forceinline__ int axis_of(const RopeArgs& a, int j) {
+    if (a.interleaved) {
+        const int r = j % a.axes;
+        return r > 0 && j < a.axes * a.sections[r] ? r : 0;
+    }
+    int axis = 0;
+    for (int i = 0, end = 0; i + 1 < a.axes; i++) {
+        end += a.sections[i];
+        if (j >= end) axis = i + 1;
+    }
+    return axis;
+}
+
+template <typename T>
+__device__ __forceinline__ float load_value(const T* p);
+template <>
+__device__ __forceinline__ float load_value(const float* p) {
+    return *p;
+}
+template <>
+__device__ __forceinline__ float load_value(const uint16_t* p) {
+    return __builtin_bit_cast(float, static_cast<uint32_t>(*p) << 16);
+}
+__device__ __forceinline__ void store_value(float* p, float x) { *p = x; }
+__device__ __forceinline__ void store_value(uint16_t* p, float x) {
+    *p = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+}
+
+// One workgroup takes TOKENS tokens: the cosines and sines of their angles once into LDS, then every head's values by
+// them. The angle is taken in turns in 64 bits (a position of a million at the first frequency is 1.6e5 turns, of which
+// fp32 would keep 6 bits of the fraction) and only its fraction goes on in 32.
+// VEC: values a thread moves at once (16 bytes where every row and the half split are that aligned, else one).
+// Bound by reading and writing q and k once.
+template <typename T, int VEC, int TOKENS>
+__global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
+    extern __shared__ float2 turn[];  // [TOKENS][half]: cos, sin
+    const int t0 = blockIdx.x * TOKENS, n = min(TOKENS, a.tokens - t0);
+    for (int i = threadIdx.x; i < n * a.half; i += kRopeThreads) {
+        const int t = t0 + i / a.half, j = i % a.half;
+        const double pos = static_cast<double>(a.positions[axis_of(a, j) * a.positions_stride + t]);
+        const double turns = pos * a.inv_freq[j] * 0.15915494309189533577;  // 1 / (2 pi)
+        float s, c;
+        sincospif(static_cast<float>(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+        turn[i] = make_float2(a.scale * c, a.scale * s);
+    }
+    __syncthreads();
+    // a head: half / VEC pairs of runs, then what is not rotated
+    const int pairs = a.half / VEC, rest = (a.head_dim - 2 * a.half) / VEC, per = pairs + rest;
+    const int heads = a.q.heads + a.k.heads;
+    for (int i = threadIdx.x; i < n * heads * per; i += kRopeThreads) {
+        const int u = i % per, th = i / per, t = th / heads, hh = th % heads;
+        const bool is_k = hh >= a.q.heads;
+        const WlRopeTensor& x = is_k ? a.k : a.q;
+        const int h = is_k ? hh - a.q.heads : hh;
+        const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token_stride + h * x.in_head_stride;
+        T* out = static_cast<T*>(x.out) + (t0 + t) * x.out_token_stride + h * x.out_head_stride;
+        struct alignas(sizeof(T) * VEC) Run {
+            T v[VEC];
+        };
+        if (u >= pairs) {
+            const int d = 2 * a.half + (u - pairs) * VEC;
+            if (in != out) *reinterpret_cast<Run*>(out + d) = *reinterpret_cast<const Run*>(in + d);
+            continue;
+        }
+        const int j = u * VEC;
+        Run lo = *reinterpret_cast<const Run*>(in + j), hi = *reinterpret_cast<const Run*>(in + a.half + j);
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float2 cs = turn[t * a.half + j + e];
+            const float p = load_value(lo.v + e), q = load_value(hi.v + e);
+            store_value(lo.v + e, p * cs.x - q * cs.y);
+            store_value(hi.v + e, q * cs.x + p * cs.y);
+        }
+        *reinterpret_cast<Run*>(out + j) = lo;
+        *reinterpret_cast<Run*>(out + a.half + j) = hi;
+    }
+}
+
+constexpr int kRopeTokens = 4;
+
+template <typename T>
+void launch_rope(bool wide, const RopeArgs& a, hipStream_t stream) {
+    const dim3 grid((a.tokens + kRopeTokens - 1) / kRopeTokens);
+    const size_t lds = sizeof(float2) * kRopeTokens * a.half;
+    if (wide)
+        k_rope<T, 16 / sizeof(T), kRopeTokens><<<grid, kRopeThreads, lds, stream>>>(a);
+    else
+        k_rope<T, 1, kRopeTokens><<<grid, kRopeThreads, lds, stream>>>(a);
+}
+
+int check_rope_tensor(const WlRopeTensor* x, int size) {
+    if (!x->in || !x->out) return WL_EINVAL_NULL;
+    if (x->heads < 1 || x->heads > 65535 || x->reserved != 0) return WL_EINVAL_SHAPE;
+    if (reinterpret_cast<uintptr_t>(x->in) % size || reinterpret_cast<uintptr_t>(x->out) % size) return WL_EINVAL_ALIGN;
+    return WL_OK;
+}
+
+bool aligned16(const WlRopeTensor* x, int size) {
+    const int64_t n = 16 / size;
+    return reinterpret_cast<uintptr_t>(x->in) % 16 == 0 && reinterpret_cast<uintptr_t>(x->out) % 16 == 0 &&
+           x->in_token_stride % n == 0 && x->in_head_stride % n == 0 && x->out_token_stride % n == 0 &&
+           x->out_head_stride % n == 0;
+}
+
+}  // namespace
+}  // namespace wl
+
+using namespace wl;
+
+extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
+                       const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
+                       const int32_t* sections_host, int interleaved, float scale, void* stream) {
+    if (!q || !positions || !inv_freq || !sections_host) return WL_EINVAL_NULL;
+    if (dtype != WL_DTYPE_F32 && dtype != WL_DTYPE_BF16) return WL_EINVAL_DTYPE;
+    const int size = dtype == WL_DTYPE_F32 ? 4 : 2;
+    if (const int rc = check_rope_tensor(q, size)) return rc;
+    if (k)
+        if (const int rc = check_rope_tensor(k, size)) return rc;
+    if (tokens < 1 || tokens >= (int64_t{1} << 31) || head_dim < 2 || head_dim > 1024 || rotary_dim < 2 ||
+        rotary_dim > head_dim || rotary_dim % 2 || axes < 1 || axes > WL_MAX_ROPE_AXES)
+        return WL_EINVAL_SHAPE;
+    if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return WL_EINVAL_ALIGN;
+    RopeArgs a = {};
+    a.half = rotary_dim / 2;
+    int64_t sum = 0;
+    for (int i = 0; i < axes; i++) {
+        const int n = sections_host[i];
+        if (n < 0 || n > a.half) return WL_EINVAL_SHAPE;
+        if (interleaved && i > 0 && n > 0 && i + axes * (n - 1) >= a.half) return WL_EINVAL_SHAPE;
+        a.sections[i] = n;
+        sum += n;
+    }
+    if (sum != a.half) return WL_EINVAL_SHAPE;
+    a.q = *q;
+    if (k) a.k = *k;
+    a.positions = positions;
+    a.positions_stride = positions_stride;
+    a.inv_freq = inv_freq;
+    a.tokens = static_cast<int32_t>(tokens);
+    a.head_dim = head_dim;
+    a.axes = axes;
+    a.interleaved = interleaved != 0;
+    a.scale = scale;
+    const int vec = 16 / size;
+    const bool wide = a.half % vec == 0 && head_dim % vec == 0 && aligned16(q, size) && (!k || aligned16(k, size));
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == WL_DTYPE_F32)
+        launch_rope<float>(wide, a, st);
+    else
+        launch_rope<uint16_t>(wide, a, st);
+    return launch_status();
+}

@@ -6,6 +6,9 @@ gemv_batch, gemv_combine, dequantize_gpu, GGMLWeight; gguf/metal.py:20,295,320-4
 Metal kernels round to bf16. It adds the fused MoE layer (moe_layer / MoELayer), which replaces Engine.moe's
 router -> host sync -> per-expert launches (engines/base.py:445-591) with device-side routing.
 
+Beside it the attention half's operators (gguf.hip.kv): rope (rotary positions with several axes), KVPages, kv_append,
+kv_attend and kv_copy (a paged 8-bit key/value cache, its writer, the attention that reads it, its page copies).
+
 There is no CPU fallback: without the built library (or without a GPU) every compute call raises.
 """
 import ctypes
@@ -22,6 +25,7 @@ MAX_BATCH_EXPERTS = 64
 DTYPE_F32, DTYPE_BF16 = 0, 1
 MOE_NO_FUSED, MOE_NO_MFMA, MOE_FORCE_MFMA, MOE_TEST_STARVE, MOE_PRE_NORM, MOE_RESIDUAL = 1, 2, 4, 8, 16, 32
 MOE_GUESS_NEXT = 64
+KV_INT8, KV_E4M3 = 0, 1
 ESYNC = -10  # wl_moe_workspace_status: a bounded wait gave up
 EINVAL_SCOPE = -12  # wl_moe_fork_begin / wl_moe_fork_end used outside their pairing
 NOALLOC_SCRATCH_BYTES = 16 << 20  # WL_NOALLOC_SCRATCH_BYTES
@@ -53,6 +57,34 @@ class WlMoeLayer(ctypes.Structure):
 
 
 _lib = None
+
+
+class WlKvCache(ctypes.Structure):
+    """Mirror of the C struct WlKvCache (include/willow_hip.h)."""
+    _fields_ = [
+        ("k", ctypes.c_void_p), ("v", ctypes.c_void_p), ("k_scale", ctypes.c_void_p), ("v_scale", ctypes.c_void_p),
+        ("pages", ctypes.c_int64), ("layers", ctypes.c_int32), ("kv_heads", ctypes.c_int32),
+        ("head_dim", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("type", ctypes.c_int32),
+        ("reserved", ctypes.c_int32),
+    ]
+
+
+class WlKvBatch(ctypes.Structure):
+    """Mirror of the C struct WlKvBatch (include/willow_hip.h)."""
+    _fields_ = [
+        ("table", ctypes.c_void_p), ("cu", ctypes.c_void_p), ("table_stride", ctypes.c_int64),
+        ("tokens", ctypes.c_int64), ("seqs", ctypes.c_int32), ("table_width", ctypes.c_int32),
+        ("max_count", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
+
+
+class WlRopeTensor(ctypes.Structure):
+    """Mirror of the C struct WlRopeTensor (include/willow_hip.h)."""
+    _fields_ = [
+        ("in_", ctypes.c_void_p), ("out", ctypes.c_void_p), ("in_token_stride", ctypes.c_int64),
+        ("in_head_stride", ctypes.c_int64), ("out_token_stride", ctypes.c_int64), ("out_head_stride", ctypes.c_int64),
+        ("heads", ctypes.c_int32), ("reserved", ctypes.c_int32),
+    ]
 
 
 def library() -> ctypes.CDLL:
@@ -90,6 +122,18 @@ def library() -> ctypes.CDLL:
     lib.wl_moe_workspace_status.argtypes, lib.wl_moe_workspace_status.restype = [vp, ctypes.c_size_t, vp], c_int
     lib.wl_moe_fork_begin.argtypes, lib.wl_moe_fork_begin.restype = [vp], c_int
     lib.wl_moe_fork_end.argtypes, lib.wl_moe_fork_end.restype = [vp], c_int
+    cache_p, batch_p, rope_p = (ctypes.POINTER(s) for s in (WlKvCache, WlKvBatch, WlRopeTensor))
+    i32p = ctypes.POINTER(i32)
+    lib.wl_kv_check.argtypes = [cache_p]
+    lib.wl_kv_append.argtypes = [cache_p, c_int, vp, i64, i64, vp, i64, i64, batch_p, vp, vp]
+    lib.wl_kv_attend_workspace_bytes.argtypes = [cache_p, c_int, batch_p, i64]
+    lib.wl_kv_attend_workspace_bytes.restype = ctypes.c_size_t
+    lib.wl_kv_attend.argtypes = [cache_p, c_int, vp, i64, i64, c_int, batch_p, vp, i64, ctypes.c_float, c_int, vp, vp,
+                                 ctypes.c_size_t, vp]
+    lib.wl_kv_copy.argtypes = [cache_p, vp, vp, i64, vp]
+    lib.wl_rope.argtypes = [rope_p, rope_p, c_int, i64, c_int, c_int, vp, i64, vp, c_int, i32p, c_int, ctypes.c_float, vp]
+    for name in ("wl_kv_check", "wl_kv_append", "wl_kv_attend", "wl_kv_copy", "wl_rope"):
+        getattr(lib, name).restype = c_int
     for name in ("wl_dequant", "wl_gemv", "wl_gemv_dtype", "wl_linear", "wl_gemv_batch", "wl_gemv_combine",
                  "wl_moe_check", "wl_moe_route", "wl_moe_layer", "wl_moe_layer_profile"):
         getattr(lib, name).restype = c_int
@@ -327,3 +371,4 @@ class GGMLWeight:
 
 
 from .moe import MoELayer, moe_layer  # noqa: E402  (needs the names above)
+from .kv import KVPages, kv_append, kv_attend, kv_copy, rope  # noqa: E402
