@@ -280,7 +280,7 @@ typedef struct WlKvCache {
     int32_t layers;
     int32_t kv_heads;   /* 1 .. 4096 */
     int32_t head_dim;   /* 64, 128 or 256 */
-    int32_t page_tokens; /* a multiple of 16, 16 .. 1024 */
+    int32_t page_tokens; /* a power of two, 16 .. 1024 */
     int32_t type;       /* WL_KV_* */
     int32_t reserved;   /* 0 */
 } WlKvCache;

@@ -28,7 +28,18 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;       // tokens of a tile
 constexpr int kRows = 16;       // query rows of a workgroup
 constexpr int kFewWaves = 4;
-constexpr int kFewGroups = 512; // workgroups of a split call: two a CU
+constexpr int kFewGroups = 256; // workgroups of a call of few rows: one a CU
+
+// A sequence of the call: its first row, its rows, its tokens.
+struct Seq {
+    int at, n, length;
+};
+
+// Where the partial results of a (sequence, kv head) lie: slot first, then two slots further for each of the other pieces,
+// from `next` on. pieces is 0 where there are none.
+struct Pieces {
+    int32_t pieces, first, next, reserved;
+};
 
 struct AttendArgs {
     KvLayer c;
@@ -37,15 +48,21 @@ struct AttendArgs {
     const uint16_t* q;
     int64_t q_token_stride, q_head_stride;
     uint16_t* out;
-    float* partial;   // [2 * workgroups][kRows][D]
-    float2* partial_ml;  // [2 * workgroups][kRows]: maximum (in log2) and sum
+    float* partial;      // [pieces of what was cut][rows][D]
+    float2* partial_ml;  // [pieces of what was cut][rows]: maximum (in log2) and sum
+    Pieces* pieces;      // [seqs][kv heads]
+    int32_t rows;        // rows of a (sequence, kv head), at most, where they are few
     int32_t q_heads, group;
     float scale_log2;  // scale * log2(e)
     int32_t causal, wide_q;
+    int32_t whole, groups;  // how a call of few rows is cut: not at all, or over how many workgroups
 
-    __device__ __forceinline__ int len(int b) const {
-        const int64_t most = static_cast<int64_t>(s.table_width) * c.page_tokens;
-        return static_cast<int>(min(static_cast<int64_t>(max(length[b], 0)), most));
+    __device__ __forceinline__ Seq seq(int b) const {
+        Seq q;
+        q.at = s.first(b);
+        q.n = s.count(b, q.at);
+        q.length = min(max(length[b], 0), s.table_width << c.page_shift);
+        return q;
     }
 };
 
@@ -77,12 +94,42 @@ __device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
     return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
 }
 
+// Over the four lanes that hold one row's values: lanes 16, 32 and 48 apart.
+template <typename F>
+__device__ __forceinline__ float over_groups(float x, F f) {
+    // a bit_cast straight from a vector's element reads element 0: each goes through a value
+    uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    const uint32_t a0 = a[0], a1 = a[1];
+    u = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
+    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    const uint32_t b0 = b[0], b1 = b[1];
+    return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
+}
+__device__ __forceinline__ float max_over_groups(float x) {
+    return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
+}
+__device__ __forceinline__ float sum_over_groups(float x) {
+    return over_groups(x, [](float a, float b) { return a + b; });
+}
+
+// Inclusive sum over the wavefront's lanes, by row shifts and broadcasts.
+__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
+    int v = static_cast<int>(x);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
+    return static_cast<uint32_t>(v);
+}
+__device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
+
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// The bytes of w whose index is below n (0 .. 4)
-__device__ __forceinline__ uint32_t keep_bytes(uint32_t w, int n) {
-    return n >= 4 ? w : n <= 0 ? 0u : w & ((1u << (8 * n)) - 1u);
-}
+// All bits of the bytes whose index is below n
+__device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 
 // One wavefront's share of rows [row0, row0 + 16) of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
 template <int TYPE, int D>
@@ -90,144 +137,184 @@ struct Rows {
     static constexpr int kChunks = D / 64;  // 16-byte loads of a K row, by four lanes each
     static constexpr int kDims = D / 16;    // 16-dimension blocks of V^T
 
-    uint4 q[2 * kChunks];  // 8 bf16 each: this lane's row, dimensions 64 i + 16 g + 8 s ..
+    static constexpr int kSteps = D / 32;   // k-steps of the first product
+
     f32x4 o[kDims];
     float m, l;
     int limit;  // tokens that this lane's row sees
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, int b, int head, int row0, int at, int n, int length) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15);
-        const int token = row / a.group;
+    __device__ __forceinline__ void begin(const AttendArgs& a, int row0, int n, int length) {
+        const int token = (row0 + static_cast<int>(threadIdx.x & 15)) / a.group;
         m = -__builtin_inff();
         l = 0.0f;
-        limit = 0;
+        limit = token >= n ? 0 : a.causal ? min(length, max(length - n + token + 1, 0)) : length;
 #pragma unroll
         for (int i = 0; i < kDims; i++) o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        if (token < n) {
-            limit = a.causal ? min(length, max(length - n + token + 1, 0)) : length;
-            const uint16_t* p = a.q + static_cast<int64_t>(at + token) * a.q_token_stride +
-                                static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 16 * g;
-            if (a.wide_q) {
-#pragma unroll
-                for (int i = 0; i < 2 * kChunks; i++)
-                    q[i] = *reinterpret_cast<const uint4*>(p + 64 * (i / 2) + 8 * (i % 2));
-            } else {
-#pragma unroll
-                for (int i = 0; i < 2 * kChunks; i++) {
-                    const uint16_t* e = p + 64 * (i / 2) + 8 * (i % 2);
-                    q[i] = make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-                }
+    }
+
+    // The rows' q in the order in which the product takes it, 16 bytes for each k-step and lane: step 2 i + s of lane
+    // (row, g) is dimensions 64 i + 16 g + 8 s .., 0 for rows that are not there. By all of the workgroup's threads.
+    static __device__ __forceinline__ void stage_q(const AttendArgs& a, uint4 (*q)[64], int head, int row0, int at, int n) {
+        for (int i = threadIdx.x; i < kSteps * 64; i += blockDim.x) {
+            const int step = i >> 6, row = row0 + (i & 15), g = (i >> 4) & 3, token = row / a.group;
+            uint4 x = make_uint4(0, 0, 0, 0);
+            if (token < n) {
+                const uint16_t* e = a.q + static_cast<int64_t>(at + token) * a.q_token_stride +
+                                    static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride +
+                                    64 * (step >> 1) + 16 * g + 8 * (step & 1);
+                x = a.wide_q ? *reinterpret_cast<const uint4*>(e)
+                             : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
             }
-        } else {
-#pragma unroll
-            for (int i = 0; i < 2 * kChunks; i++) q[i] = make_uint4(0, 0, 0, 0);
+            q[step][i & 63] = x;
         }
     }
 
-    // tokens [base, base + 64) of the sequence
-    __device__ __forceinline__ void tile(const AttendArgs& a, int b, int head, int base, int length) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
-        const int P = a.c.page_tokens;
-        // K: this lane's tokens of the four products lie in the tile's 16-token group m16 / 4; V and the scores: group g
-        const int kpos = base + 16 * (m16 >> 2), vpos = base + 16 * g;
-        const int kpage = a.s.page(b, a.c.column(kpos), a.c.pages), vpage = a.s.page(b, a.c.column(vpos), a.c.pages);
-        const uint8_t* kp = a.c.k + (a.c.block(max(kpage, 0), head) * P + a.c.within(kpos) + (m16 & 3)) * D + 16 * g;
-        const uint8_t* vp = a.c.v + a.c.block(max(vpage, 0), head) * P * D + m16 * P + a.c.within(vpos);
-        uint4 kr[4][kChunks], vr[kDims];
+    uint4 kr[4][kChunks], vr[kDims];  // the tile's bytes
+    float ks, vs;                     // scales of this lane's 16 tokens
+    int kpage, vpage, vhere;          // the tile's pages after find(); vhere: V's page of the tile that is loaded
+
+    // Tokens [base, base + 64) of the sequence: K's tokens of a lane's four products lie in the tile's 16-token group
+    // (lane % 16) / 4, V's and the scores' in group lane / 16.
+    static __device__ __forceinline__ int kpos(int base) { return base + 16 * ((threadIdx.x & 15) >> 2); }
+    static __device__ __forceinline__ int vpos(int base) { return base + 16 * ((threadIdx.x & 63) >> 4); }
+
+    __device__ __forceinline__ void find(const AttendArgs& a, int b, int base) {
+        kpage = a.s.page(b, a.c.column(kpos(base)), a.c.pages);
+        vpage = a.s.page(b, a.c.column(vpos(base)), a.c.pages);
+    }
+    __device__ __forceinline__ void load_k(const AttendArgs& a, int head, int base) {
+        const uint8_t* p = a.c.k + (a.c.block(max(kpage, 0), head) * a.c.page_tokens + a.c.within(kpos(base)) +
+                                    (threadIdx.x & 3)) * D + 16 * ((threadIdx.x & 63) >> 4);
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < kChunks; i++) kr[t][i] = *reinterpret_cast<const uint4*>(kp + 4 * t * D + 64 * i);
+            for (int i = 0; i < kChunks; i++) kr[t][i] = *reinterpret_cast<const uint4*>(p + 4 * t * D + 64 * i);
+        ks = a.c.k_scale[a.c.block(max(vpage, 0), head)] * a.scale_log2;
+    }
+    __device__ __forceinline__ void load_v(const AttendArgs& a, int head, int base) {
+        const int P = a.c.page_tokens;
+        const int64_t block = a.c.block(max(vpage, 0), head);
+        const uint8_t* p = a.c.v + block * P * D + (threadIdx.x & 15) * P + a.c.within(vpos(base));
 #pragma unroll
-        for (int i = 0; i < kDims; i++) vr[i] = *reinterpret_cast<const uint4*>(vp + 16 * i * P);
-        const float ks = a.c.k_scale[a.c.block(max(vpage, 0), head)] * a.scale_log2;
-        const float vs = a.c.v_scale[a.c.block(max(vpage, 0), head)];
-        const int mine = vpage < 0 ? 0 : min(max(limit - vpos, 0), 16);  // of this lane's 16 tokens, those that count
+        for (int i = 0; i < kDims; i++, p += 16 * P) vr[i] = *reinterpret_cast<const uint4*>(p);
+        vs = a.c.v_scale[block];
+        vhere = vpage;
+    }
 
-        f32x4 s[4];
+    __device__ __forceinline__ void first(const AttendArgs& a, int b, int head, int base) {
+        find(a, b, base);
+        load_k(a, head, base);
+        load_v(a, head, base);
+    }
+
+    // Tiles t0 (which first() has asked for), t0 + step, .. below t1. The bytes of the next tile are asked for as soon as this one's are used up: K's
+    // before the softmax and the second product, V's behind it, page numbers a tile earlier.
+    __device__ __forceinline__ void tiles(const AttendArgs& a, const uint4 (*q)[64], int b, int head, int t0, int t1, int step, int length) {
+        for (int t = t0; t < t1; t += step) {
+            const int base = t * kTile, next = base + step * kTile;
+            const bool more = t + step < t1;
+            if (more) find(a, b, next);
+            f32x4 s[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            s[t] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+            for (int j = 0; j < 4; j++) s[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < kChunks; i++) {
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[t][i].x, kr[t][i].y),
-                                                               __builtin_bit_cast(bf16x8, q[2 * i]), s[t], 0, 0, 0);
-                s[t] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[t][i].z, kr[t][i].w),
-                                                               __builtin_bit_cast(bf16x8, q[2 * i + 1]), s[t], 0, 0, 0);
+                const bf16x8 q0 = __builtin_bit_cast(bf16x8, q[2 * i][threadIdx.x & 63]),
+                             q1 = __builtin_bit_cast(bf16x8, q[2 * i + 1][threadIdx.x & 63]);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[j][i].x, kr[j][i].y),
+                                                                   q0, s[j], 0, 0, 0);
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[j][i].z, kr[j][i].w),
+                                                                   q1, s[j], 0, 0, 0);
             }
-        }
-        float top = m;
+            // of this lane's 16 tokens, those that count
+            const int mine = vhere < 0 ? 0 : min(max(limit - vpos(base), 0), 16);
+            float top = m;
 #pragma unroll
-        for (int t = 0; t < 4; t++)
+            for (int j = 0; j < 4; j++)
 #pragma unroll
-            for (int r = 0; r < 4; r++) {
-                s[t][r] = 4 * t + r < mine ? s[t][r] * ks : -__builtin_inff();
-                top = fmaxf(top, s[t][r]);
+                for (int r = 0; r < 4; r++) {
+                    s[j][r] = 4 * j + r < mine ? s[j][r] * ks : -__builtin_inff();
+                    top = fmaxf(top, s[j][r]);
+                }
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_k(a, head, next);
+            __builtin_amdgcn_sched_barrier(0);
+            top = max_over_groups(top);
+            const float safe = top == -__builtin_inff() ? 0.0f : top;  // a row that has seen no token yet
+            const float shrink = exp2_fast(m - safe);
+            m = top;
+            l *= shrink;
+            if (__any(shrink != 1.0f)) {
+#pragma unroll
+                for (int i = 0; i < kDims; i++) o[i] *= shrink;
             }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float safe = top == -__builtin_inff() ? 0.0f : top;  // a row that has seen no token yet
-        const float shrink = exp2_fast(m - safe);
-        m = top;
-        l *= shrink;
-        if (__any(shrink != 1.0f)) {
+            uint32_t p[8];
 #pragma unroll
-            for (int i = 0; i < kDims; i++) o[i] *= shrink;
-        }
-        uint32_t p[8];
+            for (int j = 0; j < 4; j++) {
+                float e[4];
 #pragma unroll
-        for (int t = 0; t < 4; t++) {
-            float e[4];
-#pragma unroll
-            for (int r = 0; r < 4; r++) {
-                e[r] = exp2_fast(s[t][r] - safe);
-                l += e[r];
-                // a token that does not count adds 0 whatever its block's scale is (it may be NaN)
-                e[r] = 4 * t + r < mine ? e[r] * vs : 0.0f;
+                for (int r = 0; r < 4; r++) {
+                    e[r] = exp2_fast(s[j][r] - safe);
+                    l += e[r];
+                    // a token that does not count adds 0 whatever its block's scale is (it may be NaN)
+                    e[r] = 4 * j + r < mine ? e[r] * vs : 0.0f;
+                }
+                p[2 * j] = pack_bf16(e[0], e[1]);
+                p[2 * j + 1] = pack_bf16(e[2], e[3]);
             }
-            p[2 * t] = pack_bf16(e[0], e[1]);
-            p[2 * t + 1] = pack_bf16(e[2], e[3]);
-        }
-        if (base + kTile > length || __any(vpage < 0)) {
-            // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
-            const int there = vpage < 0 ? 0 : min(max(length - vpos, 0), 16);
+            if (base + kTile > length || __any(vhere < 0)) {
+                // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
+                const int there = vhere < 0 ? 0 : min(max(length - vpos(base), 0), 16);
+                const uint32_t m0 = byte_mask(there), m1 = byte_mask(there - 4), m2 = byte_mask(there - 8),
+                               m3 = byte_mask(there - 12);
+#pragma unroll
+                for (int i = 0; i < kDims; i++) {
+                    vr[i].x &= m0;
+                    vr[i].y &= m1;
+                    vr[i].z &= m2;
+                    vr[i].w &= m3;
+                }
+            }
+            const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
+                         p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
 #pragma unroll
             for (int i = 0; i < kDims; i++) {
-                vr[i].x = keep_bytes(vr[i].x, there);
-                vr[i].y = keep_bytes(vr[i].y, there - 4);
-                vr[i].z = keep_bytes(vr[i].z, there - 8);
-                vr[i].w = keep_bytes(vr[i].w, there - 12);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].x, vr[i].y), p0, o[i], 0, 0, 0);
+                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].z, vr[i].w), p1, o[i], 0, 0, 0);
             }
-        }
-        const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
-                     p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
-#pragma unroll
-        for (int i = 0; i < kDims; i++) {
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].x, vr[i].y), p0, o[i], 0, 0, 0);
-            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].z, vr[i].w), p1, o[i], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            if (more) load_v(a, head, next);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
 
-template <int D>
+template <int D, int WAVES>
 struct JoinLds {
-    float o[kFewWaves][kRows][D + 4];
-    float m[kFewWaves][kRows], l[kFewWaves][kRows];
+    float o[WAVES][kRows][D + 4];
+    float m[WAVES][kRows], l[WAVES][kRows];
+    uint4 q[D / 32][64];
 };
 
-// The workgroup's four wavefronts over tiles [t0, t1) of rows [row0, row0 + 16); the rows are finished into out, or, with
+// The workgroup's wavefronts over tiles [t0, t1) of rows [row0, row0 + 16); the rows are finished into out, or, with
 // slot >= 0, left as a partial result.
-template <int TYPE, int D>
-__device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D>& lds, int b, int head, int row0, int t0, int t1,
-                                            int64_t slot) {
+template <int TYPE, int D, int WAVES>
+__device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVES>& lds, int b, Seq seq, int head, int row0, int t0,
+                                            int t1, int slot) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
-    const int at = a.s.first(b), n = a.s.count(b, at), length = a.len(b);
+    const int at = seq.at, n = seq.n, length = seq.length;
     const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group - row0, static_cast<int64_t>(kRows)));
     Rows<TYPE, D> r;
-    r.begin(a, b, head, row0, at, n, length);
-    for (int t = t0 + wave; t < t1; t += kFewWaves) r.tile(a, b, head, t * kTile, length);
-    r.l += __shfl_xor(r.l, 16);
-    r.l += __shfl_xor(r.l, 32);
+    if (t0 + wave < t1) r.first(a, b, head, (t0 + wave) * kTile);
+    r.stage_q(a, lds.q, head, row0, at, n);
+    r.begin(a, row0, n, length);
+    __syncthreads();
+    r.tiles(a, lds.q, b, head, t0 + wave, t1, WAVES, length);
+    r.l = sum_over_groups(r.l);
     if (lane < kRows) {
         lds.m[wave][lane] = r.m;
         lds.l[wave][lane] = r.l;
@@ -235,7 +322,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D>& lds
     __syncthreads();
     float top = lds.m[0][m16];
 #pragma unroll
-    for (int w = 1; w < kFewWaves; w++) top = fmaxf(top, lds.m[w][m16]);
+    for (int w = 1; w < WAVES; w++) top = fmaxf(top, lds.m[w][m16]);
     const float safe = top == -__builtin_inff() ? 0.0f : top;
     if (m16 < rows) {
         const float f = exp2_fast(r.m - safe);
@@ -244,22 +331,22 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D>& lds
             *reinterpret_cast<f32x4*>(&lds.o[wave][m16][16 * i + 4 * g]) = r.o[i] * f;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * (D / 4); i += kFewWaves * 64) {
+    for (int i = threadIdx.x; i < rows * (D / 4); i += WAVES * 64) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float m = lds.m[0][row];
 #pragma unroll
-        for (int w = 1; w < kFewWaves; w++) m = fmaxf(m, lds.m[w][row]);
+        for (int w = 1; w < WAVES; w++) m = fmaxf(m, lds.m[w][row]);
         const float ms = m == -__builtin_inff() ? 0.0f : m;
         float l = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) {
+        for (int w = 0; w < WAVES; w++) {
             l += lds.l[w][row] * exp2_fast(lds.m[w][row] - ms);
             o += *reinterpret_cast<const f32x4*>(&lds.o[w][row][d]);
         }
         if (slot >= 0) {
-            *reinterpret_cast<f32x4*>(a.partial + (slot * kRows + row) * D + d) = o;
-            if (d == 0) a.partial_ml[slot * kRows + row] = make_float2(m, l);
+            *reinterpret_cast<f32x4*>(a.partial + static_cast<int64_t>(slot * a.rows + row) * D + d) = o;
+            if (d == 0) a.partial_ml[slot * a.rows + row] = make_float2(m, l);
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int token = (row0 + row) / a.group, h = head * a.group + (row0 + row) % a.group;
@@ -267,167 +354,208 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D>& lds
                 make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
         }
     }
-    __syncthreads();
 }
 
 // Calls of more than 16 rows a sequence: a workgroup for each 16 rows, sequence and kv head.
+constexpr int kTileWaves = 4;
 template <int TYPE, int D>
-__global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_tiles(AttendArgs a) {
-    __shared__ JoinLds<D> lds;
+__global__ __launch_bounds__(kTileWaves * 64, 1) void k_attend_tiles(AttendArgs a) {
+    __shared__ JoinLds<D, kTileWaves> lds;
     const int b = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * kRows;
-    const int at = a.s.first(b), n = a.s.count(b, at), length = a.len(b);
-    if (static_cast<int64_t>(row0) >= static_cast<int64_t>(n) * a.group) return;
-    const int last = min((row0 + kRows - 1) / a.group, n - 1);
-    const int seen = a.causal ? min(length, max(length - n + last + 1, 0)) : length;
-    attend_rows<TYPE, D>(a, lds, b, head, row0, 0, (seen + kTile - 1) / kTile, -1);
+    const Seq seq = a.seq(b);
+    if (static_cast<int64_t>(row0) >= static_cast<int64_t>(seq.n) * a.group) return;
+    const int last = min((row0 + kRows - 1) / a.group, seq.n - 1);
+    const int seen = a.causal ? min(seq.length, max(seq.length - seq.n + last + 1, 0)) : seq.length;
+    attend_rows<TYPE, D, kTileWaves>(a, lds, b, seq, head, row0, 0, (seen + kTile - 1) / kTile, -1);
 }
 
 // Calls of at most 16 rows a sequence are bound by reading the cache, so the cache is what is shared out: the tiles of all
 // sequences and kv heads stand in one line, and every workgroup takes the same number of them in a row, wherever sequences
 // begin and end. A (sequence, head) that lies in one share is finished there; of one that is cut, each share leaves a
-// partial result, which k_attend_join adds up in order. A share has at most two such pieces, its first and its last.
-struct Share {
-    int64_t total, each;
+// partial result, which k_attend_join adds up in order. A share has at most two such ends, its first and its last.
+// Where every sequence's last share may stay partly empty without more workgroups than the CUs hold at once, it does
+// (`pad`): a workgroup that holds an end and a beginning runs them one after the other.
+struct Line {
+    uint32_t each, pad;  // tiles of a share; a (sequence, head) takes a multiple of pad tiles of the line
+    uint32_t heads;
+
+    __device__ __forceinline__ uint32_t padded(uint32_t tiles) const { return (tiles + pad - 1) / pad * pad; }
 };
 
-__device__ __forceinline__ int seq_tiles(const AttendArgs& a, int b) {
-    if (b >= a.s.seqs || a.s.count(b, a.s.first(b)) == 0) return 0;
-    return max((a.len(b) + kTile - 1) / kTile, 1);  // a sequence without a token still has its rows to write
+__device__ __forceinline__ uint32_t tiles_of(Seq s) {
+    return s.n == 0 ? 0 : max((s.length + kTile - 1) / kTile, 1);  // without a token there are still rows to write
 }
+__device__ __forceinline__ Seq seq_or_none(const AttendArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0}; }
 
-__device__ __forceinline__ Share share_of(const AttendArgs& a, int groups) {
-    int64_t total = 0;
-    for (int b = threadIdx.x & 63; b < a.s.seqs; b += 64) total += seq_tiles(a, b);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
-    total *= a.c.kv_heads;
-    return {total, max((total + groups - 1) / groups, static_cast<int64_t>(kFewWaves))};
-}
-
-// The sequence that tile `at` of the line belongs to, and the tiles before it (every lane gets both); at < total.
-__device__ __forceinline__ int seq_at(const AttendArgs& a, int64_t at, int64_t& before) {
+// Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`.
+__device__ __forceinline__ Line line_of(const AttendArgs& a, uint32_t mine) {
+    const uint32_t heads = a.c.kv_heads;
     const int lane = threadIdx.x & 63;
-    before = 0;
-    for (int b0 = 0;; b0 += 64) {
-        int64_t sum = static_cast<int64_t>(seq_tiles(a, b0 + lane)) * a.c.kv_heads;
-        const int64_t own = sum;
-#pragma unroll
-        for (int d = 1; d < 64; d <<= 1) {
-            const int64_t other = __shfl_up(sum, d);
-            if (lane >= d) sum += other;
-        }
-        const uint64_t past = __ballot(before + sum > at);
-        if (past) {
-            const int i = __ffsll(static_cast<unsigned long long>(past)) - 1;
-            before += __shfl(sum - own, i);
-            return b0 + i;
-        }
-        if (b0 + 64 >= a.s.seqs) return a.s.seqs;
-        before += __shfl(sum, 63);
-    }
+    uint32_t total = mine;
+    for (int b = lane + 64; b < a.s.seqs; b += 64) total += tiles_of(a.seq(b));
+    total = wave_sum(total) * heads;
+    const uint32_t each = max((total + a.groups - 1) / a.groups, static_cast<uint32_t>(kFewWaves));
+    uint32_t shares = (mine + each - 1) / each;
+    for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of(a.seq(b)) + each - 1) / each;
+    return {each, wave_sum(shares) * heads <= static_cast<uint32_t>(a.groups) ? each : 1, heads};
 }
 
 template <int TYPE, int D>
-__global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(AttendArgs a) {
-    __shared__ JoinLds<D> lds;
-    const Share share = share_of(a, gridDim.x);
-    int64_t at = blockIdx.x * share.each;
-    const int64_t end = min(at + share.each, share.total);
-    if (at >= end) return;
-    int64_t before;
-    int b = seq_at(a, at, before);
-    bool first = true;
-    while (at < end && b < a.s.seqs) {
-        const int tiles = seq_tiles(a, b);
-        if (tiles == 0) {
-            b++;
-            continue;
+__global__ __launch_bounds__(kFewWaves * 64, 1) void k_attend_few(AttendArgs a) {
+    __shared__ JoinLds<D, kFewWaves> lds;
+    const int lane = threadIdx.x & 63;
+    Line line = {1, 1, static_cast<uint32_t>(a.c.kv_heads)};
+    uint32_t at, end, before = 0;  // the share, and the line before sequence b
+    int b = 0;
+    Seq seq;
+    if (a.whole) {  // a workgroup for each (sequence, head)
+        b = blockIdx.x / line.heads;
+        seq = a.seq(b);
+        const uint32_t tiles = tiles_of(seq);
+        at = blockIdx.x % line.heads * tiles;
+        end = at + tiles;
+    } else {
+        Seq mine = seq_or_none(a, lane);
+        line = line_of(a, tiles_of(mine));
+        at = blockIdx.x * line.each;
+        end = at + line.each;
+        for (;;) {
+            const uint32_t own = line.padded(tiles_of(mine)) * line.heads, sum = wave_scan(own);
+            const uint64_t past = __ballot(before + sum > at);
+            if (past) {
+                const int i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
+                before += __builtin_amdgcn_readlane(sum - own, i);
+                seq.at = __builtin_amdgcn_readlane(mine.at, i);
+                seq.n = __builtin_amdgcn_readlane(mine.n, i);
+                seq.length = __builtin_amdgcn_readlane(mine.length, i);
+                b += i;
+                break;
+            }
+            before += __builtin_amdgcn_readlane(sum, 63);
+            b += 64;
+            if (b >= a.s.seqs) return;
+            mine = seq_or_none(a, b + lane);
         }
-        const int head = static_cast<int>((at - before) / tiles), t0 = static_cast<int>((at - before) % tiles);
-        const int t1 = static_cast<int>(min(static_cast<int64_t>(tiles), t0 + (end - at)));
-        const bool whole = t0 == 0 && t1 == tiles;
-        attend_rows<TYPE, D>(a, lds, b, head, 0, t0, t1, whole ? -1 : 2 * static_cast<int64_t>(blockIdx.x) + !first);
-        first = false;
-        at += t1 - t0;
-        if (t1 == tiles && head == a.c.kv_heads - 1) {
-            before += static_cast<int64_t>(tiles) * a.c.kv_heads;
-            b++;
+    }
+    int slot = 2 * blockIdx.x;  // of the share's first piece, where it is cut; of another one that is, the last: slot + 1
+    while (at < end) {
+        const uint32_t tiles = __builtin_amdgcn_readfirstlane(tiles_of(seq)), length = line.padded(tiles);
+        if (tiles) {
+            const uint32_t head = (at - before) / length, t0 = (at - before) % length;
+            const uint32_t t1 = min(t0 + (end - at), length), stop = min(t1, tiles);
+            const bool whole = t0 == 0 && stop == tiles;
+            if (t0 < stop) {
+                if (slot & 1) __syncthreads();  // the piece before still reads the LDS
+                attend_rows<TYPE, D, kFewWaves>(a, lds, b, seq, head, 0, t0, stop, whole ? -1 : slot);
+            }
+            if (t0 == 0 && !a.whole && threadIdx.x == 0) {
+                const int rest = whole ? 0 : (tiles - stop + line.each - 1) / line.each;
+                a.pieces[b * line.heads + head] = {rest ? 1 + rest : 0, slot, 2 * (static_cast<int>(blockIdx.x) + 1), 0};
+            }
+            slot |= 1;
+            at += t1 - t0;
+            if (t1 < length || head < line.heads - 1) continue;
+            before += length * line.heads;
         }
+        if (at >= end || ++b >= a.s.seqs) break;
+        seq = a.seq(b);
     }
 }
 
-// One row of one (sequence, kv head) that was cut: its partial results, in the order of its tokens. blockIdx: (sequence and
-// head, row). A wavefront adds up every eighth part, then the eight sums are added in order.
+// One row of one (sequence, kv head) that was cut: its pieces' results, added up in the order of its tokens over eight
+// wavefronts, then those. blockIdx: (sequence and head, row).
 constexpr int kJoinWaves = 8;
 template <int D>
-__global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(AttendArgs a, int groups) {
-    __shared__ float2 ml[kJoinWaves];
+__global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(AttendArgs a) {
+    __shared__ float weight[kFewGroups];
+    __shared__ float red[2][kJoinWaves];
     __shared__ float o[kJoinWaves][D];
     const int b = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads, row = blockIdx.y;
-    const int at = a.s.first(b), n = a.s.count(b, at);
-    if (row >= n * a.group) return;
-    const Share share = share_of(a, groups);
-    int64_t before = 0;
-    for (int i = threadIdx.x & 63; i < b; i += 64) before += seq_tiles(a, i);
-#pragma unroll
-    for (int d = 32; d; d >>= 1) before += __shfl_xor(before, d);
-    const int tiles = seq_tiles(a, b);
-    before = before * a.c.kv_heads + static_cast<int64_t>(head) * tiles;
-    const int64_t w0 = before / share.each, w1 = (before + tiles - 1) / share.each;
-    if (w0 == w1) return;
+    const Seq seq = a.seq(b);
+    if (row >= seq.n * a.group) return;
+    const Pieces cut = a.pieces[blockIdx.x];
+    const int pieces = cut.pieces;
+    if (pieces == 0) return;
+    auto slot_of = [&](int i) { return i ? cut.next + 2 * (i - 1) : cut.first; };
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    float2 part = make_float2(-__builtin_inff(), 0.0f);  // of piece threadIdx.x
+    if (static_cast<int>(threadIdx.x) < pieces) part = a.partial_ml[slot_of(threadIdx.x) * a.rows + row];
+    float top = part.x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    if (lane == 0) red[0][wave] = top;
+    __syncthreads();
+    for (int w = 0; w < kJoinWaves; w++) top = fmaxf(top, red[0][w]);
+    const float safe = top == -__builtin_inff() ? 0.0f : top;
+    const float f = exp2_fast(part.x - safe);
+    if (static_cast<int>(threadIdx.x) < pieces) weight[threadIdx.x] = f;
+    float l = part.y * f;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    if (lane == 0) red[1][wave] = l;
+    __syncthreads();
     constexpr int V = D / 64;  // values of a lane
-    float m = -__builtin_inff(), l = 0.0f, acc[V] = {};
-    for (int64_t w = w0 + wave; w <= w1; w += kJoinWaves) {
-        // the first share holds this head's beginning behind whatever it began with; the others begin with this head
-        const int64_t slot = 2 * w + (w == w0 && before != w0 * share.each);
-        const float2 part = a.partial_ml[slot * kRows + row];
-        const float top = fmaxf(m, part.x), safe = top == -__builtin_inff() ? 0.0f : top;
-        const float f = exp2_fast(m - safe), fp = exp2_fast(part.x - safe);
-        const float* p = a.partial + (slot * kRows + row) * D + lane * V;
+    typedef float Lane __attribute__((ext_vector_type(V)));
+    Lane acc = {};
+    auto values = [&](int i) {
+        return *reinterpret_cast<const Lane*>(a.partial + static_cast<int64_t>(slot_of(i) * a.rows + row) * D + lane * V);
+    };
+    int i = wave;
+    for (; i + 7 * kJoinWaves < pieces; i += 8 * kJoinWaves) {
+        Lane x[8];
 #pragma unroll
-        for (int i = 0; i < V; i++) acc[i] = acc[i] * f + p[i] * fp;
-        l = l * f + part.y * fp;
-        m = top;
+        for (int e = 0; e < 8; e++) x[e] = values(i + e * kJoinWaves);
+#pragma unroll
+        for (int e = 0; e < 8; e++) acc += x[e] * weight[i + e * kJoinWaves];
     }
+    for (; i < pieces; i += kJoinWaves) acc += values(i) * weight[i];
 #pragma unroll
-    for (int i = 0; i < V; i++) o[wave][lane * V + i] = acc[i];
-    if (lane == 0) ml[wave] = make_float2(m, l);
+    for (int e = 0; e < V; e++) o[wave][lane * V + e] = acc[e];
     __syncthreads();
     if (threadIdx.x >= D) return;
-    float top = ml[0].x;
-    for (int w = 1; w < kJoinWaves; w++) top = fmaxf(top, ml[w].x);
-    const float safe = top == -__builtin_inff() ? 0.0f : top;
     float sum = 0.0f, x = 0.0f;
     for (int w = 0; w < kJoinWaves; w++) {
-        const float f = exp2_fast(ml[w].x - safe);
-        sum += ml[w].y * f;
-        x += o[w][threadIdx.x] * f;
+        sum += red[1][w];
+        x += o[w][threadIdx.x];
     }
     const int token = row / a.group, h = head * a.group + row % a.group;
     const float y = sum == 0.0f ? 0.0f : x / sum;
-    a.out[(static_cast<int64_t>(at + token) * a.q_heads + h) * D + threadIdx.x] =
+    a.out[(static_cast<int64_t>(seq.at + token) * a.q_heads + h) * D + threadIdx.x] =
         __builtin_bit_cast(uint16_t, static_cast<__bf16>(y));
 }
 
-// How a call is split: workgroups of the one-line form, 0 for the form by rows.
-int few_groups(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
+// How a call runs. groups: workgroups of the form for few rows (0: the form by rows); whole: no (sequence, kv head) is cut.
+struct Plan {
+    int64_t groups;
+    bool whole;
+};
+
+Plan plan_of(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
     const int64_t rows = static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads);
-    if (rows > kRows) return 0;
+    if (rows > kRows) return {0, false};
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
-    const int64_t tiles = (longest + kTile - 1) / kTile * b->seqs * c->kv_heads;
-    return static_cast<int>(std::min<int64_t>(kFewGroups, (tiles + kFewWaves - 1) / kFewWaves));
+    const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
+    if (longest <= kTile * kFewWaves) return {items, true};
+    // no more shares than the bound says there can be: a workgroup without one still costs its start
+    const int64_t each = (longest + kTile * kFewWaves - 1) / (kTile * kFewWaves);
+    return {std::min<int64_t>(kFewGroups, items * each), false};
 }
 
-size_t partial_bytes(int groups, int D) {
-    return groups > 1 ? static_cast<size_t>(2 * groups) * kRows * (D * sizeof(float) + sizeof(float2)) : 0;
+// Rows of all partial results that a call can leave: two a workgroup.
+int64_t partial_rows(const Plan& p, int rows) { return p.whole ? 0 : 2 * p.groups * rows; }
+size_t partial_bytes(const Plan& p, int rows, int D, int64_t items) {
+    return partial_rows(p, rows) * (D * sizeof(float) + sizeof(float2)) + (p.whole || !p.groups ? 0 : items * sizeof(Pieces));
 }
 
 int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
     if (const int rc = check_cache(cache)) return rc;
     if (const int rc = check_batch(batch)) return rc;
     if (q_heads < 1 || q_heads > 65535 || q_heads % cache->kv_heads != 0 || max_length < 0) return WL_EINVAL_SHAPE;
-    if (static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 31)) return WL_EINVAL_SHAPE;
+    // positions fit 31 bits, and so do the tiles of all sequences and kv heads together
+    const int64_t positions = int64_t{batch->table_width} * cache->page_tokens;
+    if (positions >= (int64_t{1} << 31) || (positions + kTile) / kTile * batch->seqs * cache->kv_heads >= (int64_t{1} << 31) ||
+        static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 31))
+        return WL_EINVAL_SHAPE;
     return WL_OK;
 }
 
@@ -440,7 +568,8 @@ extern "C" {
 
 size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
     if (check_attend(cache, q_heads, batch, max_length)) return 0;
-    return partial_bytes(few_groups(cache, q_heads, batch, max_length), cache->head_dim);
+    return partial_bytes(plan_of(cache, q_heads, batch, max_length), batch->max_count * (q_heads / cache->kv_heads),
+                         cache->head_dim, static_cast<int64_t>(batch->seqs) * cache->kv_heads);
 }
 
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -451,8 +580,10 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     if (layer < 0 || layer >= cache->layers || !(scale > -__builtin_inff() && scale < __builtin_inff())) return WL_EINVAL_SHAPE;
     const auto qb = reinterpret_cast<uintptr_t>(q);
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
-    const int groups = few_groups(cache, q_heads, batch, max_length);
-    const size_t need = partial_bytes(groups, cache->head_dim);
+    const Plan plan = plan_of(cache, q_heads, batch, max_length);
+    const int64_t rows = static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads);
+    const size_t need = partial_bytes(plan, static_cast<int>(rows), cache->head_dim,
+                                      static_cast<int64_t>(batch->seqs) * cache->kv_heads);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return WL_EINVAL_WORKSPACE;
     AttendArgs a = {};
     a.c = layer_of(cache, layer);
@@ -463,29 +594,29 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.q_head_stride = q_head_stride;
     a.out = out;
     a.partial = static_cast<float*>(workspace);
-    a.partial_ml = reinterpret_cast<float2*>(a.partial + static_cast<size_t>(2 * groups) * kRows * cache->head_dim);
+    a.partial_ml = reinterpret_cast<float2*>(a.partial + partial_rows(plan, static_cast<int>(rows)) * cache->head_dim);
+    a.pieces = reinterpret_cast<Pieces*>(a.partial_ml + partial_rows(plan, static_cast<int>(rows)));
+    a.rows = static_cast<int32_t>(rows);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.causal = causal != 0;
+    a.whole = plan.whole;
+    a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t rows = static_cast<int64_t>(batch->max_count) * a.group;
     auto run = [&](auto type, auto dim) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
-        if (groups == 0) {
+        if (plan.groups == 0) {
             const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows), cache->kv_heads, batch->seqs);
-            k_attend_tiles<T, D><<<grid, kFewWaves * 64, 0, st>>>(a);
+            k_attend_tiles<T, D><<<grid, kTileWaves * 64, 0, st>>>(a);
             return launch_status();
         }
-        k_attend_few<T, D><<<groups, kFewWaves * 64, 0, st>>>(a);
+        k_attend_few<T, D><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
         if (const int rc = launch_status()) return rc;
-        if (groups > 1) {
-            k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, static_cast<uint32_t>(rows)), kJoinWaves * 64, 0, st>>>(
-                a, groups);
-            return launch_status();
-        }
-        return 0;
+        if (!plan.whole)
+            k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, static_cast<uint32_t>(rows)), kJoinWaves * 64, 0, st>>>(a);
+        return launch_status();
     };
     auto with_dim = [&](auto type) {
         if (cache->head_dim == 64) return run(type, std::integral_constant<int, 64>());

@@ -11,7 +11,7 @@ inline int check_cache(const WlKvCache* c) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return WL_EINVAL_NULL;
     if (c->type != WL_KV_INT8 && c->type != WL_KV_E4M3) return WL_EINVAL_CACHE;
     if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256) return WL_EINVAL_CACHE;
-    if (c->page_tokens < 16 || c->page_tokens > 1024 || c->page_tokens % 16 != 0) return WL_EINVAL_CACHE;
+    if (c->page_tokens < 16 || c->page_tokens > 1024 || (c->page_tokens & (c->page_tokens - 1))) return WL_EINVAL_CACHE;
     if (c->pages < 1 || c->pages >= (int64_t{1} << 31) || c->layers < 1 || c->layers > 4096 || c->kv_heads < 1 ||
         c->kv_heads > 4096 || c->reserved != 0)
         return WL_EINVAL_SHAPE;
@@ -39,19 +39,15 @@ struct KvLayer {
     uint8_t* v;
     float* k_scale;
     float* v_scale;
-    int32_t pages, kv_heads, page_tokens, page_shift;  // page_shift: log2(page_tokens), or -1
+    int32_t pages, kv_heads, page_tokens, page_shift;  // page_shift: log2(page_tokens)
 
     // Byte offset of a (page, head) block, and the index of its scale: 64 bits, a cache may be far over 4 GB.
     __device__ __forceinline__ int64_t block(int page, int head) const {
         return static_cast<int64_t>(page) * kv_heads + head;
     }
     // which page of its sequence a position is in, and where in it
-    __device__ __forceinline__ int column(int pos) const {
-        return page_shift >= 0 ? pos >> page_shift : pos / page_tokens;
-    }
-    __device__ __forceinline__ int within(int pos) const {
-        return page_shift >= 0 ? pos & (page_tokens - 1) : pos % page_tokens;
-    }
+    __device__ __forceinline__ int column(int pos) const { return pos >> page_shift; }
+    __device__ __forceinline__ int within(int pos) const { return pos & (page_tokens - 1); }
 };
 
 inline KvLayer layer_of(const WlKvCache* c, int layer) {
@@ -65,8 +61,7 @@ inline KvLayer layer_of(const WlKvCache* c, int layer) {
     l.pages = static_cast<int32_t>(c->pages);
     l.kv_heads = c->kv_heads;
     l.page_tokens = c->page_tokens;
-    l.page_shift = -1;
-    if ((c->page_tokens & (c->page_tokens - 1)) == 0) l.page_shift = __builtin_ctz(c->page_tokens);
+    l.page_shift = __builtin_ctz(c->page_tokens);
     return l;
 }
 

@@ -1752,8 +1752,8 @@ const char* wl_error_string(int code) {
             return "fork scope: wl_moe_fork_begin with a scope already open on this device, or wl_moe_fork_end "
                    "without one open on this stream";
         case WL_EINVAL_CACHE:
-            return "cache: type must be WL_KV_INT8 or WL_KV_E4M3, head_dim 64, 128 or 256, page_tokens a multiple of 16 "
-                   "in 16..1024";
+            return "cache: type must be WL_KV_INT8 or WL_KV_E4M3, head_dim 64, 128 or 256, page_tokens a power "
+                   "of two in 16..1024";
         case WL_EINVAL_PAGES:
             return "page copies: a page is out of range, written twice, or both read and written";
         case WL_EINVAL_SCRATCH:

@@ -6,53 +6,63 @@ head, shared by any number of sequences through page tables (gguf.hbm_cache keep
 every decoded token. All calls only enqueue work on the current stream of their tensors' device and read page tables,
 lengths and row offsets on the GPU, so they may be captured into a HIP graph.
 """
-import contextlib
 import ctypes
 
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F32, KV_E4M3, KV_INT8, WlKvBatch, WlKvCache, WlRopeTensor, _stream, check, library
+from . import DTYPE_BF16, DTYPE_F32, KV_E4M3, KV_INT8, WlKvBatch, WlKvCache, WlRopeTensor, check, library
 
 TYPES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
 
-def _on_device(device):
-    """The device made current where it is not (a launch goes to the current device)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+def _launch(index, call, *args):
+    """call(*args, stream) with device `index` current (a launch goes to the current device) and its current stream."""
+    if index == torch.cuda.current_device():
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+        return
+    with torch.cuda.device(index):
+        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
 
 
-def _need(t, name, device, dtype, dims=None):
-    if not isinstance(t, torch.Tensor) or t.device != device or t.dtype != dtype or (dims is not None and t.dim() != dims):
-        got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
-        raise ValueError(f"{name} must be a {'' if dims is None else f'{dims}-d '}{dtype} tensor on {device} (got {got})")
+def _refuse(t, name, device, dtype, shape):
+    got = f"{t.dtype} {list(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+    raise ValueError(f"{name} must be a {dtype} tensor {shape} on {device} (got {got})")
 
 
-def _rows(t, name, device, dtype, heads, head_dim):
-    """A [tokens, heads, head_dim] tensor whose head_dim is contiguous -> (pointer, token stride, head stride)."""
-    _need(t, name, device, dtype, 3)
-    if t.shape[2] != head_dim or (heads is not None and t.shape[1] != heads):
-        raise ValueError(f"{name} must be [tokens, {'heads' if heads is None else heads}, {head_dim}] (got {list(t.shape)})")
-    if t.shape[2] > 1 and t.stride(2) != 1:
-        raise ValueError(f"{name}'s last dimension must be contiguous")
-    return t.data_ptr(), t.stride(0), t.stride(1)
+# The checks below run before every launch, so each is one expression of cheap attributes; what is wrong is worked out
+# after one has failed.
+
+
+def _need(t, name, index, dtype, shape):
+    """shape: what to say, one name or number a dimension."""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == len(shape)):
+        _refuse(t, name, f"cuda:{index}", dtype, f"[{', '.join(map(str, shape))}]")
+
+
+def _rows(t, name, index, dtype, heads, head_dim):
+    """A [tokens, heads, head_dim] tensor whose head_dim is contiguous -> (tokens, heads, token stride, head stride)."""
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.get_device() == index and t.dim() == 3:
+        n, h, d = t.shape
+        ts, hs, ds = t.stride()
+        if d == head_dim and (ds == 1 or d == 1) and (heads is None or h == heads):
+            return n, h, ts, hs
+    _refuse(t, name, f"cuda:{index}", dtype, f"[tokens, {'heads' if heads is None else heads}, {head_dim}] with a contiguous last dimension")
 
 
 class KVPages:
     """A paged key/value cache on one GPU, all layers: k int8 or float8_e4m3fn [layers, pages, kv_heads, page_tokens,
     head_dim], v of the same type [layers, pages, kv_heads, head_dim, page_tokens] (tokens innermost: the order in which the
     matrix core takes them), k_scale and v_scale fp32 [layers, pages, kv_heads], all contiguous. A value is its byte times its
-    block's scale. head_dim 64, 128 or 256; page_tokens a multiple of 16 up to 1024."""
+    block's scale. head_dim 64, 128 or 256; page_tokens a power of two, 16 to 1024."""
 
     def __init__(self, k, v, k_scale, v_scale):
         if not isinstance(k, torch.Tensor) or k.dim() != 5 or k.dtype not in TYPES:
             raise ValueError("k must be an int8 or float8_e4m3fn tensor [layers, pages, kv_heads, page_tokens, head_dim]")
         layers, pages, heads, tokens, dim = k.shape
-        _need(v, "v", k.device, k.dtype, 5)
+        _need(v, "v", k.get_device(), k.dtype, ("layers", "pages", "kv_heads", "head_dim", "page_tokens"))
         for name, t in (("k_scale", k_scale), ("v_scale", v_scale)):
-            _need(t, name, k.device, torch.float32, 3)
+            _need(t, name, k.get_device(), torch.float32, ("layers", "pages", "kv_heads"))
             if tuple(t.shape) != (layers, pages, heads):
                 raise ValueError(f"{name} must be [layers, pages, kv_heads] = {[layers, pages, heads]} (got {list(t.shape)})")
         if tuple(v.shape) != (layers, pages, heads, dim, tokens):
@@ -62,12 +72,12 @@ class KVPages:
             raise ValueError("the cache's tensors must be contiguous")
         self.k, self.v, self.k_scale, self.v_scale = k, v, k_scale, v_scale
         self.layers, self.pages, self.kv_heads, self.page_tokens, self.head_dim = layers, pages, heads, tokens, dim
-        self.dtype, self.device = k.dtype, k.device
+        self.dtype, self.device, self.index = k.dtype, k.device, k.get_device()
         s = WlKvCache()
         s.k, s.v, s.k_scale, s.v_scale = k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr()
         s.pages, s.layers, s.kv_heads, s.page_tokens, s.head_dim = pages, layers, heads, tokens, dim
         s.type = TYPES[k.dtype]
-        self.struct = s
+        self.struct, self.ref = s, ctypes.byref(s)
         check(library().wl_kv_check(ctypes.byref(s)))
 
     @classmethod
@@ -88,21 +98,21 @@ class KVPages:
 
 def _batch(pages, table, cu, per_seq, name, tokens, max_count):
     """The WlKvBatch of one call; per_seq: start or length."""
-    _need(table, "table", pages.device, torch.int32, 2)
-    _need(cu, "cu", pages.device, torch.int32, 1)
-    _need(per_seq, name, pages.device, torch.int32, 1)
-    seqs = table.shape[0]
-    if cu.shape[0] != seqs + 1 or per_seq.shape[0] != seqs:
-        raise ValueError(f"table has {seqs} sequences: cu must have {seqs + 1} entries (got {cu.shape[0]}) and {name} {seqs} "
-                         f"(got {per_seq.shape[0]})")
-    if not cu.is_contiguous() or not per_seq.is_contiguous() or (table.shape[1] > 1 and table.stride(1) != 1):
-        raise ValueError(f"cu, {name} and the rows of table must be contiguous")
-    b = WlKvBatch()
-    b.table, b.cu = table.data_ptr(), cu.data_ptr()
-    b.table_stride = table.stride(0) if seqs > 1 else max(table.stride(0), table.shape[1])
-    b.tokens, b.seqs, b.table_width = tokens, seqs, table.shape[1]
-    b.max_count = tokens if max_count is None else min(int(max_count), tokens)
-    return b
+    index = pages.index
+    if not (isinstance(table, torch.Tensor) and table.dtype is torch.int32 and table.get_device() == index and table.dim() == 2):
+        _refuse(table, "table", pages.device, torch.int32, "[sequences, pages]")
+    seqs, width = table.shape
+    row, step = table.stride()
+    for t, what, n in ((cu, "cu", seqs + 1), (per_seq, name, seqs)):
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1
+                and t.shape[0] == n and t.is_contiguous()):
+            _refuse(t, what, pages.device, torch.int32, f"[{n}] (table has {seqs} sequences), contiguous")
+    if step != 1 and width > 1:
+        raise ValueError("the rows of table must be contiguous")
+    if max_count is None or max_count > tokens:
+        max_count = tokens
+    return WlKvBatch(table.data_ptr(), cu.data_ptr(), row if seqs > 1 and row > width else max(row, width), tokens, seqs, width,
+                     max_count, 0)
 
 
 def kv_append(pages: KVPages, layer: int, k: torch.Tensor, v: torch.Tensor, table: torch.Tensor, start: torch.Tensor,
@@ -114,15 +124,15 @@ def kv_append(pages: KVPages, layer: int, k: torch.Tensor, v: torch.Tensor, tabl
     rows, a page with older tokens its scale times the smallest power of two that does (its older bytes are divided by it and
     rounded); a NaN or an infinity makes its block's scale NaN. Rows whose page is not there (no table entry, or one outside
     the cache) are dropped. Pages written in one call must be distinct over its sequences."""
-    kp, vp = (_rows(t, n, pages.device, torch.bfloat16, pages.kv_heads, pages.head_dim) for n, t in (("k", k), ("v", v)))
-    if k.shape[0] != v.shape[0]:
-        raise ValueError(f"k has {k.shape[0]} rows, v {v.shape[0]}")
-    b = _batch(pages, table, cu, start, "start", k.shape[0], max_count)
-    if k.shape[0] == 0 or b.seqs == 0:
+    n, _, k_token, k_head = _rows(k, "k", pages.index, torch.bfloat16, pages.kv_heads, pages.head_dim)
+    rows, _, v_token, v_head = _rows(v, "v", pages.index, torch.bfloat16, pages.kv_heads, pages.head_dim)
+    if n != rows:
+        raise ValueError(f"k has {n} rows, v {rows}")
+    b = _batch(pages, table, cu, start, "start", n, max_count)
+    if n == 0 or b.seqs == 0:
         return
-    with _on_device(pages.device):
-        check(library().wl_kv_append(ctypes.byref(pages.struct), layer, *kp, *vp, ctypes.byref(b), start.data_ptr(),
-                                     _stream(pages.device)))
+    _launch(pages.index, library().wl_kv_append, pages.ref, layer, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
+            ctypes.byref(b), start.data_ptr())
 
 
 def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, length: torch.Tensor, cu: torch.Tensor,
@@ -135,33 +145,32 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     sequence has (rows beyond it are not computed; default: all rows); max_length: a bound of length that only steers how the
     work is split (default: what the table's width holds). Rows behind cu[-1] of `out` stay as they are. workspace: a uint8
     tensor of kv_attend_workspace bytes; by default it comes from torch's allocator, for this call and stream."""
-    _rows(q, "q", pages.device, torch.bfloat16, None, pages.head_dim)
-    heads = q.shape[1]
+    n, heads, token_stride, head_stride = _rows(q, "q", pages.index, torch.bfloat16, None, pages.head_dim)
     if heads == 0 or heads % pages.kv_heads:
         raise ValueError(f"{heads} query heads over {pages.kv_heads} kv heads")
     if out is None:
-        out = torch.empty(q.shape, dtype=torch.bfloat16, device=q.device)
-    else:
-        _need(out, "out", pages.device, torch.bfloat16, 3)
-        if out.shape != q.shape or not out.is_contiguous():
-            raise ValueError(f"out must be a contiguous {list(q.shape)} tensor")
-    b = _batch(pages, table, cu, length, "length", q.shape[0], max_count)
-    if q.shape[0] == 0 or b.seqs == 0:
+        out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    elif not (isinstance(out, torch.Tensor) and out.dtype is torch.bfloat16 and out.get_device() == pages.index
+              and out.shape == q.shape and out.is_contiguous()):
+        _refuse(out, "out", pages.device, torch.bfloat16, f"{list(q.shape)}, contiguous,")
+    b = _batch(pages, table, cu, length, "length", n, max_count)
+    if n == 0 or b.seqs == 0:
         return out
-    most = b.table_width * pages.page_tokens
-    longest = most if max_length is None else min(int(max_length), most)
-    lib = library()
-    need = lib.wl_kv_attend_workspace_bytes(ctypes.byref(pages.struct), heads, ctypes.byref(b), longest)
-    if workspace is None:
-        workspace = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-    elif workspace.dtype != torch.uint8 or workspace.device != q.device or not workspace.is_contiguous():
-        raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
-    with _on_device(pages.device):
-        check(lib.wl_kv_attend(ctypes.byref(pages.struct), layer, q.data_ptr(), q.stride(0), q.stride(1), heads,
-                               ctypes.byref(b), length.data_ptr(), longest,
-                               pages.head_dim ** -0.5 if scale is None else scale, int(causal), out.data_ptr(),
-                               workspace.data_ptr() if workspace is not None else None,
-                               workspace.numel() if workspace is not None else 0, _stream(pages.device)))
+    longest = b.table_width * pages.page_tokens
+    if max_length is not None and max_length < longest:
+        longest = max_length
+    lib, batch = library(), ctypes.byref(b)
+    need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, batch, longest)
+    space = None
+    if workspace is not None:
+        if workspace.dtype is not torch.uint8 or workspace.get_device() != pages.index or not workspace.is_contiguous():
+            raise ValueError("workspace must be a contiguous uint8 tensor on the cache's device")
+        space, need = workspace.data_ptr(), workspace.numel()
+    elif need:
+        workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
+        space = workspace.data_ptr()
+    _launch(pages.index, lib.wl_kv_attend, pages.ref, layer, q.data_ptr(), token_stride, head_stride, heads, batch,
+            length.data_ptr(), longest, pages.head_dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), space, need)
     return out
 
 
@@ -172,9 +181,7 @@ def kv_copy(pages: KVPages, src, dst):
     src, dst = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst))
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError(f"src and dst must be lists of the same length (got {list(src.shape)} and {list(dst.shape)})")
-    with _on_device(pages.device):
-        check(library().wl_kv_copy(ctypes.byref(pages.struct), src.ctypes.data, dst.ctypes.data, src.shape[0],
-                                   _stream(pages.device)))
+    _launch(pages.index, library().wl_kv_copy, pages.ref, src.ctypes.data, dst.ctypes.data, src.shape[0])
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections=None,
@@ -186,40 +193,46 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
     frequencies i, i + axes, i + 2 axes, ..; axis 0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2)
     turn by positions[axis(j)] * inv_freq[j], taken in 64 bits; cosine and sine are multiplied by `scale`; the rest of each head
     is copied. (engines/base.py:16-89 has the one-axis form.)"""
-    if q.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"q must be bf16 or fp32 (got {q.dtype})")
-    if not q.is_cuda:
+    dtype, index = q.dtype, q.get_device()
+    if dtype is not torch.bfloat16 and dtype is not torch.float32:
+        raise ValueError(f"q must be bf16 or fp32 (got {dtype})")
+    if index < 0:
         raise ValueError(f"q must be on the GPU (got {q.device})")
-    positions = positions.reshape(1, -1) if positions.dim() == 1 else positions
-    _need(positions, "positions", q.device, torch.int64, 2)
-    _need(inv_freq, "inv_freq", q.device, torch.float64, 1)
-    half, axes = inv_freq.shape[0], positions.shape[0]
-    sections = (half,) if sections is None else tuple(int(s) for s in sections)
+    dim = q.shape[-1]
+    n, heads, token_stride, head_stride = _rows(q, "q", index, dtype, None, dim)
+    if positions.dim() == 1:
+        positions = positions[None]
+    _need(positions, "positions", index, torch.int64, ("axes", "tokens"))
+    _need(inv_freq, "inv_freq", index, torch.float64, ("rotary_dim / 2",))
+    axes, cols = positions.shape
+    axis_stride, step = positions.stride()
+    half = inv_freq.shape[0]
+    if sections is None:
+        sections = (half,)
     if len(sections) != axes:
         raise ValueError(f"positions has {axes} axes, sections {len(sections)}")
-    if positions.shape[1] != q.shape[0] or (positions.shape[1] > 1 and positions.stride(1) != 1) or not inv_freq.is_contiguous():
-        raise ValueError(f"positions must be [axes, {q.shape[0]}] with contiguous rows, inv_freq contiguous")
-    outs = (None, None) if out is None else out
-    structs, got = [], []
-    for name, x, y in (("q", q, outs[0]), ("k", k, outs[1])):
-        if x is None:
-            structs.append(None)
-            got.append(None)
-            continue
-        p, ts, hs = _rows(x, name, q.device, q.dtype, None, q.shape[2])
-        if x.shape[0] != q.shape[0]:
-            raise ValueError(f"q has {q.shape[0]} rows, k {x.shape[0]}")
-        y = torch.empty(x.shape, dtype=x.dtype, device=x.device) if y is None else y
-        yp, yts, yhs = _rows(y, "out", q.device, q.dtype, x.shape[1], q.shape[2])
-        if y.shape != x.shape or (yp == p and (yts, yhs) != (ts, hs)):
-            raise ValueError(f"out of {name} must have its shape (and its strides where it is the same memory)")
-        structs.append(WlRopeTensor(p, yp, ts, hs, yts, yhs, x.shape[1], 0))
-        got.append(y)
-    if q.shape[0] == 0:
-        return tuple(got)
-    with _on_device(q.device):
-        check(library().wl_rope(ctypes.byref(structs[0]), ctypes.byref(structs[1]) if structs[1] is not None else None,
-                                DTYPE_BF16 if q.dtype == torch.bfloat16 else DTYPE_F32, q.shape[0], q.shape[2], 2 * half,
-                                positions.data_ptr(), positions.stride(0), inv_freq.data_ptr(), axes,
-                                (ctypes.c_int32 * axes)(*sections), int(interleaved), scale, _stream(q.device)))
-    return tuple(got)
+    if cols != n or (step != 1 and n > 1) or not inv_freq.is_contiguous():
+        raise ValueError(f"positions must be [axes, {n}] with contiguous rows, inv_freq contiguous")
+
+    def rotated(x, y, rows):
+        """The struct of one tensor and where its result goes."""
+        if rows[0] != n:
+            raise ValueError(f"q has {n} rows, k {rows[0]}")
+        if y is None:
+            y = torch.empty_like(x, memory_format=torch.contiguous_format)
+            y_token, y_head = rows[1] * dim, dim
+        else:
+            m, _, y_token, y_head = _rows(y, "out", index, dtype, rows[1], dim)
+            if m != n or (y.data_ptr() == x.data_ptr() and (y_token, y_head) != rows[2:]):
+                raise ValueError("out must have its tensor's shape, and its strides where it is the same memory")
+        return y, ctypes.byref(WlRopeTensor(x.data_ptr(), y.data_ptr(), rows[2], rows[3], y_token, y_head, rows[1], 0))
+
+    q_out, k_out = (None, None) if out is None else out
+    q_out, q_arg = rotated(q, q_out, (n, heads, token_stride, head_stride))
+    k_arg = None
+    if k is not None:
+        k_out, k_arg = rotated(k, k_out, _rows(k, "k", index, dtype, None, dim))
+    if n:
+        _launch(index, library().wl_rope, q_arg, k_arg, DTYPE_BF16 if dtype is torch.bfloat16 else DTYPE_F32, n, dim, 2 * half,
+                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, (ctypes.c_int32 * axes)(*sections), interleaved, scale)
+    return q_out, k_out
