@@ -28,7 +28,7 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 constexpr int kTile = 64;       // tokens of a tile
 constexpr int kRows = 16;       // query rows of a workgroup
 constexpr int kFewWaves = 4;
-constexpr int kFewGroups = 256; // workgroups of a call of few rows: one a CU
+constexpr int kFewGroups = 512; // workgroups of a call of few rows: two a CU
 
 // A sequence of the call: its first row, its rows, its tokens.
 struct Seq {
@@ -63,6 +63,12 @@ struct AttendArgs {
         q.n = s.count(b, q.at);
         q.length = min(max(length[b], 0), s.table_width << c.page_shift);
         return q;
+    }
+    // the same for a b that all lanes share, in scalar registers
+    __device__ __forceinline__ Seq seq_uniform(int b) const {
+        const Seq q = seq(b);
+        return {__builtin_amdgcn_readfirstlane(q.at), __builtin_amdgcn_readfirstlane(q.n),
+                __builtin_amdgcn_readfirstlane(q.length)};
     }
 };
 
@@ -132,163 +138,167 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 
 // One wavefront's share of rows [row0, row0 + 16) of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
-template <int TYPE, int D>
+// PAGE: a page holds whole tiles (64 tokens or more), so a tile has one page, one address and one pair of scales.
+template <int TYPE, int D, bool PAGE>
 struct Rows {
     static constexpr int kChunks = D / 64;  // 16-byte loads of a K row, by four lanes each
     static constexpr int kDims = D / 16;    // 16-dimension blocks of V^T
 
-    static constexpr int kSteps = D / 32;   // k-steps of the first product
 
+    uint4 q[2 * kChunks];  // 8 bf16 each: this lane's row, dimensions 64 i + 16 g + 8 s ..
     f32x4 o[kDims];
     float m, l;
     int limit;  // tokens that this lane's row sees
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, int row0, int n, int length) {
-        const int token = (row0 + static_cast<int>(threadIdx.x & 15)) / a.group;
+    __device__ __forceinline__ void begin(const AttendArgs& a, int head, int row0, int at, int n, int length) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15), token = row / a.group;
         m = -__builtin_inff();
         l = 0.0f;
         limit = token >= n ? 0 : a.causal ? min(length, max(length - n + token + 1, 0)) : length;
 #pragma unroll
         for (int i = 0; i < kDims; i++) o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-    }
-
-    // The rows' q in the order in which the product takes it, 16 bytes for each k-step and lane: step 2 i + s of lane
-    // (row, g) is dimensions 64 i + 16 g + 8 s .., 0 for rows that are not there. By all of the workgroup's threads.
-    static __device__ __forceinline__ void stage_q(const AttendArgs& a, uint4 (*q)[64], int head, int row0, int at, int n) {
-        for (int i = threadIdx.x; i < kSteps * 64; i += blockDim.x) {
-            const int step = i >> 6, row = row0 + (i & 15), g = (i >> 4) & 3, token = row / a.group;
-            uint4 x = make_uint4(0, 0, 0, 0);
-            if (token < n) {
-                const uint16_t* e = a.q + static_cast<int64_t>(at + token) * a.q_token_stride +
-                                    static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride +
-                                    64 * (step >> 1) + 16 * g + 8 * (step & 1);
-                x = a.wide_q ? *reinterpret_cast<const uint4*>(e)
-                             : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-            }
-            q[step][i & 63] = x;
+        const uint16_t* p = a.q + static_cast<int64_t>(at + token) * a.q_token_stride +
+                            static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 16 * g;
+#pragma unroll
+        for (int i = 0; i < 2 * kChunks; i++) {
+            const uint16_t* e = p + 64 * (i / 2) + 8 * (i % 2);
+            q[i] = make_uint4(0, 0, 0, 0);
+            if (token < n)
+                q[i] = a.wide_q ? *reinterpret_cast<const uint4*>(e)
+                                : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
     }
 
-    uint4 kr[4][kChunks], vr[kDims];  // the tile's bytes
-    float ks, vs;                     // scales of this lane's 16 tokens
-    int kpage, vpage, vhere;          // the tile's pages after find(); vhere: V's page of the tile that is loaded
+    // A tile as it is loaded: its bytes, the scales of this lane's 16 tokens, the page they are in (below 0: not there).
+    struct Tile {
+        uint4 k[4][kChunks], v[kDims];
+        float ks, vs;
+        int page;
+        const uint8_t* more;  // where v[0] came from
+    };
+    // V's blocks that are asked for together with K, the others are when K's registers are free: with all of them at once
+    // a wavefront of 256 dimensions would not fit the 256 registers of two on a SIMD.
+    static constexpr int kEarly = D == 256 ? kDims / 2 : kDims;
+    int kpage, vpage;  // the pages of the tile that is loaded next
 
     // Tokens [base, base + 64) of the sequence: K's tokens of a lane's four products lie in the tile's 16-token group
     // (lane % 16) / 4, V's and the scores' in group lane / 16.
-    static __device__ __forceinline__ int kpos(int base) { return base + 16 * ((threadIdx.x & 15) >> 2); }
-    static __device__ __forceinline__ int vpos(int base) { return base + 16 * ((threadIdx.x & 63) >> 4); }
+    static __device__ __forceinline__ int kgroup() { return (threadIdx.x & 15) >> 2; }
+    static __device__ __forceinline__ int vgroup() { return (threadIdx.x & 63) >> 4; }
 
     __device__ __forceinline__ void find(const AttendArgs& a, int b, int base) {
-        kpage = a.s.page(b, a.c.column(kpos(base)), a.c.pages);
-        vpage = a.s.page(b, a.c.column(vpos(base)), a.c.pages);
+        if constexpr (PAGE) {
+            kpage = vpage = __builtin_amdgcn_readfirstlane(a.s.page(b, a.c.column(base), a.c.pages));
+        } else {
+            kpage = a.s.page(b, a.c.column(base + 16 * kgroup()), a.c.pages);
+            vpage = a.s.page(b, a.c.column(base + 16 * vgroup()), a.c.pages);
+        }
     }
-    __device__ __forceinline__ void load_k(const AttendArgs& a, int head, int base) {
-        const uint8_t* p = a.c.k + (a.c.block(max(kpage, 0), head) * a.c.page_tokens + a.c.within(kpos(base)) +
-                                    (threadIdx.x & 3)) * D + 16 * ((threadIdx.x & 63) >> 4);
+    __device__ __forceinline__ void load(const AttendArgs& a, Tile& x, int head, int base) const {
+        const int P = a.c.page_tokens;
+        const int64_t block = a.c.block(max(vpage, 0), head);
+        const uint8_t *k, *v;
+        if constexpr (PAGE) {  // one base for the wavefront, a lane's own offsets are the same for every tile
+            k = a.c.k + (block * P + a.c.within(base)) * D;
+            v = a.c.v + block * P * D + a.c.within(base);
+            k += static_cast<uint32_t>((16 * kgroup() + (threadIdx.x & 3)) * D + 16 * vgroup());
+            v += static_cast<uint32_t>((threadIdx.x & 15) * P + 16 * vgroup());
+        } else {
+            k = a.c.k + (a.c.block(max(kpage, 0), head) * P + a.c.within(base + 16 * kgroup()) + (threadIdx.x & 3)) * D +
+                16 * vgroup();
+            v = a.c.v + block * P * D + (threadIdx.x & 15) * P + a.c.within(base + 16 * vgroup());
+        }
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
-            for (int i = 0; i < kChunks; i++) kr[t][i] = *reinterpret_cast<const uint4*>(p + 4 * t * D + 64 * i);
-        ks = a.c.k_scale[a.c.block(max(vpage, 0), head)] * a.scale_log2;
-    }
-    __device__ __forceinline__ void load_v(const AttendArgs& a, int head, int base) {
-        const int P = a.c.page_tokens;
-        const int64_t block = a.c.block(max(vpage, 0), head);
-        const uint8_t* p = a.c.v + block * P * D + (threadIdx.x & 15) * P + a.c.within(vpos(base));
+            for (int i = 0; i < kChunks; i++) x.k[t][i] = *reinterpret_cast<const uint4*>(k + 4 * t * D + 64 * i);
+        x.ks = a.c.k_scale[block] * a.scale_log2;
 #pragma unroll
-        for (int i = 0; i < kDims; i++, p += 16 * P) vr[i] = *reinterpret_cast<const uint4*>(p);
-        vs = a.c.v_scale[block];
-        vhere = vpage;
+        for (int i = 0; i < kEarly; i++) x.v[i] = *reinterpret_cast<const uint4*>(v + 16 * i * P);
+        x.vs = a.c.v_scale[block];
+        x.page = vpage;
+        x.more = v;
     }
 
-    __device__ __forceinline__ void first(const AttendArgs& a, int b, int head, int base) {
-        find(a, b, base);
-        load_k(a, head, base);
-        load_v(a, head, base);
-    }
-
-    // Tiles t0 (which first() has asked for), t0 + step, .. below t1. The bytes of the next tile are asked for as soon as this one's are used up: K's
-    // before the softmax and the second product, V's behind it, page numbers a tile earlier.
-    __device__ __forceinline__ void tiles(const AttendArgs& a, const uint4 (*q)[64], int b, int head, int t0, int t1, int step, int length) {
-        for (int t = t0; t < t1; t += step) {
-            const int base = t * kTile, next = base + step * kTile;
-            const bool more = t + step < t1;
-            if (more) find(a, b, next);
-            f32x4 s[4];
+    __device__ __forceinline__ void add(const AttendArgs& a, Tile& x, int base, int length) {
+        f32x4 s[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) s[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < 4; j++) {
+            s[j] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int i = 0; i < kChunks; i++) {
-                const bf16x8 q0 = __builtin_bit_cast(bf16x8, q[2 * i][threadIdx.x & 63]),
-                             q1 = __builtin_bit_cast(bf16x8, q[2 * i + 1][threadIdx.x & 63]);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[j][i].x, kr[j][i].y),
-                                                                   q0, s[j], 0, 0, 0);
-#pragma unroll
-                for (int j = 0; j < 4; j++)
-                    s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(kr[j][i].z, kr[j][i].w),
-                                                                   q1, s[j], 0, 0, 0);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(x.k[j][i].x, x.k[j][i].y),
+                                                               __builtin_bit_cast(bf16x8, q[2 * i]), s[j], 0, 0, 0);
+                s[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(x.k[j][i].z, x.k[j][i].w),
+                                                               __builtin_bit_cast(bf16x8, q[2 * i + 1]), s[j], 0, 0, 0);
             }
-            // of this lane's 16 tokens, those that count
-            const int mine = vhere < 0 ? 0 : min(max(limit - vpos(base), 0), 16);
-            float top = m;
-#pragma unroll
-            for (int j = 0; j < 4; j++)
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    s[j][r] = 4 * j + r < mine ? s[j][r] * ks : -__builtin_inff();
-                    top = fmaxf(top, s[j][r]);
-                }
+        }
+        if constexpr (kEarly < kDims) {
             __builtin_amdgcn_sched_barrier(0);
-            if (more) load_k(a, head, next);
-            __builtin_amdgcn_sched_barrier(0);
-            top = max_over_groups(top);
-            const float safe = top == -__builtin_inff() ? 0.0f : top;  // a row that has seen no token yet
-            const float shrink = exp2_fast(m - safe);
-            m = top;
-            l *= shrink;
-            if (__any(shrink != 1.0f)) {
 #pragma unroll
-                for (int i = 0; i < kDims; i++) o[i] *= shrink;
+            for (int i = kEarly; i < kDims; i++) x.v[i] = *reinterpret_cast<const uint4*>(x.more + 16 * i * a.c.page_tokens);
+        }
+        const int mine = x.page < 0 ? 0 : min(max(limit - base - 16 * vgroup(), 0), 16);  // of this lane's 16 tokens, those that count
+        float top = m;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                s[j][r] = 4 * j + r < mine ? s[j][r] * x.ks : -__builtin_inff();
+                top = fmaxf(top, s[j][r]);
             }
-            uint32_t p[8];
+        top = max_over_groups(top);
+        const float safe = top == -__builtin_inff() ? 0.0f : top;  // a row that has seen no token yet
+        const float shrink = exp2_fast(m - safe);
+        m = top;
+        l *= shrink;
+        if (__any(shrink != 1.0f)) {
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                float e[4];
+            for (int i = 0; i < kDims; i++) o[i] *= shrink;
+        }
+        uint32_t p[8];
 #pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    e[r] = exp2_fast(s[j][r] - safe);
-                    l += e[r];
-                    // a token that does not count adds 0 whatever its block's scale is (it may be NaN)
-                    e[r] = 4 * j + r < mine ? e[r] * vs : 0.0f;
-                }
-                p[2 * j] = pack_bf16(e[0], e[1]);
-                p[2 * j + 1] = pack_bf16(e[2], e[3]);
+        for (int j = 0; j < 4; j++) {
+            float e[4];
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                e[r] = exp2_fast(s[j][r] - safe);
+                l += e[r];
+                // a token that does not count adds 0 whatever its block's scale is (it may be NaN)
+                e[r] = 4 * j + r < mine ? e[r] * x.vs : 0.0f;
             }
-            if (base + kTile > length || __any(vhere < 0)) {
-                // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
-                const int there = vhere < 0 ? 0 : min(max(length - vpos(base), 0), 16);
-                const uint32_t m0 = byte_mask(there), m1 = byte_mask(there - 4), m2 = byte_mask(there - 8),
-                               m3 = byte_mask(there - 12);
-#pragma unroll
-                for (int i = 0; i < kDims; i++) {
-                    vr[i].x &= m0;
-                    vr[i].y &= m1;
-                    vr[i].z &= m2;
-                    vr[i].w &= m3;
-                }
-            }
-            const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
-                         p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
+            p[2 * j] = pack_bf16(e[0], e[1]);
+            p[2 * j + 1] = pack_bf16(e[2], e[3]);
+        }
+        if (base + kTile > length || __any(x.page < 0)) {
+            // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
+            const int there = x.page < 0 ? 0 : min(max(length - base - 16 * vgroup(), 0), 16);
+            const uint32_t m0 = byte_mask(there), m1 = byte_mask(there - 4), m2 = byte_mask(there - 8), m3 = byte_mask(there - 12);
 #pragma unroll
             for (int i = 0; i < kDims; i++) {
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].x, vr[i].y), p0, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(vr[i].z, vr[i].w), p1, o[i], 0, 0, 0);
+                x.v[i].x &= m0;
+                x.v[i].y &= m1;
+                x.v[i].z &= m2;
+                x.v[i].w &= m3;
             }
-            __builtin_amdgcn_sched_barrier(0);
-            if (more) load_v(a, head, next);
-            __builtin_amdgcn_sched_barrier(0);
+        }
+        const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
+                     p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
+#pragma unroll
+        for (int i = 0; i < kDims; i++) {
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(x.v[i].x, x.v[i].y), p0, o[i], 0, 0, 0);
+            o[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(eight_bf16<TYPE>(x.v[i].z, x.v[i].w), p1, o[i], 0, 0, 0);
+        }
+    }
+
+    // Tiles t0 (which has been found), t0 + step, .. below t1.
+    __device__ __forceinline__ void tiles(const AttendArgs& a, int b, int head, int t0, int t1, int step,
+                                          int length) {
+        for (int t = t0; t < t1; t += step) {
+            Tile x;
+            load(a, x, head, t * kTile);
+            if (t + step < t1) find(a, b, (t + step) * kTile);
+            add(a, x, t * kTile, length);
         }
     }
 };
@@ -297,23 +307,20 @@ template <int D, int WAVES>
 struct JoinLds {
     float o[WAVES][kRows][D + 4];
     float m[WAVES][kRows], l[WAVES][kRows];
-    uint4 q[D / 32][64];
 };
 
 // The workgroup's wavefronts over tiles [t0, t1) of rows [row0, row0 + 16); the rows are finished into out, or, with
 // slot >= 0, left as a partial result.
-template <int TYPE, int D, int WAVES>
+template <int TYPE, int D, bool PAGE, int WAVES>
 __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVES>& lds, int b, Seq seq, int head, int row0, int t0,
                                             int t1, int slot) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
     const int at = seq.at, n = seq.n, length = seq.length;
     const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group - row0, static_cast<int64_t>(kRows)));
-    Rows<TYPE, D> r;
-    if (t0 + wave < t1) r.first(a, b, head, (t0 + wave) * kTile);
-    r.stage_q(a, lds.q, head, row0, at, n);
-    r.begin(a, row0, n, length);
-    __syncthreads();
-    r.tiles(a, lds.q, b, head, t0 + wave, t1, WAVES, length);
+    Rows<TYPE, D, PAGE> r;
+    if (t0 + wave < t1) r.find(a, b, (t0 + wave) * kTile);
+    r.begin(a, head, row0, at, n, length);
+    r.tiles(a, b, head, t0 + wave, t1, WAVES, length);
     r.l = sum_over_groups(r.l);
     if (lane < kRows) {
         lds.m[wave][lane] = r.m;
@@ -327,7 +334,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVE
     if (m16 < rows) {
         const float f = exp2_fast(r.m - safe);
 #pragma unroll
-        for (int i = 0; i < Rows<TYPE, D>::kDims; i++)
+        for (int i = 0; i < D / 16; i++)
             *reinterpret_cast<f32x4*>(&lds.o[wave][m16][16 * i + 4 * g]) = r.o[i] * f;
     }
     __syncthreads();
@@ -358,15 +365,15 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVE
 
 // Calls of more than 16 rows a sequence: a workgroup for each 16 rows, sequence and kv head.
 constexpr int kTileWaves = 4;
-template <int TYPE, int D>
-__global__ __launch_bounds__(kTileWaves * 64, 1) void k_attend_tiles(AttendArgs a) {
+template <int TYPE, int D, bool PAGE>
+__global__ __launch_bounds__(kTileWaves * 64, 2) void k_attend_tiles(AttendArgs a) {
     __shared__ JoinLds<D, kTileWaves> lds;
     const int b = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * kRows;
-    const Seq seq = a.seq(b);
+    const Seq seq = a.seq_uniform(b);
     if (static_cast<int64_t>(row0) >= static_cast<int64_t>(seq.n) * a.group) return;
     const int last = min((row0 + kRows - 1) / a.group, seq.n - 1);
     const int seen = a.causal ? min(seq.length, max(seq.length - seq.n + last + 1, 0)) : seq.length;
-    attend_rows<TYPE, D, kTileWaves>(a, lds, b, seq, head, row0, 0, (seen + kTile - 1) / kTile, -1);
+    attend_rows<TYPE, D, PAGE, kTileWaves>(a, lds, b, seq, head, row0, 0, (seen + kTile - 1) / kTile, -1);
 }
 
 // Calls of at most 16 rows a sequence are bound by reading the cache, so the cache is what is shared out: the tiles of all
@@ -394,14 +401,15 @@ __device__ __forceinline__ Line line_of(const AttendArgs& a, uint32_t mine) {
     uint32_t total = mine;
     for (int b = lane + 64; b < a.s.seqs; b += 64) total += tiles_of(a.seq(b));
     total = wave_sum(total) * heads;
-    const uint32_t each = max((total + a.groups - 1) / a.groups, static_cast<uint32_t>(kFewWaves));
+    const uint32_t each = __builtin_amdgcn_readfirstlane(
+        max((total + a.groups - 1) / a.groups, static_cast<uint32_t>(kFewWaves)));
     uint32_t shares = (mine + each - 1) / each;
     for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of(a.seq(b)) + each - 1) / each;
     return {each, wave_sum(shares) * heads <= static_cast<uint32_t>(a.groups) ? each : 1, heads};
 }
 
-template <int TYPE, int D>
-__global__ __launch_bounds__(kFewWaves * 64, 1) void k_attend_few(AttendArgs a) {
+template <int TYPE, int D, bool PAGE>
+__global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(AttendArgs a) {
     __shared__ JoinLds<D, kFewWaves> lds;
     const int lane = threadIdx.x & 63;
     Line line = {1, 1, static_cast<uint32_t>(a.c.kv_heads)};
@@ -410,7 +418,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void k_attend_few(AttendArgs a) 
     Seq seq;
     if (a.whole) {  // a workgroup for each (sequence, head)
         b = blockIdx.x / line.heads;
-        seq = a.seq(b);
+        seq = a.seq_uniform(b);
         const uint32_t tiles = tiles_of(seq);
         at = blockIdx.x % line.heads * tiles;
         end = at + tiles;
@@ -439,14 +447,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void k_attend_few(AttendArgs a) 
     }
     int slot = 2 * blockIdx.x;  // of the share's first piece, where it is cut; of another one that is, the last: slot + 1
     while (at < end) {
-        const uint32_t tiles = __builtin_amdgcn_readfirstlane(tiles_of(seq)), length = line.padded(tiles);
+        const uint32_t tiles = tiles_of(seq), length = __builtin_amdgcn_readfirstlane(line.padded(tiles));
         if (tiles) {
-            const uint32_t head = (at - before) / length, t0 = (at - before) % length;
+            const uint32_t head = __builtin_amdgcn_readfirstlane((at - before) / length), t0 = at - before - head * length;
             const uint32_t t1 = min(t0 + (end - at), length), stop = min(t1, tiles);
             const bool whole = t0 == 0 && stop == tiles;
             if (t0 < stop) {
                 if (slot & 1) __syncthreads();  // the piece before still reads the LDS
-                attend_rows<TYPE, D, kFewWaves>(a, lds, b, seq, head, 0, t0, stop, whole ? -1 : slot);
+                attend_rows<TYPE, D, PAGE, kFewWaves>(a, lds, b, seq, head, 0, t0, stop, whole ? -1 : slot);
             }
             if (t0 == 0 && !a.whole && threadIdx.x == 0) {
                 const int rest = whole ? 0 : (tiles - stop + line.each - 1) / line.each;
@@ -458,7 +466,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 1) void k_attend_few(AttendArgs a) 
             before += length * line.heads;
         }
         if (at >= end || ++b >= a.s.seqs) break;
-        seq = a.seq(b);
+        seq = a.seq_uniform(b);
     }
 }
 
@@ -605,23 +613,27 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    auto run = [&](auto type, auto dim) {
+    auto run = [&](auto type, auto dim, auto page) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
+        constexpr bool P = decltype(page)::value;
         if (plan.groups == 0) {
             const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows), cache->kv_heads, batch->seqs);
-            k_attend_tiles<T, D><<<grid, kTileWaves * 64, 0, st>>>(a);
+            k_attend_tiles<T, D, P><<<grid, kTileWaves * 64, 0, st>>>(a);
             return launch_status();
         }
-        k_attend_few<T, D><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
+        k_attend_few<T, D, P><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
         if (const int rc = launch_status()) return rc;
         if (!plan.whole)
             k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, static_cast<uint32_t>(rows)), kJoinWaves * 64, 0, st>>>(a);
         return launch_status();
     };
+    auto with_page = [&](auto type, auto dim) {
+        return cache->page_tokens >= kTile ? run(type, dim, std::true_type()) : run(type, dim, std::false_type());
+    };
     auto with_dim = [&](auto type) {
-        if (cache->head_dim == 64) return run(type, std::integral_constant<int, 64>());
-        if (cache->head_dim == 128) return run(type, std::integral_constant<int, 128>());
-        return run(type, std::integral_constant<int, 256>());
+        if (cache->head_dim == 64) return with_page(type, std::integral_constant<int, 64>());
+        if (cache->head_dim == 128) return with_page(type, std::integral_constant<int, 128>());
+        return with_page(type, std::integral_constant<int, 256>());
     };
     if (cache->type == WL_KV_INT8) return with_dim(std::integral_constant<int, WL_KV_INT8>());
     return with_dim(std::integral_constant<int, WL_KV_E4M3>());
