@@ -394,18 +394,19 @@ __device__ __forceinline__ uint32_t tiles_of(Seq s) {
 }
 __device__ __forceinline__ Seq seq_or_none(const AttendArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0}; }
 
-// Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`.
+// Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`. Shares and (sequence, head)s are whole
+// rounds of a workgroup (a tile for each wavefront), so that only the last round of each leaves wavefronts idle.
 __device__ __forceinline__ Line line_of(const AttendArgs& a, uint32_t mine) {
-    const uint32_t heads = a.c.kv_heads;
+    constexpr uint32_t W = kFewWaves;
+    const uint32_t heads = a.c.kv_heads, groups = a.groups;
     const int lane = threadIdx.x & 63;
-    uint32_t total = mine;
-    for (int b = lane + 64; b < a.s.seqs; b += 64) total += tiles_of(a.seq(b));
-    total = wave_sum(total) * heads;
-    const uint32_t each = __builtin_amdgcn_readfirstlane(
-        max((total + a.groups - 1) / a.groups, static_cast<uint32_t>(kFewWaves)));
+    uint32_t rounds = (mine + W - 1) / W;
+    for (int b = lane + 64; b < a.s.seqs; b += 64) rounds += (tiles_of(a.seq(b)) + W - 1) / W;
+    rounds = wave_sum(rounds) * heads;
+    const uint32_t each = __builtin_amdgcn_readfirstlane(max((rounds + groups - 1) / groups, 1u) * W);
     uint32_t shares = (mine + each - 1) / each;
     for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of(a.seq(b)) + each - 1) / each;
-    return {each, wave_sum(shares) * heads <= static_cast<uint32_t>(a.groups) ? each : 1, heads};
+    return {each, wave_sum(shares) * heads <= groups ? each : W, heads};
 }
 
 template <int TYPE, int D, bool PAGE>
