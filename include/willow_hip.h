@@ -324,7 +324,7 @@ size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const W
  * length[b] - n + i. out = sum_j softmax_j(scale * q . k_j) v_j over the positions j < length[b] and, with causal != 0,
  * j <= the row's own position; a row that sees no token is 0. Softmax statistics and sums are fp32; the weights are rounded
  * to bf16 for the matrix core, which adds up in fp32.
- * max_length: a bound of length[], from which the work's split is chosen (results hold whatever it says).
+ * scale: finite, not negative. max_length: a bound of length[], from which the work's split is chosen (results hold whatever it says).
  * No counterpart in the reference, whose attention reads a bf16 cache (engines/base.py:348-366). */
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                  int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,

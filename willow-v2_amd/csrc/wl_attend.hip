@@ -1,39 +1,18 @@
-// Attention over the paged 8-bit cache (wl_kv_attend).
+// Attention over the paged 8-bit cache (wl_kv_attend): the entry points, and the form for few rows.
 //
-// Every query row of a kv head's group (row = token * group + head in the group) meets the same keys and values, so the
-// rows are the matrix core's second axis. A wavefront takes 16 rows and tiles of 64 tokens, all in registers:
-//   S^T = K Q^T    v_mfma_f32_16x16x32_bf16, A = 16 tokens of K, B = 16 rows of q; the result's lane holds one row
-//                  (lane % 16) and four of the 16 tokens, so a row's statistics are a lane's own values and two exchanges
-//                  over the four groups of lanes;
-//   O^T = V^T P^T  A = 16 of V's dimensions over 32 tokens, B = the weights, which the lanes hold in just the order in
-//                  which this product takes them: no exchange and no LDS between the two products.
-// That works because an operand's inner index may be any permutation as long as both operands share it, and the first
-// product's token rows may be any tokens: row m of its t-th product is token 16 (m / 4) + 4 t + m % 4 of the tile. A lane
-// of group g then holds the scores of tokens 16 g .. 16 g + 15, and reads 16 consecutive bytes of V^T for each dimension.
-// Bytes become bf16 exactly (|int8| <= 127 and e4m3 have at most 8 significant bits); a block's scale multiplies its
-// scores in fp32, and V's scale multiplies the weights in fp32 before they are rounded to bf16.
+// At most 16 rows of a (sequence, kv head): a wavefront takes the rows and tiles of 64 tokens, all in registers, with
+// v_mfma_f32_16x16x32_bf16. Row m of the first product's t-th operand is token 16 (m / 4) + 4 t + m % 4 of the tile, so a
+// lane of group g (of four) holds the scores of tokens 16 g .. 16 g + 15 of row lane % 16.
 #include <algorithm>
-#include <type_traits>
 
-#include "wl_kv.h"
+#include "wl_attend.h"
 
 namespace wl {
 namespace {
 
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef float f32x2 __attribute__((ext_vector_type(2)));
-typedef float f32x4 __attribute__((ext_vector_type(4)));
-
-constexpr int kTile = 64;       // tokens of a tile
-constexpr int kRows = 16;       // query rows of a workgroup
+constexpr int kRows = 16;
 constexpr int kFewWaves = 4;
-constexpr int kFewGroups = 512; // workgroups of a call of few rows: two a CU
-
-// A sequence of the call: its first row, its rows, its tokens.
-struct Seq {
-    int at, n, length;
-};
+constexpr int kFewGroups = 512;  // workgroups: two a CU
 
 // Where the partial results of a (sequence, kv head) lie: slot first, then two slots further for each of the other pieces,
 // from `next` on. pieces is 0 where there are none.
@@ -41,103 +20,15 @@ struct Pieces {
     int32_t pieces, first, next, reserved;
 };
 
-struct AttendArgs {
-    KvLayer c;
-    KvSeqs s;
-    const int32_t* length;
-    const uint16_t* q;
-    int64_t q_token_stride, q_head_stride;
-    uint16_t* out;
-    float* partial;      // [pieces of what was cut][rows][D]
-    float2* partial_ml;  // [pieces of what was cut][rows]: maximum (in log2) and sum
+struct FewArgs : AttendArgs {
+    float* partial;      // [2 * workgroups][rows][D]
+    float2* partial_ml;  // [2 * workgroups][rows]: maximum (in log2) and sum
     Pieces* pieces;      // [seqs][kv heads]
-    int32_t rows;        // rows of a (sequence, kv head), at most, where they are few
-    int32_t q_heads, group;
-    float scale_log2;  // scale * log2(e)
-    int32_t causal, wide_q;
-    int32_t whole, groups;  // how a call of few rows is cut: not at all, or over how many workgroups
-
-    __device__ __forceinline__ Seq seq(int b) const {
-        Seq q;
-        q.at = s.first(b);
-        q.n = s.count(b, q.at);
-        q.length = min(max(length[b], 0), s.table_width << c.page_shift);
-        return q;
-    }
-    // the same for a b that all lanes share, in scalar registers
-    __device__ __forceinline__ Seq seq_uniform(int b) const {
-        const Seq q = seq(b);
-        return {__builtin_amdgcn_readfirstlane(q.at), __builtin_amdgcn_readfirstlane(q.n),
-                __builtin_amdgcn_readfirstlane(q.length)};
-    }
+    int32_t rows;        // rows of a (sequence, kv head), at most
+    int32_t whole, groups;  // how the call is cut: not at all, or over how many workgroups
 };
 
-template <int TYPE>
-__device__ __forceinline__ uint32_t two_bf16(uint32_t w, bool high) {
-    if constexpr (TYPE == WL_KV_INT8) {
-        const int i0 = static_cast<int8_t>(high ? w >> 16 : w), i1 = static_cast<int8_t>(high ? w >> 24 : w >> 8);
-        const uint32_t f0 = __builtin_bit_cast(uint32_t, static_cast<float>(i0)),
-                       f1 = __builtin_bit_cast(uint32_t, static_cast<float>(i1));
-        return __builtin_amdgcn_perm(f1, f0, 0x07060302u);  // the upper halves: exact, 8 significant bits
-    } else {
-        return __builtin_bit_cast(uint32_t, high ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, true)
-                                                 : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.0f, false));
-    }
-}
-
-// 8 bytes of the cache as bf16
-template <int TYPE>
-__device__ __forceinline__ bf16x8 eight_bf16(uint32_t lo, uint32_t hi) {
-    uint4 r;
-    r.x = two_bf16<TYPE>(lo, false);
-    r.y = two_bf16<TYPE>(lo, true);
-    r.z = two_bf16<TYPE>(hi, false);
-    r.w = two_bf16<TYPE>(hi, true);
-    return __builtin_bit_cast(bf16x8, r);
-}
-
-__device__ __forceinline__ uint32_t pack_bf16(float a, float b) {
-    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, bf16x2));
-}
-
-// Over the four lanes that hold one row's values: lanes 16, 32 and 48 apart.
-template <typename F>
-__device__ __forceinline__ float over_groups(float x, F f) {
-    // a bit_cast straight from a vector's element reads element 0: each goes through a value
-    uint32_t u = __builtin_bit_cast(uint32_t, x);
-    const auto a = __builtin_amdgcn_permlane16_swap(u, u, false, false);
-    const uint32_t a0 = a[0], a1 = a[1];
-    u = __builtin_bit_cast(uint32_t, f(__builtin_bit_cast(float, a0), __builtin_bit_cast(float, a1)));
-    const auto b = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    const uint32_t b0 = b[0], b1 = b[1];
-    return f(__builtin_bit_cast(float, b0), __builtin_bit_cast(float, b1));
-}
-__device__ __forceinline__ float max_over_groups(float x) {
-    return over_groups(x, [](float a, float b) { return fmaxf(a, b); });
-}
-__device__ __forceinline__ float sum_over_groups(float x) {
-    return over_groups(x, [](float a, float b) { return a + b; });
-}
-
-// Inclusive sum over the wavefront's lanes, by row shifts and broadcasts.
-__device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
-    int v = static_cast<int>(x);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // row_shr 1, 2, 4, 8
-    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
-    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // row_bcast 15, 31
-    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);
-    return static_cast<uint32_t>(v);
-}
-__device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
-
-__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
-// All bits of the bytes whose index is below n
-__device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
-
-// One wavefront's share of rows [row0, row0 + 16) of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
+// One wavefront's share of the rows of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
 // PAGE: a page holds whole tiles (64 tokens or more), so a tile has one page, one address and one pair of scales.
 template <int TYPE, int D, bool PAGE>
 struct Rows {
@@ -150,8 +41,8 @@ struct Rows {
     float m, l;
     int limit;  // tokens that this lane's row sees
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, int head, int row0, int at, int n, int length) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15), token = row / a.group;
+    __device__ __forceinline__ void begin(const AttendArgs& a, int head, int at, int n, int length) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, row = lane & 15, token = row / a.group;
         m = -__builtin_inff();
         l = 0.0f;
         limit = token >= n ? 0 : a.causal ? min(length, max(length - n + token + 1, 0)) : length;
@@ -303,24 +194,24 @@ struct Rows {
     }
 };
 
-template <int D, int WAVES>
+template <int D>
 struct JoinLds {
-    float o[WAVES][kRows][D + 4];
-    float m[WAVES][kRows], l[WAVES][kRows];
+    float o[kFewWaves][kRows][D + 4];
+    float m[kFewWaves][kRows], l[kFewWaves][kRows];
 };
 
-// The workgroup's wavefronts over tiles [t0, t1) of rows [row0, row0 + 16); the rows are finished into out, or, with
+// The workgroup's wavefronts over tiles [t0, t1) of the rows; the rows are finished into out, or, with
 // slot >= 0, left as a partial result.
-template <int TYPE, int D, bool PAGE, int WAVES>
-__device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVES>& lds, int b, Seq seq, int head, int row0, int t0,
+template <int TYPE, int D, bool PAGE>
+__device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, int b, Seq seq, int head, int t0,
                                             int t1, int slot) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
     const int at = seq.at, n = seq.n, length = seq.length;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group - row0, static_cast<int64_t>(kRows)));
+    const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group, static_cast<int64_t>(kRows)));
     Rows<TYPE, D, PAGE> r;
     if (t0 + wave < t1) r.find(a, b, (t0 + wave) * kTile);
-    r.begin(a, head, row0, at, n, length);
-    r.tiles(a, b, head, t0 + wave, t1, WAVES, length);
+    r.begin(a, head, at, n, length);
+    r.tiles(a, b, head, t0 + wave, t1, kFewWaves, length);
     r.l = sum_over_groups(r.l);
     if (lane < kRows) {
         lds.m[wave][lane] = r.m;
@@ -329,7 +220,7 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVE
     __syncthreads();
     float top = lds.m[0][m16];
 #pragma unroll
-    for (int w = 1; w < WAVES; w++) top = fmaxf(top, lds.m[w][m16]);
+    for (int w = 1; w < kFewWaves; w++) top = fmaxf(top, lds.m[w][m16]);
     const float safe = top == -__builtin_inff() ? 0.0f : top;
     if (m16 < rows) {
         const float f = exp2_fast(r.m - safe);
@@ -338,16 +229,16 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVE
             *reinterpret_cast<f32x4*>(&lds.o[wave][m16][16 * i + 4 * g]) = r.o[i] * f;
     }
     __syncthreads();
-    for (int i = threadIdx.x; i < rows * (D / 4); i += WAVES * 64) {
+    for (int i = threadIdx.x; i < rows * (D / 4); i += kFewWaves * 64) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
         float m = lds.m[0][row];
 #pragma unroll
-        for (int w = 1; w < WAVES; w++) m = fmaxf(m, lds.m[w][row]);
+        for (int w = 1; w < kFewWaves; w++) m = fmaxf(m, lds.m[w][row]);
         const float ms = m == -__builtin_inff() ? 0.0f : m;
         float l = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < WAVES; w++) {
+        for (int w = 0; w < kFewWaves; w++) {
             l += lds.l[w][row] * exp2_fast(lds.m[w][row] - ms);
             o += *reinterpret_cast<const f32x4*>(&lds.o[w][row][d]);
         }
@@ -356,24 +247,11 @@ __device__ __forceinline__ void attend_rows(const AttendArgs& a, JoinLds<D, WAVE
             if (d == 0) a.partial_ml[slot * a.rows + row] = make_float2(m, l);
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int token = (row0 + row) / a.group, h = head * a.group + (row0 + row) % a.group;
+            const int token = (row) / a.group, h = head * a.group + (row) % a.group;
             *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(at + token) * a.q_heads + h) * D + d) =
                 make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
         }
     }
-}
-
-// Calls of more than 16 rows a sequence: a workgroup for each 16 rows, sequence and kv head.
-constexpr int kTileWaves = 4;
-template <int TYPE, int D, bool PAGE>
-__global__ __launch_bounds__(kTileWaves * 64, 2) void k_attend_tiles(AttendArgs a) {
-    __shared__ JoinLds<D, kTileWaves> lds;
-    const int b = blockIdx.z, head = blockIdx.y, row0 = blockIdx.x * kRows;
-    const Seq seq = a.seq_uniform(b);
-    if (static_cast<int64_t>(row0) >= static_cast<int64_t>(seq.n) * a.group) return;
-    const int last = min((row0 + kRows - 1) / a.group, seq.n - 1);
-    const int seen = a.causal ? min(seq.length, max(seq.length - seq.n + last + 1, 0)) : seq.length;
-    attend_rows<TYPE, D, PAGE, kTileWaves>(a, lds, b, seq, head, row0, 0, (seen + kTile - 1) / kTile, -1);
 }
 
 // Calls of at most 16 rows a sequence are bound by reading the cache, so the cache is what is shared out: the tiles of all
@@ -392,11 +270,11 @@ struct Line {
 __device__ __forceinline__ uint32_t tiles_of(Seq s) {
     return s.n == 0 ? 0 : max((s.length + kTile - 1) / kTile, 1);  // without a token there are still rows to write
 }
-__device__ __forceinline__ Seq seq_or_none(const AttendArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0}; }
+__device__ __forceinline__ Seq seq_or_none(const FewArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0}; }
 
 // Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`. Shares and (sequence, head)s are whole
 // rounds of a workgroup (a tile for each wavefront), so that only the last round of each leaves wavefronts idle.
-__device__ __forceinline__ Line line_of(const AttendArgs& a, uint32_t mine) {
+__device__ __forceinline__ Line line_of(const FewArgs& a, uint32_t mine) {
     constexpr uint32_t W = kFewWaves;
     const uint32_t heads = a.c.kv_heads, groups = a.groups;
     const int lane = threadIdx.x & 63;
@@ -410,8 +288,8 @@ __device__ __forceinline__ Line line_of(const AttendArgs& a, uint32_t mine) {
 }
 
 template <int TYPE, int D, bool PAGE>
-__global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(AttendArgs a) {
-    __shared__ JoinLds<D, kFewWaves> lds;
+__global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
+    __shared__ JoinLds<D> lds;
     const int lane = threadIdx.x & 63;
     Line line = {1, 1, static_cast<uint32_t>(a.c.kv_heads)};
     uint32_t at, end, before = 0;  // the share, and the line before sequence b
@@ -455,7 +333,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(AttendArgs a) 
             const bool whole = t0 == 0 && stop == tiles;
             if (t0 < stop) {
                 if (slot & 1) __syncthreads();  // the piece before still reads the LDS
-                attend_rows<TYPE, D, PAGE, kFewWaves>(a, lds, b, seq, head, 0, t0, stop, whole ? -1 : slot);
+                attend_rows<TYPE, D, PAGE>(a, lds, b, seq, head, t0, stop, whole ? -1 : slot);
             }
             if (t0 == 0 && !a.whole && threadIdx.x == 0) {
                 const int rest = whole ? 0 : (tiles - stop + line.each - 1) / line.each;
@@ -475,7 +353,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(AttendArgs a) 
 // wavefronts, then those. blockIdx: (sequence and head, row).
 constexpr int kJoinWaves = 8;
 template <int D>
-__global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(AttendArgs a) {
+__global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(FewArgs a) {
     __shared__ float weight[kFewGroups];
     __shared__ float red[2][kJoinWaves];
     __shared__ float o[kJoinWaves][D];
@@ -533,15 +411,17 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(AttendArgs a) {
         __builtin_bit_cast(uint16_t, static_cast<__bf16>(y));
 }
 
-// How a call runs. groups: workgroups of the form for few rows (0: the form by rows); whole: no (sequence, kv head) is cut.
-struct Plan {
+// How a call of few rows is cut. whole: a workgroup for each (sequence, kv head); else the line of tiles over `groups`.
+struct FewPlan {
     int64_t groups;
     bool whole;
 };
 
-Plan plan_of(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
-    const int64_t rows = static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads);
-    if (rows > kRows) return {0, false};
+bool is_few(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
+    return static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads) <= kRows;
+}
+
+FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length) {
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
     const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
     if (longest <= kTile * kFewWaves) return {items, true};
@@ -550,10 +430,15 @@ Plan plan_of(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_le
     return {std::min<int64_t>(kFewGroups, items * each), false};
 }
 
-// Rows of all partial results that a call can leave: two a workgroup.
-int64_t partial_rows(const Plan& p, int rows) { return p.whole ? 0 : 2 * p.groups * rows; }
-size_t partial_bytes(const Plan& p, int rows, int D, int64_t items) {
-    return partial_rows(p, rows) * (D * sizeof(float) + sizeof(float2)) + (p.whole || !p.groups ? 0 : items * sizeof(Pieces));
+// The workspace of a call of few rows: two slots of partial results a workgroup, then where they are.
+struct FewSpace {
+    size_t ml, pieces, bytes;  // offsets, total
+};
+FewSpace few_space(const WlKvCache* c, int q_heads, const WlKvBatch* b, const FewPlan& p) {
+    if (p.whole) return {0, 0, 0};
+    const size_t rows = static_cast<size_t>(2 * p.groups) * b->max_count * (q_heads / c->kv_heads);
+    const size_t ml = rows * c->head_dim * sizeof(float), pieces = ml + rows * sizeof(float2);
+    return {ml, (pieces + 15) / 16 * 16, (pieces + 15) / 16 * 16 + static_cast<size_t>(b->seqs) * c->kv_heads * sizeof(Pieces)};
 }
 
 int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
@@ -563,7 +448,7 @@ int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, in
     // positions fit 31 bits, and so do the tiles of all sequences and kv heads together
     const int64_t positions = int64_t{batch->table_width} * cache->page_tokens;
     if (positions >= (int64_t{1} << 31) || (positions + kTile) / kTile * batch->seqs * cache->kv_heads >= (int64_t{1} << 31) ||
-        static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 31))
+        static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 30))
         return WL_EINVAL_SHAPE;
     return WL_OK;
 }
@@ -577,8 +462,8 @@ extern "C" {
 
 size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
     if (check_attend(cache, q_heads, batch, max_length)) return 0;
-    return partial_bytes(plan_of(cache, q_heads, batch, max_length), batch->max_count * (q_heads / cache->kv_heads),
-                         cache->head_dim, static_cast<int64_t>(batch->seqs) * cache->kv_heads);
+    if (!is_few(cache, q_heads, batch)) return attend_rows_workspace(cache, q_heads, batch, max_length);
+    return few_space(cache, q_heads, batch, few_plan(cache, batch, max_length)).bytes;
 }
 
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
@@ -586,15 +471,12 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
                  uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_attend(cache, q_heads, batch, max_length)) return rc;
     if (!q || !length || !out) return WL_EINVAL_NULL;
-    if (layer < 0 || layer >= cache->layers || !(scale > -__builtin_inff() && scale < __builtin_inff())) return WL_EINVAL_SHAPE;
+    if (layer < 0 || layer >= cache->layers || !(scale >= 0.0f && scale < __builtin_inff())) return WL_EINVAL_SHAPE;
     const auto qb = reinterpret_cast<uintptr_t>(q);
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
-    const Plan plan = plan_of(cache, q_heads, batch, max_length);
-    const int64_t rows = static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads);
-    const size_t need = partial_bytes(plan, static_cast<int>(rows), cache->head_dim,
-                                      static_cast<int64_t>(batch->seqs) * cache->kv_heads);
+    const size_t need = wl_kv_attend_workspace_bytes(cache, q_heads, batch, max_length);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return WL_EINVAL_WORKSPACE;
-    AttendArgs a = {};
+    FewArgs a = {};
     a.c = layer_of(cache, layer);
     a.s = seqs_of(batch);
     a.length = length;
@@ -602,30 +484,27 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.q_token_stride = q_token_stride;
     a.q_head_stride = q_head_stride;
     a.out = out;
-    a.partial = static_cast<float*>(workspace);
-    a.partial_ml = reinterpret_cast<float2*>(a.partial + partial_rows(plan, static_cast<int>(rows)) * cache->head_dim);
-    a.pieces = reinterpret_cast<Pieces*>(a.partial_ml + partial_rows(plan, static_cast<int>(rows)));
-    a.rows = static_cast<int32_t>(rows);
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
     a.scale_log2 = scale * 1.44269504088896340736f;
     a.causal = causal != 0;
-    a.whole = plan.whole;
-    a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (!is_few(cache, q_heads, batch)) return launch_attend_rows(cache, a, batch, max_length, workspace, st);
+    const FewPlan plan = few_plan(cache, batch, max_length);
+    const FewSpace space = few_space(cache, q_heads, batch, plan);
+    a.partial = static_cast<float*>(workspace);
+    a.partial_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + space.ml);
+    a.pieces = reinterpret_cast<Pieces*>(static_cast<char*>(workspace) + space.pieces);
+    a.rows = batch->max_count * a.group;
+    a.whole = plan.whole;
+    a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     auto run = [&](auto type, auto dim, auto page) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
-        constexpr bool P = decltype(page)::value;
-        if (plan.groups == 0) {
-            const dim3 grid(static_cast<uint32_t>((rows + kRows - 1) / kRows), cache->kv_heads, batch->seqs);
-            k_attend_tiles<T, D, P><<<grid, kTileWaves * 64, 0, st>>>(a);
-            return launch_status();
-        }
-        k_attend_few<T, D, P><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
+        k_attend_few<T, D, decltype(page)::value><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
         if (const int rc = launch_status()) return rc;
         if (!plan.whole)
-            k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, static_cast<uint32_t>(rows)), kJoinWaves * 64, 0, st>>>(a);
+            k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, a.rows), kJoinWaves * 64, 0, st>>>(a);
         return launch_status();
     };
     auto with_page = [&](auto type, auto dim) {
