@@ -47,9 +47,9 @@ struct Shape {
     static constexpr int kSubs = kTokens / 32;   // of the first product's rows
     static constexpr int kSteps = D / 16;        // k-steps of the first product
     static constexpr int kBlocks = D / 32;       // of V's dimensions
-    // Swizzles of a k-step's 64 slots of 16 bytes: 16 lanes that write one tile's bytes fill 16 slots in a row's worth of
-    // banks, whichever k-steps those belong to.
-    static __device__ __forceinline__ constexpr int k_swizzle(int step) { return step * (256 / D) & 15; }
+    // Swizzles of a k-step's 64 slots of 16 bytes: 16 lanes that write together fill 16 slots in a row's worth of banks,
+    // whichever k-steps those belong to. Four different ones for K: a reader keeps their addresses.
+    static __device__ __forceinline__ constexpr int k_swizzle(int step) { return 4 * (step & 3); }
     static __device__ __forceinline__ constexpr int v_swizzle(int part) { return part * (16 / kParts); }
 };
 
@@ -60,32 +60,49 @@ struct Lds {
     Part part[2][Shape<D>::kParts];
 };
 
-// One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V.
-template <int TYPE, int D>
+// One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V. PAGE: a page holds
+// whole tiles, so a tile has one page and one pair of scales, all threads share its address, and the registers that other
+// tiles need for theirs are scalar ones (with 256 dimensions a wavefront has none to spare).
+template <int TYPE, int D, bool PAGE>
 struct Stage {
     using S = Shape<D>;
     uint4 k, v;
     float ks, vs;
     int kpage, vpage, count;
 
-    static __device__ __forceinline__ int k_token() { return threadIdx.x / (D / 16); }
-    static __device__ __forceinline__ int k_chunk() { return threadIdx.x % (D / 16); }
+    // 16 lanes take 4 tokens by 64 values
+    static __device__ __forceinline__ int k_token() { return (threadIdx.x >> 4) / (D / 64) * 4 + ((threadIdx.x >> 2) & 3); }
+    static __device__ __forceinline__ int k_chunk() { return (threadIdx.x >> 4) % (D / 64) * 4 + (threadIdx.x & 3); }
     static __device__ __forceinline__ int v_dim() { return threadIdx.x / S::kParts; }
     static __device__ __forceinline__ int v_part() { return threadIdx.x % S::kParts; }
 
     __device__ __forceinline__ void find(const AttendArgs& a, int b, int base) {
-        kpage = a.s.page(b, a.c.column(base + k_token()), a.c.pages);
-        vpage = a.s.page(b, a.c.column(base + 16 * v_part()), a.c.pages);
+        if constexpr (PAGE) {
+            kpage = vpage = __builtin_amdgcn_readfirstlane(a.s.page(b, a.c.column(base), a.c.pages));
+        } else {
+            kpage = a.s.page(b, a.c.column(base + k_token()), a.c.pages);
+            vpage = a.s.page(b, a.c.column(base + 16 * v_part()), a.c.pages);
+        }
     }
     __device__ __forceinline__ void load(const AttendArgs& a, int head, int base, int length) {
         const int P = a.c.page_tokens;
         const int64_t kb = a.c.block(max(kpage, 0), head), vb = a.c.block(max(vpage, 0), head);
-        k = *reinterpret_cast<const uint4*>(a.c.k + (kb * P + a.c.within(base + k_token())) * D + 16 * k_chunk());
-        v = *reinterpret_cast<const uint4*>(a.c.v + vb * P * D + v_dim() * P + a.c.within(base + 16 * v_part()));
-        count = vpage < 0 ? 0 : min(max(length - base - 16 * v_part(), 0), 16);
-        if (threadIdx.x < S::kParts) {
-            ks = a.c.k_scale[vb];
+        if constexpr (PAGE) {
+            const uint8_t* kp = a.c.k + (kb * P + a.c.within(base)) * D;
+            const uint8_t* vp = a.c.v + vb * P * D + a.c.within(base);
+            k = *reinterpret_cast<const uint4*>(kp + static_cast<uint32_t>(k_token() * D + 16 * k_chunk()));
+            v = *reinterpret_cast<const uint4*>(vp + static_cast<uint32_t>(v_dim() * P + 16 * v_part()));
+            count = vpage < 0 ? 0 : length - base;  // of the tile
+            ks = a.c.k_scale[kb];
             vs = a.c.v_scale[vb];
+        } else {
+            k = *reinterpret_cast<const uint4*>(a.c.k + (kb * P + a.c.within(base + k_token())) * D + 16 * k_chunk());
+            v = *reinterpret_cast<const uint4*>(a.c.v + vb * P * D + v_dim() * P + a.c.within(base + 16 * v_part()));
+            count = vpage < 0 ? 0 : length - base;
+            if (threadIdx.x < S::kParts) {
+                ks = a.c.k_scale[vb];
+                vs = a.c.v_scale[vb];
+            }
         }
     }
     __device__ __forceinline__ void store(const AttendArgs& a, Lds<D>& lds, int buffer) const {
@@ -96,17 +113,22 @@ struct Stage {
         to[row ^ sw] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(k.x, k.y));
         to[(32 + row) ^ sw] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(k.z, k.w));
         uint4 w = v;
-        if (count < 16) {  // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
-            w.x &= byte_mask(count);
-            w.y &= byte_mask(count - 4);
-            w.z &= byte_mask(count - 8);
-            w.w &= byte_mask(count - 12);
+        const int n = min(max(count - 16 * v_part(), 0), 16);  // tokens that are there, of this thread's part
+        if (count < S::kTokens) {  // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
+            w.x &= byte_mask(n);
+            w.y &= byte_mask(n - 4);
+            w.z &= byte_mask(n - 8);
+            w.w &= byte_mask(n - 12);
         }
         const int d = v_dim(), x = v_part(), slot = ((x & 1) * 32 + (d & 31)) ^ S::v_swizzle(x);
         uint4(*pair)[64] = &lds.v[buffer][((d >> 5) * S::kSubs + (x >> 1)) * 2];
         pair[0][slot] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(w.x, w.y));
         pair[1][slot] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(w.z, w.w));
-        if (threadIdx.x < S::kParts) lds.part[buffer][threadIdx.x] = {ks * a.scale_log2, vs, count, 0};
+        if (threadIdx.x < S::kParts) {
+            // never 0: a masked score is -inf, and times the scale it has to stay that (a block of zeros scores 0 all the same)
+            const float scaled = ks * a.scale_log2;
+            lds.part[buffer][threadIdx.x] = {scaled == 0.0f ? 1.17549435e-38f : scaled, vs, n, 0};
+        }
     }
 };
 
@@ -117,6 +139,75 @@ __device__ __forceinline__ float other_half(float x, bool add) {
     const float p = __builtin_bit_cast(float, r0), q = __builtin_bit_cast(float, r1);
     return add ? p + q : fmaxf(p, q);
 }
+
+// A wavefront's 32 rows: q, the running maximum, its lanes' sums and O^T.
+template <int D>
+struct Wave {
+    using S = Shape<D>;
+    bf16x8 q[S::kSteps];
+    f32x16 o[S::kBlocks];
+    float m, l;
+
+    // The 32 tokens of part u of a tile; seen: of this lane's 16 tokens, those that its row may see.
+    // Operands come from LDS four products ahead, V's first ones before the softmax.
+    __device__ __forceinline__ void add(const Lds<D>& lds, int buffer, int u, int seen) {
+        constexpr int kAhead = D == 256 ? 2 : 4;  // no registers for more with 256 dimensions
+        const int lane = threadIdx.x & 63, half = lane >> 5;
+        const uint4(*kt)[64] = &lds.k[buffer][u * S::kSteps];
+        f32x16 s = (f32x16)(0.0f);
+        uint4 f[kAhead];
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) f[i] = kt[i][lane ^ S::k_swizzle(i)];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int i = 0; i < S::kSteps; i++) {
+            s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[i % kAhead]), q[i], s, 0, 0, 0);
+            if (i + kAhead < S::kSteps) f[i % kAhead] = kt[i + kAhead][lane ^ S::k_swizzle(i + kAhead)];
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        const Part part = lds.part[buffer][2 * u + half];
+        const int mine = min(part.count, seen);
+        // a lane that sees no token of its block is not to meet the block's scales: they may be NaN
+        const float ks = mine > 0 ? part.ks : 1.0f, vs = mine > 0 ? part.vs : 0.0f;
+        const int slot = lane ^ S::v_swizzle(2 * u + half);
+        auto v = [&](int i) { return lds.v[buffer][(i / 2 * S::kSubs + u) * 2 + i % 2][slot]; };
+#pragma unroll
+        for (int i = 0; i < kAhead; i++) f[i] = v(i);
+        __builtin_amdgcn_sched_barrier(0);
+        if (__any(mine < 16)) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) s[i] = i < mine ? s[i] : -__builtin_inff();
+        }
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
+        top = other_half(top * ks, false);
+        if (__any(top > m + kSlack || (m == -__builtin_inff() && top > m))) {
+            const float now = fmaxf(m, top), shrink = now == -__builtin_inff() ? 1.0f : exp2_fast(m - now);
+            m = now;
+            l *= shrink;
+#pragma unroll
+            for (int i = 0; i < S::kBlocks; i++) o[i] *= shrink;
+        }
+        const float safe = m == -__builtin_inff() ? 0.0f : m;
+        uint32_t p[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            const float e0 = exp2_fast(__builtin_fmaf(s[2 * i], ks, -safe)), e1 = exp2_fast(__builtin_fmaf(s[2 * i + 1], ks, -safe));
+            l += e0 + e1;
+            p[i] = pack_bf16(e0 * vs, e1 * vs);
+        }
+        const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
+                     p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
+#pragma unroll
+        for (int i = 0; i < 2 * S::kBlocks; i++) {
+            o[i / 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[i % kAhead]), i % 2 ? p1 : p0,
+                                                               o[i / 2], 0, 0, 0);
+            if (i + kAhead < 2 * S::kBlocks) f[i % kAhead] = v(i + kAhead);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+    }
+};
 
 // Which tiles of the cache a workgroup takes of its row tile; pieces == 0: none.
 struct Cut {
@@ -133,7 +224,7 @@ __device__ __forceinline__ Cut cut_of(const RowsArgs& a, Seq seq, int row0, int 
 }
 
 // blockIdx.x: (row tile, latest tokens first as they see most of the cache; piece; kv head), blockIdx.y: sequence.
-template <int TYPE, int D>
+template <int TYPE, int D, bool PAGE>
 __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     using S = Shape<D>;
     __shared__ Lds<D> lds;
@@ -151,10 +242,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
                          static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 8 * half;
     const int most = __builtin_amdgcn_readlane(limit, 31) > 0 ? __builtin_amdgcn_readlane(limit, 31) : seq.length;
 
-    Stage<TYPE, D> st;
+    Stage<TYPE, D, PAGE> st;
     st.find(a, b, cut.t0 * S::kTokens);
     st.load(a, head, cut.t0 * S::kTokens, seq.length);
-    bf16x8 q[S::kSteps];
+    Wave<D> w;
 #pragma unroll
     for (int i = 0; i < S::kSteps; i++) {
         const uint16_t* e = qp + 16 * i;
@@ -162,12 +253,12 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
         if (there)
             x = a.wide_q ? *reinterpret_cast<const uint4*>(e)
                          : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
-        q[i] = __builtin_bit_cast(bf16x8, x);
+        w.q[i] = __builtin_bit_cast(bf16x8, x);
     }
-    f32x16 o[S::kBlocks];
 #pragma unroll
-    for (int i = 0; i < S::kBlocks; i++) o[i] = (f32x16)(0.0f);
-    float m = -__builtin_inff(), l = 0.0f;
+    for (int i = 0; i < S::kBlocks; i++) w.o[i] = (f32x16)(0.0f);
+    w.m = -__builtin_inff();
+    w.l = 0.0f;
     const bool idle = !__any(there);
 
     st.store(a, lds, 0);
@@ -182,63 +273,13 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
 #pragma unroll
         for (int u = 0; u < S::kSubs; u++) {
             if (idle || base + 32 * u >= most) break;
-            const Part part = lds.part[buffer][2 * u + half];
-            f32x16 s = (f32x16)(0.0f);
-#pragma unroll
-            for (int i = 0; i < S::kSteps; i++)
-                s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(
-                    __builtin_bit_cast(bf16x8, lds.k[buffer][u * S::kSteps + i][lane ^ S::k_swizzle(i)]), q[i], s, 0, 0, 0);
-            const int mine = min(part.count, limit - base - 32 * u - 16 * half);  // of this lane's 16 tokens
-            const bool masked = __any(mine < 16);
-            if (masked) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) s[i] = i < mine ? s[i] : -__builtin_inff();
-            }
-            float top = s[0];
-#pragma unroll
-            for (int i = 1; i < 16; i++) top = fmaxf(top, s[i]);
-            // a scale of 0 times -inf would be NaN: no token that counts leaves -inf
-            top = other_half(top == -__builtin_inff() ? top : top * part.ks, false);
-            if (__any(top > m + kSlack || (m == -__builtin_inff() && top > m))) {
-                const float now = fmaxf(m, top), shrink = now == -__builtin_inff() ? 1.0f : exp2_fast(m - now);
-                m = now;
-                l *= shrink;
-#pragma unroll
-                for (int i = 0; i < S::kBlocks; i++) o[i] *= shrink;
-            }
-            const float safe = m == -__builtin_inff() ? 0.0f : m;
-            uint32_t p[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) {
-                float e0 = exp2_fast(__builtin_fmaf(s[2 * i], part.ks, -safe)),
-                      e1 = exp2_fast(__builtin_fmaf(s[2 * i + 1], part.ks, -safe));
-                if (masked) {  // a token that does not count adds 0 whatever its block's scales are (they may be NaN)
-                    e0 = 2 * i < mine ? e0 : 0.0f;
-                    e1 = 2 * i + 1 < mine ? e1 : 0.0f;
-                }
-                l += e0 + e1;
-                e0 *= part.vs;
-                e1 *= part.vs;
-                if (masked) {
-                    e0 = 2 * i < mine ? e0 : 0.0f;
-                    e1 = 2 * i + 1 < mine ? e1 : 0.0f;
-                }
-                p[i] = pack_bf16(e0, e1);
-            }
-            const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
-                         p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
-            const int slot = lane ^ S::v_swizzle(2 * u + half);
-#pragma unroll
-            for (int i = 0; i < S::kBlocks; i++) {
-                const uint4(*v)[64] = &lds.v[buffer][(i * S::kSubs + u) * 2];
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[0][slot]), p0, o[i], 0, 0, 0);
-                o[i] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, v[1][slot]), p1, o[i], 0, 0, 0);
-            }
+            w.add(lds, buffer, u, limit - base - 32 * u - 16 * half);
         }
         if (t + 1 < cut.t1) st.store(a, lds, buffer ^ 1);
         __syncthreads();
     }
-    l = other_half(l, true);
+    const float m = w.m, l = other_half(w.l, true);
+    f32x16(&o)[S::kBlocks] = w.o;
     if (!there) return;
     const int64_t place = static_cast<int64_t>(seq.at + token) * a.q_heads + head * a.group + row % a.group;
     if (cut.pieces == 1) {
@@ -345,7 +386,10 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     const dim3 merge(static_cast<uint32_t>(p.row_tiles * (kGroupRows / kMergeRows) * c->kv_heads), b->seqs);
     auto run = [&](auto type, auto dim) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
-        k_attend_rows<T, D><<<grid, kThreads, 0, stream>>>(a);
+        if (c->page_tokens >= Shape<D>::kTokens)
+            k_attend_rows<T, D, true><<<grid, kThreads, 0, stream>>>(a);
+        else
+            k_attend_rows<T, D, false><<<grid, kThreads, 0, stream>>>(a);
         if (const int rc = launch_status()) return rc;
         if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeWaves * 64, 0, stream>>>(a);
         return launch_status();
