@@ -70,7 +70,7 @@ struct Rows {
     // V's blocks that are asked for together with K, the others are when K's registers are free: with all of them at once
     // a wavefront of 256 dimensions would not fit the 256 registers of two on a SIMD.
     static constexpr int kEarly = D == 256 ? kDims / 2 : kDims;
-    int kpage, vpage;  // the pages of the tile that is loaded next
+    int kentry, ventry;  // of the page table, for the tile that is loaded next
 
     // Tokens [base, base + 64) of the sequence: K's tokens of a lane's four products lie in the tile's 16-token group
     // (lane % 16) / 4, V's and the scores' in group lane / 16.
@@ -78,15 +78,13 @@ struct Rows {
     static __device__ __forceinline__ int vgroup() { return (threadIdx.x & 63) >> 4; }
 
     __device__ __forceinline__ void find(const AttendArgs& a, int b, int base) {
-        if constexpr (PAGE) {
-            kpage = vpage = __builtin_amdgcn_readfirstlane(a.s.page(b, a.c.column(base), a.c.pages));
-        } else {
-            kpage = a.s.page(b, a.c.column(base + 16 * kgroup()), a.c.pages);
-            vpage = a.s.page(b, a.c.column(base + 16 * vgroup()), a.c.pages);
-        }
+        kentry = a.s.entry(b, a.c.column(PAGE ? base : base + 16 * kgroup()));
+        ventry = PAGE ? kentry : a.s.entry(b, a.c.column(base + 16 * vgroup()));
     }
     __device__ __forceinline__ void load(const AttendArgs& a, Tile& x, int head, int base) const {
         const int P = a.c.page_tokens;
+        const int kpage = KvSeqs::page_of(PAGE ? __builtin_amdgcn_readfirstlane(kentry) : kentry, a.c.pages),
+                  vpage = PAGE ? kpage : KvSeqs::page_of(ventry, a.c.pages);
         const int64_t block = a.c.block(max(vpage, 0), head);
         const uint8_t *k, *v;
         if constexpr (PAGE) {  // one base for the wavefront, a lane's own offsets are the same for every tile

@@ -21,6 +21,7 @@ typedef float f32x16 __attribute__((ext_vector_type(16)));
 constexpr int kWaves = 8;
 constexpr int kThreads = kWaves * 64;
 constexpr int kGroupRows = kWaves * 32;
+constexpr int kRing = 4;  // tiles in LDS: two are multiplied between barriers, two are filled
 constexpr int kMaxPieces = 16;
 constexpr int kCus = 256;
 constexpr float kSlack = 8.0f;  // log2: how far a score may lie above the running maximum
@@ -28,9 +29,9 @@ constexpr float kSlack = 8.0f;  // log2: how far a score may lie above the runni
 struct RowsArgs : AttendArgs {
     float* partial;      // [pieces][tokens][q_heads][D]
     float2* partial_ml;  // [pieces][tokens][q_heads]: maximum (in log2) and sum
-    int32_t row_tiles;   // of 256 rows, at most
+    int32_t* each;       // tiles that a piece has at most, as the first kernel found it for the second
+    int32_t row_tiles;   // of 256 rows, in a sequence, at most
     int32_t pieces;      // a row tile's cache is cut into at most this many
-    int32_t tiles_each;  // .. of about this many tiles
 };
 
 // What a part of 16 tokens needs beside its bytes.
@@ -55,9 +56,9 @@ struct Shape {
 
 template <int D>
 struct Lds {
-    uint4 k[2][Shape<D>::kSubs * Shape<D>::kSteps][64];
-    uint4 v[2][Shape<D>::kBlocks * Shape<D>::kSubs * 2][64];
-    Part part[2][Shape<D>::kParts];
+    uint4 k[kRing][Shape<D>::kSubs * Shape<D>::kSteps][64];
+    uint4 v[kRing][Shape<D>::kBlocks * Shape<D>::kSubs * 2][64];
+    Part part[kRing][Shape<D>::kParts];
 };
 
 // One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V. PAGE: a page holds
@@ -68,7 +69,8 @@ struct Stage {
     using S = Shape<D>;
     uint4 k, v;
     float ks, vs;
-    int kpage, vpage, count;
+    int kentry, ventry;  // of the page table, for the tile that is loaded next
+    int count;
 
     // 16 lanes take 4 tokens by 64 values
     static __device__ __forceinline__ int k_token() { return (threadIdx.x >> 4) / (D / 64) * 4 + ((threadIdx.x >> 2) & 3); }
@@ -78,23 +80,24 @@ struct Stage {
 
     __device__ __forceinline__ void find(const AttendArgs& a, int b, int base) {
         if constexpr (PAGE) {
-            kpage = vpage = __builtin_amdgcn_readfirstlane(a.s.page(b, a.c.column(base), a.c.pages));
+            const int col = a.c.column(base);  // uniform, but read by a vector load: see lane_zero()
+            kentry = col < a.s.table_width ? static_cast<int>(ScalarBase(a.s.table + b * a.s.table_stride + col).load4(lane_zero())) : -1;
         } else {
-            kpage = a.s.page(b, a.c.column(base + k_token()), a.c.pages);
-            vpage = a.s.page(b, a.c.column(base + 16 * v_part()), a.c.pages);
+            kentry = a.s.entry(b, a.c.column(base + k_token()));
         }
+        ventry = PAGE ? kentry : a.s.entry(b, a.c.column(base + 16 * v_part()));
     }
     __device__ __forceinline__ void load(const AttendArgs& a, int head, int base, int length) {
         const int P = a.c.page_tokens;
+        const int kpage = KvSeqs::page_of(PAGE ? __builtin_amdgcn_readfirstlane(kentry) : kentry, a.c.pages),
+                  vpage = PAGE ? kpage : KvSeqs::page_of(ventry, a.c.pages);
         const int64_t kb = a.c.block(max(kpage, 0), head), vb = a.c.block(max(vpage, 0), head);
         if constexpr (PAGE) {
-            const uint8_t* kp = a.c.k + (kb * P + a.c.within(base)) * D;
-            const uint8_t* vp = a.c.v + vb * P * D + a.c.within(base);
-            k = *reinterpret_cast<const uint4*>(kp + static_cast<uint32_t>(k_token() * D + 16 * k_chunk()));
-            v = *reinterpret_cast<const uint4*>(vp + static_cast<uint32_t>(v_dim() * P + 16 * v_part()));
+            k = ScalarBase(a.c.k + (kb * P + a.c.within(base)) * D).load16(k_token() * D + 16 * k_chunk());
+            v = ScalarBase(a.c.v + vb * P * D + a.c.within(base)).load16(v_dim() * P + 16 * v_part());
             count = vpage < 0 ? 0 : length - base;  // of the tile
-            ks = a.c.k_scale[kb];
-            vs = a.c.v_scale[vb];
+            ks = ScalarBase(a.c.k_scale + kb).load_float(lane_zero());
+            vs = ScalarBase(a.c.v_scale + vb).load_float(lane_zero());
         } else {
             k = *reinterpret_cast<const uint4*>(a.c.k + (kb * P + a.c.within(base + k_token())) * D + 16 * k_chunk());
             v = *reinterpret_cast<const uint4*>(a.c.v + vb * P * D + v_dim() * P + a.c.within(base + 16 * v_part()));
@@ -152,7 +155,9 @@ struct Wave {
     // Operands come from LDS four products ahead, V's first ones before the softmax.
     __device__ __forceinline__ void add(const Lds<D>& lds, int buffer, int u, int seen) {
         constexpr int kAhead = D == 256 ? 2 : 4;  // no registers for more with 256 dimensions
-        const int lane = threadIdx.x & 63, half = lane >> 5;
+        int lane = threadIdx.x & 63;
+        __asm__ volatile("" : "+v"(lane));  // its slots are worked out for every tile: kept, they would cost five registers
+        const int half = lane >> 5;
         const uint4(*kt)[64] = &lds.k[buffer][u * S::kSteps];
         f32x16 s = (f32x16)(0.0f);
         uint4 f[kAhead];
@@ -209,30 +214,113 @@ struct Wave {
     }
 };
 
-// Which tiles of the cache a workgroup takes of its row tile; pieces == 0: none.
-struct Cut {
-    int t0, t1, pieces;
-};
-__device__ __forceinline__ Cut cut_of(const RowsArgs& a, Seq seq, int row0, int piece, int tile_tokens) {
-    if (row0 >= seq.n * a.group) return {0, 0, 0};
+// Tiles of the cache that rows [row0, row0 + 256) of a sequence see; at least one where there are rows, which have to be
+// written even if they see nothing.
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, Seq seq, int row0, int tile_tokens) {
+    if (row0 >= seq.n * a.group) return 0;
     const int last = min((row0 + kGroupRows - 1) / a.group, seq.n - 1);
     const int seen = a.causal ? min(seq.length, max(seq.length - seq.n + last + 1, 0)) : seq.length;
-    const int tiles = (seen + tile_tokens - 1) / tile_tokens;
-    const int pieces = max(min(a.pieces, (tiles + a.tiles_each - 1) / a.tiles_each), 1);
-    const int size = (tiles + pieces - 1) / pieces;
-    return {min(piece * size, tiles), min((piece + 1) * size, tiles), pieces};
+    return max((seen + tile_tokens - 1) / tile_tokens, 1);
 }
 
-// blockIdx.x: (row tile, latest tokens first as they see most of the cache; piece; kv head), blockIdx.y: sequence.
+// A row tile's tiles in pieces of at most `each`, as equal as can be, unless that were too many pieces.
+struct Cut {
+    int pieces, size;
+};
+__device__ __forceinline__ Cut cut_of(int tiles, int each, int most) {
+    const int pieces = min((tiles + each - 1) / each, most);
+    return {pieces, pieces ? (tiles + pieces - 1) / pieces : 0};
+}
+
+// What a workgroup takes: the pieces of all row tiles in order of their size, the largest first, one for each kv head. A
+// causal prompt's row tiles see from one to all of its tokens, and a call's sequences may differ as much: were they taken as
+// they come, the last large one would run on alone. Every workgroup ranks the pieces for itself, by 64 classes of size.
+struct Work {
+    int b, row0, piece, pieces, t0, t1;
+};
+constexpr int kClasses = 64;
+constexpr int kLeast = 4;  // tiles that are worth a piece
+struct PlanLds {
+    uint32_t classes[kClasses];
+    uint32_t sums[kWaves];
+    Work work;
+};
+
+template <int D>
+__device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work& work) {
+    constexpr int T = Shape<D>::kTokens;
+    const uint32_t wanted = blockIdx.x / a.c.kv_heads, items = a.s.seqs * a.row_tiles;
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    auto tiles_at = [&](uint32_t i) {
+        return i < items ? tiles_of(a, a.seq(i / a.row_tiles), static_cast<int>(i % a.row_tiles) * kGroupRows, T) : 0;
+    };
+    uint32_t total = 0;
+    for (uint32_t i = threadIdx.x; i < items; i += kThreads) total += tiles_at(i);
+    total = wave_sum(total);
+    if (lane == 0) lds.sums[wave] = total;
+    if (threadIdx.x < kClasses) lds.classes[threadIdx.x] = 0;
+    __syncthreads();
+    total = 0;
+    for (int i = 0; i < kWaves; i++) total += lds.sums[i];
+    const int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && a.pieces > 1) *a.each = each;
+    auto class_of = [&](Cut c) { return kClasses - 1 - min(static_cast<int>(c.size * (kClasses - 1ll) / each), kClasses - 1); };
+    for (uint32_t i = threadIdx.x; i < items; i += kThreads) {
+        const Cut c = cut_of(tiles_at(i), each, a.pieces);
+        if (c.pieces) atomicAdd(&lds.classes[class_of(c)], static_cast<uint32_t>(c.pieces));
+    }
+    __syncthreads();
+    const uint32_t own = lds.classes[lane], sum = wave_scan(own);
+    const uint64_t past = __ballot(sum > wanted);
+    if (!past) return false;
+    const int mine = __builtin_ctzll(past);
+    const uint32_t rank = wanted - __builtin_amdgcn_readlane(sum - own, mine);  // in its class, in the order of the row tiles
+    uint32_t before = 0;
+    for (uint32_t i0 = 0; i0 < items; i0 += kThreads) {
+        const uint32_t i = i0 + threadIdx.x;
+        const int tiles = tiles_at(i);
+        const Cut c = cut_of(tiles, each, a.pieces);
+        const uint32_t n = c.pieces && class_of(c) == mine ? c.pieces : 0, upto = wave_scan(n);
+        __syncthreads();  // the sums before have been read
+        if (lane == 63) lds.sums[wave] = upto;
+        __syncthreads();
+        uint32_t at = before + upto - n;
+        for (int j = 0; j < kWaves; j++) {
+            if (j < wave) at += lds.sums[j];
+            before += lds.sums[j];
+        }
+        if (at <= rank && rank < at + n) {
+            const int piece = rank - at;
+            lds.work = {static_cast<int>(i / a.row_tiles), static_cast<int>(i % a.row_tiles) * kGroupRows, piece, c.pieces,
+                        min(piece * c.size, tiles), min((piece + 1) * c.size, tiles)};
+        }
+        if (before > rank) break;
+    }
+    __syncthreads();
+    work = lds.work;
+    work.b = __builtin_amdgcn_readfirstlane(work.b);
+    work.row0 = __builtin_amdgcn_readfirstlane(work.row0);
+    work.piece = __builtin_amdgcn_readfirstlane(work.piece);
+    work.pieces = __builtin_amdgcn_readfirstlane(work.pieces);
+    work.t0 = __builtin_amdgcn_readfirstlane(work.t0);
+    work.t1 = __builtin_amdgcn_readfirstlane(work.t1);
+    return true;
+}
+
+// blockIdx: (rank of the piece, kv head).
 template <int TYPE, int D, bool PAGE>
 __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     using S = Shape<D>;
-    __shared__ Lds<D> lds;
-    const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, rest = blockIdx.x / a.c.kv_heads;
-    const int piece = rest % a.pieces, row0 = (a.row_tiles - 1 - rest / a.pieces) * kGroupRows;
+    __shared__ union {
+        Lds<D> lds;
+        PlanLds plan;
+    } shared;
+    Lds<D>& lds = shared.lds;
+    Work cut;
+    if (!find_work<D>(a, shared.plan, cut)) return;
+    __syncthreads();  // the plan has been read
+    const int b = cut.b, row0 = cut.row0, piece = cut.piece, head = blockIdx.x % a.c.kv_heads;
     const Seq seq = a.seq_uniform(b);
-    const Cut cut = cut_of(a, seq, row0, piece, S::kTokens);
-    if (piece >= cut.pieces) return;
 
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
     const int row = row0 + 32 * wave + (lane & 31), token = row / a.group;
@@ -262,26 +350,36 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     const bool idle = !__any(there);
 
     st.store(a, lds, 0);
-    st.find(a, b, (cut.t0 + 1) * S::kTokens);
+    if (cut.t0 + 1 < cut.t1) {
+        st.find(a, b, (cut.t0 + 1) * S::kTokens);
+        st.load(a, head, (cut.t0 + 1) * S::kTokens, seq.length);
+        st.store(a, lds, 1);
+    }
+    // q is here before the loop: were it still on its way, the first product of every round would wait for that round's loads
+    __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+    st.find(a, b, (cut.t0 + 2) * S::kTokens);
     __syncthreads();
     for (int t = cut.t0; t < cut.t1; t++) {
-        const int buffer = (t - cut.t0) & 1, base = t * S::kTokens;
-        if (t + 1 < cut.t1) {
-            st.load(a, head, base + S::kTokens, seq.length);
-            st.find(a, b, base + 2 * S::kTokens);
+        const int buffer = (t - cut.t0) & (kRing - 1), base = t * S::kTokens;
+        if (t + 2 < cut.t1) {
+            st.load(a, head, base + 2 * S::kTokens, seq.length);
+            st.find(a, b, base + 3 * S::kTokens);
         }
 #pragma unroll
         for (int u = 0; u < S::kSubs; u++) {
             if (idle || base + 32 * u >= most) break;
             w.add(lds, buffer, u, limit - base - 32 * u - 16 * half);
         }
-        if (t + 1 < cut.t1) st.store(a, lds, buffer ^ 1);
-        __syncthreads();
+        if (t + 2 < cut.t1) st.store(a, lds, (buffer + 2) & (kRing - 1));
+        if (buffer & 1) __syncthreads();
     }
     const float m = w.m, l = other_half(w.l, true);
     f32x16(&o)[S::kBlocks] = w.o;
-    if (!there) return;
-    const int64_t place = static_cast<int64_t>(seq.at + token) * a.q_heads + head * a.group + row % a.group;
+    // worked out again: the loop has no register to keep them in
+    const int out_row = row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero());
+    const int out_token = out_row / a.group;
+    if (out_token >= seq.n) return;
+    const int64_t place = static_cast<int64_t>(seq.at + out_token) * a.q_heads + head * a.group + out_row % a.group;
     if (cut.pieces == 1) {
         const float inv = l == 0.0f ? 0.0f : 1.0f / l;
         uint16_t* out = a.out + place * D + 4 * half;
@@ -305,50 +403,56 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     if (half == 0) a.partial_ml[slot] = make_float2(m, l);
 }
 
-// Adds up the pieces of the row tiles that were cut: a wavefront a row, 32 rows a workgroup. blockIdx as above, with 32 rows
-// for a row tile's 256 and no pieces.
-constexpr int kMergeWaves = 4, kMergeRows = 32;
+// Adds up the pieces of the row tiles that were cut: a wavefront a row. blockIdx: (four rows, kv head), sequence.
+constexpr int kMergeRows = 4;
 template <int D>
-__global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge(RowsArgs a) {
-    const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, first = blockIdx.x / a.c.kv_heads * kMergeRows;
+__global__ __launch_bounds__(kMergeRows * 64) void k_attend_merge(RowsArgs a) {
+    const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, lane = threadIdx.x & 63;
+    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x / a.c.kv_heads * kMergeRows + (threadIdx.x >> 6));
     const Seq seq = a.seq_uniform(b);
-    const Cut cut = cut_of(a, seq, first / kGroupRows * kGroupRows, 0, Shape<D>::kTokens);
-    if (cut.pieces < 2) return;
+    if (row >= seq.n * a.group) return;
+    const int pieces = cut_of(tiles_of(a, seq, row / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
+    if (pieces < 2) return;
     constexpr int V = D / 64;
     typedef float Lane __attribute__((ext_vector_type(V)));
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int64_t piece = static_cast<int64_t>(a.s.tokens) * a.q_heads;
-    for (int row = first + wave; row < first + kMergeRows && row < seq.n * a.group; row += kMergeWaves) {
-        const int64_t place = static_cast<int64_t>(seq.at + row / a.group) * a.q_heads + head * a.group + row % a.group;
-        float2 ml[kMaxPieces];
-        float top = -__builtin_inff();
+    const int64_t stride = static_cast<int64_t>(a.s.tokens) * a.q_heads;
+    const int64_t place = static_cast<int64_t>(seq.at + row / a.group) * a.q_heads + head * a.group + row % a.group;
+    const float2 ml = lane < pieces ? a.partial_ml[lane * stride + place] : make_float2(-__builtin_inff(), 0.0f);
+    float top = ml.x;
 #pragma unroll
-        for (int i = 0; i < kMaxPieces; i++)
-            if (i < cut.pieces) {
-                ml[i] = a.partial_ml[i * piece + place];
-                top = fmaxf(top, ml[i].x);
-            }
-        const float safe = top == -__builtin_inff() ? 0.0f : top;
-        Lane sum = {};
-        float l = 0.0f;
+    for (int d = kMaxPieces / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float safe = top == -__builtin_inff() ? 0.0f : top, own = exp2_fast(ml.x - safe);
+    Lane sum = {};
+    float l = 0.0f;
+    for (int i = 0; i < pieces; i += 4) {
+        Lane x[4];
 #pragma unroll
-        for (int i = 0; i < kMaxPieces; i++)
-            if (i < cut.pieces) {
-                const float f = exp2_fast(ml[i].x - safe);
-                l += ml[i].y * f;
-                sum += *reinterpret_cast<const Lane*>(a.partial + (i * piece + place) * D + lane * V) * f;
-            }
-        const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-        uint16_t* out = a.out + place * D + lane * V;
+        for (int e = 0; e < 4; e++)
+            x[e] = *reinterpret_cast<const Lane*>(a.partial + (min(i + e, pieces - 1) * stride + place) * D + lane * V);
 #pragma unroll
-        for (int e = 0; e < V; e++) out[e] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(sum[e] * inv));
+        for (int e = 0; e < 4; e++) {
+            if (i + e >= pieces) break;
+            const float f = __shfl(own, i + e);
+            l += __shfl(ml.y, i + e) * f;
+            sum += x[e] * f;
+        }
+    }
+    const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+    uint16_t* out = a.out + place * D + lane * V;
+    if constexpr (V == 4) {
+        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
+    } else if constexpr (V == 2) {
+        *reinterpret_cast<uint32_t*>(out) = pack_bf16(sum[0] * inv, sum[1] * inv);
+    } else {
+        *out = __builtin_bit_cast(uint16_t, static_cast<__bf16>(sum[0] * inv));
     }
 }
 
-// How the row tiles' caches are cut. Calls of few row tiles would leave CUs idle, and in a causal one the last row tiles
-// would run on alone: every row tile's cache is cut into pieces of a CU's share of the whole, where that is less.
+// How the row tiles' caches are cut. Calls of few row tiles would leave CUs idle, and a causal prompt's last row tiles would
+// run on alone: a cache is cut into pieces of a CU's share of the whole where that is less. From twice as many row tiles as
+// CUs on, taking the large ones first is enough, and nothing is cut.
 struct RowsPlan {
-    int64_t row_tiles, pieces, tiles_each;
+    int64_t row_tiles, pieces, groups;
 };
 RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
     const int64_t tokens = 8192 / c->head_dim, group = q_heads / c->kv_heads;
@@ -356,9 +460,12 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t row_tiles = (b->max_count * group + kGroupRows - 1) / kGroupRows;
     const int64_t items = row_tiles * c->kv_heads * b->seqs;
     const int64_t most = (longest + tokens - 1) / tokens;  // tiles of the last row tile
+    if (items >= 2 * kCus) return {row_tiles, 1, items};
     const int64_t mean = std::max<int64_t>(1, (longest - std::min<int64_t>(b->max_count, longest) / 2 + tokens - 1) / tokens);
-    const int64_t each = std::max<int64_t>(4, (items * mean + kCus - 1) / kCus);
-    return {row_tiles, std::min<int64_t>(kMaxPieces, (most + each - 1) / each), each};
+    const int64_t each = std::max<int64_t>(kLeast, (items * mean + kCus - 1) / kCus);
+    const int64_t pieces = std::min<int64_t>(kMaxPieces, (most + each - 1) / each);
+    // the pieces of n tiles are less than n / each + 1, those of all (row tile, kv head)s less than kCus + items
+    return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus)};
 }
 
 }  // namespace
@@ -366,7 +473,7 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
 size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
     const RowsPlan p = rows_plan(c, q_heads, b, max_length);
     if (p.pieces == 1) return 0;
-    return static_cast<size_t>(p.pieces * b->tokens * q_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
+    return 16 + static_cast<size_t>(p.pieces * b->tokens * q_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
 }
 
 int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBatch* b, int64_t max_length, void* workspace,
@@ -374,16 +481,15 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     const RowsPlan p = rows_plan(c, call.q_heads, b, max_length);
     RowsArgs a;
     static_cast<AttendArgs&>(a) = call;
-    a.partial = static_cast<float*>(workspace);
+    a.each = static_cast<int32_t*>(workspace);
+    a.partial = static_cast<float*>(workspace) + 4;
     a.partial_ml = reinterpret_cast<float2*>(a.partial + p.pieces * b->tokens * call.q_heads * c->head_dim);
     a.row_tiles = static_cast<int32_t>(p.row_tiles);
     a.pieces = static_cast<int32_t>(p.pieces);
-    a.tiles_each = static_cast<int32_t>(p.tiles_each);
-    const int64_t blocks = p.row_tiles * p.pieces * c->kv_heads;
-    if (blocks >= (int64_t{1} << 31) || p.row_tiles * (kGroupRows / kMergeRows) * c->kv_heads >= (int64_t{1} << 31))
-        return WL_EINVAL_SHAPE;
-    const dim3 grid(static_cast<uint32_t>(blocks), b->seqs);
-    const dim3 merge(static_cast<uint32_t>(p.row_tiles * (kGroupRows / kMergeRows) * c->kv_heads), b->seqs);
+    const int64_t merges = (b->max_count * static_cast<int64_t>(call.group) + kMergeRows - 1) / kMergeRows * c->kv_heads;
+    if (p.groups >= (int64_t{1} << 31) || merges >= (int64_t{1} << 31)) return WL_EINVAL_SHAPE;
+    const dim3 grid(static_cast<uint32_t>(p.groups));
+    const dim3 merge(static_cast<uint32_t>(merges), b->seqs);
     auto run = [&](auto type, auto dim) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
         if (c->page_tokens >= Shape<D>::kTokens)
@@ -391,7 +497,7 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
         else
             k_attend_rows<T, D, false><<<grid, kThreads, 0, stream>>>(a);
         if (const int rc = launch_status()) return rc;
-        if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeWaves * 64, 0, stream>>>(a);
+        if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeRows * 64, 0, stream>>>(a);
         return launch_status();
     };
     auto with_dim = [&](auto type) {

@@ -33,6 +33,34 @@ inline int check_batch(const WlKvBatch* b) {
     return WL_OK;
 }
 
+// 0 that the compiler takes for a lane's own: an address with it is read by a vector load. A scalar load shares its counter
+// with LDS reads and comes back out of order, so the next LDS operand would wait for it to come from memory.
+__device__ __forceinline__ uint32_t lane_zero() {
+    uint32_t z = 0;
+    __asm__("" : "+v"(z));
+    return z;
+}
+
+// Loads at a pointer that all lanes share plus a lane's 32-bit offset in bytes: the pointer is kept in scalar registers, a
+// lane holds the offset alone.
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+struct ScalarBase {
+    const __attribute__((address_space(1))) uint8_t* p;
+
+    __device__ __forceinline__ explicit ScalarBase(const void* at) {
+        uint64_t u = reinterpret_cast<uint64_t>(at);
+        __asm__("" : "+s"(u));
+        p = (const __attribute__((address_space(1))) uint8_t*)u;
+    }
+    __device__ __forceinline__ uint4 load16(uint32_t offset) const {
+        return __builtin_bit_cast(uint4, *(const __attribute__((address_space(1))) u32x4*)(p + offset));
+    }
+    __device__ __forceinline__ uint32_t load4(uint32_t offset) const {
+        return *(const __attribute__((address_space(1))) uint32_t*)(p + offset);
+    }
+    __device__ __forceinline__ float load_float(uint32_t offset) const { return __builtin_bit_cast(float, load4(offset)); }
+};
+
 // One layer of the cache, as the kernels see it.
 struct KvLayer {
     uint8_t* k;
@@ -77,12 +105,15 @@ struct KvSeqs {
     __device__ __forceinline__ int count(int b, int at) const {
         return min(max(cu[b + 1], at) - at, min(tokens - at, max_count));
     }
-    // The page that holds column `col` of sequence b, or -1.
-    __device__ __forceinline__ int page(int b, int col, int pages) const {
-        if (static_cast<uint32_t>(col) >= static_cast<uint32_t>(table_width)) return -1;
-        const int p = table[b * table_stride + col];
-        return static_cast<uint32_t>(p) < static_cast<uint32_t>(pages) ? p : -1;
+    // The table's entry for column `col` of sequence b, as it stands there (-1 behind the table's end); and the page that an
+    // entry names, or -1. Apart, so that a kernel can ask for an entry long before it uses it.
+    __device__ __forceinline__ int entry(int b, int col) const {
+        return static_cast<uint32_t>(col) < static_cast<uint32_t>(table_width) ? table[b * table_stride + col] : -1;
     }
+    static __device__ __forceinline__ int page_of(int entry, int pages) {
+        return static_cast<uint32_t>(entry) < static_cast<uint32_t>(pages) ? entry : -1;
+    }
+    __device__ __forceinline__ int page(int b, int col, int pages) const { return page_of(entry(b, col), pages); }
 };
 
 inline KvSeqs seqs_of(const WlKvBatch* b) {

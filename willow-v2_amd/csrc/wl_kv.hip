@@ -7,8 +7,6 @@
 namespace wl {
 namespace {
 
-typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
-
 constexpr int kAppendThreads = 256;
 
 template <int TYPE>
