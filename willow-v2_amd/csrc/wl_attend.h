@@ -119,8 +119,6 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return __builtin_amdg
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// All bits of the bytes whose index is below n
-__device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
 
 // Calls of more rows than the few-row form takes (wl_attend_rows.hip).
 size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);

@@ -33,6 +33,9 @@ inline int check_batch(const WlKvBatch* b) {
     return WL_OK;
 }
 
+// All bits of the bytes whose index is below n
+__device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <= 0 ? 0u : (1u << (8 * n)) - 1u; }
+
 // 0 that the compiler takes for a lane's own: an address with it is read by a vector load. A scalar load shares its counter
 // with LDS reads and comes back out of order, so the next LDS operand would wait for it to come from memory.
 __device__ __forceinline__ uint32_t lane_zero() {

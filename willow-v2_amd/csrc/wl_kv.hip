@@ -55,12 +55,38 @@ __device__ __forceinline__ float block_scale(float top, bool held, float old, in
     return ldexpf(old, n);
 }
 
+// x / s of bf16 values as a byte, rounded to nearest even, for a scale that block_scale gave.
+// The quotient is taken as x times 1 / s and then cut to 18 significant bits: with 8 significant bits each, x / s is a tie
+// between two bytes exactly, or at least 2^-16 (relative) away from one, and the product is off by less than 2^-22, so the
+// cut brings every tie back to itself and moves nothing else across one. A scale whose reciprocal leaves fp32 is divided by.
+template <int TYPE>
+struct Quantizer {
+    float scale, inverse;
+    bool dead, tiny;  // nothing but zeros, or a NaN scale: every byte is 0
+
+    __device__ __forceinline__ explicit Quantizer(float s)
+        : scale(s), inverse(1.0f / s), dead(!(s > 0.0f)), tiny(s < 1.0e-30f) {}
+    __device__ __forceinline__ uint32_t operator()(uint32_t bits) const {
+        const float x = bf16_to_float(bits);
+        const uint32_t y = __builtin_bit_cast(uint32_t, x * inverse);
+        float q = __builtin_bit_cast(float, (y + 0x20u) & ~0x3Fu);
+        if (tiny) q = x / scale;
+        return dead ? 0u : to_byte<TYPE>(q);
+    }
+    // a pair of bf16 in one word -> two bytes
+    __device__ __forceinline__ uint32_t pair(uint32_t two) const { return (*this)(two & 0xFFFFu) | (*this)(two >> 16) << 8; }
+};
+
+__device__ __forceinline__ uint32_t top_of(uint32_t two, uint32_t top) {
+    return max(top, max(two & 0x7FFFu, (two >> 16) & 0x7FFFu));
+}
+
 // One workgroup writes one block: a page of a sequence, one kv head, K or V (blockIdx.y's low bit), so the block's scale
-// and its older bytes have one writer. Two passes over the block's new rows: their largest magnitude, then the bytes; the
-// second finds them in the caches. K's bytes lie as the rows do, 16 values of a token to a thread. V's lie with the
-// tokens innermost: a thread takes two neighbouring values of 16 tokens, its loads run along the rows over the lanes, and
-// it writes 16 bytes for each value; where those 16 tokens are not all new, the bytes there are read first.
-// Bound by its reads and writes for prompts (6 bytes a value), by the launch and one round trip for single tokens.
+// and its older bytes have one writer. Two passes over the block's new rows: their largest magnitude, then the bytes; a
+// thread keeps what it read in the first one (all of it, up to 16384 new values). K's bytes lie as the rows do, 16 values of
+// a token to a thread. V's lie with the tokens innermost: a thread takes two neighbouring values of 16 tokens, its loads run
+// along the rows over the lanes, and it writes 16 bytes for each value; where those 16 tokens are not all new, the bytes
+// there are read first. Bound by latency: a prompt has one such workgroup for each CU or two, a step's single tokens less.
 template <int TYPE, int D, bool WIDE>
 __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs s, const int32_t* __restrict__ start,
                                                               const uint16_t* __restrict__ kx, int64_t k_ts, int64_t k_hs,
@@ -80,99 +106,157 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
     const int stop = static_cast<int>(min(end - page0, static_cast<int64_t>(P)));  // tokens [held, stop) are new
     const int64_t ts = is_v ? v_ts : k_ts;
     // row of token t (in the page): at + (page0 + t - from)
-    const uint16_t* __restrict__ x =
-        (is_v ? vx + head * v_hs : kx + head * k_hs) + (at + (page0 - from)) * ts;
+    const uint16_t* __restrict__ x = (is_v ? vx + head * v_hs : kx + head * k_hs) + (at + (page0 - from)) * ts;
     const int64_t block = c.block(page, head);
     uint8_t* __restrict__ out = (is_v ? c.v : c.k) + block * P * D;
     float* scale = (is_v ? c.v_scale : c.k_scale) + block;
+    const float old = *scale;
+
+    // K: unit i is 16 values of token held + i / (D / 16). V: unit i is two values of the 16 tokens from 16 (i / (D / 2)).
+    const int k_units = (stop - held) * (D / 16), g_new = held / 16, g_end = (stop + 15) / 16,
+              v_units = (g_end - g_new) * (D / 2);
+    auto read_k = [&](int i, uint32_t (&w)[8]) {
+        const uint16_t* row = x + (held + i / (D / 16)) * ts + i % (D / 16) * 16;
+        if constexpr (WIDE) {
+            const uint4 lo = *reinterpret_cast<const uint4*>(row), hi = *reinterpret_cast<const uint4*>(row + 8);
+            w[0] = lo.x, w[1] = lo.y, w[2] = lo.z, w[3] = lo.w, w[4] = hi.x, w[5] = hi.y, w[6] = hi.z, w[7] = hi.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = row[2 * j] | static_cast<uint32_t>(row[2 * j + 1]) << 16;
+        }
+    };
+    auto read_v = [&](int i, uint32_t (&w)[16]) {
+        const int t0 = (g_new + i / (D / 2)) * 16, d = i % (D / 2) * 2;
+#pragma unroll
+        for (int j = 0; j < 16; j++) {
+            const int t = t0 + j;
+            w[j] = 0;
+            if (t < held || t >= stop) continue;
+            const uint16_t* e = x + t * ts + d;
+            if constexpr (WIDE)
+                w[j] = *reinterpret_cast<const uint32_t*>(e);
+            else
+                w[j] = e[0] | static_cast<uint32_t>(e[1]) << 16;
+        }
+    };
 
     // the largest magnitude, as bits (bf16 magnitudes order as their bits do; infinities and NaN come out largest)
-    uint32_t top = 0;
-    if constexpr (WIDE) {
-        for (int i = threadIdx.x; i < (stop - held) * (D / 8); i += kAppendThreads) {
-            const uint4 w = *reinterpret_cast<const uint4*>(x + (held + i / (D / 8)) * ts + i % (D / 8) * 8);
-            for (uint32_t u : {w.x, w.y, w.z, w.w}) top = max(top, max(u & 0x7FFFu, (u >> 16) & 0x7FFFu));
+    constexpr int kKeepK = 4, kKeepV = 2;
+    uint32_t top = 0, kept[32];
+    uint32_t(&kk)[kKeepK][8] = reinterpret_cast<uint32_t(&)[kKeepK][8]>(kept);
+    uint32_t(&vv)[kKeepV][16] = reinterpret_cast<uint32_t(&)[kKeepV][16]>(kept);
+    if (!is_v) {
+#pragma unroll
+        for (int r = 0; r < kKeepK; r++) {
+            const int i = threadIdx.x + r * kAppendThreads;
+            if (i < k_units) read_k(i, kk[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kKeepK; r++)
+            if (static_cast<int>(threadIdx.x) + r * kAppendThreads < k_units)
+#pragma unroll
+                for (int j = 0; j < 8; j++) top = top_of(kk[r][j], top);
+        for (int i = threadIdx.x + kKeepK * kAppendThreads; i < k_units; i += kAppendThreads) {
+            uint32_t w[8];
+            read_k(i, w);
+#pragma unroll
+            for (int j = 0; j < 8; j++) top = top_of(w[j], top);
         }
     } else {
-        for (int i = threadIdx.x; i < (stop - held) * D; i += kAppendThreads)
-            top = max(top, x[(held + i / D) * ts + i % D] & 0x7FFFu);
+#pragma unroll
+        for (int r = 0; r < kKeepV; r++) {
+            const int i = threadIdx.x + r * kAppendThreads;
+            if (i < v_units) read_v(i, vv[r]);
+        }
+#pragma unroll
+        for (int r = 0; r < kKeepV; r++)
+            if (static_cast<int>(threadIdx.x) + r * kAppendThreads < v_units)
+#pragma unroll
+                for (int j = 0; j < 16; j++) top = top_of(vv[r][j], top);
+        for (int i = threadIdx.x + kKeepV * kAppendThreads; i < v_units; i += kAppendThreads) {
+            uint32_t w[16];
+            read_v(i, w);
+#pragma unroll
+            for (int j = 0; j < 16; j++) top = top_of(w[j], top);
+        }
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) top = max(top, __shfl_xor(top, d));
     if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
-    const float old = *scale;
     __syncthreads();
     top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
 
     int shrink = 0;
-    float now = top < 0x7F80u ? block_scale<TYPE>(bf16_to_float(top), held > 0, old, shrink)
-                              : __builtin_nanf("");
-    const bool dead = !(now > 0.0f);  // nothing but zeros, or a NaN scale: the bytes are 0
-    const float per = dead ? 1.0f : now;
-    auto quantize = [&](uint32_t bits) { return dead ? 0u : to_byte<TYPE>(bf16_to_float(bits) / per); };
+    const float now =
+        top < 0x7F80u ? block_scale<TYPE>(bf16_to_float(top), held > 0, old, shrink) : __builtin_nanf("");
+    const Quantizer<TYPE> quantize(now);
     auto older = [&](uint32_t byte) { return to_byte<TYPE>(ldexpf(from_byte<TYPE>(byte), -shrink)); };
+    auto older4 = [&](uint32_t w) {
+        return older(w & 0xFFu) | older(w >> 8 & 0xFFu) << 8 | older(w >> 16 & 0xFFu) << 16 | older(w >> 24) << 24;
+    };
     if (threadIdx.x == 0) *scale = now;
 
     if (!is_v) {
-        for (int i = threadIdx.x; i < (stop - held) * (D / 16); i += kAppendThreads) {
-            const int t = held + i / (D / 16), d = i % (D / 16) * 16;
-            const uint16_t* row = x + t * ts + d;
-            uint32_t in[8], w[4];
-            if constexpr (WIDE) {
-                const uint4 lo = *reinterpret_cast<const uint4*>(row), hi = *reinterpret_cast<const uint4*>(row + 8);
-                in[0] = lo.x, in[1] = lo.y, in[2] = lo.z, in[3] = lo.w;
-                in[4] = hi.x, in[5] = hi.y, in[6] = hi.z, in[7] = hi.w;
-            } else {
-                for (int j = 0; j < 8; j++) in[j] = row[2 * j] | static_cast<uint32_t>(row[2 * j + 1]) << 16;
-            }
+        auto write_k = [&](int i, const uint32_t (&w)[8]) {
+            uint32_t y[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                w[j] = quantize(in[2 * j] & 0xFFFFu) | quantize(in[2 * j] >> 16) << 8 |
-                       quantize(in[2 * j + 1] & 0xFFFFu) << 16 | quantize(in[2 * j + 1] >> 16) << 24;
-            *reinterpret_cast<uint4*>(out + t * D + d) = make_uint4(w[0], w[1], w[2], w[3]);
+            for (int j = 0; j < 4; j++) y[j] = quantize.pair(w[2 * j]) | quantize.pair(w[2 * j + 1]) << 16;
+            *reinterpret_cast<uint4*>(out + (held + i / (D / 16)) * D + i % (D / 16) * 16) = make_uint4(y[0], y[1], y[2], y[3]);
+        };
+#pragma unroll
+        for (int r = 0; r < kKeepK; r++) {
+            const int i = threadIdx.x + r * kAppendThreads;
+            if (i < k_units) write_k(i, kk[r]);
+        }
+        for (int i = threadIdx.x + kKeepK * kAppendThreads; i < k_units; i += kAppendThreads) {
+            uint32_t w[8];
+            read_k(i, w);
+            write_k(i, w);
         }
         if (shrink)
-            for (int i = threadIdx.x; i < held * (D / 4); i += kAppendThreads) {
-                const uint32_t w = reinterpret_cast<uint32_t*>(out)[i];
-                reinterpret_cast<uint32_t*>(out)[i] = older(w & 0xFFu) | older(w >> 8 & 0xFFu) << 8 |
-                                                      older(w >> 16 & 0xFFu) << 16 | older(w >> 24) << 24;
-            }
+            for (int i = threadIdx.x; i < held * (D / 4); i += kAppendThreads)
+                reinterpret_cast<uint32_t*>(out)[i] = older4(reinterpret_cast<uint32_t*>(out)[i]);
         return;
     }
-    const int g0 = shrink ? 0 : held / 16, g1 = (stop + 15) / 16;  // the groups of 16 tokens that change
-    for (int i = threadIdx.x; i < (g1 - g0) * (D / 2); i += kAppendThreads) {
-        const int t0 = (g0 + i / (D / 2)) * 16, d = i % (D / 2) * 2;
-        uint32_t w[2][4] = {};
-        uint4* to[2] = {reinterpret_cast<uint4*>(out + d * P + t0), reinterpret_cast<uint4*>(out + (d + 1) * P + t0)};
-        if (t0 < held || t0 + 16 > stop) {
+    auto write_v = [&](int i, const uint32_t (&w)[16]) {
+        const int t0 = (g_new + i / (D / 2)) * 16, d = i % (D / 2) * 2;
+        const bool mixed = t0 < held || t0 + 16 > stop;
 #pragma unroll
-            for (int e = 0; e < 2; e++) {
-                const uint4 was = *to[e];
-                w[e][0] = was.x, w[e][1] = was.y, w[e][2] = was.z, w[e][3] = was.w;
+        for (int e = 0; e < 2; e++) {
+            uint4* to = reinterpret_cast<uint4*>(out + (d + e) * P + t0);
+            uint32_t y[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                y[j] = quantize(w[4 * j] >> (16 * e) & 0xFFFFu) | quantize(w[4 * j + 1] >> (16 * e) & 0xFFFFu) << 8 |
+                       quantize(w[4 * j + 2] >> (16 * e) & 0xFFFFu) << 16 | quantize(w[4 * j + 3] >> (16 * e) & 0xFFFFu) << 24;
+            if (mixed) {
+                const uint4 was = *to;
+                const uint32_t o[4] = {was.x, was.y, was.z, was.w};
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    // bytes of this word below `held` are older, those from `stop` on nobody's
+                    const uint32_t low = byte_mask(held - t0 - 4 * j), high = ~byte_mask(stop - t0 - 4 * j);
+                    y[j] = ((shrink ? older4(o[j]) : o[j]) & low) | (o[j] & high) | (y[j] & ~(low | high));
+                }
             }
+            *to = make_uint4(y[0], y[1], y[2], y[3]);
         }
+    };
 #pragma unroll
-        for (int j = 0; j < 16; j++) {
-            const int t = t0 + j;
-            const uint32_t sh = 8 * (j % 4);
-            if (t >= stop) continue;
-            if (t >= held) {
-                uint32_t two;
-                if constexpr (WIDE)
-                    two = *reinterpret_cast<const uint32_t*>(x + t * ts + d);
-                else
-                    two = x[t * ts + d] | static_cast<uint32_t>(x[t * ts + d + 1]) << 16;
-                w[0][j / 4] = (w[0][j / 4] & ~(0xFFu << sh)) | quantize(two & 0xFFFFu) << sh;
-                w[1][j / 4] = (w[1][j / 4] & ~(0xFFu << sh)) | quantize(two >> 16) << sh;
-            } else if (shrink) {
-#pragma unroll
-                for (int e = 0; e < 2; e++)
-                    w[e][j / 4] = (w[e][j / 4] & ~(0xFFu << sh)) | older(w[e][j / 4] >> sh & 0xFFu) << sh;
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; e++) *to[e] = make_uint4(w[e][0], w[e][1], w[e][2], w[e][3]);
+    for (int r = 0; r < kKeepV; r++) {
+        const int i = threadIdx.x + r * kAppendThreads;
+        if (i < v_units) write_v(i, vv[r]);
     }
+    for (int i = threadIdx.x + kKeepV * kAppendThreads; i < v_units; i += kAppendThreads) {
+        uint32_t w[16];
+        read_v(i, w);
+        write_v(i, w);
+    }
+    if (shrink)  // the groups of 16 tokens before the first that changes
+        for (int i = threadIdx.x; i < D * g_new * 4; i += kAppendThreads) {
+            uint32_t* w = reinterpret_cast<uint32_t*>(out + i / (4 * g_new) * P) + i % (4 * g_new);
+            *w = older4(*w);
+        }
 }
 
 template <int TYPE, int D>
@@ -185,7 +269,7 @@ void launch_append(bool wide, dim3 grid, hipStream_t stream, const KvLayer& c, c
 }
 
 // Page copies: the pairs of one launch travel in its arguments, so nothing is uploaded and a graph keeps them.
-constexpr int kCopyPairs = 256;
+constexpr int kCopyPairs = 480;  // 3840 of the 4096 bytes that arguments may take
 constexpr int kCopyThreads = 256;
 constexpr int kCopyChunk = kCopyThreads * 16 * 4;  // bytes of one workgroup: four 16-byte loads a thread in flight
 

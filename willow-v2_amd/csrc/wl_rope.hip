@@ -63,48 +63,48 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
         turn[i] = make_float2(a.scale * c, a.scale * s);
     }
     __syncthreads();
-    // a head: half / VEC pairs of runs, then what is not rotated
-    const int pairs = a.half / VEC, rest = (a.head_dim - 2 * a.half) / VEC, per = pairs + rest;
-    const int heads = a.q.heads + a.k.heads;
-    for (int i = threadIdx.x; i < n * heads * per; i += kRopeThreads) {
-        const int u = i % per, th = i / per, t = th / heads, hh = th % heads;
+    // a head: half / VEC pairs of runs, then what is not rotated; 32 lanes a head
+    struct alignas(sizeof(T) * VEC) Run {
+        T v[VEC];
+    };
+    const int pairs = a.half / VEC, rest = (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
+#pragma unroll 4
+    for (int i = threadIdx.x / 32; i < n * heads; i += kRopeThreads / 32) {
+        const int t = TOKENS == 1 ? 0 : i / heads, hh = TOKENS == 1 ? i : i % heads;
         const bool is_k = hh >= a.q.heads;
         const WlRopeTensor& x = is_k ? a.k : a.q;
         const int h = is_k ? hh - a.q.heads : hh;
         const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token_stride + h * x.in_head_stride;
         T* out = static_cast<T*>(x.out) + (t0 + t) * x.out_token_stride + h * x.out_head_stride;
-        struct alignas(sizeof(T) * VEC) Run {
-            T v[VEC];
-        };
-        if (u >= pairs) {
-            const int d = 2 * a.half + (u - pairs) * VEC;
-            if (in != out) *reinterpret_cast<Run*>(out + d) = *reinterpret_cast<const Run*>(in + d);
-            continue;
-        }
-        const int j = u * VEC;
-        Run lo = *reinterpret_cast<const Run*>(in + j), hi = *reinterpret_cast<const Run*>(in + a.half + j);
+        for (int u = threadIdx.x % 32; u < pairs + rest; u += 32) {
+            if (u >= pairs) {
+                const int d = 2 * a.half + (u - pairs) * VEC;
+                if (in != out) *reinterpret_cast<Run*>(out + d) = *reinterpret_cast<const Run*>(in + d);
+                continue;
+            }
+            const int j = u * VEC;
+            Run lo = *reinterpret_cast<const Run*>(in + j), hi = *reinterpret_cast<const Run*>(in + a.half + j);
 #pragma unroll
-        for (int e = 0; e < VEC; e++) {
-            const float2 cs = turn[t * a.half + j + e];
-            const float p = load_value(lo.v + e), q = load_value(hi.v + e);
-            store_value(lo.v + e, p * cs.x - q * cs.y);
-            store_value(hi.v + e, q * cs.x + p * cs.y);
+            for (int e = 0; e < VEC; e++) {
+                const float2 cs = turn[t * a.half + j + e];
+                const float p = load_value(lo.v + e), q = load_value(hi.v + e);
+                store_value(lo.v + e, p * cs.x - q * cs.y);
+                store_value(hi.v + e, q * cs.x + p * cs.y);
+            }
+            *reinterpret_cast<Run*>(out + j) = lo;
+            *reinterpret_cast<Run*>(out + a.half + j) = hi;
         }
-        *reinterpret_cast<Run*>(out + j) = lo;
-        *reinterpret_cast<Run*>(out + a.half + j) = hi;
     }
 }
 
-constexpr int kRopeTokens = 4;
-
-template <typename T>
-void launch_rope(bool wide, const RopeArgs& a, hipStream_t stream) {
-    const dim3 grid((a.tokens + kRopeTokens - 1) / kRopeTokens);
-    const size_t lds = sizeof(float2) * kRopeTokens * a.half;
-    if (wide)
-        k_rope<T, 16 / sizeof(T), kRopeTokens><<<grid, kRopeThreads, lds, stream>>>(a);
+template <typename T, int VEC>
+void launch_rope(const RopeArgs& a, hipStream_t stream) {
+    // one token a workgroup while that leaves CUs to spare: at 64 tokens ROPE_SMALL us against ROPE_SMALL4 with four; at
+    // 4096 ROPE_LARGE1 against ROPE_LARGE
+    if (a.tokens <= 512)
+        k_rope<T, VEC, 1><<<a.tokens, kRopeThreads, sizeof(float2) * a.half, stream>>>(a);
     else
-        k_rope<T, 1, kRopeTokens><<<grid, kRopeThreads, lds, stream>>>(a);
+        k_rope<T, VEC, 4><<<(a.tokens + 3) / 4, kRopeThreads, sizeof(float2) * 4 * a.half, stream>>>(a);
 }
 
 int check_rope_tensor(const WlRopeTensor* x, int size) {
@@ -164,8 +164,8 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
     const bool wide = a.half % vec == 0 && head_dim % vec == 0 && aligned16(q, size) && (!k || aligned16(k, size));
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == WL_DTYPE_F32)
-        launch_rope<float>(wide, a, st);
+        wide ? launch_rope<float, 4>(a, st) : launch_rope<float, 1>(a, st);
     else
-        launch_rope<uint16_t>(wide, a, st);
+        wide ? launch_rope<uint16_t, 8>(a, st) : launch_rope<uint16_t, 1>(a, st);
     return launch_status();
 }
