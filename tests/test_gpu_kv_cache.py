@@ -1,0 +1,299 @@
+"""HBMKVCache, the rotary positions and HipAttention together on the GPU, as a model's loop uses them: prompts, decoding,
+forks, truncation, compaction, HIP graphs, several streams; against oracle/kv_ref.py on the cache's own contents."""
+import random
+
+import numpy as np
+import pytest
+import torch
+import torch.nn.functional as F
+
+from engines.qwen36 import HipAttention, Rotary
+from gguf import synth
+from gguf.hbm_cache import HBMKVCache, OutOfPages
+from gguf.hip import GGMLWeight, kv_attend
+from oracle import kv_ref
+
+pytestmark = pytest.mark.gpu
+DEV = "cuda"
+
+
+def bf16(g, *shape, scale=1.0):
+    return (torch.randn(*shape, generator=g) * scale).to(torch.bfloat16).to(DEV)
+
+
+def oracle_attend(cache, layer, step, q, **kw):
+    p = cache.pages
+    return kv_ref.attend(p.k[layer].cpu(), p.v[layer].cpu(), p.k_scale[layer].cpu(), p.v_scale[layer].cpu(), q.cpu(),
+                         step.table.cpu(), step.length.cpu(), step.cu.cpu(), **kw)
+
+
+def assert_within(got, want, tol):
+    err = (got.cpu().double() - want).abs()
+    assert (err <= tol).all(), f"off by {float((err / (tol + 1e-300)).max()):.2f} of the bound"
+
+
+def stored(cache, layer, seq):
+    """(keys, values) of a sequence as the cache holds them, fp64 [tokens, kv_heads, head_dim], and each value's step."""
+    p, (length, pages) = cache.pages, cache.book.sequences[seq]
+    ids = torch.tensor(pages, dtype=torch.long)
+    out = []
+    for pool, scale, flip in ((p.k, p.k_scale, False), (p.v, p.v_scale, True)):
+        x, s = pool[layer].cpu().double()[ids], scale[layer].cpu().double()[ids]
+        x = x.transpose(2, 3) if flip else x
+        tokens = lambda y: y.transpose(1, 2).reshape(-1, *y.shape[1:2], y.shape[3])[:length]  # noqa: E731
+        out.append((tokens(x * s[:, :, None, None]), tokens((s[:, :, None, None] * torch.ones_like(x)))))
+    return out
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_lives_of_sequences(hip, dtype):
+    """Prompts, single tokens, forks, cuts, frees and compactions in random order: every live sequence holds its own keys and
+    values, each within one step of its block, and attends to just those."""
+    rng, g = random.Random(5), torch.Generator().manual_seed(5)
+    cache = HBMKVCache(layers=2, pages=12, kv_heads=2, head_dim=64, page_tokens=16, dtype=dtype)
+    kept = {}  # seq -> [(k, v) of each layer]
+    full = 0
+    for i in range(90):
+        live = list(kept)
+        what = rng.choice(("new", "fork", "truncate", "free", "compact") + 6 * ("step",))
+        if what == "new" or not live:
+            kept[cache.new()] = [(torch.empty(0, 2, 64), torch.empty(0, 2, 64))] * 2
+        elif what == "step":
+            seqs = rng.sample(live, rng.randint(1, min(3, len(live))))
+            counts = [rng.choice((1, 1, 3, 17, 40)) for _ in seqs]
+            try:
+                step = cache.step(seqs, counts)
+            except OutOfPages:
+                full += 1
+                s = rng.choice(live)
+                cache.free(s)
+                del kept[s]
+                continue
+            for layer in range(2):
+                k, v = bf16(g, sum(counts), 2, 64, scale=1 + i % 4), bf16(g, sum(counts), 2, 64)
+                q = bf16(g, sum(counts), 6, 64)
+                cache.append(layer, step, k, v)
+                out = cache.attend(layer, step, q)
+                assert_within(out, *oracle_attend(cache, layer, step, q))
+                at = 0
+                for s, n in zip(seqs, counts):
+                    old = kept[s][layer]
+                    new = tuple(torch.cat((o, x[at:at + n].float().cpu())) for o, x in zip(old, (k, v)))
+                    kept[s] = [new if l == layer else kept[s][l] for l in range(2)]
+                    at += n
+        elif what == "fork":
+            s = rng.choice(live)
+            kept[cache.fork(s)] = list(kept[s])
+        elif what == "truncate":
+            s = rng.choice(live)
+            n = rng.randint(0, cache.length(s))
+            cache.truncate(s, n)
+            kept[s] = [tuple(x[:n] for x in kv) for kv in kept[s]]
+        elif what == "free":
+            s = rng.choice(live)
+            cache.free(s)
+            del kept[s]
+        else:
+            cache.compact()
+            assert all(p < cache.book.used() for v in cache.book.sequences.values() for p in v[1])
+        for s, layers in kept.items():
+            assert cache.length(s) == len(layers[0][0])
+            if not cache.length(s):
+                continue
+            for layer in range(2):
+                for (x, step_size), want in zip(stored(cache, layer, s), layers[layer]):
+                    # int8: under one step of the final scale. e4m3: half a step of its own magnitude (2^-4), and where a
+                    # grown scale pushed it below the normal ones, one of the smallest steps (2^-9) of the final scale
+                    tol = step_size if dtype == torch.int8 else 2.0 ** -4 * want.double().abs() + 2.0 ** -9 * step_size
+                    assert ((x - want.double()).abs() <= tol).all(), f"sequence {s}, layer {layer}"
+    assert full  # the cache did run out of pages on the way
+
+
+def test_prompt_by_pages(hip):
+    """A prompt in chunks that end with pages leaves the same bytes as the prompt at once, and the same answers."""
+    g = torch.Generator().manual_seed(6)
+    k, v, q = bf16(g, 300, 2, 128), bf16(g, 300, 2, 128), bf16(g, 300, 8, 128)
+    caches = [HBMKVCache(1, 8, 2, 128, 64) for _ in range(2)]
+    a, b = (c.new() for c in caches)
+    step = caches[0].step([a], [300])
+    caches[0].append(0, step, k, v)
+    whole = caches[0].attend(0, step, q)
+    parts = []
+    for lo, hi in ((0, 64), (64, 256), (256, 300)):
+        step = caches[1].step([b], [hi - lo])
+        caches[1].append(0, step, k[lo:hi], v[lo:hi])
+        parts.append(caches[1].attend(0, step, q[lo:hi]))
+    for name in ("k", "v", "k_scale", "v_scale"):
+        assert torch.equal(getattr(caches[0].pages, name), getattr(caches[1].pages, name))
+    want, tol = oracle_attend(caches[0], 0, _as_step(caches[0], a, 300), q)
+    assert_within(whole, want, tol)
+    assert_within(torch.cat(parts), want, tol)
+
+
+def _as_step(cache, seq, count):
+    class S:
+        pass
+    s, (length, pages) = S(), cache.book.sequences[seq]
+    s.table, s.length = torch.tensor([pages], dtype=torch.int32), torch.tensor([length], dtype=torch.int32)
+    s.cu = torch.tensor([0, count], dtype=torch.int32)
+    return s
+
+
+def test_decode_graph(hip):
+    """One decode step (rotary, append, attend over two layers) captured once and replayed for later tokens after refresh(),
+    with eager work and synchronizations in between: the same bits as eager steps on a cache of its own."""
+    g = torch.Generator().manual_seed(7)
+    rotary = Rotary(256, 64, 1e7, (11, 11, 10))
+    prompt, T = (70, 33, 128), 3
+    caches, seqs = [HBMKVCache(2, 24, 2, 256, 64) for _ in range(2)], []
+    filled = [(bf16(g, sum(prompt), 2, 256), bf16(g, sum(prompt), 2, 256)) for _ in range(2)]
+    for c in caches:
+        ids = [c.new() for _ in prompt]
+        seqs.append(ids)
+        s = c.step(ids, prompt)
+        for layer in range(2):
+            c.append(layer, s, *filled[layer])
+
+    def run(cache, step, x, positions):
+        outs = []
+        for layer in range(2):
+            q, k = rotary(x[layer][0], x[layer][1], positions)
+            cache.append(layer, step, k, x[layer][2])
+            outs.append(cache.attend(layer, step, q))
+        return torch.stack(outs)
+
+    def fresh():
+        return [(bf16(g, T, 16, 256), bf16(g, T, 2, 256), bf16(g, T, 2, 256)) for _ in range(2)]
+
+    inputs = fresh()
+    positions = rotary.positions(torch.tensor(prompt))
+    step = caches[0].step(seqs[0], [1] * T, width=6)
+    first = caches[1].step(seqs[1], [1] * T, width=6)
+    want = run(caches[1], first, inputs, positions)
+    torch.cuda.synchronize()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = run(caches[0], step, inputs, positions)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    for i in range(1, 9):
+        new = fresh()
+        for old, x in zip(inputs, new):
+            for a, b in zip(old, x):
+                a.copy_(b)
+        positions.add_(1)
+        caches[0].refresh(step, seqs[0], [1] * T)
+        want = run(caches[1], caches[1].step(seqs[1], [1] * T, width=6), inputs, positions)
+        if i % 3 == 0:
+            torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want), f"replay {i}"
+    with pytest.raises(ValueError):
+        caches[0].refresh(step, seqs[0], [2] * T)
+    with pytest.raises(ValueError):
+        caches[0].step([seqs[0][0]], [400], width=6)
+
+
+def test_streams_and_workspaces(hip):
+    """Calls on two streams at once on one cache, each with its own workspace from the allocator, and with one given."""
+    g = torch.Generator().manual_seed(8)
+    cache = HBMKVCache(1, 200, 2, 128, 64)
+    ids = [cache.new() for _ in range(3)]
+    step = cache.step(ids, [3000, 5000, 77])
+    cache.append(0, step, bf16(g, 8077, 2, 128), bf16(g, 8077, 2, 128))
+    step = cache.step(ids, [1, 1, 1])
+    cache.append(0, step, bf16(g, 3, 2, 128), bf16(g, 3, 2, 128))
+    qs = [bf16(g, 3, 16, 128) for _ in range(6)]
+    want = [cache.attend(0, step, q) for q in qs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for i, q in enumerate(qs):
+            with torch.cuda.stream(streams[i % 2]):
+                got.append(cache.attend(0, step, q))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    args = (cache.pages, 0, qs[0], step.table, step.length, step.cu)
+    ws = torch.full((64 << 20,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(kv_attend(*args, max_count=1, workspace=ws), want[0])  # whatever the workspace held
+    for bad in (ws[:64], ws.view(torch.int8), ws.cpu()):
+        with pytest.raises(ValueError):
+            kv_attend(*args, max_count=1, workspace=bad)
+
+
+class TinyEngine(HipAttention):
+    prefix = "model."
+
+    def __init__(self, weights, cache, rotary):
+        self.weights, self.kv_cache, self.rotary = weights, cache, rotary
+
+
+def engine(g, gated, quantized, norm):
+    hidden, heads, kv_heads, dim = 256, 4, 2, 64
+    p = "model.layers.3.self_attn"
+    rows = {"q_proj": (2 if gated else 1) * heads * dim, "k_proj": kv_heads * dim, "v_proj": kv_heads * dim, "o_proj": hidden}
+    w = {}
+    for i, (name, n) in enumerate(rows.items()):
+        if quantized and name != "o_proj":
+            raw = synth.q4_k_blocks(np.random.default_rng(i), n * hidden // 256)
+            w[f"{p}.{name}.weight"] = GGMLWeight(torch.from_numpy(raw.reshape(-1)).to(DEV), "Q4_K", (n, hidden))
+        else:
+            w[f"{p}.{name}.weight"] = bf16(g, n, heads * dim if name == "o_proj" else hidden, scale=hidden ** -0.5)
+    if norm:
+        w[f"{p}.q_norm.weight"], w[f"{p}.k_norm.weight"] = (0.1 * torch.randn(dim, generator=g) for _ in range(2))
+    return TinyEngine(w, HBMKVCache(1, 16, kv_heads, dim, 16), Rotary(dim, 32, 1e6, (6, 5, 5))), heads, dim
+
+
+@pytest.mark.parametrize("gated,quantized,norm", [(True, False, True), (False, False, False), (True, True, True)])
+def test_engine_attention(hip, gated, quantized, norm):
+    """HipAttention over a ragged prompt and decode steps, against its formula in 64 bits on the projections' own outputs and the
+    cache's own contents."""
+    g = torch.Generator().manual_seed(9)
+    eng, heads, dim = engine(g, gated, quantized, norm)
+    cache, p = eng.kv_cache, "model.layers.3.self_attn"
+    seqs = [cache.new(), cache.new()]
+    at = [0, 0]
+    for counts in ((21, 9), (1, 1), (1, 3)):
+        n = sum(counts)
+        x = bf16(g, n, 256, scale=2.0 ** -9 if quantized else 1.0)
+        step = cache.step(seqs, counts)
+        ids = torch.cat([torch.arange(a, a + c) for a, c in zip(at, counts)])
+        at = [a + c for a, c in zip(at, counts)]
+        positions = eng.rotary.positions(torch.stack((ids, ids // 3, ids % 5)))
+        y = eng.hip_attention(x, 3, 0, step, positions)
+        assert y.shape == (n, 256) and y.dtype == torch.bfloat16
+        wide = F.linear(x, eng.weights[f"{p}.q_proj.weight"]).cpu()
+        q, gate = wide.view(n, heads, 2, dim).unbind(2) if gated else (wide.view(n, heads, dim), None)
+        q64 = q.double()
+        if norm:
+            q64 = q64 * torch.rsqrt(q64.square().mean(-1, keepdim=True) + 1e-6) * (1 + eng.weights[f"{p}.q_norm.weight"].double())
+            q64 = q64.to(torch.float32).to(torch.bfloat16).double()
+        turned = kv_ref.rope(q64, positions.cpu(), eng.rotary.inv_freq.cpu(), (6, 5, 5), True)
+        want, tol = oracle_attend(cache, 0, step, turned.to(torch.float32).to(torch.bfloat16))
+        # q's norm and rotation round to bf16 twice, perhaps to the other neighbour (2^-7 of each value, 2^-6 together): scores
+        # move by at most that times sum |q k|, weights by twice as much, relatively
+        keys, values = zip(*[[z[0].abs().max() for z in stored(cache, 0, s)] for s in seqs])
+        move = 2.0 ** -6 * turned.abs().sum(-1, keepdim=True) * float(max(keys)) * dim ** -0.5
+        tol = tol + torch.expm1(2 * move) * float(max(values))
+        o, tol = want, tol
+        if gated:
+            s = torch.sigmoid(gate.double())
+            o, tol = o * s, tol * s + 2.0 ** -7 * (o * s).abs()
+        w = eng.weights[f"{p}.o_proj.weight"].cpu().double()
+        ref = o.reshape(n, -1) @ w.T
+        bound = (tol + 2.0 ** -8 * o.abs()).reshape(n, -1) @ w.abs().T + 2.0 ** -8 * ref.abs() + 1e-6
+        assert_within(y, ref, bound)
+
+
+def test_engine_attention_refuses(hip):
+    g = torch.Generator().manual_seed(10)
+    eng, _, _ = engine(g, True, False, True)
+    step = eng.kv_cache.step([eng.kv_cache.new()], [2])
+    eng.weights["model.layers.3.self_attn.k_proj.weight"] = bf16(g, 192, 256)
+    with pytest.raises(ValueError):
+        eng.hip_attention(bf16(g, 2, 256), 3, 0, step, eng.rotary.positions(torch.arange(2)))

@@ -1,0 +1,309 @@
+"""The attention half without a GPU: the page book's bookkeeping, the C ABI's refusals, the Python side's checks."""
+import ctypes
+import math
+import random
+
+import pytest
+import torch
+
+from engines.qwen36 import Rotary
+from gguf import hip
+from gguf.hbm_cache import OutOfPages, PageBook
+from oracle import kv_ref
+
+FAKE = 0x10000  # a non-NULL, aligned address that is never dereferenced
+
+
+# -- the page book ---------------------------------------------------------------------------------------------------
+
+
+def check_book(book):
+    """Every page is free, or used as often as sequences hold it; sequences hold just the pages that their tokens need."""
+    uses = [0] * book.pages
+    for length, pages in book.sequences.values():
+        assert len(pages) == -(-length // book.page_tokens) and len(set(pages)) == len(pages)
+        for p in pages:
+            uses[p] += 1
+    assert uses == book.uses
+    assert sorted(book.free_pages) == [p for p in range(book.pages) if not uses[p]]
+
+
+class Contents:
+    """What a device would hold, by the book's copies and a writer that writes where the book says."""
+
+    def __init__(self, book):
+        self.book, self.page, self.want = book, [[None] * book.page_tokens for _ in range(book.pages)], {}
+
+    def copy(self, src, dst):
+        assert len(set(dst)) == len(dst) and not set(src) & set(dst)
+        for a, b in zip(src, dst):
+            self.page[b] = list(self.page[a])
+
+    def grow(self, seqs, counts, stamp):
+        self.copy(*self.book.grow(seqs, counts))
+        for s, n in zip(seqs, counts):
+            length, pages = self.book.sequences[s]
+            for t in range(length - n, length):
+                self.page[pages[t // self.book.page_tokens]][t % self.book.page_tokens] = (stamp, s, t)
+                self.want.setdefault(s, []).append((stamp, s, t))
+
+    def check(self):
+        for s, (length, pages) in self.book.sequences.items():
+            got = [self.page[pages[t // self.book.page_tokens]][t % self.book.page_tokens] for t in range(length)]
+            assert got == self.want.get(s, []), f"sequence {s}"
+
+
+@pytest.mark.parametrize("seed", range(8))
+def test_page_book_random(seed):
+    """Random lives of sequences: what each one reads is always what was written for it, whatever was forked, cut, freed,
+    copied and compacted in between."""
+    rng = random.Random(seed)
+    book = PageBook(40, 16)
+    c = Contents(book)
+    for i in range(400):
+        live = list(book.sequences)
+        what = rng.choice(("new", "grow", "grow", "grow", "fork", "free", "truncate", "compact"))
+        if what == "new" or not live:
+            c.want[book.new()] = []
+        elif what == "grow":
+            seqs = rng.sample(live, rng.randint(1, min(4, len(live))))
+            counts = [rng.choice((0, 1, 1, 5, 16, 33)) for _ in seqs]
+            before = {s: [v[0], list(v[1])] for s, v in book.sequences.items()}
+            try:
+                c.grow(seqs, counts, i)
+            except OutOfPages:
+                assert before == book.sequences
+                book.free(rng.choice(live))
+        elif what == "fork":
+            s = rng.choice(live)
+            c.want[book.fork(s)] = list(c.want[s])
+        elif what == "free":
+            book.free(rng.choice(live))
+        elif what == "truncate":
+            s = rng.choice(live)
+            n = rng.randint(0, book.length(s))
+            book.truncate(s, n)
+            c.want[s] = c.want[s][:n]
+        else:
+            c.copy(*book.compact())
+            assert all(p < book.used() for v in book.sequences.values() for p in v[1])
+        check_book(book)
+        c.check()
+
+
+def test_page_book_takes_the_lowest():
+    book = PageBook(8, 16)
+    a, b = book.new(), book.new()
+    assert book.grow([a, b], [20, 1]) == ([], []) and book.sequences[a][1] == [0, 1] and book.sequences[b][1] == [2]
+    book.free(a)
+    d = book.new()
+    book.grow([d], [40])
+    assert book.sequences[d][1] == [0, 1, 3]
+
+
+def test_page_book_shared_last_page():
+    """Of a page that n sequences share and all write, n - 1 take copies; of one that only some write, each of those."""
+    book = PageBook(8, 16)
+    a = book.new()
+    book.grow([a], [20])
+    b, c = book.fork(a), book.fork(a)
+    src, dst = book.grow([a, b, c], [1, 1, 1])
+    assert src == [1, 1] and dst == [2, 3] and book.sequences[c][1] == [0, 1]
+    e = book.fork(a)
+    assert book.grow([e], [1]) == ([2], [4]) and book.grow([a], [1]) == ([], [])
+    f = book.fork(a)
+    book.truncate(f, 16)
+    assert book.grow([f], [1]) == ([], [])  # the page behind whole shared ones is its own
+
+
+def test_page_book_refuses():
+    book = PageBook(2, 16)
+    a = book.new()
+    for bad in (lambda: book.grow([a, a], [1, 1]), lambda: book.grow([a], [-1]), lambda: book.grow([a], [1, 2]),
+                lambda: book.truncate(a, 1), lambda: book.truncate(a, -1)):
+        with pytest.raises(ValueError):
+            bad()
+    for bad in (lambda: book.grow([7], [1]), lambda: book.free(7), lambda: book.fork(7), lambda: book.length(7)):
+        with pytest.raises(KeyError):
+            bad()
+    with pytest.raises(OutOfPages):
+        book.grow([a], [33])
+    assert book.used() == 0 and book.length(a) == 0
+
+
+# -- the C ABI -------------------------------------------------------------------------------------------------------
+
+
+def cache_struct(**over):
+    s = hip.WlKvCache(FAKE, FAKE, FAKE, FAKE, 8, 2, 2, 64, 16, 0, 0)
+    for k, v in over.items():
+        setattr(s, k, v)
+    return s
+
+
+def batch_struct(**over):
+    b = hip.WlKvBatch(FAKE, FAKE, 4, 6, 2, 4, 3, 0)
+    for k, v in over.items():
+        setattr(b, k, v)
+    return b
+
+
+def test_struct_layout():
+    assert ctypes.sizeof(hip.WlKvCache) == 4 * 8 + 8 + 6 * 4 == 64
+    assert ctypes.sizeof(hip.WlKvBatch) == 4 * 8 + 4 * 4 == 48
+    assert ctypes.sizeof(hip.WlRopeTensor) == 6 * 8 + 2 * 4 == 56
+
+
+BAD_CACHES = [({"k": None}, -3), ({"v_scale": None}, -3), ({"type": 2}, -13), ({"head_dim": 96}, -13), ({"page_tokens": 8}, -13),
+              ({"page_tokens": 48}, -13), ({"page_tokens": 2048}, -13), ({"pages": 0}, -2), ({"pages": 1 << 31}, -2),
+              ({"layers": 0}, -2), ({"kv_heads": 0}, -2), ({"reserved": 1}, -2), ({"v": FAKE + 8}, -4), ({"k_scale": FAKE + 2}, -4)]
+BAD_BATCHES = [({"table": None}, -3), ({"cu": None}, -3), ({"seqs": 0}, -2), ({"seqs": 65536}, -2), ({"table_width": 0}, -2),
+               ({"table_stride": 3}, -2), ({"tokens": 0}, -2), ({"max_count": 0}, -2), ({"max_count": 7}, -2), ({"reserved": 1}, -2),
+               ({"cu": FAKE + 2}, -4)]
+
+
+def calls(cache, batch, layer=0):
+    lib = hip.library()
+    c, b = ctypes.byref(cache), ctypes.byref(batch)
+    return [lib.wl_kv_append(c, layer, FAKE, 128, 64, FAKE, 128, 64, b, FAKE, None),
+            lib.wl_kv_attend(c, layer, FAKE, 256, 64, 4, b, FAKE, 64, 0.125, 1, FAKE, None, 0, None)]
+
+
+@pytest.mark.parametrize("over,code", BAD_CACHES)
+def test_bad_caches(over, code):
+    lib, cache = hip.library(), cache_struct(**over)
+    assert lib.wl_kv_check(ctypes.byref(cache)) == code and calls(cache, batch_struct()) == [code, code]
+    assert lib.wl_kv_copy(ctypes.byref(cache), FAKE, FAKE, 1, None) == code
+    assert lib.wl_kv_attend_workspace_bytes(ctypes.byref(cache), 4, ctypes.byref(batch_struct()), 64) == 0
+
+
+@pytest.mark.parametrize("over,code", BAD_BATCHES)
+def test_bad_batches(over, code):
+    assert calls(cache_struct(), batch_struct(**over)) == [code, code]
+
+
+def test_bad_calls():
+    lib = hip.library()
+    c, b = ctypes.byref(cache_struct()), ctypes.byref(batch_struct())
+    assert calls(cache_struct(), batch_struct(), layer=2) == [-2, -2] and calls(cache_struct(), batch_struct(), layer=-1) == [-2, -2]
+    append = lambda k=FAKE, v=FAKE, start=FAKE: lib.wl_kv_append(c, 0, k, 128, 64, v, 128, 64, b, start, None)  # noqa: E731
+    assert append(k=None) == append(v=None) == append(start=None) == -3 and append(k=FAKE + 1) == append(start=FAKE + 2) == -4
+
+    def attend(q=FAKE, heads=4, batch=b, length=FAKE, bound=64, scale=0.125, out=FAKE, ws=None, n=0):
+        return lib.wl_kv_attend(c, 0, q, 256, 64, heads, batch, length, bound, scale, 1, out, ws, n, None)
+    assert attend(q=None) == attend(length=None) == attend(out=None) == -3
+    assert attend(q=FAKE + 1) == attend(out=FAKE + 8) == attend(length=FAKE + 1) == -4
+    assert attend(heads=3) == attend(heads=0) == attend(bound=-1) == -2
+    assert attend(scale=-1.0) == attend(scale=math.inf) == attend(scale=math.nan) == -2
+    long = ctypes.byref(batch_struct(table_width=64, table_stride=64))
+    need = lib.wl_kv_attend_workspace_bytes(c, 4, long, 1024)
+    assert need > 0 and attend(batch=long, bound=1024) == attend(batch=long, bound=1024, ws=FAKE, n=need - 1) == -6
+    assert attend(batch=long, bound=1024, ws=FAKE + 4, n=need) == -6
+    huge = ctypes.byref(batch_struct(seqs=65535, table_width=1 << 20, table_stride=1 << 20))
+    assert attend(batch=huge) == -2  # more tiles than 31 bits count
+
+
+@pytest.mark.parametrize("src,dst,code", [([0], [8], -14), ([-1], [2], -14), ([8], [2], -14), ([0, 1], [3, 3], -14),
+                                          ([0, 1], [1, 2], -14), ([4], [4], -14)])
+def test_bad_copies(src, dst, code):
+    a, b = ((ctypes.c_int32 * len(x))(*x) for x in (src, dst))
+    assert hip.library().wl_kv_copy(ctypes.byref(cache_struct()), a, b, len(src), None) == code
+
+
+def test_copy_counts():
+    lib, c = hip.library(), ctypes.byref(cache_struct())
+    one = (ctypes.c_int32 * 1)(0)
+    assert lib.wl_kv_copy(c, None, None, 0, None) == 0 and lib.wl_kv_copy(c, None, one, 1, None) == -3
+    assert lib.wl_kv_copy(c, one, one, -1, None) == lib.wl_kv_copy(c, one, one, 9, None) == -2
+
+
+def test_bad_rope():
+    lib = hip.library()
+
+    def call(q={}, k=None, dtype=1, tokens=4, dim=64, rotary=32, pos=FAKE, inv=FAKE, axes=3, sections=(6, 5, 5), inter=1):  # noqa: B006
+        def tensor(over):
+            t = hip.WlRopeTensor(FAKE, FAKE, 256, 64, 256, 64, 4, 0)
+            for n, v in over.items():
+                setattr(t, n, v)
+            return ctypes.byref(t)
+        return lib.wl_rope(tensor(q), None if k is None else tensor(k), dtype, tokens, dim, rotary, pos, 4, inv, axes,
+                           (ctypes.c_int32 * len(sections))(*sections), inter, 1.0, None)
+    assert call(dtype=2) == -7 and call(q={"in_": None}) == call(q={"out": None}) == call(k={"in_": None}) == -3
+    assert call(pos=None) == call(inv=None) == -3 and call(pos=FAKE + 4) == call(inv=FAKE + 4) == call(q={"in_": FAKE + 1}) == -4
+    assert call(dtype=0, q={"out": FAKE + 2}) == -4
+    for bad in (dict(tokens=0), dict(dim=1), dict(dim=2048), dict(rotary=33), dict(rotary=66), dict(rotary=0), dict(axes=0),
+                dict(axes=5, sections=(4, 4, 4, 4, 0)), dict(sections=(6, 5, 4)), dict(sections=(16, 1, -1)), dict(sections=(4, 5, 7)),
+                dict(q={"heads": 0}), dict(k={"heads": 0}), dict(q={"reserved": 1})):
+        assert call(**bad) == -2, bad
+
+
+def test_error_strings():
+    for code in (-13, -14):
+        assert hip.library().wl_error_string(code) != hip.library().wl_error_string(-99)
+
+
+# -- the Python side -------------------------------------------------------------------------------------------------
+
+
+def test_pages_refuse():
+    z = torch.zeros
+    ok = dict(k=z(1, 2, 1, 16, 64, dtype=torch.int8), v=z(1, 2, 1, 64, 16, dtype=torch.int8), k_scale=z(1, 2, 1), v_scale=z(1, 2, 1))
+    hip.KVPages(**ok)
+    for bad in (dict(k=z(1, 2, 1, 16, 64)), dict(v=z(1, 2, 1, 16, 64, dtype=torch.int8)), dict(v=z(1, 2, 1, 64, 16)),
+                dict(k_scale=z(1, 2)), dict(v_scale=z(1, 2, 2)), dict(k_scale=z(1, 2, 1, dtype=torch.float64)),
+                dict(k=z(1, 2, 1, 64, 16, dtype=torch.int8).transpose(3, 4)),
+                dict(k=z(1, 2, 1, 16, 96, dtype=torch.int8), v=z(1, 2, 1, 96, 16, dtype=torch.int8)),
+                dict(k=z(1, 2, 1, 24, 64, dtype=torch.int8), v=z(1, 2, 1, 64, 24, dtype=torch.int8))):
+        with pytest.raises(ValueError):
+            hip.KVPages(**{**ok, **bad})
+
+
+def test_call_checks():
+    """What the wrappers refuse before they reach the library (on tensors of the CPU, which they take for a device's)."""
+    z = torch.zeros
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    k, q = z(3, 2, 64, dtype=torch.bfloat16), z(3, 4, 64, dtype=torch.bfloat16)
+    i = dict(dtype=torch.int32)
+    good = dict(table=z(1, 2, **i), cu=z(2, **i))
+    for bad in (dict(table=z(1, 2)), dict(table=z(2, **i)), dict(cu=z(3, **i)), dict(cu=z(2, dtype=torch.int64)), dict(cu=z(4, **i)[::2]),
+                dict(table=z(1, 4, **i)[:, ::2]), dict(cu=[0, 3])):
+        a = {**good, **bad}
+        with pytest.raises(ValueError):
+            hip.kv_append(p, 0, k, k, a["table"], z(1, **i), a["cu"])
+        with pytest.raises(ValueError):
+            hip.kv_attend(p, 0, q, a["table"], z(1, **i), a["cu"])
+    for bad in (k.float(), z(3, 1, 64, dtype=torch.bfloat16), z(3, 2, 32, dtype=torch.bfloat16), z(2, 2, 64, dtype=torch.bfloat16), None,
+                z(3, 2, 128, dtype=torch.bfloat16)[:, :, ::2]):
+        with pytest.raises(ValueError):
+            hip.kv_append(p, 0, k, bad, good["table"], z(1, **i), good["cu"])
+    for bad in (q.float(), z(3, 3, 64, dtype=torch.bfloat16), z(3, 0, 64, dtype=torch.bfloat16), z(3, 4, 32, dtype=torch.bfloat16)):
+        with pytest.raises(ValueError):
+            hip.kv_attend(p, 0, bad, good["table"], z(1, **i), good["cu"])
+    for out in (q.float(), z(2, 4, 64, dtype=torch.bfloat16), z(3, 4, 128, dtype=torch.bfloat16)[:, :, :64]):
+        with pytest.raises(ValueError):
+            hip.kv_attend(p, 0, q, good["table"], z(1, **i), good["cu"], out=out)
+    with pytest.raises(ValueError):
+        hip.kv_copy(p, [0, 1], [2])
+    with pytest.raises(ValueError):
+        hip.rope(z(2, 1, 64), None, z(2, dtype=torch.int64), z(8, dtype=torch.float64))  # not on a GPU
+
+
+def test_rotary():
+    r = Rotary(256, 64, 1e7, (11, 11, 10), device="cpu")
+    assert r.inv_freq.dtype == torch.float64 and float(r.inv_freq[0]) == 1.0
+    assert float(r.inv_freq[16]) == pytest.approx(1e7 ** -0.5, rel=1e-15)
+    assert r.positions(torch.arange(5)).shape == (3, 5)
+    for bad in (dict(rotary_dim=63), dict(rotary_dim=512), dict(sections=(11, 11, 11), rotary_dim=64), dict(inv_freq=[1.0], rotary_dim=64)):
+        with pytest.raises(ValueError):
+            Rotary(256, device="cpu", **bad)
+
+
+# -- the oracle's own pieces -----------------------------------------------------------------------------------------
+
+
+def test_oracle_rounding():
+    assert kv_ref.bf16_not_below(1.0) == 1.0 and kv_ref.bf16_not_below(1.0 + 2.0 ** -20) == 1.0 + 2.0 ** -7
+    x = torch.linspace(-448, 448, 30001, dtype=torch.float64)
+    assert torch.equal(kv_ref.nearest(x, torch.float8_e4m3fn), x.to(torch.float32).to(torch.float8_e4m3fn).double())
+    tiny = torch.linspace(-0.03, 0.03, 30001, dtype=torch.float64)
+    assert torch.equal(kv_ref.nearest(tiny, torch.float8_e4m3fn), tiny.to(torch.float32).to(torch.float8_e4m3fn).double())

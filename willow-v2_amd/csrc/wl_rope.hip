@@ -45,66 +45,84 @@ __device__ __forceinline__ void store_value(uint16_t* p, float x) {
     *p = __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
 }
 
-// One workgroup takes TOKENS tokens: the cosines and sines of their angles once into LDS, then every head's values by
-// them. The angle is taken in turns in 64 bits (a position of a million at the first frequency is 1.6e5 turns, of which
-// fp32 would keep 6 bits of the fraction) and only its fraction goes on in 32.
+// One workgroup takes a token: the cosines and sines of its angles once into LDS, then every head's values by them, 32 lanes
+// a head. The first eight heads' values are asked for before the angles are worked out (more of them help few tokens by less
+// than 0.4 us and cost many 2 to 3). The angle is taken in turns in 64 bits (a
+// position of a million at the first frequency is 1.6e5 turns, of which fp32 would keep 6 bits of the fraction) and only its
+// fraction goes on in 32.
 // VEC: values a thread moves at once (16 bytes where every row and the half split are that aligned, else one).
-// Bound by reading and writing q and k once.
-template <typename T, int VEC, int TOKENS>
+// Bound by reading and writing q and k once (4096 tokens of 16 + 2 heads of 256 in bf16, 75 MB: 20.9 us, 3.6 TB/s); a token
+// a workgroup, since one with more runs through their heads one pass after the other (1024 tokens: 9.0 us, with two tokens a
+// workgroup 10.8, with four 13.9; 4096 tokens: all within 0.6 us).
+template <typename T, int VEC>
 __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
-    extern __shared__ float2 turn[];  // [TOKENS][half]: cos, sin
-    const int t0 = blockIdx.x * TOKENS, n = min(TOKENS, a.tokens - t0);
-    for (int i = threadIdx.x; i < n * a.half; i += kRopeThreads) {
-        const int t = t0 + i / a.half, j = i % a.half;
-        const double pos = static_cast<double>(a.positions[axis_of(a, j) * a.positions_stride + t]);
-        const double turns = pos * a.inv_freq[j] * 0.15915494309189533577;  // 1 / (2 pi)
-        float s, c;
-        sincospif(static_cast<float>(2.0 * (turns - __builtin_rint(turns))), &s, &c);
-        turn[i] = make_float2(a.scale * c, a.scale * s);
-    }
-    __syncthreads();
-    // a head: half / VEC pairs of runs, then what is not rotated; 32 lanes a head
+    extern __shared__ float2 turn[];  // [half]: cos, sin
     struct alignas(sizeof(T) * VEC) Run {
         T v[VEC];
     };
-    const int pairs = a.half / VEC, rest = (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
-#pragma unroll 4
-    for (int i = threadIdx.x / 32; i < n * heads; i += kRopeThreads / 32) {
-        const int t = TOKENS == 1 ? 0 : i / heads, hh = TOKENS == 1 ? i : i % heads;
-        const bool is_k = hh >= a.q.heads;
-        const WlRopeTensor& x = is_k ? a.k : a.q;
-        const int h = is_k ? hh - a.q.heads : hh;
-        const T* in = static_cast<const T*>(x.in) + (t0 + t) * x.in_token_stride + h * x.in_head_stride;
-        T* out = static_cast<T*>(x.out) + (t0 + t) * x.out_token_stride + h * x.out_head_stride;
-        for (int u = threadIdx.x % 32; u < pairs + rest; u += 32) {
-            if (u >= pairs) {
-                const int d = 2 * a.half + (u - pairs) * VEC;
-                if (in != out) *reinterpret_cast<Run*>(out + d) = *reinterpret_cast<const Run*>(in + d);
-                continue;
-            }
-            const int j = u * VEC;
-            Run lo = *reinterpret_cast<const Run*>(in + j), hi = *reinterpret_cast<const Run*>(in + a.half + j);
-#pragma unroll
-            for (int e = 0; e < VEC; e++) {
-                const float2 cs = turn[t * a.half + j + e];
-                const float p = load_value(lo.v + e), q = load_value(hi.v + e);
-                store_value(lo.v + e, p * cs.x - q * cs.y);
-                store_value(hi.v + e, q * cs.x + p * cs.y);
-            }
-            *reinterpret_cast<Run*>(out + j) = lo;
-            *reinterpret_cast<Run*>(out + a.half + j) = hi;
+    constexpr int kRows = kRopeThreads / 32, kEarly = 1;
+    const int token = blockIdx.x, lane = threadIdx.x % 32;
+    // a head: half / VEC pairs of runs, then what is not rotated
+    const int pairs = a.half / VEC, units = pairs + (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
+    struct Head {
+        const T* in;
+        T* out;
+    };
+    auto head_at = [&](int i) -> Head {
+        const WlRopeTensor& x = i >= a.q.heads ? a.k : a.q;
+        const int h = i >= a.q.heads ? i - a.q.heads : i;
+        return {static_cast<const T*>(x.in) + token * x.in_token_stride + h * x.in_head_stride,
+                static_cast<T*>(x.out) + token * x.out_token_stride + h * x.out_head_stride};
+    };
+    auto load = [&](const Head& x, int u, Run& lo, Run& hi) {
+        lo = *reinterpret_cast<const Run*>(x.in + (u < pairs ? u : u + pairs) * VEC);
+        if (u < pairs) hi = *reinterpret_cast<const Run*>(x.in + a.half + u * VEC);
+    };
+    auto finish = [&](const Head& x, int u, Run lo, Run hi) {
+        if (u >= pairs) {
+            if (x.in != x.out) *reinterpret_cast<Run*>(x.out + (u + pairs) * VEC) = lo;
+            return;
         }
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float2 cs = turn[u * VEC + e];
+            const float p = load_value(lo.v + e), q = load_value(hi.v + e);
+            store_value(lo.v + e, p * cs.x - q * cs.y);
+            store_value(hi.v + e, q * cs.x + p * cs.y);
+        }
+        *reinterpret_cast<Run*>(x.out + u * VEC) = lo;
+        *reinterpret_cast<Run*>(x.out + a.half + u * VEC) = hi;
+    };
+    Run lo[kEarly], hi[kEarly];
+#pragma unroll
+    for (int r = 0; r < kEarly; r++) {
+        const int i = threadIdx.x / 32 + r * kRows;
+        if (i < heads && lane < units) load(head_at(i), lane, lo[r], hi[r]);
     }
+    for (int j = threadIdx.x; j < a.half; j += kRopeThreads) {
+        const double pos = static_cast<double>(a.positions[axis_of(a, j) * a.positions_stride + token]);
+        const double turns = pos * a.inv_freq[j] * 0.15915494309189533577;  // 1 / (2 pi)
+        float s, c;
+        sincospif(static_cast<float>(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+        turn[j] = make_float2(a.scale * c, a.scale * s);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int r = 0; r < kEarly; r++) {
+        const int i = threadIdx.x / 32 + r * kRows;
+        if (i < heads && lane < units) finish(head_at(i), lane, lo[r], hi[r]);
+    }
+    for (int i = threadIdx.x / 32; i < heads; i += kRows)
+        for (int u = i < kEarly * kRows ? lane + 32 : lane; u < units; u += 32) {
+            Run x, y;
+            load(head_at(i), u, x, y);
+            finish(head_at(i), u, x, y);
+        }
 }
 
 template <typename T, int VEC>
 void launch_rope(const RopeArgs& a, hipStream_t stream) {
-    // one token a workgroup while that leaves CUs to spare: at 64 tokens ROPE_SMALL us against ROPE_SMALL4 with four; at
-    // 4096 ROPE_LARGE1 against ROPE_LARGE
-    if (a.tokens <= 512)
-        k_rope<T, VEC, 1><<<a.tokens, kRopeThreads, sizeof(float2) * a.half, stream>>>(a);
-    else
-        k_rope<T, VEC, 4><<<(a.tokens + 3) / 4, kRopeThreads, sizeof(float2) * 4 * a.half, stream>>>(a);
+    k_rope<T, VEC><<<a.tokens, kRopeThreads, sizeof(float2) * a.half, stream>>>(a);
 }
 
 int check_rope_tensor(const WlRopeTensor* x, int size) {

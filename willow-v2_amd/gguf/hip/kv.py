@@ -181,6 +181,8 @@ def kv_copy(pages: KVPages, src, dst):
     src, dst = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst))
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError(f"src and dst must be lists of the same length (got {list(src.shape)} and {list(dst.shape)})")
+    if src.shape[0] == 0:
+        return
     _launch(pages.index, library().wl_kv_copy, pages.ref, src.ctypes.data, dst.ctypes.data, src.shape[0])
 
 
