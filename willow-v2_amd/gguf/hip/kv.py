@@ -7,6 +7,7 @@ every decoded token. All calls only enqueue work on the current stream of their 
 lengths and row offsets on the GPU, so they may be captured into a HIP graph.
 """
 import ctypes
+import functools
 
 import numpy as np
 import torch
@@ -18,11 +19,13 @@ TYPES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
 def _launch(index, call, *args):
     """call(*args, stream) with device `index` current (a launch goes to the current device) and its current stream."""
-    if index == torch.cuda.current_device():
-        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
-        return
-    with torch.cuda.device(index):
-        check(call(*args, torch._C._cuda_getCurrentRawStream(index)))
+    if index == torch._C._cuda_getDevice():
+        rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
+    if rc:
+        check(rc)
 
 
 def _refuse(t, name, device, dtype, shape):
@@ -132,7 +135,7 @@ def kv_append(pages: KVPages, layer: int, k: torch.Tensor, v: torch.Tensor, tabl
     if n == 0 or b.seqs == 0:
         return
     _launch(pages.index, library().wl_kv_append, pages.ref, layer, k.data_ptr(), k_token, k_head, v.data_ptr(), v_token, v_head,
-            ctypes.byref(b), start.data_ptr())
+            b, start.data_ptr())
 
 
 def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, length: torch.Tensor, cu: torch.Tensor,
@@ -159,8 +162,8 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     longest = b.table_width * pages.page_tokens
     if max_length is not None and max_length < longest:
         longest = max_length
-    lib, batch = library(), ctypes.byref(b)
-    need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, batch, longest)
+    lib = library()
+    need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, b, longest)
     space = None
     if workspace is not None:
         if workspace.dtype is not torch.uint8 or workspace.get_device() != pages.index or not workspace.is_contiguous():
@@ -169,7 +172,7 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     elif need:
         workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
         space = workspace.data_ptr()
-    _launch(pages.index, lib.wl_kv_attend, pages.ref, layer, q.data_ptr(), token_stride, head_stride, heads, batch,
+    _launch(pages.index, lib.wl_kv_attend, pages.ref, layer, q.data_ptr(), token_stride, head_stride, heads, b,
             length.data_ptr(), longest, pages.head_dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), space, need)
     return out
 
@@ -184,6 +187,19 @@ def kv_copy(pages: KVPages, src, dst):
     if src.shape[0] == 0:
         return
     _launch(pages.index, library().wl_kv_copy, pages.ref, src.ctypes.data, dst.ctypes.data, src.shape[0])
+
+
+@functools.lru_cache(maxsize=64)
+def _sections(sections):
+    return (ctypes.c_int32 * len(sections))(*sections)
+
+
+def _rotated_into(out, x, index, dim):
+    """(token stride, head stride) of the tensor that x's rotated values go to."""
+    n, _, token, head = _rows(out, "out", index, x.dtype, x.shape[1], dim)
+    if n != x.shape[0] or (out.data_ptr() == x.data_ptr() and (token, head) != x.stride()[:2]):
+        raise ValueError("out must have its tensor's shape, and its strides where it is the same memory")
+    return token, head
 
 
 def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, sections=None,
@@ -201,40 +217,37 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
     if index < 0:
         raise ValueError(f"q must be on the GPU (got {q.device})")
     dim = q.shape[-1]
-    n, heads, token_stride, head_stride = _rows(q, "q", index, dtype, None, dim)
+    n, heads, token, head = _rows(q, "q", index, dtype, None, dim)
     if positions.dim() == 1:
         positions = positions[None]
-    _need(positions, "positions", index, torch.int64, ("axes", "tokens"))
-    _need(inv_freq, "inv_freq", index, torch.float64, ("rotary_dim / 2",))
+    if not (positions.dtype is torch.int64 and positions.get_device() == index and positions.dim() == 2):
+        _refuse(positions, "positions", q.device, torch.int64, "[axes, tokens]")
+    if not (inv_freq.dtype is torch.float64 and inv_freq.get_device() == index and inv_freq.dim() == 1 and inv_freq.is_contiguous()):
+        _refuse(inv_freq, "inv_freq", q.device, torch.float64, "[rotary_dim / 2], contiguous")
     axes, cols = positions.shape
     axis_stride, step = positions.stride()
     half = inv_freq.shape[0]
-    if sections is None:
-        sections = (half,)
-    if len(sections) != axes:
-        raise ValueError(f"positions has {axes} axes, sections {len(sections)}")
-    if cols != n or (step != 1 and n > 1) or not inv_freq.is_contiguous():
-        raise ValueError(f"positions must be [axes, {n}] with contiguous rows, inv_freq contiguous")
-
-    def rotated(x, y, rows):
-        """The struct of one tensor and where its result goes."""
-        if rows[0] != n:
-            raise ValueError(f"q has {n} rows, k {rows[0]}")
-        if y is None:
-            y = torch.empty_like(x, memory_format=torch.contiguous_format)
-            y_token, y_head = rows[1] * dim, dim
-        else:
-            m, _, y_token, y_head = _rows(y, "out", index, dtype, rows[1], dim)
-            if m != n or (y.data_ptr() == x.data_ptr() and (y_token, y_head) != rows[2:]):
-                raise ValueError("out must have its tensor's shape, and its strides where it is the same memory")
-        return y, ctypes.byref(WlRopeTensor(x.data_ptr(), y.data_ptr(), rows[2], rows[3], y_token, y_head, rows[1], 0))
-
+    sections = (half,) if sections is None else tuple(sections)
+    if len(sections) != axes or cols != n or (step != 1 and n > 1):
+        raise ValueError(f"positions must be [{len(sections)}, {n}] (axes as in sections {sections}, q's tokens) with contiguous "
+                         f"rows (got {list(positions.shape)})")
     q_out, k_out = (None, None) if out is None else out
-    q_out, q_arg = rotated(q, q_out, (n, heads, token_stride, head_stride))
+    if q_out is None:
+        q_out, to = torch.empty_like(q, memory_format=torch.contiguous_format), (heads * dim, dim)
+    else:
+        to = _rotated_into(q_out, q, index, dim)
+    q_arg = WlRopeTensor(q.data_ptr(), q_out.data_ptr(), token, head, *to, heads, 0)
     k_arg = None
     if k is not None:
-        k_out, k_arg = rotated(k, k_out, _rows(k, "k", index, dtype, None, dim))
+        rows, heads, token, head = _rows(k, "k", index, dtype, None, dim)
+        if rows != n:
+            raise ValueError(f"q has {n} rows, k {rows}")
+        if k_out is None:
+            k_out, to = torch.empty_like(k, memory_format=torch.contiguous_format), (heads * dim, dim)
+        else:
+            to = _rotated_into(k_out, k, index, dim)
+        k_arg = WlRopeTensor(k.data_ptr(), k_out.data_ptr(), token, head, *to, heads, 0)
     if n:
         _launch(index, library().wl_rope, q_arg, k_arg, DTYPE_BF16 if dtype is torch.bfloat16 else DTYPE_F32, n, dim, 2 * half,
-                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, (ctypes.c_int32 * axes)(*sections), interleaved, scale)
+                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, _sections(sections), interleaved, scale)
     return q_out, k_out
