@@ -24,6 +24,7 @@ constexpr int kGroupRows = kWaves * 32;
 constexpr int kRing = 4;  // tiles in LDS: two are multiplied between barriers, two are filled
 constexpr int kMaxPieces = 16;
 constexpr int kCus = 256;
+constexpr int64_t kPartialBytes = 256 << 20;  // for partial results, at most
 constexpr float kSlack = 8.0f;  // log2: how far a score may lie above the running maximum
 
 struct RowsArgs : AttendArgs {
@@ -403,48 +404,62 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     if (half == 0) a.partial_ml[slot] = make_float2(m, l);
 }
 
-// Adds up the pieces of the row tiles that were cut: a wavefront a row. blockIdx: (four rows, kv head), sequence.
-constexpr int kMergeRows = 4;
+// Adds up the pieces of the row tiles that were cut: a wavefront takes four rows, so that a row's chain of loads is shared
+// (one row each: 21 and 12 us where this takes MERGE_4096 and MERGE_RAGGED). blockIdx: (16 rows, kv head), sequence.
+constexpr int kMergeWaves = 4, kWaveRows = 4, kMergeRows = kMergeWaves * kWaveRows;
+static_assert(64 / kWaveRows == kMaxPieces && kGroupRows % kMergeRows == 0, "a lane for each piece of each row");
 template <int D>
-__global__ __launch_bounds__(kMergeRows * 64) void k_attend_merge(RowsArgs a) {
+__global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge(RowsArgs a) {
     const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, lane = threadIdx.x & 63;
-    const int row = __builtin_amdgcn_readfirstlane(blockIdx.x / a.c.kv_heads * kMergeRows + (threadIdx.x >> 6));
+    const int first = __builtin_amdgcn_readfirstlane(blockIdx.x / a.c.kv_heads * kMergeRows + (threadIdx.x >> 6) * kWaveRows);
     const Seq seq = a.seq_uniform(b);
-    if (row >= seq.n * a.group) return;
-    const int pieces = cut_of(tiles_of(a, seq, row / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
+    const int rows = seq.n * a.group;
+    if (first >= rows) return;
+    const int pieces = cut_of(tiles_of(a, seq, first / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
     if (pieces < 2) return;
     constexpr int V = D / 64;
     typedef float Lane __attribute__((ext_vector_type(V)));
     const int64_t stride = static_cast<int64_t>(a.s.tokens) * a.q_heads;
-    const int64_t place = static_cast<int64_t>(seq.at + row / a.group) * a.q_heads + head * a.group + row % a.group;
-    const float2 ml = lane < pieces ? a.partial_ml[lane * stride + place] : make_float2(-__builtin_inff(), 0.0f);
+    const int row = min(first + lane / kMaxPieces, rows - 1), piece = lane % kMaxPieces;
+    const int place = (seq.at + row / a.group) * a.q_heads + head * a.group + row % a.group;
+    const float2 ml = piece < pieces ? a.partial_ml[piece * stride + place] : make_float2(-__builtin_inff(), 0.0f);
     float top = ml.x;
 #pragma unroll
     for (int d = kMaxPieces / 2; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
-    const float safe = top == -__builtin_inff() ? 0.0f : top, own = exp2_fast(ml.x - safe);
-    Lane sum = {};
-    float l = 0.0f;
-    for (int i = 0; i < pieces; i += 4) {
-        Lane x[4];
+    const float own = exp2_fast(ml.x - (top == -__builtin_inff() ? 0.0f : top));
+    float l = ml.y * own;
 #pragma unroll
-        for (int e = 0; e < 4; e++)
-            x[e] = *reinterpret_cast<const Lane*>(a.partial + (min(i + e, pieces - 1) * stride + place) * D + lane * V);
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (i + e >= pieces) break;
-            const float f = __shfl(own, i + e);
-            l += __shfl(ml.y, i + e) * f;
-            sum += x[e] * f;
-        }
-    }
+    for (int d = kMaxPieces / 2; d; d >>= 1) l += __shfl_xor(l, d);
     const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-    uint16_t* out = a.out + place * D + lane * V;
-    if constexpr (V == 4) {
-        *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(sum[0] * inv, sum[1] * inv), pack_bf16(sum[2] * inv, sum[3] * inv));
-    } else if constexpr (V == 2) {
-        *reinterpret_cast<uint32_t*>(out) = pack_bf16(sum[0] * inv, sum[1] * inv);
-    } else {
-        *out = __builtin_bit_cast(uint16_t, static_cast<__bf16>(sum[0] * inv));
+    int at[kWaveRows];
+    Lane sum[kWaveRows];
+#pragma unroll
+    for (int r = 0; r < kWaveRows; r++) {
+        at[r] = __builtin_amdgcn_readlane(place, r * kMaxPieces);
+        sum[r] = (Lane)(0.0f);
+    }
+    auto of_lane = [](float x, int i) {
+        return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, x), i));
+    };
+    for (int i = 0; i < pieces; i++) {
+        Lane x[kWaveRows];
+#pragma unroll
+        for (int r = 0; r < kWaveRows; r++) x[r] = *reinterpret_cast<const Lane*>(a.partial + (i * stride + at[r]) * D + lane * V);
+#pragma unroll
+        for (int r = 0; r < kWaveRows; r++) sum[r] += x[r] * of_lane(own, r * kMaxPieces + i);
+    }
+#pragma unroll
+    for (int r = 0; r < kWaveRows; r++) {
+        if (first + r >= rows) break;
+        const float f = of_lane(inv, r * kMaxPieces);
+        uint16_t* out = a.out + static_cast<int64_t>(at[r]) * D + lane * V;
+        if constexpr (V == 4) {
+            *reinterpret_cast<uint2*>(out) = make_uint2(pack_bf16(sum[r][0] * f, sum[r][1] * f), pack_bf16(sum[r][2] * f, sum[r][3] * f));
+        } else if constexpr (V == 2) {
+            *reinterpret_cast<uint32_t*>(out) = pack_bf16(sum[r][0] * f, sum[r][1] * f);
+        } else {
+            *out = __builtin_bit_cast(uint16_t, static_cast<__bf16>(sum[r][0] * f));
+        }
     }
 }
 
@@ -461,9 +476,9 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t items = row_tiles * c->kv_heads * b->seqs;
     const int64_t most = (longest + tokens - 1) / tokens;  // tiles of the last row tile
     if (items >= 2 * kCus) return {row_tiles, 1, items};
-    const int64_t mean = std::max<int64_t>(1, (longest - std::min<int64_t>(b->max_count, longest) / 2 + tokens - 1) / tokens);
-    const int64_t each = std::max<int64_t>(kLeast, (items * mean + kCus - 1) / kCus);
-    const int64_t pieces = std::min<int64_t>(kMaxPieces, (most + each - 1) / each);
+    // how many pieces come of it is known on the device alone: room for as many as the partial results may take
+    const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
+    const int64_t pieces = std::max<int64_t>(1, std::min({int64_t{kMaxPieces}, (most + kLeast - 1) / kLeast, room}));
     // the pieces of n tiles are less than n / each + 1, those of all (row tile, kv head)s less than kCus + items
     return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus)};
 }
@@ -497,7 +512,7 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
         else
             k_attend_rows<T, D, false><<<grid, kThreads, 0, stream>>>(a);
         if (const int rc = launch_status()) return rc;
-        if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeRows * 64, 0, stream>>>(a);
+        if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeWaves * 64, 0, stream>>>(a);
         return launch_status();
     };
     auto with_dim = [&](auto type) {
