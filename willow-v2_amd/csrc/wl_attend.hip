@@ -422,7 +422,10 @@ bool is_few(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
 FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length) {
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
     const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
-    if (longest <= kTile * kFewWaves) return {items, true};
+    // two rounds of a workgroup cost what one and the join do: 300 tokens of 8 sequences of 8 kv heads of 128 8.3 against 10.4
+    // us, 500 tokens of 64 sequences of 2 heads of 256 16.0 against 17.8, of one sequence 14.5 against 13.5; three (700
+    // tokens, one sequence) 18.5 against 13.4
+    if (longest <= kTile * kFewWaves * 2) return {items, true};
     // no more shares than the bound says there can be: a workgroup without one still costs its start
     const int64_t each = (longest + kTile * kFewWaves - 1) / (kTile * kFewWaves);
     return {std::min<int64_t>(kFewGroups, items * each), false};

@@ -35,11 +35,14 @@ struct RowsArgs : AttendArgs {
     int32_t pieces;      // a row tile's cache is cut into at most this many
 };
 
-// What a part of 16 tokens needs beside its bytes.
+// What a part of 16 tokens needs beside its bytes. V's scale goes into the exponent, so that a weight comes out of its exp2
+// with the scale on it and the sum of the weights takes it off once for all 16: a multiplication less for each weight. Not so
+// a scale that would push the weights out of fp32's range on the way (or is 0 or NaN): `rest` is that scale, and else 1.
 struct Part {
-    float ks, vs;  // scales (K's with the softmax's scale and log2 e)
-    int count;     // tokens that are there
-    int unused;
+    float ks;       // K's scale with the softmax's scale and log2 e
+    float log2_vs;  // log2 of what V's scale puts into the exponent
+    float inverse;  // 1 / that
+    float rest;
 };
 
 template <int D>
@@ -60,6 +63,7 @@ struct Lds {
     uint4 k[kRing][Shape<D>::kSubs * Shape<D>::kSteps][64];
     uint4 v[kRing][Shape<D>::kBlocks * Shape<D>::kSubs * 2][64];
     Part part[kRing][Shape<D>::kParts];
+    int count[kRing][Shape<D>::kParts];  // tokens that are there
 };
 
 // One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V. PAGE: a page holds
@@ -131,7 +135,10 @@ struct Stage {
         if (threadIdx.x < S::kParts) {
             // never 0: a masked score is -inf, and times the scale it has to stay that (a block of zeros scores 0 all the same)
             const float scaled = ks * a.scale_log2;
-            lds.part[buffer][threadIdx.x] = {scaled == 0.0f ? 1.17549435e-38f : scaled, vs, n, 0};
+            const bool fold = vs >= 8.6736174e-19f && vs <= 1.1529215e18f;  // 2^-60 .. 2^60
+            lds.part[buffer][threadIdx.x] = {scaled == 0.0f ? 1.17549435e-38f : scaled, fold ? __builtin_amdgcn_logf(vs) : 0.0f,
+                                             fold ? 1.0f / vs : 1.0f, fold ? 1.0f : vs};
+            lds.count[buffer][threadIdx.x] = n;
         }
     }
 };
@@ -157,7 +164,8 @@ struct Wave {
     __device__ __forceinline__ void add(const Lds<D>& lds, int buffer, int u, int seen) {
         constexpr int kAhead = D == 256 ? 2 : 4;  // no registers for more with 256 dimensions
         int lane = threadIdx.x & 63;
-        __asm__ volatile("" : "+v"(lane));  // its slots are worked out for every tile: kept, they would cost five registers
+        // with 256 dimensions its slots are worked out for every tile: kept, they would cost five registers
+        if constexpr (D == 256) __asm__ volatile("" : "+v"(lane));
         const int half = lane >> 5;
         const uint4(*kt)[64] = &lds.k[buffer][u * S::kSteps];
         f32x16 s = (f32x16)(0.0f);
@@ -165,16 +173,18 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) f[i] = kt[i][lane ^ S::k_swizzle(i)];
         __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
 #pragma unroll
         for (int i = 0; i < S::kSteps; i++) {
             s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, f[i % kAhead]), q[i], s, 0, 0, 0);
             if (i + kAhead < S::kSteps) f[i % kAhead] = kt[i + kAhead][lane ^ S::k_swizzle(i + kAhead)];
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
         const Part part = lds.part[buffer][2 * u + half];
-        const int mine = min(part.count, seen);
+        const int mine = min(lds.count[buffer][2 * u + half], seen);
         // a lane that sees no token of its block is not to meet the block's scales: they may be NaN
-        const float ks = mine > 0 ? part.ks : 1.0f, vs = mine > 0 ? part.vs : 0.0f;
+        const float ks = mine > 0 ? part.ks : 1.0f, rest = mine > 0 ? part.rest : 1.0f;
         const int slot = lane ^ S::v_swizzle(2 * u + half);
         auto v = [&](int i) { return lds.v[buffer][(i / 2 * S::kSubs + u) * 2 + i % 2][slot]; };
 #pragma unroll
@@ -195,14 +205,22 @@ struct Wave {
 #pragma unroll
             for (int i = 0; i < S::kBlocks; i++) o[i] *= shrink;
         }
-        const float safe = m == -__builtin_inff() ? 0.0f : m;
+        const float shift = part.log2_vs - (m == -__builtin_inff() ? 0.0f : m);
+        float sum = 0.0f;
         uint32_t p[8];
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            const float e0 = exp2_fast(__builtin_fmaf(s[2 * i], ks, -safe)), e1 = exp2_fast(__builtin_fmaf(s[2 * i + 1], ks, -safe));
-            l += e0 + e1;
-            p[i] = pack_bf16(e0 * vs, e1 * vs);
+            const float e0 = exp2_fast(__builtin_fmaf(s[2 * i], ks, shift)), e1 = exp2_fast(__builtin_fmaf(s[2 * i + 1], ks, shift));
+            sum += e0 + e1;
+            p[i] = pack_bf16(e0, e1);
         }
+        l = __builtin_fmaf(sum, part.inverse, l);
+        if (__any(rest != 1.0f)) {  // rounded once more, where a scale is as far out as that
+#pragma unroll
+            for (int i = 0; i < 8; i++)
+                p[i] = pack_bf16(__builtin_bit_cast(float, p[i] << 16) * rest, __builtin_bit_cast(float, p[i] & 0xFFFF0000u) * rest);
+        }
+        __builtin_amdgcn_s_setprio(1);
         const bf16x8 p0 = __builtin_bit_cast(bf16x8, make_uint4(p[0], p[1], p[2], p[3])),
                      p1 = __builtin_bit_cast(bf16x8, make_uint4(p[4], p[5], p[6], p[7]));
 #pragma unroll
@@ -212,6 +230,7 @@ struct Wave {
             if (i + kAhead < 2 * S::kBlocks) f[i % kAhead] = v(i + kAhead);
             __builtin_amdgcn_sched_barrier(0);
         }
+        __builtin_amdgcn_s_setprio(0);
     }
 };
 
