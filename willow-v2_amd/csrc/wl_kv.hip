@@ -86,7 +86,7 @@ __device__ __forceinline__ uint32_t top_of(uint32_t two, uint32_t top) {
 // thread keeps what it read in the first one (all of it, up to 16384 new values). K's bytes lie as the rows do, 16 values of
 // a token to a thread. V's lie with the tokens innermost: a thread takes two neighbouring values of 16 tokens, its loads run
 // along the rows over the lanes, and it writes 16 bytes for each value; where those 16 tokens are not all new, the bytes
-// there are read first. Bound by latency: a prompt has one such workgroup for each CU or two, a step's single tokens less.
+// there are read with them. Bound by latency: a prompt has one such workgroup for each CU or two, a step's single tokens less.
 template <int TYPE, int D, bool WIDE>
 __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs s, const int32_t* __restrict__ start,
                                                               const uint16_t* __restrict__ kx, int64_t k_ts, int64_t k_hs,
@@ -140,11 +140,20 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
         }
     };
 
+    // what stands in V's bytes where a unit's 16 tokens are not all new
+    auto read_old = [&](int i, uint4 (&w)[2]) {
+        const int t0 = (g_new + i / (D / 2)) * 16, d = i % (D / 2) * 2;
+        if (t0 >= held && t0 + 16 <= stop) return;
+#pragma unroll
+        for (int e = 0; e < 2; e++) w[e] = *reinterpret_cast<const uint4*>(out + (d + e) * P + t0);
+    };
+
     // the largest magnitude, as bits (bf16 magnitudes order as their bits do; infinities and NaN come out largest)
     constexpr int kKeepK = 4, kKeepV = 2;
     uint32_t top = 0, kept[32];
     uint32_t(&kk)[kKeepK][8] = reinterpret_cast<uint32_t(&)[kKeepK][8]>(kept);
     uint32_t(&vv)[kKeepV][16] = reinterpret_cast<uint32_t(&)[kKeepV][16]>(kept);
+    uint4 was[kKeepV][2] = {};
     if (!is_v) {
 #pragma unroll
         for (int r = 0; r < kKeepK; r++) {
@@ -166,7 +175,10 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
 #pragma unroll
         for (int r = 0; r < kKeepV; r++) {
             const int i = threadIdx.x + r * kAppendThreads;
-            if (i < v_units) read_v(i, vv[r]);
+            if (i < v_units) {
+                read_v(i, vv[r]);
+                read_old(i, was[r]);
+            }
         }
 #pragma unroll
         for (int r = 0; r < kKeepV; r++)
@@ -218,7 +230,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
                 reinterpret_cast<uint32_t*>(out)[i] = older4(reinterpret_cast<uint32_t*>(out)[i]);
         return;
     }
-    auto write_v = [&](int i, const uint32_t (&w)[16]) {
+    auto write_v = [&](int i, const uint32_t (&w)[16], const uint4 (&before)[2]) {
         const int t0 = (g_new + i / (D / 2)) * 16, d = i % (D / 2) * 2;
         const bool mixed = t0 < held || t0 + 16 > stop;
 #pragma unroll
@@ -230,8 +242,7 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
                 y[j] = quantize(w[4 * j] >> (16 * e) & 0xFFFFu) | quantize(w[4 * j + 1] >> (16 * e) & 0xFFFFu) << 8 |
                        quantize(w[4 * j + 2] >> (16 * e) & 0xFFFFu) << 16 | quantize(w[4 * j + 3] >> (16 * e) & 0xFFFFu) << 24;
             if (mixed) {
-                const uint4 was = *to;
-                const uint32_t o[4] = {was.x, was.y, was.z, was.w};
+                const uint32_t o[4] = {before[e].x, before[e].y, before[e].z, before[e].w};
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     // bytes of this word below `held` are older, those from `stop` on nobody's
@@ -245,12 +256,14 @@ __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs 
 #pragma unroll
     for (int r = 0; r < kKeepV; r++) {
         const int i = threadIdx.x + r * kAppendThreads;
-        if (i < v_units) write_v(i, vv[r]);
+        if (i < v_units) write_v(i, vv[r], was[r]);
     }
     for (int i = threadIdx.x + kKeepV * kAppendThreads; i < v_units; i += kAppendThreads) {
         uint32_t w[16];
+        uint4 before[2] = {};
         read_v(i, w);
-        write_v(i, w);
+        read_old(i, before);
+        write_v(i, w, before);
     }
     if (shrink)  // the groups of 16 tokens before the first that changes
         for (int i = threadIdx.x; i < D * g_new * 4; i += kAppendThreads) {
