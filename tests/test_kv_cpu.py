@@ -307,3 +307,24 @@ def test_oracle_rounding():
     assert torch.equal(kv_ref.nearest(x, torch.float8_e4m3fn), x.to(torch.float32).to(torch.float8_e4m3fn).double())
     tiny = torch.linspace(-0.03, 0.03, 30001, dtype=torch.float64)
     assert torch.equal(kv_ref.nearest(tiny, torch.float8_e4m3fn), tiny.to(torch.float32).to(torch.float8_e4m3fn).double())
+
+
+def test_table_rows_lie_apart(monkeypatch):
+    """A table whose rows overlap in memory (an expanded one) is refused: the kernels step from row to row by at least its
+    width. Of one sequence the stride between rows means nothing."""
+    z = torch.zeros
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    k, q = z(3, 2, 64, dtype=torch.bfloat16), z(3, 4, 64, dtype=torch.bfloat16)
+    strides = []
+    monkeypatch.setattr("gguf.hip.kv._launch", lambda index, call, *args: strides.extend(
+        a.table_stride for a in args if isinstance(a, hip.WlKvBatch)))
+    i = dict(dtype=torch.int32)
+    for table in (z(1, 2, **i).expand(3, 2), z(4, **i).as_strided((3, 2), (1, 1)), z(1, 1, **i).expand(3, 1)):
+        with pytest.raises(ValueError, match="apart"):
+            hip.kv_append(p, 0, k, k, table, z(3, **i), z(4, **i))
+        with pytest.raises(ValueError, match="apart"):
+            hip.kv_attend(p, 0, q, table, z(3, **i), z(4, **i))
+    assert not strides
+    for table, want in ((z(3, 2, **i), 2), (z(3, 5, **i)[:, :2], 5), (z(5, **i)[:2][None], 2), (z(3, 1, **i), 1)):
+        hip.kv_append(p, 0, k, k, table, z(len(table), **i), z(len(table) + 1, **i))
+        assert strides.pop() == want

@@ -110,11 +110,11 @@ def _batch(pages, table, cu, per_seq, name, tokens, max_count):
         if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1
                 and t.shape[0] == n and t.is_contiguous()):
             _refuse(t, what, pages.device, torch.int32, f"[{n}] (table has {seqs} sequences), contiguous")
-    if step != 1 and width > 1:
-        raise ValueError("the rows of table must be contiguous")
+    if (step != 1 and width > 1) or (seqs > 1 and row < width):
+        raise ValueError("the rows of table must be contiguous, and lie apart (not expanded)")
     if max_count is None or max_count > tokens:
         max_count = tokens
-    return WlKvBatch(table.data_ptr(), cu.data_ptr(), row if seqs > 1 and row > width else max(row, width), tokens, seqs, width,
+    return WlKvBatch(table.data_ptr(), cu.data_ptr(), max(row, width), tokens, seqs, width,
                      max_count, 0)
 
 
