@@ -328,3 +328,22 @@ def test_table_rows_lie_apart(monkeypatch):
     for table, want in ((z(3, 2, **i), 2), (z(3, 5, **i)[:, :2], 5), (z(5, **i)[:2][None], 2), (z(3, 1, **i), 1)):
         hip.kv_append(p, 0, k, k, table, z(len(table), **i), z(len(table) + 1, **i))
         assert strides.pop() == want
+
+
+def test_cpu_tensors_are_not_launched(monkeypatch):
+    """Calls that are right but for their device, on a machine that may well have a GPU: an error, and no kernel."""
+    z = torch.zeros
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    k, q, i = z(3, 2, 64, dtype=torch.bfloat16), z(3, 4, 64, dtype=torch.bfloat16), dict(dtype=torch.int32)
+
+    class Calls:
+        wl_kv_append = wl_kv_attend = wl_kv_copy = staticmethod(lambda *args: pytest.fail("reached the library"))
+        wl_kv_attend_workspace_bytes = staticmethod(lambda *args: 0)
+
+    monkeypatch.setattr("gguf.hip.kv.library", lambda: Calls)
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: -1, raising=False)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: 0, raising=False)
+    for call in (lambda: hip.kv_append(p, 0, k, k, z(1, 2, **i), z(1, **i), z(2, **i)),
+                 lambda: hip.kv_attend(p, 0, q, z(1, 2, **i), z(1, **i), z(2, **i)), lambda: hip.kv_copy(p, [0], [1])):
+        with pytest.raises(ValueError, match="GPU"):
+            call()

@@ -19,6 +19,8 @@ TYPES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
 def _launch(index, call, *args):
     """call(*args, stream) with device `index` current (a launch goes to the current device) and its current stream."""
+    if index < 0:
+        raise ValueError("the tensors must be on the GPU (got tensors on the CPU)")
     if index == torch._C._cuda_getDevice():
         rc = call(*args, torch._C._cuda_getCurrentRawStream(index))
     else:
