@@ -347,3 +347,24 @@ def test_cpu_tensors_are_not_launched(monkeypatch):
                  lambda: hip.kv_attend(p, 0, q, z(1, 2, **i), z(1, **i), z(2, **i)), lambda: hip.kv_copy(p, [0], [1])):
         with pytest.raises(ValueError, match="GPU"):
             call()
+
+
+def test_copied_pages_stay_the_pages_named(monkeypatch):
+    """Page numbers are cut to 32 bits for the library: none may become another one on the way."""
+    import numpy as np
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    got = []
+    monkeypatch.setattr("gguf.hip.kv._launch", lambda index, call, pages, src, dst, n: got.extend(
+        (ctypes.c_int32 * n).from_address(a)[:] for a in (src, dst)))
+    for bad in (np.array([2 ** 32 + 1]), np.array([2 ** 31], dtype=np.uint32), [-1], [1.5], [True], [2 ** 70], np.array([-2 ** 32])):
+        with pytest.raises(ValueError):
+            hip.kv_copy(p, bad, [2])
+        with pytest.raises(ValueError):
+            hip.kv_copy(p, [2], bad)
+    hip.kv_copy(p, [], [])
+    assert not got
+    for kind in (list, np.array, lambda x: np.array(x, dtype=np.int32), lambda x: np.array(x, dtype=np.uint8),
+                 lambda x: np.array([v for n in x for v in (n, 9)], dtype=np.int32)[::2]):
+        hip.kv_copy(p, kind([0, 1]), kind([2, 3]))
+        assert got == [[0, 1], [2, 3]]
+        got.clear()

@@ -179,11 +179,21 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     return out
 
 
+def _page_numbers(x, name):
+    """x as int32, unless a number would become another one by that."""
+    a = np.asarray(x)
+    if a.dtype != np.int32:
+        if a.size and (a.dtype.kind not in "iu" or int(a.min()) < 0 or int(a.max()) >= 2 ** 31):
+            raise ValueError(f"{name} must be page numbers")
+        a = a.astype(np.int32)
+    return np.ascontiguousarray(a)
+
+
 def kv_copy(pages: KVPages, src, dst):
     """Copies pages src[i] -> dst[i] of every layer, bytes and scales. src, dst: page numbers on the host (lists or integer
     arrays); they travel in the kernels' arguments, so nothing is uploaded. Refused (ValueError): a page out of range, one
     written twice, one both read and written."""
-    src, dst = (np.ascontiguousarray(x, dtype=np.int32) for x in (src, dst))
+    src, dst = _page_numbers(src, "src"), _page_numbers(dst, "dst")
     if src.ndim != 1 or src.shape != dst.shape:
         raise ValueError(f"src and dst must be lists of the same length (got {list(src.shape)} and {list(dst.shape)})")
     if src.shape[0] == 0:
