@@ -8,7 +8,7 @@ import torch
 
 from engines.qwen36 import Rotary
 from gguf import hip
-from gguf.hbm_cache import OutOfPages, PageBook
+from gguf.hbm_cache import HBMKVCache, OutOfPages, PageBook
 from oracle import kv_ref
 
 FAKE = 0x10000  # a non-NULL, aligned address that is never dereferenced
@@ -368,3 +368,22 @@ def test_copied_pages_stay_the_pages_named(monkeypatch):
         hip.kv_copy(p, kind([0, 1]), kind([2, 3]))
         assert got == [[0, 1], [2, 3]]
         got.clear()
+
+
+def test_step_needs_all_its_rows(monkeypatch):
+    cache = HBMKVCache(1, 4, 2, 64, 16, device="cpu")
+    step = cache.step([cache.new(), cache.new()], [3, 2])
+    calls = []
+    monkeypatch.setattr("gguf.hbm_cache.kv_append", lambda *args, **kw: calls.append("append"))
+    monkeypatch.setattr("gguf.hbm_cache.kv_attend", lambda *args, **kw: calls.append("attend"))
+    k = torch.zeros(7, 2, 64, dtype=torch.bfloat16)
+    for rows in (0, 4):
+        with pytest.raises(ValueError, match="5 tokens"):
+            cache.append(0, step, k[:rows], k[:rows])
+        with pytest.raises(ValueError, match="5 tokens"):
+            cache.attend(0, step, k[:rows])
+    assert not calls
+    for rows in (5, 7):  # all of them, and a padded batch
+        cache.append(0, step, k[:rows], k[:rows])
+        cache.attend(0, step, k[:rows])
+    assert calls == ["append", "attend"] * 2

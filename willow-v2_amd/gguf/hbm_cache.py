@@ -143,6 +143,12 @@ class KVStep:
     counts: list
     max_count: int
     max_length: int
+    tokens: int           # of all sequences; a call's rows are these, and any padding behind them
+
+    def check(self, rows: torch.Tensor, name: str):
+        """The book counts the step's tokens as written: fewer rows than those would leave some of them unwritten."""
+        if rows.shape[0] < self.tokens:
+            raise ValueError(f"{name} has {rows.shape[0]} rows, the step {self.tokens} tokens")
 
 
 class HBMKVCache:
@@ -208,7 +214,7 @@ class HBMKVCache:
         host, start, length, cu = self._host_step(list(seqs), [int(c) for c in counts], width)
         up = [torch.from_numpy(a).to(self.device) for a in (host, start, length, cu)]
         return KVStep(*up, [int(c) for c in counts], max(int(c) for c in counts),
-                      int(length.max()) if width is None else width * self.book.page_tokens)
+                      int(length.max()) if width is None else width * self.book.page_tokens, int(cu[-1]))
 
     def _check_width(self, seqs, counts, width):
         for s, c in zip(seqs, counts):
@@ -230,10 +236,12 @@ class HBMKVCache:
 
     def append(self, layer: int, step: KVStep, k: torch.Tensor, v: torch.Tensor):
         """The step's new keys and values of one layer, bf16 [tokens, kv_heads, head_dim]; kv_append."""
+        step.check(k, "k")
         kv_append(self.pages, layer, k, v, step.table, step.start, step.cu, max_count=step.max_count or 1)
 
     def attend(self, layer: int, step: KVStep, q: torch.Tensor, scale: float = None, causal: bool = True,
                out: torch.Tensor = None) -> torch.Tensor:
         """The step's rows' attention over one layer of their sequences, bf16 [tokens, heads, head_dim]; kv_attend."""
+        step.check(q, "q")
         return kv_attend(self.pages, layer, q, step.table, step.length, step.cu, max_count=step.max_count or 1,
                          max_length=step.max_length, scale=scale, causal=causal, out=out)
