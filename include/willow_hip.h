@@ -288,7 +288,8 @@ typedef struct WlKvCache {
 /* The sequences of one call. Their tokens lie packed in rows [cu[b], cu[b + 1]) of the call's arrays, of which `tokens`
  * rows exist; rows behind cu[seqs] are neither read nor written. Page numbers are read on the device: an entry outside
  * [0, pages) stands for a page that is not there (its tokens are not written, and attended by nobody), as does a
- * position behind table_width pages. cu is taken as if cut to [0, tokens], and a sequence's rows to max_count. */
+ * position behind table_width pages. cu is taken as if cut to [0, tokens], and a sequence's rows to max_count (the rest
+ * count as if they were not there). cu must not decrease: a row may belong to one sequence only. */
 typedef struct WlKvBatch {
     const int32_t* table; /* [seqs][table_width] page numbers, rows table_stride entries apart */
     const int32_t* cu;    /* [seqs + 1] */
@@ -324,7 +325,9 @@ size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const W
  * length[b] - n + i. out = sum_j softmax_j(scale * q . k_j) v_j over the positions j < length[b] and, with causal != 0,
  * j <= the row's own position; a row that sees no token is 0. Softmax statistics and sums are fp32; the weights are rounded
  * to bf16 for the matrix core, which adds up in fp32.
- * scale: finite, not negative. max_length: a bound of length[], from which the work's split is chosen (results hold whatever it says).
+ * scale: finite (times log2 e too), not negative; the cache's scales: not negative (a NaN one reaches the rows that see its
+ * block). out may not overlap q. max_length: a bound of length[], from which the work's split is chosen (results
+ * hold whatever it says). workspace: what it holds before does not matter; calls that may overlap need one each.
  * No counterpart in the reference, whose attention reads a bf16 cache (engines/base.py:348-366). */
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                  int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,
@@ -335,7 +338,8 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
 int wl_kv_copy(const WlKvCache* cache, const int32_t* src_host, const int32_t* dst_host, int64_t n, void* stream);
 
 #define WL_MAX_ROPE_AXES 4
-/* One tensor to rotate: [tokens][heads][head_dim], element strides given (head_dim contiguous). out may be in. */
+/* One tensor to rotate: [tokens][heads][head_dim], element strides given (head_dim contiguous). out may be in, with the
+ * same strides; memory that overlaps otherwise may be overwritten before it is read. */
 typedef struct WlRopeTensor {
     const void* in;
     void* out;

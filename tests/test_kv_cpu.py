@@ -387,3 +387,28 @@ def test_step_needs_all_its_rows(monkeypatch):
         cache.append(0, step, k[:rows], k[:rows])
         cache.attend(0, step, k[:rows])
     assert calls == ["append", "attend"] * 2
+
+
+def test_launch_limits():
+    """Sizes that no launch holds are refused before one is made (2^32 threads along an axis)."""
+    lib = hip.library()
+    c = cache_struct()
+    huge = dict(tokens=2 ** 31 - 1, max_count=2 ** 31 - 1)
+    assert calls(c, batch_struct(**huge)) == [-2, -2]
+    tensor = ctypes.byref(hip.WlRopeTensor(FAKE, FAKE, 256, 64, 256, 64, 4, 0))
+    sections = (ctypes.c_int32 * 1)(16)
+    assert lib.wl_rope(tensor, None, 1, 2 ** 24, 64, 32, FAKE, 4, FAKE, 1, sections, 1, 1.0, None) == -2
+    wide = cache_struct(kv_heads=256)
+    many = batch_struct(seqs=65535)
+    assert lib.wl_kv_attend(ctypes.byref(wide), 0, FAKE, 256, 64, 256, ctypes.byref(many), FAKE, 64, 0.125, 1, FAKE, None, 0, None) == -2
+    long = batch_struct(seqs=65535, tokens=2 ** 26, max_count=2 ** 26)  # of the form for many rows
+    assert lib.wl_kv_attend(ctypes.byref(c), 0, FAKE, 256, 64, 4, ctypes.byref(long), FAKE, 64, 0.125, 1, FAKE, FAKE, 2 ** 40, None) == -2
+    # a scale that times log2 e is infinite
+    assert lib.wl_kv_attend(ctypes.byref(c), 0, FAKE, 256, 64, 4, ctypes.byref(batch_struct()), FAKE, 64, 3e38, 1, FAKE, None, 0, None) == -2
+
+
+def test_out_is_not_q():
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    q, i = torch.zeros(3, 4, 64, dtype=torch.bfloat16), dict(dtype=torch.int32)
+    with pytest.raises(ValueError, match="not q's memory"):
+        hip.kv_attend(p, 0, q, torch.zeros(1, 2, **i), torch.zeros(1, **i), torch.zeros(2, **i), out=q)

@@ -449,7 +449,8 @@ int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, in
     // positions fit 31 bits, and so do the tiles of all sequences and kv heads together
     const int64_t positions = int64_t{batch->table_width} * cache->page_tokens;
     if (positions >= (int64_t{1} << 31) || (positions + kTile) / kTile * batch->seqs * cache->kv_heads >= (int64_t{1} << 31) ||
-        static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 30))
+        static_cast<int64_t>(batch->max_count) * (q_heads / cache->kv_heads) >= (int64_t{1} << 30) ||
+        !fits_a_launch(int64_t{batch->seqs} * cache->kv_heads, kJoinWaves * 64))
         return WL_EINVAL_SHAPE;
     return WL_OK;
 }
@@ -472,7 +473,8 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
                  uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_attend(cache, q_heads, batch, max_length)) return rc;
     if (!q || !length || !out) return WL_EINVAL_NULL;
-    if (layer < 0 || layer >= cache->layers || !(scale >= 0.0f && scale < __builtin_inff())) return WL_EINVAL_SHAPE;
+    const float scale_log2 = scale * 1.44269504088896340736f;
+    if (layer < 0 || layer >= cache->layers || !(scale >= 0.0f && scale_log2 < __builtin_inff())) return WL_EINVAL_SHAPE;
     const auto qb = reinterpret_cast<uintptr_t>(q);
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
     const size_t need = wl_kv_attend_workspace_bytes(cache, q_heads, batch, max_length);
@@ -487,7 +489,7 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.out = out;
     a.q_heads = q_heads;
     a.group = q_heads / cache->kv_heads;
-    a.scale_log2 = scale * 1.44269504088896340736f;
+    a.scale_log2 = scale_log2;
     a.causal = causal != 0;
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -493,7 +493,8 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t tokens = 8192 / c->head_dim, group = q_heads / c->kv_heads;
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
     const int64_t row_tiles = (b->max_count * group + kGroupRows - 1) / kGroupRows;
-    const int64_t items = row_tiles * c->kv_heads * b->seqs;
+    // (row tile, kv head)s: as many as the sequences' most rows have room for, and no more than all rows together fill
+    const int64_t items = std::min(row_tiles * b->seqs, b->tokens * group / kGroupRows + b->seqs) * c->kv_heads;
     const int64_t most = (longest + tokens - 1) / tokens;  // tiles of the last row tile
     if (items >= 2 * kCus) return {row_tiles, 1, items};
     // how many pieces come of it is known on the device alone: room for as many as the partial results may take
@@ -522,7 +523,9 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     a.row_tiles = static_cast<int32_t>(p.row_tiles);
     a.pieces = static_cast<int32_t>(p.pieces);
     const int64_t merges = (b->max_count * static_cast<int64_t>(call.group) + kMergeRows - 1) / kMergeRows * c->kv_heads;
-    if (p.groups >= (int64_t{1} << 31) || merges >= (int64_t{1} << 31)) return WL_EINVAL_SHAPE;
+    if (p.row_tiles * b->seqs >= (int64_t{1} << 31) || !fits_a_launch(p.groups, kThreads) ||
+        !fits_a_launch(merges, kMergeWaves * 64))
+        return WL_EINVAL_SHAPE;
     const dim3 grid(static_cast<uint32_t>(p.groups));
     const dim3 merge(static_cast<uint32_t>(merges), b->seqs);
     auto run = [&](auto type, auto dim) {

@@ -6,6 +6,8 @@
 namespace wl {
 
 constexpr int64_t kMaxTokens = int64_t{1} << 31;
+// A launch has less than 2^32 threads along its first axis.
+inline bool fits_a_launch(int64_t groups, int threads) { return groups < (int64_t{1} << 32) / threads; }
 
 inline int check_cache(const WlKvCache* c) {
     if (!c || !c->k || !c->v || !c->k_scale || !c->v_scale) return WL_EINVAL_NULL;

@@ -352,7 +352,9 @@ int wl_kv_append(const WlKvCache* cache, int layer, const uint16_t* k, int64_t k
                       v_token_stride % 8 == 0 && v_head_stride % 8 == 0;
     const int P = cache->page_tokens;
     // a sequence's rows touch at most this many pages: one more than fill, where they begin inside one
-    const dim3 grid((batch->max_count + P - 2) / P + 1, 2 * cache->kv_heads, batch->seqs);
+    const int64_t touched = (int64_t{batch->max_count} + P - 2) / P + 1;
+    if (!fits_a_launch(touched, kAppendThreads)) return WL_EINVAL_SHAPE;
+    const dim3 grid(static_cast<uint32_t>(touched), 2 * cache->kv_heads, batch->seqs);
     const KvLayer c = layer_of(cache, layer);
     const KvSeqs s = seqs_of(batch);
     const hipStream_t st = static_cast<hipStream_t>(stream);

@@ -153,7 +153,7 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
     if (const int rc = check_rope_tensor(q, size)) return rc;
     if (k)
         if (const int rc = check_rope_tensor(k, size)) return rc;
-    if (tokens < 1 || tokens >= (int64_t{1} << 31) || head_dim < 2 || head_dim > 1024 || rotary_dim < 2 ||
+    if (tokens < 1 || tokens >= (int64_t{1} << 32) / kRopeThreads || head_dim < 2 || head_dim > 1024 || rotary_dim < 2 ||
         rotary_dim > head_dim || rotary_dim % 2 || axes < 1 || axes > WL_MAX_ROPE_AXES)
         return WL_EINVAL_SHAPE;
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return WL_EINVAL_ALIGN;

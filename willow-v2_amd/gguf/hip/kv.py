@@ -146,18 +146,20 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     """Grouped-query attention of one layer: q bf16 [tokens, q_heads, head_dim] (any strides over tokens and heads) -> bf16
     [tokens, q_heads, head_dim]. Sequence b's rows are cu[b] .. cu[b + 1], the last of its length[b] tokens in the cache (so
     append them first); query head i reads kv head i / (q_heads / kv_heads). causal: a row sees the positions up to its own;
-    otherwise all length[b]. A row that sees none is 0. scale defaults to head_dim ** -0.5. max_count: the most rows any
-    sequence has (rows beyond it are not computed; default: all rows); max_length: a bound of length that only steers how the
-    work is split (default: what the table's width holds). Rows behind cu[-1] of `out` stay as they are. workspace: a uint8
-    tensor of kv_attend_workspace bytes; by default it comes from torch's allocator, for this call and stream."""
+    otherwise all length[b]. A row that sees none is 0. scale (finite, not negative) defaults to head_dim ** -0.5. max_count: the
+    most rows any sequence has (rows beyond it count as if they were not there; default: all rows, which costs calls of short
+    sequences the form that is made for them); cu must not decrease; max_length: a bound of length that only steers how the
+    work is split (default: what the table's width holds). Rows behind cu[-1] of `out` (which may not overlap q) stay as they are.
+    workspace: a uint8 tensor that is large enough (wl_kv_attend_workspace_bytes), for calls that do not overlap in time; by
+    default it comes from torch's allocator, for this call and stream."""
     n, heads, token_stride, head_stride = _rows(q, "q", pages.index, torch.bfloat16, None, pages.head_dim)
     if heads == 0 or heads % pages.kv_heads:
         raise ValueError(f"{heads} query heads over {pages.kv_heads} kv heads")
     if out is None:
         out = torch.empty_like(q, memory_format=torch.contiguous_format)
     elif not (isinstance(out, torch.Tensor) and out.dtype is torch.bfloat16 and out.get_device() == pages.index
-              and out.shape == q.shape and out.is_contiguous()):
-        _refuse(out, "out", pages.device, torch.bfloat16, f"{list(q.shape)}, contiguous,")
+              and out.shape == q.shape and out.is_contiguous() and out.data_ptr() != q.data_ptr()):
+        _refuse(out, "out", pages.device, torch.bfloat16, f"{list(q.shape)}, contiguous and not q's memory,")
     b = _batch(pages, table, cu, length, "length", n, max_count)
     if n == 0 or b.seqs == 0:
         return out
@@ -218,7 +220,7 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
          interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions with several axes: q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (or None), both bf16
     or both fp32 (any strides over tokens and heads), rotated into new tensors (or into `out`, a (q, k) pair, which may be
-    q and k themselves) -> (q, k). positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2],
+    q and k themselves, but not overlap them otherwise) -> (q, k). positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2],
     the angle of one position step; sections[i] of its frequencies belong to axis i, interleaved (axis i > 0 has the
     frequencies i, i + axes, i + 2 axes, ..; axis 0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2)
     turn by positions[axis(j)] * inv_freq[j], taken in 64 bits; cosine and sine are multiplied by `scale`; the rest of each head
