@@ -73,9 +73,9 @@ def append(pool, scale, new, table, start, cu, page_tokens, v=False, max_count=N
     return (out.transpose(2, 3) if v else out), sc
 
 
-def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True, max_count=None):
+def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True, max_count=None, weight_roundings=1):
     """k, v, scales: one layer on the CPU. -> (out fp64 [tokens, heads, dim] with NaN in rows that belong to no sequence, the
-    bound of |error| of a bf16 result whose scores and sums are fp32 and whose weights are rounded to bf16)."""
+    bound of |error| of a bf16 result whose scores and sums are fp32 and whose weights are rounded to bf16, so many times)."""
     pages, kv_heads, page, dim = k.shape
     group = q.shape[1] // kv_heads
     scale = dim ** -0.5 if scale is None else scale
@@ -107,7 +107,7 @@ def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True
                 # a score: dim products added in fp32, then two multiplications; its exponential: 2 steps of the argument
                 slack = (dim + 4) * 2.0 ** -23 * float((Kk.abs() @ x.abs()).max()) * abs(scale) + 2.0 ** -21 * float(s.abs().max())
                 # a weight is rounded to bf16 (2^-8), the sums are fp32; the result is rounded once more
-                per = 2.0 ** -8 + 2 * slack + (len(keep) + 8) * 2.0 ** -23
+                per = weight_roundings * 2.0 ** -8 + 2 * slack + (len(keep) + 8) * 2.0 ** -23
                 tol[lo + i, h] = 2.0 ** -8 * o.abs() + per * (w @ Vk.abs())
     return out, tol
 

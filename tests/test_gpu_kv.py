@@ -160,6 +160,8 @@ def test_append_out_of_range(hip, counts, starts, cu, max_count):
 
 def check_attend(hip, pages, layer, q, table, length, cu, **kw):
     ref = {n: kw[n] for n in ("scale", "causal", "max_count") if n in kw}
+    if "weight_roundings" in kw:
+        ref["weight_roundings"] = kw.pop("weight_roundings")
     want, tol = kv_ref.attend(pages.k[layer].cpu(), pages.v[layer].cpu(), pages.k_scale[layer].cpu(), pages.v_scale[layer].cpu(),
                               q.cpu(), table.cpu(), length.cpu(), cu.cpu(), **ref)
     out = torch.full(q.shape, 7.0, dtype=torch.bfloat16, device=DEV)
@@ -285,6 +287,100 @@ def test_attend_long(hip, dim, count):
     table = table_of(g, (n,), 64, n // 64 + 2)
     q = (4 * torch.randn(count, 2, dim, generator=g)).to(torch.bfloat16).to(DEV)
     check_attend(hip, pages, 0, q, table, i32([n]), i32([0, count]))
+
+
+@pytest.mark.parametrize("count", [1, 24])
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_attend_scales_far_out(hip, count, dtype):
+    """V's scales from where weights still are normal bf16 values to where sums would leave fp32, zeros among them, K's of 0 and nearly: a sequence
+    of each, and one with a mixture, whose largest pages drown the others."""
+    g = gen(11)
+    v_scales = (2.0 ** -100, 1e-30, 2.0 ** -61, 2.0 ** -60, 2.0 ** -59, 2.0 ** 59, 2.0 ** 60, 2.0 ** 61, 1e25, 0.0)
+    n = len(v_scales)
+    pages = random_pages(hip, g, 1, 2 * n + 6, 2, 32, 128, dtype)
+    for i, s in enumerate(v_scales):
+        pages.v_scale[0, 2 * i:2 * i + 2] = s
+    for i, s in enumerate((1.0, 0.0, 1e-30, 2.0 ** -60, 1e25, 3.0)):
+        pages.v_scale[0, 2 * n + i] = s
+    pages.k_scale[0, 4:6], pages.k_scale[0, 8], pages.k_scale[0, 2 * n + 1] = 0.0, 0.0, 1e-38
+    table = torch.full((n + 1, 6), -1, dtype=torch.int32)
+    table[:n, :2] = torch.arange(2 * n).view(n, 2)
+    table[n] = torch.arange(2 * n, 2 * n + 6)
+    lengths = [61 - i for i in range(n)] + [190]
+    q = torch.randn((n + 1) * count, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+    # the form for many rows rounds weights twice where a scale is that far out
+    check_attend(hip, pages, 0, q, table.to(DEV), i32(lengths), cu_of([count] * (n + 1)), max_count=count,
+                 weight_roundings=1 if count == 1 else 2)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("max_count", [2, 30])
+def test_attend_rows_beyond_max_count(hip, causal, max_count):
+    """What an append with the same max_count has left: rows beyond it are not there for either."""
+    g = gen(12)
+    counts = (max_count + 3, 1, max_count + 40)
+    lengths = (200, 5, max_count + 1)
+    pages = random_pages(hip, g, 1, 12, 2, 32, 64, torch.int8)
+    table = table_of(g, lengths, 32, 12)
+    q = torch.randn(sum(counts), 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+    check_attend(hip, pages, 0, q, table, i32(lengths), cu_of(counts), max_count=max_count, causal=causal)
+
+
+@pytest.mark.parametrize("count", [2, 24])
+def test_attend_shared_pages(hip, count):
+    """Sequences on the same pages (forks), with other lengths."""
+    g = gen(13)
+    pages = random_pages(hip, g, 1, 12, 2, 32, 64, torch.float8_e4m3fn)
+    table = table_of(g, (300,), 32, 12).repeat(3, 1)
+    q = torch.randn(3 * count, 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+    check_attend(hip, pages, 0, q, table, i32((300, 299, 40)), cu_of([count] * 3), max_count=count)
+
+
+def test_attend_many_ragged_prompts(hip):
+    """The form for many rows over hundreds of sequences, some without rows, some without tokens; no bound of the rows given."""
+    g = gen(14)
+    rng = np.random.default_rng(14)
+    counts = [int(x) for x in rng.integers(0, 8, 300)]
+    counts[100], counts[299] = 150, 40
+    lengths = [c + int(x) for c, x in zip(counts, rng.integers(0, 60, 300))]
+    lengths[5] = 0
+    need = sum(-(-n // 16) for n in lengths)
+    pages = random_pages(hip, g, 1, need, 2, 16, 64, torch.int8)
+    table = table_of(g, lengths, 16, need)
+    q = torch.randn(sum(counts) + 3, 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+    check_attend(hip, pages, 0, q, table, i32(lengths), cu_of(counts))
+    check_attend(hip, pages, 0, q, table, i32(lengths), cu_of(counts), causal=False)
+
+
+@pytest.mark.parametrize("page,dim,total", [(64, 256, 140_000), (16, 128, 1_100_000)])
+def test_past_32_bits(hip, page, dim, total):
+    """Pages whose bytes lie more than 2^32 into the cache: the same bits as on a small cache that holds just them."""
+    g = gen(15)
+    assert total * 2 * page * dim > 2 ** 32
+    far = hip.KVPages(*(torch.empty(1, total, 2, *t, dtype=torch.int8, device=DEV) for t in ((page, dim), (dim, page))),
+                      *(torch.zeros(1, total, 2, device=DEV) for _ in range(2)))
+    ids = [total - 1, total - 2, 0, total - 1000, total // 2 + 1, total - 77, 5, total - 3]
+    small = hip.KVPages.empty(1, len(ids), 2, dim, page)
+    for t in (far.k, far.v):
+        t[:, ids] = 0
+    rows = 3 * page + 5
+    x = torch.randn(rows + 40, 2, 2, dim, generator=g).to(torch.bfloat16).to(DEV)
+    table = torch.tensor([[0, 1, 2, 3], [4, 5, 6, -1]], dtype=torch.int32)
+    numbers = torch.tensor(ids + [-1], dtype=torch.int32)
+    cu = cu_of((rows, 40))
+    outs = []
+    for pages, t in ((small, table.to(DEV)), (far, numbers[table.long()].to(DEV))):
+        hip.kv_append(pages, 0, x[:, 0], x[:, 1], t, i32([0, 3]), cu)
+        outs.append([hip.kv_attend(pages, 0, q, t, i32([rows, 43]), c, max_count=m) for q, c, m in (
+            (torch.randn(2, 8, dim, generator=gen(16)).to(torch.bfloat16).to(DEV), i32([0, 1, 2]), 1),
+            (torch.randn(60, 8, dim, generator=gen(17)).to(torch.bfloat16).to(DEV), i32([0, 35, 60]), 35))])
+    assert all(torch.equal(a, b) and torch.isfinite(a.float()).all() for a, b in zip(*outs))
+    hip.kv_copy(far, [ids[0], 5], [total // 3, ids[7]])
+    hip.kv_copy(small, [0, 6], [4, 7])
+    for name in ("k", "v", "k_scale", "v_scale"):
+        a, b = getattr(small, name)[0], getattr(far, name)[0]
+        for i, n in enumerate(ids[:4] + [total // 3] + ids[5:]):
+            assert torch.equal(a[i], b[n]), (name, i)
 
 
 # -- copy ------------------------------------------------------------------------------------------------------------

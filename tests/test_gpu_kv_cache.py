@@ -226,6 +226,38 @@ def test_streams_and_workspaces(hip):
             kv_attend(*args, max_count=1, workspace=bad)
 
 
+def test_two_prompt_graphs(hip):
+    """Two captured calls of many rows that leave partial results in workspaces of their own, replayed in turn with other
+    inputs and lengths, eager calls and synchronizations in between: the eager calls' bits every time."""
+    g = torch.Generator().manual_seed(12)
+    cache = HBMKVCache(1, 80, 2, 128, 64)
+    seqs = [cache.new(), cache.new()]
+    first = cache.step(seqs, [2500, 1300])
+    cache.append(0, first, bf16(g, 3800, 2, 128), bf16(g, 3800, 2, 128))
+    lengths = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ((2500, 1300), (900, 1100))]
+    cus = [torch.tensor(x, dtype=torch.int32, device=DEV) for x in ((0, 40, 60), (0, 5, 25))]
+    qs = [bf16(g, 60, 16, 128), bf16(g, 25, 16, 128)]
+
+    def call(i):
+        return kv_attend(cache.pages, 0, qs[i], first.table, lengths[i], cus[i], max_count=40, max_length=2500)
+    want = [call(i) for i in range(2)]
+    graphs, got = [torch.cuda.CUDAGraph() for _ in range(2)], []
+    for i in range(2):
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graphs[i]):
+            got.append(call(i))
+    for turn in range(6):
+        for i in (0, 1) if turn % 2 else (1, 0):
+            qs[i].copy_(bf16(g, *qs[i].shape))
+            lengths[i].sub_(turn * 31)
+            want[i] = call(i)
+            if turn % 3 == 0:
+                torch.cuda.synchronize()
+            graphs[i].replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), f"turn {turn}"
+
+
 class TinyEngine(HipAttention):
     prefix = "model."
 
