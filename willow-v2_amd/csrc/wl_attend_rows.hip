@@ -269,10 +269,25 @@ struct PlanLds {
 template <int D>
 __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work& work) {
     constexpr int T = Shape<D>::kTokens;
-    const uint32_t wanted = blockIdx.x / a.c.kv_heads, items = a.s.seqs * a.row_tiles;
+    const uint32_t wanted = blockIdx.x / a.c.kv_heads;
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    // max_count may say nothing (all rows of the call): where that makes for many empty row tiles, the longest sequence
+    // says how many there are (1000 sequences of 8 rows: 8.9 ms without, 0.45 ms with, 0.43 ms where max_count says it)
+    uint32_t row_tiles = a.row_tiles;
+    if (row_tiles > 1 && a.s.seqs * row_tiles > 2 * kThreads) {
+        int most = 1;
+        for (int b = threadIdx.x; b < a.s.seqs; b += kThreads) most = max(most, a.seq(b).n);
+#pragma unroll
+        for (int d = 32; d; d >>= 1) most = max(most, __shfl_xor(most, d));
+        if (lane == 0) lds.sums[wave] = most;
+        __syncthreads();
+        for (int i = 0; i < kWaves; i++) most = max(most, static_cast<int>(lds.sums[i]));
+        row_tiles = __builtin_amdgcn_readfirstlane((most * a.group + kGroupRows - 1) / kGroupRows);
+        __syncthreads();  // the maxima have been read
+    }
+    const uint32_t items = a.s.seqs * row_tiles;
     auto tiles_at = [&](uint32_t i) {
-        return i < items ? tiles_of(a, a.seq(i / a.row_tiles), static_cast<int>(i % a.row_tiles) * kGroupRows, T) : 0;
+        return i < items ? tiles_of(a, a.seq(i / row_tiles), static_cast<int>(i % row_tiles) * kGroupRows, T) : 0;
     };
     uint32_t total = 0;
     for (uint32_t i = threadIdx.x; i < items; i += kThreads) total += tiles_at(i);
@@ -311,7 +326,7 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
         }
         if (at <= rank && rank < at + n) {
             const int piece = rank - at;
-            lds.work = {static_cast<int>(i / a.row_tiles), static_cast<int>(i % a.row_tiles) * kGroupRows, piece, c.pieces,
+            lds.work = {static_cast<int>(i / row_tiles), static_cast<int>(i % row_tiles) * kGroupRows, piece, c.pieces,
                         min(piece * c.size, tiles), min((piece + 1) * c.size, tiles)};
         }
         if (before > rank) break;
