@@ -326,8 +326,9 @@ size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const W
  * j <= the row's own position; a row that sees no token is 0. Softmax statistics and sums are fp32; the weights are rounded
  * to bf16 for the matrix core, which adds up in fp32.
  * scale: finite (times log2 e too), not negative; the cache's scales: not negative (a NaN one reaches the rows that see its
- * block; below 2^-100 or so V's products leave bf16's normal values). out may not overlap q. max_length: a bound of length[], from which the work's split is chosen (results
- * hold whatever it says). workspace: what it holds before does not matter; calls that may overlap need one each.
+ * block; below 2^-100 or so V's products leave bf16's normal values). out may not overlap q. max_length: a bound of
+ * length[], from which the work's split is chosen (results hold whatever it says). workspace: what it holds before does not
+ * matter; calls that may overlap need one each.
  * No counterpart in the reference, whose attention reads a bf16 cache (engines/base.py:348-366). */
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
                  int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,

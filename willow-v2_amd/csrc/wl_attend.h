@@ -10,7 +10,8 @@
 // product's token rows may be any tokens: they are dealt out so that a lane holds the scores of 16 consecutive tokens of a
 // page, whose values are 16 consecutive bytes of V^T for each dimension.
 // Bytes become bf16 exactly (|int8| <= 127 and e4m3 have at most 8 significant bits); a block's scale multiplies its
-// scores in fp32, and V's scale multiplies the weights in fp32 before they are rounded to bf16.
+// scores in fp32, and V's scale multiplies the weights in fp32 before they are rounded to bf16 (the weights' one rounding: the
+// matrix core takes them in no more bits at this rate).
 #pragma once
 
 #include <type_traits>
@@ -118,7 +119,6 @@ __device__ __forceinline__ uint32_t wave_scan(uint32_t x) {
 __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return __builtin_amdgcn_readlane(wave_scan(x), 63); }
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
-
 
 // Calls of more rows than the few-row form takes (wl_attend_rows.hip).
 size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);

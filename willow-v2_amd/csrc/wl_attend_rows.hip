@@ -3,12 +3,20 @@
 // A workgroup takes 256 rows, a wavefront 32 of them (v_mfma_f32_32x32x16_bf16), and goes through the cache in tiles of
 // 8192 / D tokens. The workgroup turns a tile's bytes into bf16 once, into LDS, in the order in which the products take
 // them (16 bytes a lane, 1 KB a k-step, so every read is a straight run over the lanes): each of K's and V's values is
-// converted by one of eight wavefronts and used by all. Two tiles are in LDS: while one is multiplied, the next one's
-// bytes are on their way in registers, and are converted into the other.
+// converted by one of eight wavefronts and used by all. LDS holds a ring of four tiles: while one is multiplied, the
+// bytes of the tile two ahead are on their way in registers, and are converted into its place; a barrier stands behind every
+// second tile (behind every one: 2% slower).
 // Token 16 h + i of a 32-token part is row 8 (i / 4) + 4 h + i % 4 of the first product, so a lane of half h holds the
 // scores of tokens 16 h .. 16 h + 15 of row lane % 32, which is how the second product takes the weights.
 // The running maximum is moved only when a score exceeds it by 2^8 (the weights stay below 2^8, fp32 sums hold them): the
 // multiplication of a wavefront's 32 x D sums by the change is the dearest step of the softmax, and becomes rare.
+// Bound by what a wavefront does between its products: 4096 tokens of 16 heads of 256 on 2 kv heads take 185 to 200 us (the
+// card in hand), 740 to 690 TFLOP/s where a large product of matrices reaches 1213; 32 on 8 heads of 128 167 to 177 us, 825 to
+// 780. The matrix core is busy half of the time, the rest is softmax and conversion, of which two wavefronts a SIMD hide some
+// behind each other's products: more wavefronts, or two tiles in flight in one, have no registers (192 of 256 hold q and the
+// sums with 256 dimensions; 64 rows a wavefront of 512 registers spill 500). 16 rows a tile straight from registers, as the
+// form for few rows has it, took 435 us, every wavefront converting all bytes for itself. Bytes copied into LDS by the loads
+// themselves and converted from there: 240 against 225 us at that stage, since LDS reads then wait for the copies.
 #include <algorithm>
 
 #include "wl_attend.h"
@@ -160,7 +168,7 @@ struct Wave {
     float m, l;
 
     // The 32 tokens of part u of a tile; seen: of this lane's 16 tokens, those that its row may see.
-    // Operands come from LDS four products ahead, V's first ones before the softmax.
+    // Operands come from LDS four products ahead (two with 256 dimensions), V's first ones before the softmax.
     __device__ __forceinline__ void add(const Lds<D>& lds, int buffer, int u, int seen) {
         constexpr int kAhead = D == 256 ? 2 : 4;  // no registers for more with 256 dimensions
         int lane = threadIdx.x & 63;
