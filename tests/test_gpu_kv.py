@@ -289,6 +289,27 @@ def test_attend_long(hip, dim, count):
     check_attend(hip, pages, 0, q, table, i32([n]), i32([0, count]))
 
 
+@pytest.mark.parametrize("heads,kv_heads,dim,counts,lengths", [
+    (16, 2, 256, (512,), (16512,)), (32, 8, 128, (301, 180, 65, 256, 37), (1700, 999, 65, 1300, 437)), (8, 1, 64, (700,), (30000,)),
+    (4, 4, 256, (1100, 300), (1500, 5000))])
+def test_attend_prompts_in_pieces(hip, heads, kv_heads, dim, counts, lengths):
+    """Prompts whose caches are cut into about a piece a CU, by shares that the device chooses: rows of every part of them."""
+    g = gen(18)
+    need = sum(-(-n // 64) for n in lengths)
+    pages = random_pages(hip, g, 1, need, kv_heads, 64, dim, torch.int8)
+    table = table_of(g, lengths, 64, need)
+    q = torch.randn(sum(counts), heads, dim, generator=g).to(torch.bfloat16).to(DEV)
+    out = hip.kv_attend(pages, 0, q, table, i32(lengths), cu_of(counts), max_count=max(counts), max_length=max(lengths)).cpu().double()
+    cache = [x[0].cpu() for x in (pages.k, pages.v, pages.k_scale, pages.v_scale)]
+    at = 0
+    for b, (n, length) in enumerate(zip(counts, lengths)):
+        for i in sorted({0, 1, n // 3, n // 2, min(255, n - 1), n - 2, n - 1}):
+            want, tol = kv_ref.attend(*cache, q[at + i:at + i + 1].cpu(), table[b:b + 1].cpu(), torch.tensor([length - n + i + 1]),
+                                      torch.tensor([0, 1]))
+            assert ((out[at + i] - want[0]).abs() <= tol[0]).all(), (b, i)
+        at += n
+
+
 @pytest.mark.parametrize("count", [1, 24])
 @pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
 def test_attend_scales_far_out(hip, count, dtype):
