@@ -13,7 +13,6 @@ float8_e4m3fn), k_scale and v_scale fp32 [layers, pages, kv_heads]; a value is b
 bfloat16 s with M * s >= max |x| over the page's tokens (M = 127 or 448), a value's byte x / s rounded to nearest even.
 When tokens join a page that holds some, its scale grows by the smallest power of two that covers the new ones, and
 the older bytes are divided by it and rounded to nearest even."""
-import functools
 import math
 import os
 import random
@@ -29,7 +28,6 @@ TYPES = {"int8": torch.int8, "e4m3": torch.float8_e4m3fn}
 DEVICE = "cuda"
 
 
-@functools.lru_cache(maxsize=None)  # a program imports its module once, not on every call
 def _hip():
     root = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "willow-v2_amd")
     if root not in sys.path:
