@@ -482,3 +482,16 @@ def test_rope_refusals(hip):
                 lambda: hip.rope(q.cpu(), None, p, f, sections=(3, 3, 2)), lambda: hip.rope(q, torch.zeros(3, 1, 64, device=DEV), p, f, sections=(3, 3, 2))):
         with pytest.raises(ValueError):
             bad()
+
+
+@pytest.mark.parametrize("page", [16, 64])
+@pytest.mark.parametrize("counts", [(4, 2, 3), (70, 3, 33)])
+def test_attend_length_beyond_the_table(hip, counts, page):
+    """Lengths that the table has no pages for: the tokens behind its width are not there, and the rows stand at the positions
+    that the lengths say, so the last ones see all that is there."""
+    g = gen(19)
+    pages = random_pages(hip, g, 1, 10, 2, page, 64, torch.int8)
+    table = table_of(g, (3 * page,) * 3, page, 10)
+    q = torch.randn(sum(counts), 8, 64, generator=g).to(torch.bfloat16).to(DEV)
+    for beyond in (1, counts[0] - 2, 2 ** 31 - 1 - 3 * page):
+        check_attend(hip, pages, 0, q, table, i32([3 * page + beyond, 3 * page - 1, 3 * page + 2]), cu_of(counts), max_count=max(counts))

@@ -27,9 +27,15 @@ typedef float f32x4 __attribute__((ext_vector_type(4)));
 
 constexpr int kTile = 64;       // tokens of a tile
 
-// A sequence of the call: its first row, its rows, its tokens.
+// A sequence of the call: its first row, its rows, its tokens (as many as the table has pages for), and the position of its
+// first row, which its whole length says.
 struct Seq {
-    int at, n, length;
+    int at, n, length, begin;
+
+    // tokens that its row `i` may see
+    __device__ __forceinline__ int seen(int i, bool causal) const {
+        return causal ? min(length, max(begin + i + 1, 0)) : length;
+    }
 };
 
 struct AttendArgs {
@@ -47,14 +53,16 @@ struct AttendArgs {
         Seq q;
         q.at = s.first(b);
         q.n = s.count(b, q.at);
-        q.length = min(max(length[b], 0), s.table_width << c.page_shift);
+        const int all = max(length[b], 0);
+        q.length = min(all, s.table_width << c.page_shift);
+        q.begin = all - q.n;
         return q;
     }
     // the same for a b that all lanes share, in scalar registers
     __device__ __forceinline__ Seq seq_uniform(int b) const {
         const Seq q = seq(b);
         return {__builtin_amdgcn_readfirstlane(q.at), __builtin_amdgcn_readfirstlane(q.n),
-                __builtin_amdgcn_readfirstlane(q.length)};
+                __builtin_amdgcn_readfirstlane(q.length), __builtin_amdgcn_readfirstlane(q.begin)};
     }
 };
 

@@ -45,20 +45,20 @@ struct Rows {
     float m, l;
     int limit;  // tokens that this lane's row sees
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, int head, int at, int n, int length) {
+    __device__ __forceinline__ void begin(const AttendArgs& a, int head, Seq seq) {
         const int lane = threadIdx.x & 63, g = lane >> 4, row = lane & 15, token = row / a.group;
         m = -__builtin_inff();
         l = 0.0f;
-        limit = token >= n ? 0 : a.causal ? min(length, max(length - n + token + 1, 0)) : length;
+        limit = token >= seq.n ? 0 : seq.seen(token, a.causal);
 #pragma unroll
         for (int i = 0; i < kDims; i++) o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
-        const uint16_t* p = a.q + static_cast<int64_t>(at + token) * a.q_token_stride +
+        const uint16_t* p = a.q + static_cast<int64_t>(seq.at + token) * a.q_token_stride +
                             static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 16 * g;
 #pragma unroll
         for (int i = 0; i < 2 * kChunks; i++) {
             const uint16_t* e = p + 64 * (i / 2) + 8 * (i % 2);
             q[i] = make_uint4(0, 0, 0, 0);
-            if (token < n)
+            if (token < seq.n)
                 q[i] = a.wide_q ? *reinterpret_cast<const uint4*>(e)
                                 : make_uint4(e[0] | e[1] << 16, e[2] | e[3] << 16, e[4] | e[5] << 16, e[6] | e[7] << 16);
         }
@@ -212,7 +212,7 @@ __device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, i
     const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group, static_cast<int64_t>(kRows)));
     Rows<TYPE, D, PAGE> r;
     if (t0 + wave < t1) r.find(a, b, (t0 + wave) * kTile);
-    r.begin(a, head, at, n, length);
+    r.begin(a, head, seq);
     r.tiles(a, b, head, t0 + wave, t1, kFewWaves, length);
     r.l = sum_over_groups(r.l);
     if (lane < kRows) {
@@ -272,7 +272,7 @@ struct Line {
 __device__ __forceinline__ uint32_t tiles_of(Seq s) {
     return s.n == 0 ? 0 : max((s.length + kTile - 1) / kTile, 1);  // without a token there are still rows to write
 }
-__device__ __forceinline__ Seq seq_or_none(const FewArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0}; }
+__device__ __forceinline__ Seq seq_or_none(const FewArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0, 0}; }
 
 // Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`. Shares and (sequence, head)s are whole
 // rounds of a workgroup (a tile for each wavefront), so that only the last round of each leaves wavefronts idle.
@@ -317,6 +317,7 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
                 seq.at = __builtin_amdgcn_readlane(mine.at, i);
                 seq.n = __builtin_amdgcn_readlane(mine.n, i);
                 seq.length = __builtin_amdgcn_readlane(mine.length, i);
+                seq.begin = __builtin_amdgcn_readlane(mine.begin, i);
                 b += i;
                 break;
             }

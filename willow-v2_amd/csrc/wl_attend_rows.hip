@@ -247,8 +247,7 @@ struct Wave {
 __device__ __forceinline__ int tiles_of(const AttendArgs& a, Seq seq, int row0, int tile_tokens) {
     if (row0 >= seq.n * a.group) return 0;
     const int last = min((row0 + kGroupRows - 1) / a.group, seq.n - 1);
-    const int seen = a.causal ? min(seq.length, max(seq.length - seq.n + last + 1, 0)) : seq.length;
-    return max((seen + tile_tokens - 1) / tile_tokens, 1);
+    return max((seq.seen(last, a.causal) + tile_tokens - 1) / tile_tokens, 1);
 }
 
 // A row tile's tiles in pieces of at most `each`, as equal as can be, unless that were too many pieces.
@@ -400,7 +399,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
     const int row = row0 + 32 * wave + (lane & 31), token = row / a.group;
     const bool there = token < seq.n;
-    const int limit = !there ? 0 : a.causal ? min(seq.length, max(seq.length - seq.n + token + 1, 0)) : seq.length;
+    const int limit = there ? seq.seen(token, a.causal) : 0;
     const uint16_t* qp = a.q + static_cast<int64_t>(seq.at + token) * a.q_token_stride +
                          static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 8 * half;
     const int most = __builtin_amdgcn_readlane(limit, 31) > 0 ? __builtin_amdgcn_readlane(limit, 31) : seq.length;
