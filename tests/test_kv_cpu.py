@@ -412,3 +412,31 @@ def test_out_is_not_q():
     q, i = torch.zeros(3, 4, 64, dtype=torch.bfloat16), dict(dtype=torch.int32)
     with pytest.raises(ValueError, match="not q's memory"):
         hip.kv_attend(p, 0, q, torch.zeros(1, 2, **i), torch.zeros(1, **i), torch.zeros(2, **i), out=q)
+
+
+def test_numbers_keep_their_value(monkeypatch):
+    """The library takes 32-bit numbers: a layer or a count that does not fit is refused, not cut to another one."""
+    z = torch.zeros
+    p = hip.KVPages.empty(2, 4, 2, 64, 16, device="cpu")
+    k, q, i = z(3, 2, 64, dtype=torch.bfloat16), z(3, 4, 64, dtype=torch.bfloat16), dict(dtype=torch.int32)
+    launched = []
+    monkeypatch.setattr("gguf.hip.kv._launch", lambda index, call, *args: launched.append(args[1]))
+    args = (z(1, 2, **i), z(1, **i), z(2, **i))
+    for layer in (2, -1, 2 ** 32, 2 ** 32 + 1, -2 ** 32, 2 ** 64 + 1):
+        with pytest.raises(ValueError, match="layer"):
+            hip.kv_append(p, layer, k, k, *args)
+        with pytest.raises(ValueError, match="layer"):
+            hip.kv_attend(p, layer, q, *args)
+    for count in (-1, 1 - 2 ** 32, 2 - 2 ** 64):
+        with pytest.raises(ValueError, match="max_count"):
+            hip.kv_append(p, 0, k, k, *args, max_count=count)
+        with pytest.raises(ValueError, match="max_count"):
+            hip.kv_attend(p, 0, q, *args, max_count=count)
+    for length in (-1, 64 - 2 ** 64):
+        with pytest.raises(ValueError, match="max_length"):
+            hip.kv_attend(p, 0, q, *args, max_length=length)
+    assert not launched
+    for layer in (0, 1):
+        hip.kv_append(p, layer, k, k, *args, max_count=2 ** 40)
+        hip.kv_attend(p, layer, q, *args, max_count=2 ** 40, max_length=2 ** 70)
+    assert launched == [0, 0, 1, 1]

@@ -55,6 +55,11 @@ def _rows(t, name, index, dtype, heads, head_dim):
     _refuse(t, name, f"cuda:{index}", dtype, f"[tokens, {'heads' if heads is None else heads}, {head_dim}] with a contiguous last dimension")
 
 
+def _in_cache(pages, layer):
+    if not 0 <= layer < pages.layers:
+        raise ValueError(f"layer {layer}: the cache has {pages.layers}")
+
+
 class KVPages:
     """A paged key/value cache on one GPU, all layers: k int8 or float8_e4m3fn [layers, pages, kv_heads, page_tokens,
     head_dim], v of the same type [layers, pages, kv_heads, head_dim, page_tokens] (tokens innermost: the order in which the
@@ -116,6 +121,8 @@ def _batch(pages, table, cu, per_seq, name, tokens, max_count):
         raise ValueError("the rows of table must be contiguous, and lie apart (not expanded)")
     if max_count is None or max_count > tokens:
         max_count = tokens
+    if (seqs | width | tokens | max_count) >> 31:  # below 0, or more than the library's 32 bits: it would see another number
+        raise ValueError(f"max_count {max_count} with {seqs} sequences of {width} pages and {tokens} rows")
     return WlKvBatch(table.data_ptr(), cu.data_ptr(), max(row, width), tokens, seqs, width,
                      max_count, 0)
 
@@ -129,6 +136,7 @@ def kv_append(pages: KVPages, layer: int, k: torch.Tensor, v: torch.Tensor, tabl
     rows, a page with older tokens its scale times the smallest power of two that does (its older bytes are divided by it and
     rounded); a NaN or an infinity makes its block's scale NaN. Rows whose page is not there (no table entry, or one outside
     the cache) are dropped. Pages written in one call must be distinct over its sequences."""
+    _in_cache(pages, layer)
     n, _, k_token, k_head = _rows(k, "k", pages.index, torch.bfloat16, pages.kv_heads, pages.head_dim)
     rows, _, v_token, v_head = _rows(v, "v", pages.index, torch.bfloat16, pages.kv_heads, pages.head_dim)
     if n != rows:
@@ -152,6 +160,7 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     work is split (default: what the table's width holds). Rows behind cu[-1] of `out` (which may not overlap q) stay as they are.
     workspace: a uint8 tensor that is large enough (wl_kv_attend_workspace_bytes), for calls that do not overlap in time; by
     default it comes from torch's allocator, for this call and stream."""
+    _in_cache(pages, layer)
     n, heads, token_stride, head_stride = _rows(q, "q", pages.index, torch.bfloat16, None, pages.head_dim)
     if heads == 0 or heads % pages.kv_heads:
         raise ValueError(f"{heads} query heads over {pages.kv_heads} kv heads")
@@ -165,6 +174,8 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
         return out
     longest = b.table_width * pages.page_tokens
     if max_length is not None and max_length < longest:
+        if max_length < 0:
+            raise ValueError(f"max_length {max_length}")
         longest = max_length
     lib = library()
     need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, b, longest)
