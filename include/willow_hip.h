@@ -340,7 +340,8 @@ int wl_kv_copy(const WlKvCache* cache, const int32_t* src_host, const int32_t* d
 
 #define WL_MAX_ROPE_AXES 4
 /* One tensor to rotate: [tokens][heads][head_dim], element strides given (head_dim contiguous). out may be in, with the
- * same strides; memory that overlaps otherwise may be overwritten before it is read. */
+ * same strides; memory that overlaps otherwise may be overwritten before it is read. No two rows of out may share memory
+ * (refused). */
 typedef struct WlRopeTensor {
     const void* in;
     void* out;

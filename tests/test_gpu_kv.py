@@ -495,3 +495,23 @@ def test_attend_length_beyond_the_table(hip, counts, page):
     q = torch.randn(sum(counts), 8, 64, generator=g).to(torch.bfloat16).to(DEV)
     for beyond in (1, counts[0] - 2, 2 ** 31 - 1 - 3 * page):
         check_attend(hip, pages, 0, q, table, i32([3 * page + beyond, 3 * page - 1, 3 * page + 2]), cu_of(counts), max_count=max(counts))
+
+
+def test_rope_into_rows_that_share_memory(hip):
+    q = torch.randn(4, 2, 64, device=DEV)
+    f, p = torch.ones(32, dtype=torch.float64, device=DEV), torch.zeros(4, dtype=torch.int64, device=DEV)
+    one = torch.zeros(1, 2, 64, device=DEV)
+    for out in (one.expand(4, 2, 64), torch.zeros(4, 1, 64, device=DEV).expand(4, 2, 64),
+                torch.zeros(1000, device=DEV).as_strided((4, 2, 64), (100, 50, 1))):
+        before = out.clone()
+        with pytest.raises(ValueError):
+            hip.rope(q, None, p, f, out=(out, None))
+        with pytest.raises(ValueError):
+            hip.rope(q, q, p, f, out=(None, out))
+        assert torch.equal(out, before)
+    with pytest.raises(ValueError):
+        hip.rope(one.expand(4, 2, 64), None, p, f, out=(one.expand(4, 2, 64), None))  # in place
+    a, _ = hip.rope(one.expand(4, 2, 64), None, p, f)  # to be read they may
+    assert torch.equal(a, torch.zeros_like(q))
+    apart = torch.zeros(2, 4, 64, device=DEV).transpose(0, 1)  # heads outermost
+    assert torch.equal(hip.rope(q, None, p, f, out=(apart, None))[0], hip.rope(q, None, p, f)[0])

@@ -440,3 +440,27 @@ def test_numbers_keep_their_value(monkeypatch):
         hip.kv_append(p, layer, k, k, *args, max_count=2 ** 40)
         hip.kv_attend(p, layer, q, *args, max_count=2 ** 40, max_length=2 ** 70)
     assert launched == [0, 0, 1, 1]
+
+
+@pytest.mark.parametrize("side", ["q", "k"])
+@pytest.mark.parametrize("heads,token,head,apart", [
+    (4, 256, 64, True), (4, 1000, 64, True), (4, 64, 64 * 5, True), (1, 64, 0, True), (1, 64, 7, True), (4, -256, 64, True),
+    (4, 256, -64, True), (2, 150, 100, False), (3, 160, 64, False), (2, 192, 64, True), (2, 64, 96, False), (4, 0, 64, False),
+    (4, 256, 0, False), (4, 63, 64 * 5, False), (4, 255, 64, False), (4, 256, 63, False), (4, 256, 32, False), (4, -255, 64, False),
+    (2, 128, 320, True), (2, 128, 340, False), (2, 128, 319, False), (8, 128, 192, False)])
+def test_rope_rows_lie_apart(side, heads, token, head, apart):
+    """Results whose tokens or heads share memory would be written twice, in no order: refused before anything is launched. What
+    overlaps is worked out from every pair of rows."""
+    tokens, dim = 5, 64
+    at = sorted(t * token + h * head for t in range(tokens) for h in range(heads))
+    assert apart == all(b - a >= dim for a, b in zip(at, at[1:]))
+    lib, sections = hip.library(), (ctypes.c_int32 * 1)(16)
+    good = hip.WlRopeTensor(FAKE, FAKE, 256, 64, 256, 64, 4, 0)
+    over = hip.WlRopeTensor(FAKE, FAKE, 256, 64, token, head, heads, 0)
+    # positions on no 8-byte address are refused behind the tensors: what a call ends with whose tensors are right
+    rc = lib.wl_rope(over if side == "q" else good, over if side == "k" else None, 1, tokens, dim, 32, FAKE + 4, tokens, FAKE, 1,
+                     sections, 1, 1.0, None)
+    assert rc == (-4 if apart else -2)
+    one = lib.wl_rope(over if side == "q" else good, over if side == "k" else None, 1, 1, dim, 32, FAKE + 4, 1, FAKE, 1, sections, 1,
+                      1.0, None)
+    assert one == (-4 if heads == 1 or abs(head) >= dim else -2)  # of one token the stride between tokens means nothing

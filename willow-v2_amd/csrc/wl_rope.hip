@@ -132,6 +132,23 @@ int check_rope_tensor(const WlRopeTensor* x, int size) {
     return WL_OK;
 }
 
+// Whether no two of the rows [t * token, + dim) + h * head (t < tokens, h < heads) share an element. Rows dt tokens and dh heads
+// apart lie |dt token + dh head| apart; of each dh the nearest two dt are looked at.
+bool rows_apart(int64_t token, int64_t head, int64_t tokens, int64_t heads, int64_t dim) {
+    using wide = __int128;  // strides are the caller's: no product of them may overflow
+    auto size = [](wide x) { return x < 0 ? -x : x; };
+    const wide ts = size(token), hs = size(head);
+    if ((heads == 1 || hs >= dim) && (tokens == 1 || ts >= hs * (heads - 1) + dim)) return true;  // all of a token, then the next
+    if (tokens > 1 && ts < dim) return false;
+    if (tokens == 1) return false;
+    for (int64_t dh = 1; dh < heads; dh++) {
+        const wide off = wide{head} * dh, near = -off / token;
+        for (wide dt = near - 1; dt <= near + 1; dt++)
+            if (size(dt) < tokens && size(off + dt * token) < dim) return false;
+    }
+    return true;
+}
+
 bool aligned16(const WlRopeTensor* x, int size) {
     const int64_t n = 16 / size;
     return reinterpret_cast<uintptr_t>(x->in) % 16 == 0 && reinterpret_cast<uintptr_t>(x->out) % 16 == 0 &&
@@ -156,6 +173,8 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
     if (tokens < 1 || tokens >= (int64_t{1} << 32) / kRopeThreads || head_dim < 2 || head_dim > 1024 || rotary_dim < 2 ||
         rotary_dim > head_dim || rotary_dim % 2 || axes < 1 || axes > WL_MAX_ROPE_AXES)
         return WL_EINVAL_SHAPE;
+    for (const WlRopeTensor* x : {q, k})
+        if (x && !rows_apart(x->out_token_stride, x->out_head_stride, tokens, x->heads, head_dim)) return WL_EINVAL_SHAPE;
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return WL_EINVAL_ALIGN;
     RopeArgs a = {};
     a.half = rotary_dim / 2;

@@ -231,7 +231,7 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
          interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions with several axes: q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (or None), both bf16
     or both fp32 (any strides over tokens and heads), rotated into new tensors (or into `out`, a (q, k) pair, which may be
-    q and k themselves, but not overlap them otherwise) -> (q, k). positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2],
+    q and k themselves, but not overlap them otherwise; rows of one that share memory are refused) -> (q, k). positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2],
     the angle of one position step; sections[i] of its frequencies belong to axis i, interleaved (axis i > 0 has the
     frequencies i, i + axes, i + 2 axes, ..; axis 0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2)
     turn by positions[axis(j)] * inv_freq[j], taken in 64 bits; cosine and sine are multiplied by `scale`; the rest of each head
