@@ -44,7 +44,7 @@ extern "C" {
 #define WL_EINVAL_COUNT -8     /* too many experts for one batched call */
 #define WL_EINVAL_SCRATCH -9   /* wl_moe_layer_noalloc: the call needs more than WL_NOALLOC_SCRATCH_BYTES */
 #define WL_ESYNC -10           /* wl_moe_workspace_status: a bounded wait gave up since the last query */
-#define WL_EINVAL_OVERLAP -11  /* wl_moe_layer: y overlaps x */
+#define WL_EINVAL_OVERLAP -11  /* wl_moe_layer: y overlaps x; wl_kv_attend: out overlaps q */
 #define WL_EINVAL_SCOPE -12    /* wl_moe_fork_begin with a scope open on the device; wl_moe_fork_end without one on
                                   this stream */
 
@@ -326,7 +326,7 @@ size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const W
  * j <= the row's own position; a row that sees no token is 0. Softmax statistics and sums are fp32; the weights are rounded
  * to bf16 for the matrix core, which adds up in fp32.
  * scale: finite (times log2 e too), not negative; the cache's scales: not negative (a NaN one reaches the rows that see its
- * block; below 2^-100 or so V's products leave bf16's normal values). out may not overlap q. max_length: a bound of
+ * block; below 2^-100 or so V's products leave bf16's normal values). out may not overlap q (refused). max_length: a bound of
  * length[], from which the work's split is chosen (results hold whatever it says). workspace: what it holds before does not
  * matter; calls that may overlap need one each.
  * No counterpart in the reference, whose attention reads a bf16 cache (engines/base.py:348-366). */

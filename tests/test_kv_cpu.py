@@ -464,3 +464,27 @@ def test_rope_rows_lie_apart(side, heads, token, head, apart):
     one = lib.wl_rope(over if side == "q" else good, over if side == "k" else None, 1, 1, dim, 32, FAKE + 4, 1, FAKE, 1, sections, 1,
                       1.0, None)
     assert one == (-4 if heads == 1 or abs(head) >= dim else -2)  # of one token the stride between tokens means nothing
+
+
+def test_out_overlaps_q():
+    """out in the memory of q's rows is refused wherever they meet, before anything is launched; between the rows, or beside them,
+    it may lie. Against every pair of elements."""
+    lib, rng = hip.library(), random.Random(3)
+    c = cache_struct(kv_heads=1)
+    seen = [0, 0]
+    for _ in range(3000):
+        tokens, heads = rng.randint(1, 5), rng.randint(1, 4)
+        token, head = (rng.choice((0, 64, 72, 128, 256, 300, 1000, 2000, -64, -256, -700)) for _ in range(2))
+        at = 8 * rng.randint(-400, 400)  # out's beginning behind q's, in elements
+        rows = {t * token + h * head for t in range(tokens) for h in range(heads)}
+        meet = any(r < at + tokens * heads * 64 and r + 64 > at for r in rows)
+        b = batch_struct(tokens=tokens, max_count=1, table_width=64, table_stride=64)
+        args = (FAKE, token, head, heads, ctypes.byref(b), FAKE, 1024, 0.125, 1, FAKE + 2 * at)
+        need = lib.wl_kv_attend_workspace_bytes(ctypes.byref(c), heads, ctypes.byref(b), 1024)
+        assert need
+        if meet:
+            assert lib.wl_kv_attend(ctypes.byref(c), 0, *args, FAKE, need, None) == -11
+        elif not torch.cuda.is_available():  # nothing stands in the way of a launch, which ends without a device
+            assert lib.wl_kv_attend(ctypes.byref(c), 0, *args, FAKE, need, None) > 0
+        seen[meet] += 1
+    assert min(seen) > 500

@@ -130,6 +130,7 @@ __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_ex
 
 // Calls of more rows than the few-row form takes (wl_attend_rows.hip).
 size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);
+bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);  // launches hold the call
 int launch_attend_rows(const WlKvCache* c, const AttendArgs& a, const WlKvBatch* b, int64_t max_length, void* workspace,
                        hipStream_t stream);
 

@@ -460,6 +460,24 @@ int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, in
     return WL_OK;
 }
 
+// Whether a row of q (element strides ts, hs) lies in out's memory (dense). For each head the first row that ends behind out's
+// beginning is the one that would begin before its end.
+bool out_meets_q(const uint16_t* out, const uint16_t* q, int64_t ts, int64_t hs, int64_t tokens, int64_t heads, int64_t dim) {
+    using wide = __int128;  // strides are the caller's: no product of them may overflow
+    const wide lo = (static_cast<wide>(reinterpret_cast<uintptr_t>(out)) - static_cast<wide>(reinterpret_cast<uintptr_t>(q))) / 2,
+               hi = lo + static_cast<wide>(tokens) * heads * dim;
+    const wide t_end = static_cast<wide>(ts) * (tokens - 1), h_end = static_cast<wide>(hs) * (heads - 1);
+    if (std::min<wide>(t_end, 0) + std::min<wide>(h_end, 0) >= hi || std::max<wide>(t_end, 0) + std::max<wide>(h_end, 0) + dim <= lo)
+        return false;  // what most calls are: apart as a whole
+    for (int64_t h = 0; h < heads; h++) {
+        const wide off = static_cast<wide>(hs) * h + (ts < 0 ? t_end : 0), step = ts < 0 ? -ts : ts;
+        const wide gap = lo - dim - off;  // rows that begin at or before off + gap end before out
+        const wide t = gap < 0 ? 0 : step == 0 ? tokens : gap / step + 1;
+        if (t < tokens && off + t * step < hi) return true;
+    }
+    return false;
+}
+
 }  // namespace
 }  // namespace wl
 
@@ -484,6 +502,9 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
     const size_t need = wl_kv_attend_workspace_bytes(cache, q_heads, batch, max_length);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return WL_EINVAL_WORKSPACE;
+    const bool few = is_few(cache, q_heads, batch);
+    if (!few && !attend_rows_fit(cache, q_heads, batch, max_length)) return WL_EINVAL_SHAPE;
+    if (out_meets_q(out, q, q_token_stride, q_head_stride, batch->tokens, q_heads, cache->head_dim)) return WL_EINVAL_OVERLAP;
     FewArgs a = {};
     a.c = layer_of(cache, layer);
     a.s = seqs_of(batch);
@@ -498,7 +519,7 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.causal = causal != 0;
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!is_few(cache, q_heads, batch)) return launch_attend_rows(cache, a, batch, max_length, workspace, st);
+    if (!few) return launch_attend_rows(cache, a, batch, max_length, workspace, st);
     const FewPlan plan = few_plan(cache, batch, max_length);
     const FewSpace space = few_space(cache, q_heads, batch, plan);
     a.partial = static_cast<float*>(workspace);

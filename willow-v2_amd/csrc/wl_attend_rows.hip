@@ -566,6 +566,16 @@ size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b
     return 16 + static_cast<size_t>(p.pieces * b->tokens * q_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
 }
 
+static int64_t merge_groups(const WlKvCache* c, int64_t group, const WlKvBatch* b) {
+    return (b->max_count * group + kMergeRows - 1) / kMergeRows * c->kv_heads;
+}
+
+bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
+    const RowsPlan p = rows_plan(c, q_heads, b, max_length);
+    return p.row_tiles * b->seqs < (int64_t{1} << 31) && fits_a_launch(p.groups, kThreads) &&
+           fits_a_launch(merge_groups(c, q_heads / c->kv_heads, b), kMergeWaves * 64);
+}
+
 int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBatch* b, int64_t max_length, void* workspace,
                        hipStream_t stream) {
     const RowsPlan p = rows_plan(c, call.q_heads, b, max_length);
@@ -576,12 +586,8 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     a.partial_ml = reinterpret_cast<float2*>(a.partial + p.pieces * b->tokens * call.q_heads * c->head_dim);
     a.row_tiles = static_cast<int32_t>(p.row_tiles);
     a.pieces = static_cast<int32_t>(p.pieces);
-    const int64_t merges = (b->max_count * static_cast<int64_t>(call.group) + kMergeRows - 1) / kMergeRows * c->kv_heads;
-    if (p.row_tiles * b->seqs >= (int64_t{1} << 31) || !fits_a_launch(p.groups, kThreads) ||
-        !fits_a_launch(merges, kMergeWaves * 64))
-        return WL_EINVAL_SHAPE;
     const dim3 grid(static_cast<uint32_t>(p.groups));
-    const dim3 merge(static_cast<uint32_t>(merges), b->seqs);
+    const dim3 merge(static_cast<uint32_t>(merge_groups(c, call.group, b)), b->seqs);
     auto run = [&](auto type, auto dim) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
         if (c->page_tokens >= Shape<D>::kTokens)
