@@ -488,3 +488,32 @@ def test_out_overlaps_q():
             assert lib.wl_kv_attend(ctypes.byref(c), 0, *args, FAKE, need, None) > 0
         seen[meet] += 1
     assert min(seen) > 500
+
+
+def test_counts_are_whole(monkeypatch):
+    """Fractions of tokens are refused with nothing changed (they were cut to whole ones, or left a book of fractions)."""
+    book = PageBook(4, 16)
+    a = book.new()
+    book.grow([a], [20])
+    for bad in (1.5, 0.999, float("nan"), float("inf"), "1", None):
+        with pytest.raises((ValueError, TypeError)):
+            book.grow([a], [bad])
+        with pytest.raises((ValueError, TypeError)):
+            book.truncate(a, bad)
+        assert book.length(a) == 20 and book.sequences[a][1] == [0, 1]
+    cache = HBMKVCache(1, 8, 2, 64, 16, device="cpu")
+    s = cache.new()
+    step = cache.step([s], [3], width=4)
+    for bad in ([1.5], [3.5], ["3"]):
+        with pytest.raises((ValueError, TypeError)):
+            cache.step([s], bad)
+        with pytest.raises((ValueError, TypeError)):
+            cache.refresh(step, [s], bad)
+        assert cache.length(s) == 3
+    import numpy as np
+    for one in (1, 1.0, np.int32(1), np.float32(1), torch.tensor(1)):
+        cache.step([s], [one])
+    cache.truncate(s, np.int64(4))
+    cache.truncate(s, 2.0)
+    assert cache.length(s) == 2 and type(cache.length(s)) is int
+    check_book(cache.book)

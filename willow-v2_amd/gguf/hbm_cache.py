@@ -26,6 +26,13 @@ class OutOfPages(RuntimeError):
     """A step needs more pages than are free; nothing was changed."""
 
 
+def _whole(n) -> int:
+    """A number of tokens as an int; a fraction of one is refused."""
+    if isinstance(n, str) or n - n != 0 or int(n) != n:  # infinities less themselves are not 0
+        raise ValueError(f"{n!r} is no number of tokens")
+    return int(n)
+
+
 class PageBook:
     """Which pages each sequence has, on the host alone: no call here touches a device."""
 
@@ -78,7 +85,7 @@ class PageBook:
 
     def truncate(self, seq: int, length: int):
         """Forgets the tokens from `length` on."""
-        s = self._sequence(seq)
+        s, length = self._sequence(seq), _whole(length)
         if not 0 <= length <= s[0]:
             raise ValueError(f"sequence {seq} has {s[0]} tokens: cannot keep {length}")
         keep = -(-length // self.page_tokens)
@@ -92,6 +99,7 @@ class PageBook:
         for unknown or repeated sequences and negative counts, with nothing changed."""
         if len(seqs) != len(counts) or len(set(seqs)) != len(seqs):
             raise ValueError("seqs must be different sequences, one count for each")
+        counts = [_whole(n) for n in counts]
         need, shared = 0, {}
         for seq, n in zip(seqs, counts):
             length, pages = self._sequence(seq)
@@ -209,22 +217,23 @@ class HBMKVCache:
         (for refresh() of longer sequences; default: as many as the longest has). The tables are uploaded: not under capture."""
         if not seqs:
             raise ValueError("a step needs a sequence")
+        counts = [_whole(c) for c in counts]
         if width is not None:
             self._check_width(seqs, counts, width)
-        host, start, length, cu = self._host_step(list(seqs), [int(c) for c in counts], width)
+        host, start, length, cu = self._host_step(list(seqs), counts, width)
         up = [torch.from_numpy(a).to(self.device) for a in (host, start, length, cu)]
-        return KVStep(*up, [int(c) for c in counts], max(int(c) for c in counts),
+        return KVStep(*up, counts, max(counts),
                       int(length.max()) if width is None else width * self.book.page_tokens, int(cu[-1]))
 
     def _check_width(self, seqs, counts, width):
         for s, c in zip(seqs, counts):
-            if self.book.length(s) + int(c) > width * self.book.page_tokens:
+            if self.book.length(s) + c > width * self.book.page_tokens:
                 raise ValueError(f"sequence {s} does not fit {width} pages")
 
     def refresh(self, step: KVStep, seqs, counts) -> KVStep:
         """A later step of as many sequences with the same counts, written into `step`'s tensors on the current stream: a
         graph that was captured with them then runs this step."""
-        counts = [int(c) for c in counts]
+        counts = [_whole(c) for c in counts]
         if len(seqs) != step.table.shape[0] or counts != step.counts:
             raise ValueError(f"the step was made for {step.table.shape[0]} sequences with counts {step.counts}")
         self._check_width(seqs, counts, step.table.shape[1])
