@@ -1,4 +1,5 @@
 """The attention half without a GPU: the page book's bookkeeping, the C ABI's refusals, the Python side's checks."""
+import contextlib
 import ctypes
 import math
 import random
@@ -516,4 +517,25 @@ def test_counts_are_whole(monkeypatch):
     cache.truncate(s, np.int64(4))
     cache.truncate(s, 2.0)
     assert cache.length(s) == 2 and type(cache.length(s)) is int
+    check_book(cache.book)
+
+
+def test_nothing_is_booked_under_capture(monkeypatch):
+    """step, refresh and compact upload tables or move pages that the book counts as moved at once: under capture, where nothing
+    runs, they are refused with nothing changed."""
+    cache = HBMKVCache(1, 8, 2, 64, 16, device="cpu")
+    a, b = cache.new(), cache.new()
+    step = cache.step([a], [20], width=4)
+    cache.step([b], [3])
+    cache.truncate(a, 0)
+    cache.step([a], [1])
+    before = {s: [v[0], list(v[1])] for s, v in cache.book.sequences.items()}
+    monkeypatch.setattr("torch.cuda.is_current_stream_capturing", lambda: True)
+    monkeypatch.setattr("torch.cuda.device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(cache.pages, "index", 0)
+    monkeypatch.setattr("gguf.hbm_cache.kv_copy", lambda *args: pytest.fail("copied"))
+    for call in (lambda: cache.step([a], [1]), lambda: cache.refresh(step, [a], [20]), lambda: cache.compact()):
+        with pytest.raises(RuntimeError, match="captur"):
+            call()
+        assert before == cache.book.sequences
     check_book(cache.book)

@@ -191,14 +191,23 @@ class HBMKVCache:
 
     def compact(self) -> int:
         """Moves the live pages to the lowest numbers -> how many moved. Steps made before hold pages that are no longer
-        theirs: make them anew."""
+        theirs: make them anew. Not under capture."""
+        self._not_captured()
         src, dst = self.book.compact()
         kv_copy(self.pages, src, dst)
         return len(src)
 
     # -- one forward pass -----------------------------------------------------------------------------------------
 
+    def _not_captured(self):
+        """The book counts pages as moved and tokens as there at once: not in a captured graph, which runs later, and often."""
+        if self.pages.index >= 0:
+            with torch.cuda.device(self.pages.index):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("a cache's step(), refresh() and compact() cannot be captured into a graph")
+
     def _host_step(self, seqs, counts, width):
+        self._not_captured()
         src, dst = self.book.grow(seqs, counts)
         kv_copy(self.pages, src, dst)
         n = len(seqs)
