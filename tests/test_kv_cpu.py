@@ -539,3 +539,25 @@ def test_nothing_is_booked_under_capture(monkeypatch):
             call()
         assert before == cache.book.sequences
     check_book(cache.book)
+
+
+@pytest.mark.parametrize("after", range(4))
+def test_steps_whose_tables_do_not_arrive(monkeypatch, after):
+    """An upload that fails (no memory, say) leaves no token counted that no step can write."""
+    cache = HBMKVCache(1, 8, 2, 64, 16, device="cpu")
+    a, b = cache.new(), cache.new()
+    step = cache.step([a, b], [10, 40], width=4)
+    real, left = torch.from_numpy, [after]
+
+    def upload(array):
+        if not left[0]:
+            raise RuntimeError("out of memory")
+        left[0] -= 1
+        return real(array)
+    monkeypatch.setattr(torch, "from_numpy", upload)
+    for call in (lambda: cache.step([b, a], [20, 7]), lambda: cache.refresh(step, [b, a], [10, 40])):
+        left[0] = min(after, 2) if "refresh" in call.__code__.co_names else after
+        with pytest.raises(RuntimeError, match="memory"):
+            call()
+        assert (cache.length(a), cache.length(b), cache.book.used()) == (10, 40, 4)
+        check_book(cache.book)

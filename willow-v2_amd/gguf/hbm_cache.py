@@ -13,6 +13,7 @@ what is live to the lowest page numbers. The lowest free page is always taken fi
         cache.append(layer, step, k, v)                       # k, v bf16 [tokens, kv_heads, head_dim]
         out = cache.attend(layer, step, q)                    # q bf16 [tokens, heads, head_dim]
 """
+import contextlib
 import heapq
 from dataclasses import dataclass
 
@@ -220,6 +221,16 @@ class HBMKVCache:
         cu = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
         return host, start, length, cu
 
+    @contextlib.contextmanager
+    def _given_back(self, seqs, counts):
+        """Takes the step's tokens off the book again where its tables do not reach the device."""
+        try:
+            yield
+        except BaseException:
+            for s, n in zip(seqs, counts):
+                self.book.truncate(s, self.book.length(s) - n)
+            raise
+
     def step(self, seqs, counts, width: int = None) -> KVStep:
         """Room for counts[i] new tokens of sequence seqs[i], which count as its own from here on -> what append and attend
         take. Pages that a fork shares and that are about to be written are copied. width: pages the table has columns for
@@ -230,7 +241,8 @@ class HBMKVCache:
         if width is not None:
             self._check_width(seqs, counts, width)
         host, start, length, cu = self._host_step(list(seqs), counts, width)
-        up = [torch.from_numpy(a).to(self.device) for a in (host, start, length, cu)]
+        with self._given_back(seqs, counts):
+            up = [torch.from_numpy(a).to(self.device) for a in (host, start, length, cu)]
         return KVStep(*up, counts, max(counts),
                       int(length.max()) if width is None else width * self.book.page_tokens, int(cu[-1]))
 
@@ -247,8 +259,9 @@ class HBMKVCache:
             raise ValueError(f"the step was made for {step.table.shape[0]} sequences with counts {step.counts}")
         self._check_width(seqs, counts, step.table.shape[1])
         host, start, length, _ = self._host_step(list(seqs), counts, step.table.shape[1])
-        for t, a in ((step.table, host), (step.start, start), (step.length, length)):
-            t.copy_(torch.from_numpy(a))
+        with self._given_back(seqs, counts):
+            for t, a in ((step.table, host), (step.start, start), (step.length, length)):
+                t.copy_(torch.from_numpy(a))
         step.max_length = max(step.max_length, int(length.max()))
         return step
 
