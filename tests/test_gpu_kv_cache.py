@@ -329,3 +329,22 @@ def test_engine_attention_refuses(hip):
     eng.weights["model.layers.3.self_attn.k_proj.weight"] = bf16(g, 192, 256)
     with pytest.raises(ValueError):
         eng.hip_attention(bf16(g, 2, 256), 3, 0, step, eng.rotary.positions(torch.arange(2)))
+
+
+@pytest.mark.parametrize("counts,pad", [((3, 1), 12), ((40, 9), 15)])
+def test_padded_layer(hip, monkeypatch, counts, pad):
+    """A layer over a batch with padding rows behind its tokens: the tokens' rows have the bits of the call without padding, the
+    others come out as zeros, whatever the allocator's memory held. Projections in 64 bits, rounded once, since a library's product
+    may add up in another order for another number of rows."""
+    monkeypatch.setattr(F, "linear", lambda x, w: (x.double() @ w.double().T).to(torch.bfloat16))
+    g, n, outs = torch.Generator().manual_seed(14), sum(counts), []
+    x = bf16(g, n + pad, 256)
+    for rows in (n, n + pad):
+        eng = engine(torch.Generator().manual_seed(11), True, False, False)[0]
+        step = eng.kv_cache.step([eng.kv_cache.new() for _ in counts], counts)
+        positions = eng.rotary.positions(torch.arange(rows))
+        full = [torch.full((rows * 256,), float("nan"), device=DEV, dtype=torch.bfloat16) for _ in range(8)]
+        del full
+        outs.append(eng.hip_attention(x[:rows], 3, 0, step, positions))
+    assert torch.equal(outs[1][:n], outs[0]) and outs[0].abs().max() > 0
+    assert (outs[1][n:] == 0).all()

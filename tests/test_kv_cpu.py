@@ -561,3 +561,25 @@ def test_steps_whose_tables_do_not_arrive(monkeypatch, after):
             call()
         assert (cache.length(a), cache.length(b), cache.book.used()) == (10, 40, 4)
         check_book(cache.book)
+
+
+def test_padding_rows_are_zeros(monkeypatch):
+    """Rows behind the step's tokens, which no kernel writes, come out as zeros where the cache makes the result: what goes on
+    through a layer (its projection, the next one's router) is not what the memory held before."""
+    cache = HBMKVCache(1, 4, 2, 64, 16, device="cpu")
+    step = cache.step([cache.new(), cache.new()], [3, 2])
+    outs = []
+
+    def attend(pages, layer, q, *args, out=None, **kw):
+        out = torch.full(q.shape, float("nan"), dtype=q.dtype) if out is None else out  # memory that held something else
+        outs.append(out)
+        out[:5] = 1.0
+        return out
+    monkeypatch.setattr("gguf.hbm_cache.kv_attend", attend)
+    wide = torch.zeros(8, 4, 128, dtype=torch.bfloat16)
+    for q in (wide[:5, :, :64], wide[:8, :, :64], wide[:8, :, :64].contiguous()):
+        got = cache.attend(0, step, q)
+        assert got is outs.pop() and got.shape == q.shape and got.is_contiguous()
+        assert (got[:5] == 1).all() and (got[5:] == 0).all()
+    mine = torch.full((8, 4, 64), 7.0, dtype=torch.bfloat16)
+    assert cache.attend(0, step, wide[..., :64], out=mine) is mine and (mine[5:] == 7).all()  # the caller's own stay

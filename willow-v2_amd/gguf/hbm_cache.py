@@ -272,7 +272,11 @@ class HBMKVCache:
 
     def attend(self, layer: int, step: KVStep, q: torch.Tensor, scale: float = None, causal: bool = True,
                out: torch.Tensor = None) -> torch.Tensor:
-        """The step's rows' attention over one layer of their sequences, bf16 [tokens, heads, head_dim]; kv_attend."""
+        """The step's rows' attention over one layer of their sequences, bf16 [tokens, heads, head_dim]; kv_attend. Rows of q behind
+        the step's tokens (padding) come out as zeros, or stay as they are in `out`."""
         step.check(q, "q")
+        if out is None and q.shape[0] > step.tokens:
+            out = torch.empty_like(q, memory_format=torch.contiguous_format)
+            out[step.tokens:].zero_()
         return kv_attend(self.pages, layer, q, step.table, step.length, step.cu, max_count=step.max_count or 1,
                          max_length=step.max_length, scale=scale, causal=causal, out=out)

@@ -157,7 +157,8 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     otherwise all length[b]. A row that sees none is 0. scale (finite, not negative) defaults to head_dim ** -0.5. max_count: the
     most rows any sequence has (rows beyond it count as if they were not there; default: all rows, which costs calls of short
     sequences the form that is made for them); cu must not decrease; max_length: a bound of length that only steers how the
-    work is split (default: what the table's width holds). Rows behind cu[-1] of `out` (which may not overlap q) stay as they are.
+    work is split (default: what the table's width holds). Rows of no sequence stay as they are in `out` (which may not overlap
+    q), and hold anything without it.
     workspace: a uint8 tensor that is large enough (wl_kv_attend_workspace_bytes), for calls that do not overlap in time; by
     default it comes from torch's allocator, for this call and stream."""
     _in_cache(pages, layer)
@@ -231,10 +232,11 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
          interleaved: bool = True, scale: float = 1.0, out=None):
     """Rotary positions with several axes: q [tokens, heads, head_dim] and k [tokens, kv_heads, head_dim] (or None), both bf16
     or both fp32 (any strides over tokens and heads), rotated into new tensors (or into `out`, a (q, k) pair, which may be
-    q and k themselves, but not overlap them otherwise; rows of one that share memory are refused) -> (q, k). positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2],
-    the angle of one position step; sections[i] of its frequencies belong to axis i, interleaved (axis i > 0 has the
-    frequencies i, i + axes, i + 2 axes, ..; axis 0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2)
-    turn by positions[axis(j)] * inv_freq[j], taken in 64 bits; cosine and sine are multiplied by `scale`; the rest of each head
+    q and k themselves, but not overlap them otherwise; rows of one that share memory are refused) -> (q, k).
+    positions: int64 [axes, tokens] (or [tokens], one axis); inv_freq: fp64 [rotary_dim / 2], the angle of one position step;
+    sections[i] of its frequencies belong to axis i, interleaved (axis i > 0 has the frequencies i, i + axes, i + 2 axes, ..; axis
+    0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2) turn by positions[axis(j)] * inv_freq[j], taken in
+    64 bits; cosine and sine are multiplied by `scale`; the rest of each head
     is copied. (engines/base.py:16-89 has the one-axis form.)"""
     dtype, index = q.dtype, q.get_device()
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
