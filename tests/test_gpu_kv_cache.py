@@ -348,3 +348,71 @@ def test_padded_layer(hip, monkeypatch, counts, pad):
         outs.append(eng.hip_attention(x[:rows], 3, 0, step, positions))
     assert torch.equal(outs[1][:n], outs[0]) and outs[0].abs().max() > 0
     assert (outs[1][n:] == 0).all()
+
+
+@pytest.mark.parametrize("seed", [0, 1])
+def test_calls_on_changing_streams(hip, seed):
+    """The same lives of sequences (prompts, forks, single tokens, frees, compactions, a replayed graph) on one stream and on three in
+    turn, without a synchronization: the same answers and the same cache, bit for bit."""
+    streams = [torch.cuda.current_stream()] + [torch.cuda.Stream() for _ in range(2)]
+    g = torch.Generator().manual_seed(20)
+    k, v, q = bf16(g, 4000, 2, 128), bf16(g, 4000, 2, 128), bf16(g, 4000, 16, 128)
+    torch.cuda.synchronize()
+
+    def lives(changing):
+        rng, which = random.Random(seed), random.Random(seed + 50)
+        cache = HBMKVCache(1, 300, 2, 128, 64)
+        torch.cuda.synchronize()
+        live, outs = [], []
+        decoded, graph = cache.new(), torch.cuda.CUDAGraph()
+        step = cache.step([decoded], [1], width=4)
+        cache.append(0, step, k[:1], v[:1])
+        cache.attend(0, step, q[:1])
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            cache.append(0, step, k[:1], v[:1])
+            answer = cache.attend(0, step, q[:1])
+        graph.replay()
+        for i in range(60):
+            torch.cuda.set_stream(streams[which.randrange(3) if changing else 0])
+            what = rng.choice(("new", "fork", "token", "token", "token", "free", "compact", "replay"))
+            if what == "replay" and cache.length(decoded) < 250:
+                cache.refresh(step, [decoded], [1])
+                graph.replay()
+                outs.append(answer.clone())
+                continue
+            if what in ("compact", "free") and len(live) > 3:
+                if what == "free":
+                    cache.free(live.pop(rng.randrange(len(live))))
+                else:
+                    cache.compact()
+                continue
+            if what == "fork" and live:
+                live.append(cache.fork(rng.choice(live)))
+                continue
+            if what == "new" or not live:
+                live.append(cache.new())
+                seqs, counts = live[-1:], [rng.randint(500, 3000)]
+            else:
+                seqs = rng.sample(live, min(len(live), 3))
+                counts = [rng.randint(1, 3) for _ in seqs]
+            if cache.book.used() > 220:
+                cache.free(live.pop(0))
+                continue
+            n, at = sum(counts), rng.randint(0, 900)
+            s = cache.step(seqs, counts)
+            cache.append(0, s, k[at:at + n], v[at:at + n])
+            if changing:
+                torch.cuda.set_stream(streams[which.randrange(3)])
+            outs.append(cache.attend(0, s, q[at:at + n]))
+        torch.cuda.set_stream(streams[0])
+        torch.cuda.synchronize()
+        return outs, [getattr(cache.pages, name) for name in ("k", "v", "k_scale", "v_scale")]
+    want, pools = lives(False)
+    try:
+        for _ in range(3):
+            got, mine = lives(True)
+            assert len(got) == len(want) and all(torch.equal(a, b) for a, b in zip(got, want))
+            assert all(torch.equal(a, b) for a, b in zip(mine, pools))
+    finally:
+        torch.cuda.set_stream(streams[0])

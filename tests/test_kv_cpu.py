@@ -583,3 +583,95 @@ def test_padding_rows_are_zeros(monkeypatch):
         assert (got[:5] == 1).all() and (got[5:] == 0).all()
     mine = torch.full((8, 4, 64), 7.0, dtype=torch.bfloat16)
     assert cache.attend(0, step, wide[..., :64], out=mine) is mine and (mine[5:] == 7).all()  # the caller's own stay
+
+
+class FakeStreams:
+    """Streams as clocks: what each one's work so far is known to come after. Every call of the cache is checked against all before
+    it: a write comes after everything, a read after every write."""
+
+    def __init__(self):
+        self.current, self.capturing, self.clocks, self.log, self.held = 0, False, {}, [], []
+
+    def stream(self, raw):
+        outer = self
+
+        class Stream:
+            cuda_stream = raw
+
+            def wait_stream(self, other):
+                mine, theirs = (outer.clocks.setdefault(s, {}) for s in (raw, other.cuda_stream))
+                for s, t in theirs.items():
+                    mine[s] = max(mine.get(s, 0), t)
+        return Stream()
+
+    def work(self, writes):
+        if self.capturing:
+            return
+        clock = self.clocks.setdefault(self.current, {})
+        for s, t, wrote in self.log:
+            assert not (writes or wrote) or clock.get(s, 0) >= t, f"stream {self.current} does not wait for stream {s}"
+        clock[self.current] = clock.get(self.current, 0) + 1
+        self.log.append((self.current, clock[self.current], writes))
+
+
+@pytest.mark.parametrize("seed", range(6))
+def test_calls_on_several_streams_keep_their_order(monkeypatch, seed):
+    """Pages that a call reads or writes are another call's before it, which the caller cannot see (forks share them, freed ones are
+    used again): work on one cache is ordered as its calls are, whatever streams they come on; reads beside reads are not."""
+    rng, fake = random.Random(seed), FakeStreams()
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda index: fake.current, raising=False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda index=None: fake.stream(fake.current))
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: fake.capturing)
+    monkeypatch.setattr(torch.cuda, "device", lambda index: contextlib.nullcontext())
+    monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: fake.held.append((t, s.cuda_stream)))
+    monkeypatch.setattr("gguf.hbm_cache.kv_append", lambda *args, **kw: fake.work(True))
+    monkeypatch.setattr("gguf.hbm_cache.kv_attend", lambda *args, **kw: fake.work(False))
+    monkeypatch.setattr("gguf.hbm_cache.kv_copy", lambda pages, src, dst: fake.work(True) if len(src) else None)
+    empty = hip.KVPages.empty
+
+    def made(*args):
+        pages = empty(*args[:-1], device="cpu")
+        pages.index = 0
+        fake.work(True)  # the zeros
+        return pages
+    monkeypatch.setattr("gguf.hbm_cache.KVPages.empty", made)
+    cache = HBMKVCache(1, 400, 2, 64, 16)
+    live, steps, x = [], [], torch.zeros(64, 2, 64, dtype=torch.bfloat16)
+    for _ in range(300):
+        fake.current = rng.choice((0, 0, 11, 22, 33)) if rng.random() < 0.5 else fake.current
+        fake.capturing = rng.random() < 0.1
+        what = rng.choice(("step", "append", "attend", "attend", "attend", "fork", "free", "compact", "refresh"))
+        if fake.capturing and what in ("step", "compact", "refresh"):
+            continue
+        if what == "step" or not steps:
+            if fake.capturing:
+                continue
+            live.append(cache.new() if not live or rng.random() < 0.5 else cache.fork(rng.choice(live)))
+            step = cache.step(live[-1:], [rng.randint(1, 20)], width=100)
+            steps = steps[-3:] + [(step, live[-1], fake.current)]
+        elif what == "append":
+            cache.append(0, rng.choice(steps)[0], x, x)
+        elif what == "attend":
+            step, _, made_on = rng.choice(steps)
+            cache.attend(0, step, x)
+            if fake.current != made_on and not fake.capturing:  # its tables are not to be used again before this is done
+                for t in (step.table, step.start, step.length, step.cu):
+                    assert any(u is t and s == fake.current for u, s in fake.held)
+        elif what == "refresh":
+            step, seq, _ = rng.choice(steps)
+            if seq in live and cache.length(seq) < 1000:
+                cache.refresh(step, [seq], step.counts)
+                fake.work(True)  # the graph's replay, on this stream
+        elif what == "fork" and live:
+            live.append(cache.fork(rng.choice(live)))
+        elif what == "free" and len(live) > 4:
+            cache.free(live.pop(rng.randrange(len(live))))
+        elif what == "compact":
+            cache.compact()
+    # two streams that only read wait for the last write, not for each other
+    fake.capturing, fake.current = False, 0
+    step = cache.step([live[-1]], [1])
+    cache.append(0, step, x, x)
+    for fake.current in (11, 22, 11, 22):
+        cache.attend(0, step, x)
+    assert fake.clocks[11].get(22, 0) < fake.log[-1][1] and fake.clocks[22].get(11, 0) < fake.log[-2][1]

@@ -12,10 +12,13 @@ what is live to the lowest page numbers. The lowest free page is always taken fi
     for layer in range(10):
         cache.append(layer, step, k, v)                       # k, v bf16 [tokens, kv_heads, head_dim]
         out = cache.attend(layer, step, q)                    # q bf16 [tokens, heads, head_dim]
+
+Calls may come on any streams: the cache orders its work as its calls are (_StreamOrder). A captured graph's replays it does
+not see: replay on the stream on which refresh() was called for it.
 """
 import contextlib
 import heapq
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 
 import numpy as np
 import torch
@@ -153,11 +156,49 @@ class KVStep:
     max_count: int
     max_length: int
     tokens: int           # of all sequences; a call's rows are these, and any padding behind them
+    streams: set = field(default_factory=set, repr=False)  # that the allocator knows to read the tensors
 
     def check(self, rows: torch.Tensor, name: str):
         """The book counts the step's tokens as written: fewer rows than those would leave some of them unwritten."""
         if rows.shape[0] < self.tokens:
             raise ValueError(f"{name} has {rows.shape[0]} rows, the step {self.tokens} tokens")
+
+
+class _StreamOrder:
+    """The order of one cache's work on the GPU: what writes pages comes after all calls before it, what reads them after every
+    write before it. Which pages those are the caller cannot see (a fork shares pages until one side writes, a freed page is
+    another sequence's next), so the cache itself makes the streams wait for each other where they change; on one stream that is a
+    comparison. A wait is for all that the other stream has enqueued by then, replayed graphs too. Streams that made a call
+    have to live as long as the cache."""
+
+    def __init__(self, index: int):
+        self.index, self.raw, self.writer, self.readers = index, None, None, {}
+        if index >= 0:
+            self(True)  # the cache's zeros
+
+    def __call__(self, writes: bool, step: KVStep = None):
+        if self.index < 0:
+            return
+        raw = torch._C._cuda_getCurrentRawStream(self.index)
+        known = step is None or raw in step.streams
+        if known and (raw == self.raw and not self.readers if writes else raw == self.raw or raw in self.readers):
+            return
+        with torch.cuda.device(self.index):
+            if torch.cuda.is_current_stream_capturing():  # this work runs at a replay
+                return
+        here = torch.cuda.current_stream(self.index)
+        if not known:
+            for t in (step.table, step.start, step.length, step.cu):
+                t.record_stream(here)
+            step.streams.add(raw)
+        if writes:
+            for other in (self.writer, *self.readers.values()):
+                if other is not None and other.cuda_stream != raw:
+                    here.wait_stream(other)
+            self.raw, self.writer, self.readers = raw, here, {}
+        elif raw != self.raw and raw not in self.readers:
+            here.wait_stream(self.writer)
+            self.readers[raw] = here
 
 
 class HBMKVCache:
@@ -169,6 +210,7 @@ class HBMKVCache:
         self.pages = KVPages.empty(layers, pages, kv_heads, head_dim, page_tokens, dtype, device)
         self.device = self.pages.device
         self.book = PageBook(pages, page_tokens)
+        self._order = _StreamOrder(self.pages.index)
 
     def nbytes(self) -> int:
         return self.pages.nbytes()
@@ -194,6 +236,7 @@ class HBMKVCache:
         """Moves the live pages to the lowest numbers -> how many moved. Steps made before hold pages that are no longer
         theirs: make them anew. Not under capture."""
         self._not_captured()
+        self._order(True)
         src, dst = self.book.compact()
         kv_copy(self.pages, src, dst)
         return len(src)
@@ -210,6 +253,7 @@ class HBMKVCache:
     def _host_step(self, seqs, counts, width):
         self._not_captured()
         src, dst = self.book.grow(seqs, counts)
+        self._order(True)
         kv_copy(self.pages, src, dst)
         n = len(seqs)
         rows = [self.book.sequences[s] for s in seqs]
@@ -243,8 +287,9 @@ class HBMKVCache:
         host, start, length, cu = self._host_step(list(seqs), counts, width)
         with self._given_back(seqs, counts):
             up = [torch.from_numpy(a).to(self.device) for a in (host, start, length, cu)]
-        return KVStep(*up, counts, max(counts),
-                      int(length.max()) if width is None else width * self.book.page_tokens, int(cu[-1]))
+        streams = {self._order.raw}  # the one that this was made on
+        return KVStep(*up, counts, max(counts), int(length.max()) if width is None else width * self.book.page_tokens, int(cu[-1]),
+                      streams)
 
     def _check_width(self, seqs, counts, width):
         for s, c in zip(seqs, counts):
@@ -259,6 +304,7 @@ class HBMKVCache:
             raise ValueError(f"the step was made for {step.table.shape[0]} sequences with counts {step.counts}")
         self._check_width(seqs, counts, step.table.shape[1])
         host, start, length, _ = self._host_step(list(seqs), counts, step.table.shape[1])
+        self._order(True, step)
         with self._given_back(seqs, counts):
             for t, a in ((step.table, host), (step.start, start), (step.length, length)):
                 t.copy_(torch.from_numpy(a))
@@ -268,6 +314,7 @@ class HBMKVCache:
     def append(self, layer: int, step: KVStep, k: torch.Tensor, v: torch.Tensor):
         """The step's new keys and values of one layer, bf16 [tokens, kv_heads, head_dim]; kv_append."""
         step.check(k, "k")
+        self._order(True, step)
         kv_append(self.pages, layer, k, v, step.table, step.start, step.cu, max_count=step.max_count or 1)
 
     def attend(self, layer: int, step: KVStep, q: torch.Tensor, scale: float = None, causal: bool = True,
@@ -278,5 +325,6 @@ class HBMKVCache:
         if out is None and q.shape[0] > step.tokens:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             out[step.tokens:].zero_()
+        self._order(False, step)
         return kv_attend(self.pages, layer, q, step.table, step.length, step.cu, max_count=step.max_count or 1,
                          max_length=step.max_length, scale=scale, causal=causal, out=out)
