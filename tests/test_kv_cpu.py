@@ -675,3 +675,26 @@ def test_calls_on_several_streams_keep_their_order(monkeypatch, seed):
     for fake.current in (11, 22, 11, 22):
         cache.attend(0, step, x)
     assert fake.clocks[11].get(22, 0) < fake.log[-1][1] and fake.clocks[22].get(11, 0) < fake.log[-2][1]
+
+
+def test_a_step_that_was_not_run_is_taken_back():
+    """Where a layer fails, truncating to the lengths before it takes the step back: the book is as after that, whether pages were
+    begun, filled or copied for it, and the next step writes the same positions."""
+    book = PageBook(12, 16)
+    c = Contents(book)
+    a, b = book.new(), book.new()
+    c.want[a], c.want[b] = [], []
+    c.grow([a], [20], 0)
+    f = book.fork(a)
+    c.want[f] = list(c.want[a])
+    before = {s: book.length(s) for s in (a, b, f)}
+    for counts in ((1, 40, 13), (12, 16, 1)):
+        c.copy(*book.grow([a, b, f], list(counts)))  # and nothing is written
+        for s, n in zip((a, b, f), counts):
+            book.truncate(s, book.length(s) - n)
+        assert {s: book.length(s) for s in (a, b, f)} == before
+        check_book(book)
+        c.check()
+    c.grow([a, b, f], [3, 3, 3], 1)
+    c.check()
+    check_book(book)

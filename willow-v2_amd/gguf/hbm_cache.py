@@ -278,7 +278,9 @@ class HBMKVCache:
     def step(self, seqs, counts, width: int = None) -> KVStep:
         """Room for counts[i] new tokens of sequence seqs[i], which count as its own from here on -> what append and attend
         take. Pages that a fork shares and that are about to be written are copied. width: pages the table has columns for
-        (for refresh() of longer sequences; default: as many as the longest has). The tables are uploaded: not under capture."""
+        (for refresh() of longer sequences; default: as many as the longest has). The tables are uploaded: not under capture.
+        The tokens count as written at once: append them on every layer before the sequences are forked, compacted or in another
+        step, and where a layer fails take the step back, truncate(seq, length(seq) - count) for each sequence."""
         if not seqs:
             raise ValueError("a step needs a sequence")
         counts = [_whole(c) for c in counts]
