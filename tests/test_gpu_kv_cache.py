@@ -1,6 +1,7 @@
 """HBMKVCache, the rotary positions and HipAttention together on the GPU, as a model's loop uses them: prompts, decoding,
 forks, truncation, compaction, HIP graphs, several streams; against oracle/kv_ref.py on the cache's own contents."""
 import random
+import types
 
 import numpy as np
 import pytest
@@ -416,3 +417,103 @@ def test_calls_on_changing_streams(hip, seed):
             assert all(torch.equal(a, b) for a, b in zip(mine, pools))
     finally:
         torch.cuda.set_stream(streams[0])
+
+
+def worst(got, want, bound):
+    """The largest error over its bound."""
+    return float(((got.cpu().double() - want).abs() / (bound + 1e-300)).max())
+
+
+@pytest.mark.parametrize("gated,quantized,norm", [(True, False, True), (False, False, False), (True, True, True), (True, False, False)])
+def test_engine_attention_link_by_link(hip, monkeypatch, gated, quantized, norm):
+    """HipAttention's every link against its formula in 64 bits, each on what the link before it gave, so that a bound holds just the
+    link's own roundings; and what a wrong link would give lies far outside of it: a result of zeros, a query that is not turned,
+    one that is not normed, attention to later tokens, a gate left out, the gate's half taken for the query's."""
+    g = torch.Generator().manual_seed(15)
+    eng, heads, dim = engine(g, gated, quantized, norm)
+    cache, p, seen = eng.kv_cache, "model.layers.3.self_attn", {}
+    turn, append, attend, linear = eng.rotary, cache.append, cache.attend, F.linear
+
+    def rotary(q, k, positions):
+        seen["q in"], seen["k in"] = q, k
+        seen["q"], seen["k"] = turn(q, k, positions)
+        return seen["q"], seen["k"]
+
+    def append_(layer, step, k, v):
+        seen["k kept"], seen["v kept"] = k, v
+        return append(layer, step, k, v)
+
+    def attend_(layer, step, q, **kw):
+        seen["q asked"], seen["o"] = q, attend(layer, step, q, **kw)
+        return seen["o"].clone()
+
+    def linear_(x, w):
+        name = next(n for n in ("q", "k", "v", "o") if eng.weights[f"{p}.{n}_proj.weight"] is w)
+        seen[name + " from"], seen[name + " proj"] = x, linear(x, w)
+        return seen[name + " proj"]
+    eng.rotary, cache.append, cache.attend = rotary, append_, attend_
+    monkeypatch.setattr("engines.qwen36.attention_hip.F", types.SimpleNamespace(linear=linear_))
+
+    def normed(x, name):
+        w = eng.weights.get(f"{p}.{name}_norm.weight")
+        return x if w is None else x * torch.rsqrt(x.square().mean(-1, keepdim=True) + 1e-6) * (1 + w.double())
+    seqs, at = [cache.new(), cache.new()], [0, 0]
+    for counts in ((21, 9), (1, 1), (1, 3), (17, 2)):
+        n = sum(counts)
+        x = bf16(g, n, 256, scale=2.0 ** -9 if quantized else 1.0)
+        step = cache.step(seqs, counts)
+        ids = torch.cat([torch.arange(a, a + c) for a, c in zip(at, counts)])
+        at = [a + c for a, c in zip(at, counts)]
+        positions = turn.positions(torch.stack((ids, ids // 3, ids % 5)))
+        y = eng.hip_attention(x, 3, 0, step, positions)
+        # the projections of x (quantized ones have tests of their own): 256 products in fp32, one rounding
+        for name in "qkv":
+            assert torch.equal(seen[name + " from"], x)
+            if not quantized:
+                w = eng.weights[f"{p}.{name}_proj.weight"].cpu().double()
+                want = x.cpu().double() @ w.T
+                bound = 2.0 ** -8 * want.abs() + 2.0 ** -14 * (x.cpu().double().abs() @ w.T.abs())  # 257 * 2^-23 < 2^-14
+                assert worst(seen[name + " proj"], want, bound) <= 1
+        # each head's query, its gate behind it; norms in fp32 (64 squares, a root, two products: under 2^-16), one rounding
+        wide = seen["q proj"].cpu().double()
+        q, gate = wide.view(n, heads, 2, dim).unbind(2) if gated else (wide.view(n, heads, dim), None)
+        k = seen["k proj"].cpu().double().view(n, 2, dim)
+        for name, raw in (("q", q), ("k", k)):
+            want = normed(raw, name)
+            bound = (2.0 ** -8 + 2.0 ** -15) * want.abs() if norm else 0 * want
+            assert worst(seen[name + " in"], want, bound) <= 1
+            if norm:
+                assert worst(seen[name + " in"], raw, bound) > 10
+        if gated:
+            assert worst(seen["q in"], normed(gate, "q"), (2.0 ** -8 + 2.0 ** -15) * want.abs().max()) > 10
+        # positions
+        for name in "qk":
+            z = seen[name + " in"].cpu().double()
+            want = kv_ref.rope(z, positions.cpu(), turn.inv_freq.cpu(), (6, 5, 5), True)
+            pair = torch.zeros_like(z)
+            pair[..., :32] = (z[..., :16].abs() + z[..., 16:32].abs()).repeat(1, 1, 2)
+            bound = pair * 2.0 ** -20 + want.abs() * 2.0 ** -8
+            assert worst(seen[name], want, bound) <= 1
+        assert seen["q asked"] is seen["q"] and seen["k kept"] is seen["k"]
+        assert torch.equal(seen["v kept"], seen["v proj"].view(n, 2, dim))
+        # attention over what the cache holds
+        want, tol = oracle_attend(cache, 0, step, seen["q"])
+        assert worst(seen["o"], want, tol) <= 1
+        assert worst(torch.zeros_like(want), want, tol) > 10
+        assert worst(seen["o"], *oracle_attend(cache, 0, step, seen["q in"])) > 4
+        assert worst(seen["o"], *oracle_attend(cache, 0, step, seen["q"].flip(1))) > 10
+        if max(counts) > 4:
+            assert worst(seen["o"], *oracle_attend(cache, 0, step, seen["q"], causal=False)) > 10
+        # the gate: a sigmoid and a product in fp32, one rounding; then 256 products in fp32 and one rounding
+        o = seen["o"].cpu().double()
+        w = eng.weights[f"{p}.o_proj.weight"].cpu().double()
+        if gated:
+            o = o * torch.sigmoid(gate)
+        o = o.reshape(n, -1)
+        assert worst(seen["o from"], o, (2.0 ** -8 + 2.0 ** -20) * o.abs() if gated else 0 * o) <= 1
+        if gated:
+            assert worst(seen["o from"], seen["o"].cpu().double().reshape(n, -1), 2.0 ** -7 * o.abs()) > 10
+        z = seen["o from"].cpu().double()
+        want = z @ w.T
+        assert worst(y, want, 2.0 ** -8 * want.abs() + 2.0 ** -14 * (z.abs() @ w.T.abs())) <= 1
+        assert torch.equal(y, seen["o proj"])
