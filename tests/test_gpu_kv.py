@@ -515,3 +515,86 @@ def test_rope_into_rows_that_share_memory(hip):
     assert torch.equal(a, torch.zeros_like(q))
     apart = torch.zeros(2, 4, 64, device=DEV).transpose(0, 1)  # heads outermost
     assert torch.equal(hip.rope(q, None, p, f, out=(apart, None))[0], hip.rope(q, None, p, f)[0])
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("dim,page,counts,starts", [(256, 128, (300,), (37,)), (64, 1024, (1500,), (3,)), (128, 512, (700, 513), (0, 511)),
+                                                    (256, 1024, (2100,), (1023,))])
+@pytest.mark.parametrize("layout", ["fused", "odd"])
+def test_append_large_blocks(hip, dtype, dim, page, counts, starts, layout):
+    """Blocks with more new values than the threads keep (16384): what is beyond is read a second time."""
+    g = gen(dim + page + 1)
+    pages = random_pages(hip, g, 1, 6, 2, page, dim, dtype)
+    table = table_of(g, [c + s for c, s in zip(counts, starts)], page, 6)
+    wide = torch.randn(sum(counts), 2, 2, dim + (3 if layout == "odd" else 0), generator=g)
+    wide[:, 0] *= 1 + 20 * (torch.rand(wide.shape[-1], generator=g) < 0.05)
+    wide[-1, :, :, 5] = 90.0  # the largest of the last block is in its last row
+    x = wide.to(torch.bfloat16).to(DEV)[..., 1 if layout == "odd" else 0:][..., :dim]
+    check_append(hip, pages, 0, x[:, 0], x[:, 1], table, i32(starts), cu_of(counts))
+
+
+@pytest.mark.parametrize("count", [1, 20])
+@pytest.mark.parametrize("dim,page", [(256, 64), (128, 64), (64, 128), (256, 32), (128, 1024)])
+def test_attend_nan_stays_where_it_is_on_whole_pages(hip, dim, page, count):
+    """As on small pages, where a page holds whole tiles: stray e4m3 NaN bytes reach no row, a NaN scale just the rows that see its
+    block, missing pages nobody."""
+    g = gen(21)
+    lengths = [n * page // 32 for n in (75, 130, 40)]
+    pages = random_pages(hip, g, 1, 10, 2, page, dim, torch.float8_e4m3fn)
+    table = table_of(g, lengths, page, 10)
+    raw_k, raw_v = pages.k.view(torch.uint8), pages.v.view(torch.uint8)
+    used = set()
+    for b, n in enumerate(lengths):
+        for c in range(-(-n // page)):
+            p = int(table[b, c])
+            used.add(p)
+            raw_k[0, p, :, max(0, n - page * c):] = 0x7F
+            raw_v[0, p, :, :, max(0, n - page * c):] = 0xFF
+    for p in set(range(10)) - used:
+        raw_k[0, p], raw_v[0, p] = 0x7F, 0x7F
+        pages.k_scale[0, p], pages.v_scale[0, p] = math.nan, math.nan
+    q = torch.randn(3 * count, 4, dim, generator=g).to(torch.bfloat16).to(DEV)
+    args = (i32(lengths), cu_of((count,) * 3))
+    for causal in (True, False):
+        out = check_attend(hip, pages, 0, q, table, *args, causal=causal)
+        assert torch.isfinite(out.float()).all()
+        missing = table.clone()
+        missing[1, 2], missing[2, 0], missing[0, 0] = -1, 10, 2 ** 31 - 1
+        check_attend(hip, pages, 0, q, missing, *args, causal=causal)
+    last = int(table[1, 4])
+    for scale, head in ((pages.v_scale, 1), (pages.k_scale, 0)):
+        scale[0, last, head] = math.nan  # the last tokens of sequence 1
+        out = check_attend(hip, pages, 0, q, table, *args)
+        assert torch.isnan(out[2 * count - 1, 2 * head:2 * head + 2].float()).all()
+    seen = torch.isnan(check_attend(hip, pages, 0, q, table, *args).float())
+    assert seen[2 * count - 1].all() and not seen[:count].any() and not seen[2 * count:].any()
+
+
+@pytest.mark.parametrize("dim,kv_heads,seqs", [(64, 8, 64), (128, 8, 64), (64, 16, 33)])
+def test_attend_one_long_sequence_among_many(hip, dim, kv_heads, seqs):
+    """As many short (sequence, kv head)s as leave nothing to be cut, and a long one among them."""
+    g = gen(22)
+    lengths = [7 + i % 90 for i in range(seqs)]
+    lengths[seqs // 2] = 6000
+    need = sum(-(-n // 64) for n in lengths)
+    pages = random_pages(hip, g, 1, need, kv_heads, 64, dim, torch.int8)
+    table = table_of(g, lengths, 64, need)
+    q = torch.randn(5 * seqs, 4 * kv_heads, dim, generator=g).to(torch.bfloat16).to(DEV)
+    check_attend(hip, pages, 0, q, table, i32(lengths), cu_of([5] * seqs), max_count=5)
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+@pytest.mark.parametrize("heads,kv_heads,dim,count", [(16, 2, 256, 1), (16, 2, 256, 40), (32, 8, 128, 4), (32, 8, 128, 30), (8, 8, 64, 20)])
+def test_attend_error_as_a_whole(hip, dtype, heads, kv_heads, dim, count):
+    """The 2-norm of the error over that of the result, for a long cache, where the largest possible error says little. Independent
+    values: rounding the result leaves 2^-8 / sqrt(3) at most (an error spread evenly over a step, of the smallest significand), and
+    rounding the weights as much again, since weights and result have the same relative spread."""
+    g = gen(23)
+    lengths, seqs = (3000, 2500), 2
+    pages = random_pages(hip, g, 1, 90, kv_heads, 64, dim, dtype)
+    table = table_of(g, lengths, 64, 90)
+    q = torch.randn(count * seqs, heads, dim, generator=g).to(torch.bfloat16).to(DEV)
+    out = hip.kv_attend(pages, 0, q, table, i32(lengths), cu_of([count] * seqs), max_count=count).cpu().double()
+    want, _ = kv_ref.attend(pages.k[0].cpu(), pages.v[0].cpu(), pages.k_scale[0].cpu(), pages.v_scale[0].cpu(), q.cpu(), table.cpu(),
+                            i32(lengths).cpu(), cu_of([count] * seqs).cpu())
+    assert (out - want).norm() <= 2 ** 0.5 * 2.0 ** -8 / 3 ** 0.5 * want.norm()
