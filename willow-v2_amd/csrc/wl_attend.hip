@@ -427,9 +427,11 @@ bool is_few(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
 FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length) {
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
     const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
-    // two rounds of a workgroup cost what one and the join do: 300 tokens of 8 sequences of 8 kv heads of 128 8.3 against 10.4
-    // us, 500 tokens of 64 sequences of 2 heads of 256 16.0 against 17.8, of one sequence 14.5 against 13.5; three (700
-    // tokens, one sequence) 18.5 against 13.4
+    // Two rounds of a workgroup cost less than one and the join: 500 tokens of 1 to 256 sequences on 8 kv heads of 128 9.2 to 45.6
+    // against 10.1 to 61.5 us in a graph, on 8 of 64 5.8 to 24.1 against 8.3 to 32.8, of 32 to 256 on 2 of 256 15.3 to 28.0 against
+    // 16.1 to 35.0; 300 tokens of 1 to 256 of those 12.6 to 21.5 against 13.2 to 28.5. Only where 256 dimensions, more than about
+    // 400 tokens and at most 31 sequences meet do they cost more (500 tokens of one 14.2 against 13.3): the rule is not made finer
+    // for that. Three rounds cost more in general (700 tokens of one sequence 18.5 against 13.4).
     if (longest <= kTile * kFewWaves * 2) return {items, true};
     // no more shares than the bound says there can be: a workgroup without one still costs its start
     const int64_t each = (longest + kTile * kFewWaves - 1) / (kTile * kFewWaves);

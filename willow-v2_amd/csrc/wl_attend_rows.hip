@@ -41,6 +41,7 @@ struct RowsArgs : AttendArgs {
     int32_t* each;       // tiles that a piece has at most, as the first kernel found it for the second
     int32_t row_tiles;   // of 256 rows, in a sequence, at most
     int32_t pieces;      // a row tile's cache is cut into at most this many
+    int32_t few_tiles;   // less than 2 kCus (row tile, kv head)s
 };
 
 // What a part of 16 tokens needs beside its bytes. V's scale goes into the exponent, so that a weight comes out of its exp2
@@ -308,7 +309,9 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
     total = 0;
     for (int i = 0; i < kWaves; i++) total += lds.sums[i];
     int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast);
-    if (a.pieces > 1) {
+    if (a.pieces > 1 && !a.few_tiles) {
+        each += each / 2;  // more than a CU's share alone, see rows_plan
+    } else if (a.pieces > 1) {
         // A CU's share of the whole, or up to three quarters more of it where that brings the pieces down to one a CU: every
         // row tile's last piece makes them more than the shares are, and the few that are left over run on alone
         // (512 tokens of 16 on 2 heads of 256 behind 16000: 243 us without, 170 with; five ragged prompts of up to 301 of 32
@@ -539,10 +542,16 @@ __global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge(RowsArgs a) {
 
 // How the row tiles' caches are cut. Calls of few row tiles would leave CUs idle, and a causal prompt's last row tiles would
 // run on alone: a cache is cut into pieces of a CU's share of the whole where that is less. From twice as many row tiles as
-// CUs on, taking the large ones first is enough, and nothing is cut.
+// CUs on, taking the large ones first is enough while none is more than a CU's share: so for the rows of one sequence, which see
+// the same cache or up to it. Of several sequences one may be far longer than the others, which the device alone sees: where its
+// tiles would take longer than the second kernel costs, a row tile of more than one and a half shares is cut (64 sequences of 8 kv
+// heads of 128, 5 tokens each, of which one has 100000 in the cache, the others 100: 2616 us without, 183 with; all of them 5000:
+// 280 and 286; all 100 with a bound that says 8192: 17.3 and 20.9). Where there is no room for at least four pieces, the rows are so many that none stands out.
 struct RowsPlan {
     int64_t row_tiles, pieces, groups;
+    bool few_tiles;
 };
+constexpr int kLong = 64;  // tiles: about 80 us for one workgroup
 RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
     const int64_t tokens = 8192 / c->head_dim, group = q_heads / c->kv_heads;
     const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
@@ -550,12 +559,13 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     // (row tile, kv head)s: as many as the sequences' most rows have room for, and no more than all rows together fill
     const int64_t items = std::min(row_tiles * b->seqs, b->tokens * group / kGroupRows + b->seqs) * c->kv_heads;
     const int64_t most = (longest + tokens - 1) / tokens;  // tiles of the last row tile
-    if (items >= 2 * kCus) return {row_tiles, 1, items};
     // how many pieces come of it is known on the device alone: room for as many as the partial results may take
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
+    const bool few_tiles = items < 2 * kCus;
+    if (!few_tiles && (b->seqs == 1 || most < kLong || room < 4)) return {row_tiles, 1, items, false};
     const int64_t pieces = std::max<int64_t>(1, std::min({int64_t{kMaxPieces}, (most + kLeast - 1) / kLeast, room}));
     // the pieces of n tiles are less than n / each + 1, those of all (row tile, kv head)s less than kCus + items
-    return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus)};
+    return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus), few_tiles};
 }
 
 }  // namespace
@@ -586,6 +596,7 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     a.partial_ml = reinterpret_cast<float2*>(a.partial + p.pieces * b->tokens * call.q_heads * c->head_dim);
     a.row_tiles = static_cast<int32_t>(p.row_tiles);
     a.pieces = static_cast<int32_t>(p.pieces);
+    a.few_tiles = p.few_tiles;
     const dim3 grid(static_cast<uint32_t>(p.groups));
     const dim3 merge(static_cast<uint32_t>(merge_groups(c, call.group, b)), b->seqs);
     auto run = [&](auto type, auto dim) {
