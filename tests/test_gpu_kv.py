@@ -598,3 +598,38 @@ def test_attend_error_as_a_whole(hip, dtype, heads, kv_heads, dim, count):
     want, _ = kv_ref.attend(pages.k[0].cpu(), pages.v[0].cpu(), pages.k_scale[0].cpu(), pages.v_scale[0].cpu(), q.cpu(), table.cpu(),
                             i32(lengths).cpu(), cu_of([count] * seqs).cpu())
     assert (out - want).norm() <= 2 ** 0.5 * 2.0 ** -8 / 3 ** 0.5 * want.norm()
+
+
+@pytest.mark.parametrize("dim,kv_heads,group,seqs,count,far", [
+    (64, 16, 4, 33, 5, (9000, 8300)), (128, 8, 4, 70, 5, (5000, 4100, 4500)), (256, 2, 8, 260, 3, (2100, 4000)), (128, 8, 2, 40, 200, (6000,))])
+def test_attend_long_ones_are_cut(hip, dim, kv_heads, group, seqs, count, far):
+    """From 512 (row tile, kv head)s on, where the bound of the lengths allows for long ones: some are, among short ones, ones without
+    rows and ones without tokens. The same with a bound that is far too small (nothing is cut) or none, and with any workspace."""
+    g = gen(24)
+    rng = np.random.default_rng(24)
+    lengths = [int(x) for x in rng.integers(0, 120, seqs)]
+    counts = [int(x) for x in rng.integers(0, count + 1, seqs)]
+    for i, n in enumerate(far):
+        lengths[5 + 7 * i], counts[5 + 7 * i] = n, count
+    lengths[seqs - 1], counts[0] = 0, 0
+    need = sum(-(-n // 64) for n in lengths)
+    pages = random_pages(hip, g, 1, need, kv_heads, 64, dim, torch.float8_e4m3fn)
+    table = table_of(g, lengths, 64, need)
+    q = torch.randn(sum(counts), group * kv_heads, dim, generator=g).to(torch.bfloat16).to(DEV)
+    args = (q, table, i32(lengths), cu_of(counts))
+    rows_of = [5 + 7 * i for i in range(len(far))]
+    bounds = args[3].tolist()
+    out = hip.kv_attend(pages, 0, *args, max_count=count)
+    some = sorted({r for b in rows_of for r in (bounds[b], bounds[b + 1] - 1)} | set(range(0, q.shape[0], max(1, q.shape[0] // 60))))
+    cache = [x[0].cpu() for x in (pages.k, pages.v, pages.k_scale, pages.v_scale)]
+    for r in some:
+        b = next(b for b in range(seqs) if bounds[b] <= r < bounds[b + 1])
+        seen = lengths[b] - (bounds[b + 1] - 1 - r)
+        want, tol = kv_ref.attend(*cache, q[r:r + 1].cpu(), table[b:b + 1].cpu(), torch.tensor([max(seen, 0)]), torch.tensor([0, 1]))
+        assert ((out[r].cpu().double() - want[0]).abs() <= tol[0]).all(), (r, b)
+    assert torch.equal(out, hip.kv_attend(pages, 0, *args, max_count=count, max_length=max(far)))
+    ws = torch.full((300 << 20,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(out, hip.kv_attend(pages, 0, *args, max_count=count, workspace=ws))
+    uncut = hip.kv_attend(pages, 0, *args, max_count=count, max_length=64)
+    # both lie within their bound of the exact result: 2^-8 of themselves and of the mean weighted value
+    assert (out.float() - uncut.float()).abs().max() <= 2.0 ** -5 * out.float().abs().max()

@@ -430,7 +430,7 @@ FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length) {
     // Two rounds of a workgroup cost less than one and the join: 500 tokens of 1 to 256 sequences on 8 kv heads of 128 9.2 to 45.6
     // against 10.1 to 61.5 us in a graph, on 8 of 64 5.8 to 24.1 against 8.3 to 32.8, of 32 to 256 on 2 of 256 15.3 to 28.0 against
     // 16.1 to 35.0; 300 tokens of 1 to 256 of those 12.6 to 21.5 against 13.2 to 28.5. Only where 256 dimensions, more than about
-    // 400 tokens and at most 31 sequences meet do they cost more (500 tokens of one 14.2 against 13.3): the rule is not made finer
+    // 400 tokens and at most 16 sequences meet do they cost more (500 tokens of one 14.2 against 13.3): the rule is not made finer
     // for that. Three rounds cost more in general (700 tokens of one sequence 18.5 against 13.4).
     if (longest <= kTile * kFewWaves * 2) return {items, true};
     // no more shares than the bound says there can be: a workgroup without one still costs its start
