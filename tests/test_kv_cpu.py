@@ -698,3 +698,10 @@ def test_a_step_that_was_not_run_is_taken_back():
     c.grow([a, b, f], [3, 3, 3], 1)
     c.check()
     check_book(book)
+
+
+def test_rotary_frequencies_stay_in_64_bits():
+    """Frequencies given as plain numbers: a fp32 one is off by 2^-25 of itself, 3e-3 of a turn's angle at position 10^6."""
+    want = [0.1, 1 / 3, 7e-5, 1.0]
+    for given in (want, tuple(want), torch.tensor(want, dtype=torch.float64), __import__("numpy").array(want)):
+        assert Rotary(8, 8, inv_freq=given, device="cpu").inv_freq.tolist() == want

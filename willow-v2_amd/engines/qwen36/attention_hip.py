@@ -35,7 +35,7 @@ class Rotary:
             raise ValueError(f"sections {self.sections} must add up to rotary_dim / 2 = {half}")
         if inv_freq is None:
             inv_freq = theta ** (-torch.arange(half, dtype=torch.float64) / half)
-        self.inv_freq = torch.as_tensor(inv_freq).to(device=device, dtype=torch.float64).contiguous()
+        self.inv_freq = torch.as_tensor(inv_freq, dtype=torch.float64).to(device).contiguous()
         if self.inv_freq.shape != (half,):
             raise ValueError(f"inv_freq must have {half} entries")
         self.interleaved, self.scale = bool(interleaved), float(scale)
