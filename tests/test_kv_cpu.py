@@ -705,3 +705,15 @@ def test_rotary_frequencies_stay_in_64_bits():
     want = [0.1, 1 / 3, 7e-5, 1.0]
     for given in (want, tuple(want), torch.tensor(want, dtype=torch.float64), __import__("numpy").array(want)):
         assert Rotary(8, 8, inv_freq=given, device="cpu").inv_freq.tolist() == want
+
+
+@pytest.mark.parametrize("width", [2.5, 4.0, "4", 1 << 40])
+def test_widths_that_make_no_table(width):
+    """No table comes of such a width: nothing is counted."""
+    cache = HBMKVCache(1, 8, 2, 64, 16, device="cpu")
+    a = cache.new()
+    cache.step([a], [3])
+    with pytest.raises((TypeError, ValueError, MemoryError)):
+        cache.step([a], [20], width=width)
+    assert cache.length(a) == 3 and cache.book.used() == 1
+    check_book(cache.book)

@@ -250,30 +250,31 @@ class HBMKVCache:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("a cache's step(), refresh() and compact() cannot be captured into a graph")
 
-    def _host_step(self, seqs, counts, width):
-        self._not_captured()
-        src, dst = self.book.grow(seqs, counts)
-        self._order(True)
-        kv_copy(self.pages, src, dst)
-        n = len(seqs)
-        rows = [self.book.sequences[s] for s in seqs]
-        host = np.full((n, width or max([1] + [len(r[1]) for r in rows])), -1, dtype=np.int32)
-        for i, r in enumerate(rows):
-            host[i, :len(r[1])] = r[1]
-        length = np.array([r[0] for r in rows], dtype=np.int32)
-        start = length - np.array(counts, dtype=np.int32)
-        cu = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
-        return host, start, length, cu
-
     @contextlib.contextmanager
     def _given_back(self, seqs, counts):
-        """Takes the step's tokens off the book again where its tables do not reach the device."""
+        """Takes the step's tokens off the book again where its tables are not made, or do not reach the device."""
         try:
             yield
         except BaseException:
             for s, n in zip(seqs, counts):
                 self.book.truncate(s, self.book.length(s) - n)
             raise
+
+    def _host_step(self, seqs, counts, width):
+        self._not_captured()
+        src, dst = self.book.grow(seqs, counts)
+        self._order(True)
+        kv_copy(self.pages, src, dst)
+        with self._given_back(seqs, counts):
+            n = len(seqs)
+            rows = [self.book.sequences[s] for s in seqs]
+            host = np.full((n, width or max([1] + [len(r[1]) for r in rows])), -1, dtype=np.int32)
+            for i, r in enumerate(rows):
+                host[i, :len(r[1])] = r[1]
+            length = np.array([r[0] for r in rows], dtype=np.int32)
+            start = length - np.array(counts, dtype=np.int32)
+            cu = np.concatenate(([0], np.cumsum(counts))).astype(np.int32)
+            return host, start, length, cu
 
     def step(self, seqs, counts, width: int = None) -> KVStep:
         """Room for counts[i] new tokens of sequence seqs[i], which count as its own from here on -> what append and attend
