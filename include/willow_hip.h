@@ -44,7 +44,8 @@ extern "C" {
 #define WL_EINVAL_COUNT -8     /* too many experts for one batched call */
 #define WL_EINVAL_SCRATCH -9   /* wl_moe_layer_noalloc: the call needs more than WL_NOALLOC_SCRATCH_BYTES */
 #define WL_ESYNC -10           /* wl_moe_workspace_status: a bounded wait gave up since the last query */
-#define WL_EINVAL_OVERLAP -11  /* wl_moe_layer: y overlaps x; wl_kv_attend: out overlaps q */
+#define WL_EINVAL_OVERLAP -11  /* wl_moe_layer: y overlaps x; wl_kv_attend: out overlaps q; wl_rope: one
+                                  tensor's out is the other's in or out */
 #define WL_EINVAL_SCOPE -12    /* wl_moe_fork_begin with a scope open on the device; wl_moe_fork_end without one on
                                   this stream */
 

@@ -457,7 +457,7 @@ def test_rope_rows_lie_apart(side, heads, token, head, apart):
     assert apart == all(b - a >= dim for a, b in zip(at, at[1:]))
     lib, sections = hip.library(), (ctypes.c_int32 * 1)(16)
     good = hip.WlRopeTensor(FAKE, FAKE, 256, 64, 256, 64, 4, 0)
-    over = hip.WlRopeTensor(FAKE, FAKE, 256, 64, token, head, heads, 0)
+    over = hip.WlRopeTensor(3 * FAKE, 3 * FAKE, 256, 64, token, head, heads, 0)
     # positions on no 8-byte address are refused behind the tensors: what a call ends with whose tensors are right
     rc = lib.wl_rope(over if side == "q" else good, over if side == "k" else None, 1, tokens, dim, 32, FAKE + 4, tokens, FAKE, 1,
                      sections, 1, 1.0, None)
@@ -717,3 +717,17 @@ def test_widths_that_make_no_table(width):
         cache.step([a], [20], width=width)
     assert cache.length(a) == 3 and cache.book.used() == 1
     check_book(cache.book)
+
+
+def test_rope_results_apart_from_the_other_tensor():
+    """q's result where k is read or written, or k's where q is read, would be read or written in no order."""
+    lib, sections = hip.library(), (ctypes.c_int32 * 1)(16)
+
+    def call(q, k):
+        q, k = (hip.WlRopeTensor(a, b, 256, 64, 256, 64, 4, 0) for a, b in (q, k))
+        return lib.wl_rope(q, k, 1, 4, 64, 32, FAKE + 4, 4, FAKE, 1, sections, 1, 1.0, None)
+    a, b, c, d = (FAKE * i for i in (1, 2, 3, 4))
+    for q, k in (((a, b), (c, b)), ((a, b), (b, c)), ((a, b), (c, a)), ((a, a), (a, a)), ((a, a), (a, b)), ((a, b), (a, a))):
+        assert call(q, k) == -11
+    for q, k in (((a, b), (c, d)), ((a, a), (b, b)), ((a, a), (b, c)), ((a, b), (a, c))):
+        assert call(q, k) == -4  # the positions, which are looked at last

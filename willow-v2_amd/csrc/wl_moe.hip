@@ -1743,7 +1743,8 @@ const char* wl_error_string(int code) {
         case WL_EINVAL_WORKSPACE: return "workspace is NULL or smaller than wl_moe_workspace_bytes()";
         case WL_EINVAL_DTYPE: return "output dtype must be WL_DTYPE_F32 or WL_DTYPE_BF16";
         case WL_EINVAL_COUNT: return "expert count must be in 1..64";
-        case WL_EINVAL_OVERLAP: return "y overlaps x (out overlaps q): it is written while that is still being read";
+        case WL_EINVAL_OVERLAP:
+            return "y overlaps x (out overlaps q, or another tensor): it is written while that is still being read";
         case WL_ESYNC:
             return "a bounded wait gave up: a fused-kernel workgroup waiting for another (not every workgroup was "
                    "resident; those outputs hold NaN) or a fork-scope hand-off (the scope's MFMA experts were "

@@ -175,6 +175,8 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
         return WL_EINVAL_SHAPE;
     for (const WlRopeTensor* x : {q, k})
         if (x && !rows_apart(x->out_token_stride, x->out_head_stride, tokens, x->heads, head_dim)) return WL_EINVAL_SHAPE;
+    // one tensor's result where the other is read or written
+    if (k && (q->out == k->out || q->out == k->in || k->out == q->in)) return WL_EINVAL_OVERLAP;
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return WL_EINVAL_ALIGN;
     RopeArgs a = {};
     a.half = rotary_dim / 2;
