@@ -11,12 +11,13 @@
 // The running maximum is moved only when a score exceeds it by 2^8 (the weights stay below 2^8, fp32 sums hold them): the
 // multiplication of a wavefront's 32 x D sums by the change is the dearest step of the softmax, and becomes rare.
 // Bound by what a wavefront does between its products: 4096 tokens of 16 heads of 256 on 2 kv heads take 185 to 200 us (the
-// card in hand), 740 to 690 TFLOP/s where a large product of matrices reaches 1213; 32 on 8 heads of 128 167 to 177 us, 825 to
-// 780. The matrix core is busy half of the time, the rest is softmax and conversion, of which two wavefronts a SIMD hide some
-// behind each other's products: more wavefronts, or two tiles in flight in one, have no registers (192 of 256 hold q and the
-// sums with 256 dimensions; 64 rows a wavefront of 512 registers spill 500). 16 rows a tile straight from registers, as the
-// form for few rows has it, took 435 us, every wavefront converting all bytes for itself. Bytes copied into LDS by the loads
-// themselves and converted from there: 240 against 225 us at that stage, since LDS reads then wait for the copies.
+// card in hand), 740 to 690 TFLOP/s where a large product of matrices reaches 1213; 32 on 8 heads of 128 158 to 177 us, 870 to
+// 780; 32 on 8 of 64 111 us, 620. The matrix core is busy half of the time, the rest is softmax and conversion, of which two
+// wavefronts a SIMD hide some behind each other's products: more wavefronts, or two tiles in flight in one, have no registers with
+// 256 dimensions (192 of 256 hold q and the sums; 64 rows a wavefront of 512 registers spill 500); with 128 and 64, where 188 and
+// 142 are used, two in flight would fit and have not been built. 16 rows a tile straight from registers, as the form for few rows
+// has it, took 435 us, every wavefront converting all bytes for itself. Bytes copied into LDS by the loads themselves and converted
+// from there: 240 against 225 us at that stage, since LDS reads then wait for the copies.
 #include <algorithm>
 
 #include "wl_attend.h"

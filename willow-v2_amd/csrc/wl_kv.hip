@@ -87,8 +87,9 @@ __device__ __forceinline__ uint32_t top_of(uint32_t two, uint32_t top) {
 // a token to a thread. V's lie with the tokens innermost: a thread takes two neighbouring values of 16 tokens, its loads run
 // along the rows over the lanes, and it writes 16 bytes for each value; where those 16 tokens are not all new, the bytes
 // there are read with them. Bound by latency: a prompt has one such workgroup for each CU or two, a step's single tokens less.
-// One token of 64 sequences, 2 heads of 256: 6.0 us; 4096 tokens: 10.1 us (12.6 MB, 1.2 TB/s); with the rows read again for
-// the second pass and divisions in place of the reciprocal: 14.3.
+// One token of 64 sequences, 2 heads of 256: 6.0 us; 4096 tokens: 9.4 us (12.6 MB, 1.3 TB/s); with the rows read again for
+// the second pass and divisions in place of the reciprocal: 14.3. Larger pages leave CUs without a workgroup: 4096 tokens take 14,
+// 26, 50 and 97 us on pages of 128, 256, 512 and 1024.
 template <int TYPE, int D, bool WIDE>
 __global__ __launch_bounds__(kAppendThreads) void k_kv_append(KvLayer c, KvSeqs s, const int32_t* __restrict__ start,
                                                               const uint16_t* __restrict__ kx, int64_t k_ts, int64_t k_hs,
