@@ -32,6 +32,8 @@ class OutOfPages(RuntimeError):
 
 def _whole(n) -> int:
     """A number of tokens as an int; a fraction of one is refused."""
+    if type(n) is int:
+        return n
     if isinstance(n, str) or n - n != 0 or int(n) != n:  # infinities less themselves are not 0
         raise ValueError(f"{n!r} is no number of tokens")
     return int(n)
@@ -197,7 +199,8 @@ class _StreamOrder:
                     here.wait_stream(other)
             self.raw, self.writer, self.readers = raw, here, {}
         elif raw != self.raw and raw not in self.readers:
-            here.wait_stream(self.writer)
+            if self.writer is not None:
+                here.wait_stream(self.writer)
             self.readers[raw] = here
 
 
