@@ -335,6 +335,45 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
                  int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,
                  uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* What the rows of a causal call see less than all tokens up to their own position. window > 0: a row at position p sees the
+ * tokens j <= p with j > p - window (so `window` of them, its own included) or j < sinks; window == 0: no window (and no sinks).
+ * tree != NULL: the call's rows are a sequence's drafted tokens, and of these a row sees those whose bit is set: bit j % 64 of
+ * word tree[row * tree_stride + j / 64] for the sequence's own row j (bits of rows that it does not have are ignored). All tokens
+ * before the sequence's rows count as before, and its position (which the window starts from) is that of its first row plus the
+ * number of drafted tokens that it sees, less one (wl_kv_tree makes these words). A window that begins inside a tree is refused
+ * (window < max_count). */
+typedef struct WlKvMask {
+    const uint64_t* tree; /* or NULL; 8-byte aligned */
+    int64_t tree_stride;  /* words from row to row, at least max_count / 64 rounded up */
+    int64_t window;       /* 0: none */
+    int64_t sinks;
+} WlKvMask;
+
+/* wl_kv_attend with causal != 0 and a mask (NULL: none), and its workspace. Only the pages of the sinks and of the window are
+ * read; values of tokens that no row of a sequence sees never reach it, NaN or not. */
+size_t wl_kv_attend_masked_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length,
+                                           const WlKvMask* mask);
+int wl_kv_attend_masked(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                        int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale,
+                        const WlKvMask* mask, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/* A tree of drafted tokens as wl_kv_attend_masked takes it. parents[row]: the row's parent among its sequence's rows, before it
+ * (anything else: the row is a root, behind the last token before the draft). tree[row][words]: the row's ancestors' bits and its
+ * own (words >= max_count / 64 rounded up); positions[row] = start[b] + how many ancestors it has. Rows that belong to no
+ * sequence get no bits and position 0. batch: cu, tokens, seqs and max_count are read; table may be NULL. */
+int wl_kv_tree(const WlKvBatch* batch, const int32_t* parents, const int32_t* start, uint64_t* tree, int64_t words,
+               int64_t* positions, void* stream);
+
+/* Moves tokens up inside their sequences, on every layer: row i of sequence b's rows in `batch` says that the token at position
+ * start[b] + keep[row] goes to position start[b] + i (0 <= i <= keep[row]; a smaller keep[row] is taken as i), as if all were read
+ * before any is written. Positions from start[b] + the sequence's rows on are no longer the sequence's; their bytes stay as they
+ * are. A page that receives tokens keeps its scale s, or takes s * 2^n with the smallest n that covers the tokens kept in it
+ * (s == 0: the smallest bf16 value that does); a value is its byte times its page's scale in fp32, divided by that and rounded to
+ * nearest even, so bytes that stay in a page that keeps its scale are moved as they are. Bytes before start[b] are divided by 2^n
+ * and rounded as wl_kv_append does. Tokens whose source or target page is not there are not moved. A NaN scale, or a value past
+ * fp32's range, makes the target's scale NaN. Pages that a call writes must be distinct over its sequences. */
+int wl_kv_keep(const WlKvCache* cache, const WlKvBatch* batch, const int32_t* start, const int32_t* keep, void* stream);
+
 /* Copies pages src_host[i] to dst_host[i], i < n, of every layer (bytes and scales). HOST arrays, passed by value to the
  * kernels. Refused: a page out of range, a page written twice, a page both read and written. */
 int wl_kv_copy(const WlKvCache* cache, const int32_t* src_host, const int32_t* dst_host, int64_t n, void* stream);
@@ -360,6 +399,15 @@ typedef struct WlRopeTensor {
 int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
             const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
             const int32_t* sections_host, int interleaved, float scale, void* stream);
+
+/* wl_rope on queries and keys that are normed first, head by head: y = x * (1 / sqrt(mean(x^2) + eps)) * w over a head's
+ * head_dim values, then the rotation of y, in fp32 throughout and rounded once to the tensors' dtype. w = 1 + weight with
+ * zero_centered != 0, else weight; fp32 or bf16 [head_dim] (weight_dtype, of both), NULL: w = 1. eps: finite, not negative.
+ * (The reference norms and turns in two steps, engines/base.py:16-89, rounding in between.) */
+int wl_norm_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
+                 const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
+                 const int32_t* sections_host, int interleaved, float scale, const void* q_weight, const void* k_weight,
+                 int weight_dtype, float eps, int zero_centered, void* stream);
 
 #ifdef __cplusplus
 }

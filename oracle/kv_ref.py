@@ -1,5 +1,5 @@
 """The attention half's operators in plain torch on the CPU, in 64 bits: the paged 8-bit cache's append, attention over it,
-rotary positions. Written from the definitions, one block, row or frequency at a time; used by the tests only."""
+rotary positions behind a norm, trees of drafts and their accepted tokens. Written from the definitions, one block, row or frequency at a time; used by the tests only."""
 import math
 
 import torch
@@ -73,8 +73,9 @@ def append(pool, scale, new, table, start, cu, page_tokens, v=False, max_count=N
     return (out.transpose(2, 3) if v else out), sc
 
 
-def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True, max_count=None, weight_roundings=1):
-    """k, v, scales: one layer on the CPU. -> (out fp64 [tokens, heads, dim] with NaN in rows that belong to no sequence, the
+def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True, max_count=None, weight_roundings=1, window=None, sinks=0,
+           tree=None):
+    """window, sinks, tree (int64 [tokens, words]): what a causal call's rows see. k, v, scales: one layer on the CPU. -> (out fp64 [tokens, heads, dim] with NaN in rows that belong to no sequence, the
     bound of |error| of a bf16 result whose scores and sums are fp32 and whose weights are rounded to bf16, so many times)."""
     pages, kv_heads, page, dim = k.shape
     group = q.shape[1] // kv_heads
@@ -93,8 +94,22 @@ def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True
             K = (k[use, g].double() * k_scale[use, g].double()[:, None, None]).reshape(-1, dim)[:total]
             V = (v[use, g].double() * v_scale[use, g].double()[:, None, None]).transpose(1, 2).reshape(-1, dim)[:total]
             for i in range(n):
-                seen = min(total, max(int(length[b]) - n + i + 1, 0)) if causal else total
-                keep = there[:seen].nonzero()[:, 0]
+                begin = int(length[b]) - n
+                seen = there.clone()
+                if tree is not None:
+                    own = drafted(tree[lo + i], n)
+                    seen[max(begin, 0):] = False
+                    for j in own:
+                        if 0 <= begin + j < total:
+                            seen[begin + j] = there[begin + j]
+                    at = begin + max(len(own) - 1, 0)
+                else:
+                    at = begin + i
+                    if causal:
+                        seen[max(at + 1, 0):] = False
+                if window is not None:
+                    seen[min(sinks, total):max(at + 1 - window, min(sinks, total), 0)] = False
+                keep = seen.nonzero()[:, 0]
                 x = q[lo + i, h].double()
                 if len(keep) == 0:
                     out[lo + i, h] = 0
@@ -110,6 +125,77 @@ def attend(k, v, k_scale, v_scale, q, table, length, cu, scale=None, causal=True
                 per = weight_roundings * 2.0 ** -8 + 2 * slack + (len(keep) + 8) * 2.0 ** -23
                 tol[lo + i, h] = 2.0 ** -8 * o.abs() + per * (w @ Vk.abs())
     return out, tol
+
+
+def drafted(words, n):
+    """The rows below n whose bits are set in a row's words."""
+    return [j for j in range(min(n, 64 * len(words))) if int(words[j // 64]) >> j % 64 & 1]
+
+
+def tree(parents, start, cu, words, max_count=None):
+    """-> (masks int64 [tokens, words], positions int64 [tokens]) of drafted trees, zeros in rows of no sequence."""
+    masks, positions = torch.zeros(len(parents), words, dtype=torch.int64), torch.zeros(len(parents), dtype=torch.int64)
+    for b in range(len(start)):
+        lo = min(max(int(cu[b]), 0), len(parents))
+        n = min(max(int(cu[b + 1]), lo) - lo, len(parents) - lo, len(parents) if max_count is None else max_count)
+        for i in range(n):
+            line = [i]
+            while 0 <= int(parents[lo + line[-1]]) < line[-1]:
+                line.append(int(parents[lo + line[-1]]))
+            for w in range(words):
+                bits = sum(1 << j % 64 for j in line if j // 64 == w)
+                masks[lo + i, w] = bits - (1 << 64) if bits >> 63 else bits
+            positions[lo + i] = int(start[b]) + len(line) - 1
+    return masks, positions
+
+
+def keep(pool, scale, table, start, keep, cu, page_tokens, v=False, max_count=None):
+    """K (or V) of all layers [layers, pages, heads, page_tokens, dim] (V: [.., dim, page_tokens]) and scale [layers, pages, heads] on
+    the CPU -> (pool as fp64, scale) with each sequence's kept tokens moved up, read before any is written."""
+    dtype, top = pool.dtype, LARGEST[pool.dtype]
+    old, sc = (pool.double().transpose(3, 4) if v else pool.double()).clone(), scale.double()
+    out, now_sc, pages = old.clone(), sc.clone(), pool.shape[1]
+
+    def page(b, pos):
+        p = int(table[b, pos // page_tokens]) if pos // page_tokens < table.shape[1] else -1
+        return p if 0 <= p < pages else None
+    for b in range(len(start)):
+        lo = min(max(int(cu[b]), 0), len(keep))
+        n = min(max(int(cu[b + 1]), lo) - lo, len(keep) - lo, len(keep) if max_count is None else max_count)
+        first = max(int(start[b]), 0)
+        moves = {}  # target page -> [(place in it, source page, place in it)]
+        for i in range(n):
+            source, target = first + max(int(keep[lo + i]), i), first + i
+            if page(b, target) is not None and page(b, source) is not None:
+                moves.setdefault(target // page_tokens, []).append((target % page_tokens, page(b, source), source % page_tokens))
+        for column, tokens in moves.items():
+            p, held = page(b, column * page_tokens), max(first - column * page_tokens, 0)
+            for layer in range(pool.shape[0]):
+                for h in range(pool.shape[2]):
+                    x = torch.stack([old[layer, s, h, t] * sc[layer, s, h] for _, s, t in tokens])
+                    a, was = float(x.abs().max()), float(sc[layer, p, h])
+                    if not math.isfinite(a) or a >= 2.0 ** 128:
+                        now = math.nan
+                    elif math.isnan(was):
+                        now = was
+                    elif was > 0:
+                        now = grown(was, top, a)
+                        out[layer, p, h, :held] = nearest(old[layer, p, h, :held] * (was / now), dtype)
+                    else:
+                        now = bf16_not_below(a / top)
+                        if now > 0:
+                            out[layer, p, h, :held] = 0
+                    now_sc[layer, p, h] = now
+                    for (t, _, _), y in zip(tokens, x):
+                        out[layer, p, h, t] = nearest(y / now, dtype) if now > 0 else 0.0
+    return (out.transpose(3, 4) if v else out), now_sc
+
+
+def norm(x, weight, eps, zero_centered=True):
+    """Each head's x / sqrt(mean(x^2) + eps) * w in fp64."""
+    x = x.double()
+    w = 1.0 if weight is None else weight.double() + (1.0 if zero_centered else 0.0)
+    return x / (x.square().mean(-1, keepdim=True) + eps).sqrt() * w
 
 
 def rope(x, positions, inv_freq, sections, interleaved, scale=1.0):

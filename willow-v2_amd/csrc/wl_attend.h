@@ -14,6 +14,7 @@
 // matrix core takes them in no more bits at this rate).
 #pragma once
 
+#include <algorithm>
 #include <type_traits>
 
 #include "wl_kv.h"
@@ -38,6 +39,15 @@ struct Seq {
     }
 };
 
+// What a masked call's rows see beside their place in the sequence (kernels with MASK; the others know nothing of it). A row at
+// position p sees the tokens j <= p with j > p - window or j < sinks. With a tree, of the call's own tokens it sees those
+// whose bits are set, and stands as many positions behind the first of them as it sees others.
+struct Mask {
+    const uint32_t* tree;  // the rows' bits, lowest first, or null
+    int64_t tree_stride;   // words of 32 bits
+    int32_t window, sinks;  // none: 2^31 - 1, 0
+};
+
 struct AttendArgs {
     KvLayer c;
     KvSeqs s;
@@ -48,6 +58,7 @@ struct AttendArgs {
     int32_t q_heads, group;
     float scale_log2;  // scale * log2(e)
     int32_t causal, wide_q;
+    Mask mask;
 
     __device__ __forceinline__ Seq seq(int b) const {
         Seq q;
@@ -65,6 +76,65 @@ struct AttendArgs {
                 __builtin_amdgcn_readfirstlane(q.length), __builtin_amdgcn_readfirstlane(q.begin)};
     }
 };
+
+// The lowest n of 16 bits
+__device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), 16)) - 1u; }
+
+// All bits of the four bytes whose bits (the lowest four) are set
+__device__ __forceinline__ uint32_t bytes_of(uint32_t bits) { return ((bits & 15u) * 0x00204081u & 0x01010101u) * 0xFFu; }
+
+// One row of a masked call: `limit` is its position plus 1 (0: it is not there).
+// Which of the 16 tokens from position p on it sees, as bits. `count` of them are there, counting from the first; `drafted`: the
+// bits of the tree that fall on them.
+__device__ __forceinline__ uint32_t seen_bits(const AttendArgs& a, Seq seq, int limit, int p, int count, uint32_t drafted) {
+    const uint32_t upto = a.mask.tree ? low_bits(seq.begin - p) | drafted : low_bits(limit - p);
+    return upto & low_bits(count) & (~low_bits(max(limit - a.mask.window, 0) - p) | low_bits(a.mask.sinks - p));
+}
+// The tree's bits of 16 tokens from position p on, for row `token` of the sequence.
+__device__ __forceinline__ uint32_t tree_bits(const AttendArgs& a, Seq seq, int token, int p) {
+    const int off = p - seq.begin;
+    if (off <= -16 || off >= seq.n || token >= seq.n) return 0;
+    const uint32_t* row = a.mask.tree + (seq.at + token) * a.mask.tree_stride;
+    if (off < 0) return row[0] << -off & 0xFFFFu & low_bits(seq.n - off);
+    const int word = off >> 5, bit = off & 31;
+    uint64_t two = row[word];
+    if (bit > 16 && 32 * (word + 1) < seq.n) two |= static_cast<uint64_t>(row[word + 1]) << 32;
+    return static_cast<uint32_t>(two >> bit) & low_bits(seq.n - off);
+}
+// Row `token`'s limit. Of the tree's rows only a window asks for it.
+__device__ __forceinline__ int limit_of(const AttendArgs& a, Seq seq, int token) {
+    if (token >= seq.n) return 0;
+    int behind = token;
+    if (a.mask.tree) {
+        behind = 0;
+        if (a.mask.window != 0x7FFFFFFF) {
+            const uint32_t* row = a.mask.tree + (seq.at + token) * a.mask.tree_stride;
+            for (int i = 0; 32 * i < seq.n; i++) behind += __popc(row[i] & (seq.n - 32 * i >= 32 ? ~0u : (1u << (seq.n - 32 * i)) - 1u));
+            behind = max(behind - 1, 0);
+        }
+    }
+    return max(seq.begin + behind + 1, 0);
+}
+// The first position of the window of row `token` and of every one behind it.
+__device__ __forceinline__ int window_begin(const AttendArgs& a, Seq seq, int token) {
+    return max(max(seq.begin + (a.mask.tree ? 0 : token) + 1, 0) - a.mask.window, 0);
+}
+
+// The tiles that rows from `token` on have to go through, up to position `end`: those of the sinks, and from the window's
+// begin on. They are numbered without the gap between.
+struct Span {
+    int sink_tiles, gap, tiles;
+
+    __device__ __forceinline__ int tile(int t) const { return t < sink_tiles ? t : t + gap; }
+};
+template <bool MASK>
+__device__ __forceinline__ Span span_of(const AttendArgs& a, Seq seq, int token, int end, int tile_tokens) {
+    const int all = (end + tile_tokens - 1) / tile_tokens;
+    if constexpr (!MASK) return {0, 0, all};
+    const int sinks = min(a.mask.sinks, end), sink_tiles = (sinks + tile_tokens - 1) / tile_tokens;
+    const int gap = max(min(window_begin(a, seq, token) / tile_tokens, all) - sink_tiles, 0);
+    return {sink_tiles, gap, all - gap};
+}
 
 template <int TYPE>
 __device__ __forceinline__ uint32_t two_bf16(uint32_t w, bool high) {
@@ -128,10 +198,17 @@ __device__ __forceinline__ uint32_t wave_sum(uint32_t x) { return __builtin_amdg
 
 __device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }
 
-// Calls of more rows than the few-row form takes (wl_attend_rows.hip).
-size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);
-bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length);  // launches hold the call
-int launch_attend_rows(const WlKvCache* c, const AttendArgs& a, const WlKvBatch* b, int64_t max_length, void* workspace,
-                       hipStream_t stream);
+// A bound of the tokens in the tiles that `rows` rows of a sequence in a row go through.
+inline int64_t longest_span(const WlKvCache* c, const WlKvBatch* b, int64_t max_length, const WlKvMask* m, int64_t rows, int64_t tile) {
+    const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
+    if (!m || m->window == 0 || m->window >= longest || m->sinks >= longest) return longest;
+    return std::min(longest, (m->sinks + tile - 1) / tile * tile + m->window + rows + 2 * tile - 3);
+}
+
+// Calls of more rows than the few-row form takes (wl_attend_rows.hip). mask: null, or one that hides something.
+size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask);
+bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask);  // launches hold the call
+int launch_attend_rows(const WlKvCache* c, const AttendArgs& a, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask,
+                       void* workspace, hipStream_t stream);
 
 }  // namespace wl

@@ -35,7 +35,8 @@ struct FewArgs : AttendArgs {
 
 // One wavefront's share of the rows of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
 // PAGE: a page holds whole tiles (64 tokens or more), so a tile has one page, one address and one pair of scales.
-template <int TYPE, int D, bool PAGE>
+// MASK: rows see what their window, the sinks and a tree leave them.
+template <int TYPE, int D, bool PAGE, bool MASK>
 struct Rows {
     static constexpr int kChunks = D / 64;  // 16-byte loads of a K row, by four lanes each
     static constexpr int kDims = D / 16;    // 16-dimension blocks of V^T
@@ -43,13 +44,19 @@ struct Rows {
     uint4 q[2 * kChunks];  // 8 bf16 each: this lane's row, dimensions 64 i + 16 g + 8 s ..
     f32x4 o[kDims];
     float m, l;
-    int limit;  // tokens that this lane's row sees
+    int limit;  // tokens that this lane's row sees; of a masked call its position plus 1
+    uint32_t tree;  // the 16 rows' bits of the tree
 
     __device__ __forceinline__ void begin(const AttendArgs& a, int head, Seq seq) {
         const int lane = threadIdx.x & 63, g = lane >> 4, row = lane & 15, token = row / a.group;
         m = -__builtin_inff();
         l = 0.0f;
-        limit = token >= seq.n ? 0 : seq.seen(token, a.causal);
+        if constexpr (MASK) {
+            limit = limit_of(a, seq, token);
+            tree = a.mask.tree ? tree_bits(a, seq, token, seq.begin) : 0;
+        } else {
+            limit = token >= seq.n ? 0 : seq.seen(token, a.causal);
+        }
 #pragma unroll
         for (int i = 0; i < kDims; i++) o[i] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
         const uint16_t* p = a.q + static_cast<int64_t>(seq.at + token) * a.q_token_stride +
@@ -113,7 +120,8 @@ struct Rows {
         x.more = v;
     }
 
-    __device__ __forceinline__ void add(const AttendArgs& a, Tile& x, int base, int length) {
+    __device__ __forceinline__ void add(const AttendArgs& a, Tile& x, int base, Seq seq) {
+        const int length = seq.length;
         f32x4 s[4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
@@ -131,13 +139,22 @@ struct Rows {
 #pragma unroll
             for (int i = kEarly; i < kDims; i++) x.v[i] = *reinterpret_cast<const uint4*>(x.more + 16 * i * a.c.page_tokens);
         }
-        const int mine = x.page < 0 ? 0 : min(max(limit - base - 16 * vgroup(), 0), 16);  // of this lane's 16 tokens, those that count
+        const int first = base + 16 * vgroup();
+        // of this lane's 16 tokens, those that count: so many, or these
+        const int mine = x.page < 0 ? 0 : min(max(limit - first, 0), 16);
+        uint32_t bits = 0;
+        if constexpr (MASK) {
+            const int off = seq.begin - first;  // where the tree's first token lies
+            const uint32_t drafted = off >= 16 || off <= -16 ? 0 : off < 0 ? tree >> -off : tree << off;
+            bits = x.page < 0 ? 0 : seen_bits(a, seq, limit, first, length - first, drafted);
+        }
+        auto counts = [&](int i) { return MASK ? (bits >> i & 1) != 0 : i < mine; };
         float top = m;
 #pragma unroll
         for (int j = 0; j < 4; j++)
 #pragma unroll
             for (int r = 0; r < 4; r++) {
-                s[j][r] = 4 * j + r < mine ? s[j][r] * x.ks : -__builtin_inff();
+                s[j][r] = counts(4 * j + r) ? s[j][r] * x.ks : -__builtin_inff();
                 top = fmaxf(top, s[j][r]);
             }
         top = max_over_groups(top);
@@ -158,14 +175,28 @@ struct Rows {
                 e[r] = exp2_fast(s[j][r] - safe);
                 l += e[r];
                 // a token that does not count adds 0 whatever its block's scale is (it may be NaN)
-                e[r] = 4 * j + r < mine ? e[r] * x.vs : 0.0f;
+                e[r] = counts(4 * j + r) ? e[r] * x.vs : 0.0f;
             }
             p[2 * j] = pack_bf16(e[0], e[1]);
             p[2 * j + 1] = pack_bf16(e[2], e[3]);
         }
-        if (base + kTile > length || __any(x.page < 0)) {
+        if constexpr (MASK) {
+            // the same for tokens that no row sees, before the window
+            const int lowest = window_begin(a, seq, 0);
+            if (base + kTile > length || base < lowest || __any(x.page < 0)) {
+                const uint32_t kept = x.page < 0 ? 0 : low_bits(length - first) & (~low_bits(lowest - first) | low_bits(a.mask.sinks - first));
+                const uint32_t m0 = bytes_of(kept), m1 = bytes_of(kept >> 4), m2 = bytes_of(kept >> 8), m3 = bytes_of(kept >> 12);
+#pragma unroll
+                for (int i = 0; i < kDims; i++) {
+                    x.v[i].x &= m0;
+                    x.v[i].y &= m1;
+                    x.v[i].z &= m2;
+                    x.v[i].w &= m3;
+                }
+            }
+        } else if (base + kTile > length || __any(x.page < 0)) {
             // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
-            const int there = x.page < 0 ? 0 : min(max(length - base - 16 * vgroup(), 0), 16);
+            const int there = x.page < 0 ? 0 : min(max(length - first, 0), 16);
             const uint32_t m0 = byte_mask(there), m1 = byte_mask(there - 4), m2 = byte_mask(there - 8), m3 = byte_mask(there - 12);
 #pragma unroll
             for (int i = 0; i < kDims; i++) {
@@ -184,14 +215,14 @@ struct Rows {
         }
     }
 
-    // Tiles t0 (which has been found), t0 + step, .. below t1.
-    __device__ __forceinline__ void tiles(const AttendArgs& a, int b, int head, int t0, int t1, int step,
-                                          int length) {
+    // Tiles t0 (which has been found), t0 + step, .. below t1, as `span` numbers them.
+    __device__ __forceinline__ void tiles(const AttendArgs& a, int b, int head, Span span, int t0, int t1, int step, Seq seq) {
         for (int t = t0; t < t1; t += step) {
             Tile x;
-            load(a, x, head, t * kTile);
-            if (t + step < t1) find(a, b, (t + step) * kTile);
-            add(a, x, t * kTile, length);
+            const int base = span.tile(t) * kTile;
+            load(a, x, head, base);
+            if (t + step < t1) find(a, b, span.tile(t + step) * kTile);
+            add(a, x, base, seq);
         }
     }
 };
@@ -204,16 +235,17 @@ struct JoinLds {
 
 // The workgroup's wavefronts over tiles [t0, t1) of the rows; the rows are finished into out, or, with
 // slot >= 0, left as a partial result.
-template <int TYPE, int D, bool PAGE>
+template <int TYPE, int D, bool PAGE, bool MASK>
 __device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, int b, Seq seq, int head, int t0,
                                             int t1, int slot) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
-    const int at = seq.at, n = seq.n, length = seq.length;
+    const int at = seq.at, n = seq.n;
     const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group, static_cast<int64_t>(kRows)));
-    Rows<TYPE, D, PAGE> r;
-    if (t0 + wave < t1) r.find(a, b, (t0 + wave) * kTile);
+    Rows<TYPE, D, PAGE, MASK> r;
+    const Span span = MASK ? span_of<MASK>(a, seq, 0, seq.length, kTile) : Span{0, 0, 0};
+    if (t0 + wave < t1) r.find(a, b, span.tile(t0 + wave) * kTile);
     r.begin(a, head, seq);
-    r.tiles(a, b, head, t0 + wave, t1, kFewWaves, length);
+    r.tiles(a, b, head, span, t0 + wave, t1, kFewWaves, seq);
     r.l = sum_over_groups(r.l);
     if (lane < kRows) {
         lds.m[wave][lane] = r.m;
@@ -269,27 +301,29 @@ struct Line {
     __device__ __forceinline__ uint32_t padded(uint32_t tiles) const { return (tiles + pad - 1) / pad * pad; }
 };
 
-__device__ __forceinline__ uint32_t tiles_of(Seq s) {
-    return s.n == 0 ? 0 : max((s.length + kTile - 1) / kTile, 1);  // without a token there are still rows to write
+template <bool MASK>
+__device__ __forceinline__ uint32_t tiles_of(const FewArgs& a, Seq s) {
+    return s.n == 0 ? 0 : max(span_of<MASK>(a, s, 0, s.length, kTile).tiles, 1);  // without a token there are still rows to write
 }
 __device__ __forceinline__ Seq seq_or_none(const FewArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0, 0}; }
 
 // Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`. Shares and (sequence, head)s are whole
 // rounds of a workgroup (a tile for each wavefront), so that only the last round of each leaves wavefronts idle.
+template <bool MASK>
 __device__ __forceinline__ Line line_of(const FewArgs& a, uint32_t mine) {
     constexpr uint32_t W = kFewWaves;
     const uint32_t heads = a.c.kv_heads, groups = a.groups;
     const int lane = threadIdx.x & 63;
     uint32_t rounds = (mine + W - 1) / W;
-    for (int b = lane + 64; b < a.s.seqs; b += 64) rounds += (tiles_of(a.seq(b)) + W - 1) / W;
+    for (int b = lane + 64; b < a.s.seqs; b += 64) rounds += (tiles_of<MASK>(a, a.seq(b)) + W - 1) / W;
     rounds = wave_sum(rounds) * heads;
     const uint32_t each = __builtin_amdgcn_readfirstlane(max((rounds + groups - 1) / groups, 1u) * W);
     uint32_t shares = (mine + each - 1) / each;
-    for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of(a.seq(b)) + each - 1) / each;
+    for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of<MASK>(a, a.seq(b)) + each - 1) / each;
     return {each, wave_sum(shares) * heads <= groups ? each : W, heads};
 }
 
-template <int TYPE, int D, bool PAGE>
+template <int TYPE, int D, bool PAGE, bool MASK>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
     __shared__ JoinLds<D> lds;
     const int lane = threadIdx.x & 63;
@@ -300,16 +334,16 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
     if (a.whole) {  // a workgroup for each (sequence, head)
         b = blockIdx.x / line.heads;
         seq = a.seq_uniform(b);
-        const uint32_t tiles = tiles_of(seq);
+        const uint32_t tiles = tiles_of<MASK>(a, seq);
         at = blockIdx.x % line.heads * tiles;
         end = at + tiles;
     } else {
         Seq mine = seq_or_none(a, lane);
-        line = line_of(a, tiles_of(mine));
+        line = line_of<MASK>(a, tiles_of<MASK>(a, mine));
         at = blockIdx.x * line.each;
         end = at + line.each;
         for (;;) {
-            const uint32_t own = line.padded(tiles_of(mine)) * line.heads, sum = wave_scan(own);
+            const uint32_t own = line.padded(tiles_of<MASK>(a, mine)) * line.heads, sum = wave_scan(own);
             const uint64_t past = __ballot(before + sum > at);
             if (past) {
                 const int i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
@@ -329,14 +363,14 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
     }
     int slot = 2 * blockIdx.x;  // of the share's first piece, where it is cut; of another one that is, the last: slot + 1
     while (at < end) {
-        const uint32_t tiles = tiles_of(seq), length = __builtin_amdgcn_readfirstlane(line.padded(tiles));
+        const uint32_t tiles = tiles_of<MASK>(a, seq), length = __builtin_amdgcn_readfirstlane(line.padded(tiles));
         if (tiles) {
             const uint32_t head = __builtin_amdgcn_readfirstlane((at - before) / length), t0 = at - before - head * length;
             const uint32_t t1 = min(t0 + (end - at), length), stop = min(t1, tiles);
             const bool whole = t0 == 0 && stop == tiles;
             if (t0 < stop) {
                 if (slot & 1) __syncthreads();  // the piece before still reads the LDS
-                attend_rows<TYPE, D, PAGE>(a, lds, b, seq, head, t0, stop, whole ? -1 : slot);
+                attend_rows<TYPE, D, PAGE, MASK>(a, lds, b, seq, head, t0, stop, whole ? -1 : slot);
             }
             if (t0 == 0 && !a.whole && threadIdx.x == 0) {
                 const int rest = whole ? 0 : (tiles - stop + line.each - 1) / line.each;
@@ -424,8 +458,8 @@ bool is_few(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
     return static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads) <= kRows;
 }
 
-FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length) {
-    const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
+FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
+    const int64_t longest = longest_span(c, b, max_length, mask, b->max_count, kTile);
     const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
     // Two rounds of a workgroup cost less than one and the join: 500 tokens of 1 to 256 sequences on 8 kv heads of 128 9.2 to 45.6
     // against 10.1 to 61.5 us in a graph, on 8 of 64 5.8 to 24.1 against 8.3 to 32.8, of 32 to 256 on 2 of 256 15.3 to 28.0 against
@@ -480,32 +514,39 @@ bool out_meets_q(const uint16_t* out, const uint16_t* q, int64_t ts, int64_t hs,
     return false;
 }
 
-}  // namespace
-}  // namespace wl
+int check_mask(const WlKvMask* m, const WlKvBatch* b) {
+    if (!m) return WL_OK;
+    if (m->window < 0 || m->sinks < 0) return WL_EINVAL_SHAPE;
+    if (!m->tree) return WL_OK;
+    if (reinterpret_cast<uintptr_t>(m->tree) % 8) return WL_EINVAL_ALIGN;
+    if (m->tree_stride < (b->max_count + 63) / 64 || m->tree_stride >= (int64_t{1} << 31)) return WL_EINVAL_SHAPE;
+    // a window that begins inside the tree would have to know each drafted token's own depth
+    return m->window && m->window < b->max_count ? WL_EINVAL_SHAPE : WL_OK;
+}
+bool hides_nothing(const WlKvMask* m) { return !m || (!m->tree && m->window == 0); }
 
-using namespace wl;
-
-extern "C" {
-
-size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
-    if (check_attend(cache, q_heads, batch, max_length)) return 0;
-    if (!is_few(cache, q_heads, batch)) return attend_rows_workspace(cache, q_heads, batch, max_length);
-    return few_space(cache, q_heads, batch, few_plan(cache, batch, max_length)).bytes;
+Mask device_mask(const WlKvMask* m) {
+    constexpr int64_t most = 0x7FFFFFFF;  // no position is as far
+    return {reinterpret_cast<const uint32_t*>(m->tree), 2 * m->tree_stride, static_cast<int32_t>(m->window ? std::min(m->window, most) : most),
+            static_cast<int32_t>(std::min(m->sinks, most))};
 }
 
-int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
-                 int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,
-                 uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+// A call of either entry point; mask: null, or what it hides (of a causal call).
+int attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride, int q_heads,
+           const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal, const WlKvMask* mask,
+           uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
     if (const int rc = check_attend(cache, q_heads, batch, max_length)) return rc;
+    if (const int rc = check_mask(mask, batch)) return rc;
+    if (hides_nothing(mask)) mask = nullptr;
     if (!q || !length || !out) return WL_EINVAL_NULL;
     const float scale_log2 = scale * 1.44269504088896340736f;
     if (layer < 0 || layer >= cache->layers || !(scale >= 0.0f && scale_log2 < __builtin_inff())) return WL_EINVAL_SHAPE;
     const auto qb = reinterpret_cast<uintptr_t>(q);
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
-    const size_t need = wl_kv_attend_workspace_bytes(cache, q_heads, batch, max_length);
+    const size_t need = wl_kv_attend_masked_workspace_bytes(cache, q_heads, batch, max_length, mask);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return WL_EINVAL_WORKSPACE;
     const bool few = is_few(cache, q_heads, batch);
-    if (!few && !attend_rows_fit(cache, q_heads, batch, max_length)) return WL_EINVAL_SHAPE;
+    if (!few && !attend_rows_fit(cache, q_heads, batch, max_length, mask)) return WL_EINVAL_SHAPE;
     if (out_meets_q(out, q, q_token_stride, q_head_stride, batch->tokens, q_heads, cache->head_dim)) return WL_EINVAL_OVERLAP;
     FewArgs a = {};
     a.c = layer_of(cache, layer);
@@ -519,10 +560,11 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.group = q_heads / cache->kv_heads;
     a.scale_log2 = scale_log2;
     a.causal = causal != 0;
+    if (mask) a.mask = device_mask(mask);
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!few) return launch_attend_rows(cache, a, batch, max_length, workspace, st);
-    const FewPlan plan = few_plan(cache, batch, max_length);
+    if (!few) return launch_attend_rows(cache, a, batch, max_length, mask, workspace, st);
+    const FewPlan plan = few_plan(cache, batch, max_length, mask);
     const FewSpace space = few_space(cache, q_heads, batch, plan);
     a.partial = static_cast<float*>(workspace);
     a.partial_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + space.ml);
@@ -532,7 +574,12 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     auto run = [&](auto type, auto dim, auto page) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
-        k_attend_few<T, D, decltype(page)::value><<<static_cast<uint32_t>(plan.groups), kFewWaves * 64, 0, st>>>(a);
+        constexpr bool P = decltype(page)::value;
+        const uint32_t groups = static_cast<uint32_t>(plan.groups);
+        if (mask)
+            k_attend_few<T, D, P, true><<<groups, kFewWaves * 64, 0, st>>>(a);
+        else
+            k_attend_few<T, D, P, false><<<groups, kFewWaves * 64, 0, st>>>(a);
         if (const int rc = launch_status()) return rc;
         if (!plan.whole)
             k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, a.rows), kJoinWaves * 64, 0, st>>>(a);
@@ -548,6 +595,39 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
     };
     if (cache->type == WL_KV_INT8) return with_dim(std::integral_constant<int, WL_KV_INT8>());
     return with_dim(std::integral_constant<int, WL_KV_E4M3>());
+}
+
+}  // namespace
+}  // namespace wl
+
+using namespace wl;
+
+extern "C" {
+
+size_t wl_kv_attend_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
+    return wl_kv_attend_masked_workspace_bytes(cache, q_heads, batch, max_length, nullptr);
+}
+
+size_t wl_kv_attend_masked_workspace_bytes(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length,
+                                           const WlKvMask* mask) {
+    if (check_attend(cache, q_heads, batch, max_length) || check_mask(mask, batch)) return 0;
+    if (hides_nothing(mask)) mask = nullptr;
+    if (!is_few(cache, q_heads, batch)) return attend_rows_workspace(cache, q_heads, batch, max_length, mask);
+    return few_space(cache, q_heads, batch, few_plan(cache, batch, max_length, mask)).bytes;
+}
+
+int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                 int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale, int causal,
+                 uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(cache, layer, q, q_token_stride, q_head_stride, q_heads, batch, length, max_length, scale, causal, nullptr, out,
+                  workspace, workspace_bytes, stream);
+}
+
+int wl_kv_attend_masked(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,
+                        int q_heads, const WlKvBatch* batch, const int32_t* length, int64_t max_length, float scale,
+                        const WlKvMask* mask, uint16_t* out, void* workspace, size_t workspace_bytes, void* stream) {
+    return attend(cache, layer, q, q_token_stride, q_head_stride, q_heads, batch, length, max_length, scale, 1, mask, out, workspace,
+                  workspace_bytes, stream);
 }
 
 }  // extern "C"

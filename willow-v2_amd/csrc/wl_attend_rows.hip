@@ -79,7 +79,7 @@ struct Lds {
 // One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V. PAGE: a page holds
 // whole tiles, so a tile has one page and one pair of scales, all threads share its address, and the registers that other
 // tiles need for theirs are scalar ones (with 256 dimensions a wavefront has none to spare).
-template <int TYPE, int D, bool PAGE>
+template <int TYPE, int D, bool PAGE, bool MASK>
 struct Stage {
     using S = Shape<D>;
     uint4 k, v;
@@ -123,7 +123,8 @@ struct Stage {
             }
         }
     }
-    __device__ __forceinline__ void store(const AttendArgs& a, Lds<D>& lds, int buffer) const {
+    // hidden_from, hidden_to: no row sees the tokens between, counted from the sequence's end
+    __device__ __forceinline__ void store(const AttendArgs& a, Lds<D>& lds, int buffer, int hidden_from, int hidden_to) const {
         const int t = k_token(), step = k_chunk(), i = t & 15;
         const int row = 8 * (i >> 2) + 4 * ((t >> 4) & 1) + (i & 3);
         uint4* to = lds.k[buffer][(t >> 5) * S::kSteps + step];
@@ -132,7 +133,14 @@ struct Stage {
         to[(32 + row) ^ sw] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(k.z, k.w));
         uint4 w = v;
         const int n = min(max(count - 16 * v_part(), 0), 16);  // tokens that are there, of this thread's part
-        if (count < S::kTokens) {  // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
+        if (MASK && count > 0) {  // see below
+            const int behind = 16 * v_part() - count;  // where this part begins, counted as well
+            const uint32_t kept = low_bits(count - 16 * v_part()) & (~low_bits(hidden_to - behind) | low_bits(hidden_from - behind));
+            w.x &= bytes_of(kept);
+            w.y &= bytes_of(kept >> 4);
+            w.z &= bytes_of(kept >> 8);
+            w.w &= bytes_of(kept >> 12);
+        } else if (count < S::kTokens) {  // bytes that nobody wrote may be NaN in e4m3, which a weight of 0 does not silence
             w.x &= byte_mask(n);
             w.y &= byte_mask(n - 4);
             w.z &= byte_mask(n - 8);
@@ -169,8 +177,10 @@ struct Wave {
     f32x16 o[S::kBlocks];
     float m, l;
 
-    // The 32 tokens of part u of a tile; seen: of this lane's 16 tokens, those that its row may see.
+    // The 32 tokens of part u of a tile; seen: of this lane's 16 tokens, those that its row may see, as many from the first on or,
+    // with MASK, as bits.
     // Operands come from LDS four products ahead (two with 256 dimensions), V's first ones before the softmax.
+    template <bool MASK>
     __device__ __forceinline__ void add(const Lds<D>& lds, int buffer, int u, int seen) {
         constexpr int kAhead = D == 256 ? 2 : 4;  // no registers for more with 256 dimensions
         int lane = threadIdx.x & 63;
@@ -192,7 +202,8 @@ struct Wave {
         }
         __builtin_amdgcn_s_setprio(0);
         const Part part = lds.part[buffer][2 * u + half];
-        const int mine = min(lds.count[buffer][2 * u + half], seen);
+        const int there = lds.count[buffer][2 * u + half];
+        const int mine = MASK ? seen & low_bits(there) : min(there, seen);
         // a lane that sees no token of its block is not to meet the block's scales: they may be NaN
         const float ks = mine > 0 ? part.ks : 1.0f, rest = mine > 0 ? part.rest : 1.0f;
         const int slot = lane ^ S::v_swizzle(2 * u + half);
@@ -200,9 +211,9 @@ struct Wave {
 #pragma unroll
         for (int i = 0; i < kAhead; i++) f[i] = v(i);
         __builtin_amdgcn_sched_barrier(0);
-        if (__any(mine < 16)) {
+        if (__any(MASK ? mine != 0xFFFF : mine < 16)) {
 #pragma unroll
-            for (int i = 0; i < 16; i++) s[i] = i < mine ? s[i] : -__builtin_inff();
+            for (int i = 0; i < 16; i++) s[i] = (MASK ? mine >> i & 1 : i < mine) ? s[i] : -__builtin_inff();
         }
         float top = s[0];
 #pragma unroll
@@ -246,10 +257,14 @@ struct Wave {
 
 // Tiles of the cache that rows [row0, row0 + 256) of a sequence see; at least one where there are rows, which have to be
 // written even if they see nothing.
-__device__ __forceinline__ int tiles_of(const AttendArgs& a, Seq seq, int row0, int tile_tokens) {
-    if (row0 >= seq.n * a.group) return 0;
+template <bool MASK>
+__device__ __forceinline__ Span span_at(const AttendArgs& a, Seq seq, int row0, int tile_tokens) {
     const int last = min((row0 + kGroupRows - 1) / a.group, seq.n - 1);
-    return max((seq.seen(last, a.causal) + tile_tokens - 1) / tile_tokens, 1);
+    return span_of<MASK>(a, seq, row0 / a.group, MASK && a.mask.tree ? seq.length : seq.seen(last, a.causal), tile_tokens);
+}
+template <bool MASK>
+__device__ __forceinline__ int tiles_of(const AttendArgs& a, Seq seq, int row0, int tile_tokens) {
+    return row0 >= seq.n * a.group ? 0 : max(span_at<MASK>(a, seq, row0, tile_tokens).tiles, 1);
 }
 
 // A row tile's tiles in pieces of at most `each`, as equal as can be, unless that were too many pieces.
@@ -276,7 +291,7 @@ struct PlanLds {
     Work work;
 };
 
-template <int D>
+template <int D, bool MASK>
 __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work& work) {
     constexpr int T = Shape<D>::kTokens;
     const uint32_t wanted = blockIdx.x / a.c.kv_heads;
@@ -297,7 +312,7 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
     }
     const uint32_t items = a.s.seqs * row_tiles;
     auto tiles_read = [&](uint32_t i) {
-        return i < items ? tiles_of(a, a.seq(i / row_tiles), static_cast<int>(i % row_tiles) * kGroupRows, T) : 0;
+        return i < items ? tiles_of<MASK>(a, a.seq(i / row_tiles), static_cast<int>(i % row_tiles) * kGroupRows, T) : 0;
     };
     const int own_tiles = tiles_read(threadIdx.x);  // for most calls all there is
     auto tiles_at = [&](uint32_t i) { return i == threadIdx.x ? own_tiles : tiles_read(i); };
@@ -386,7 +401,7 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
 }
 
 // blockIdx: (rank of the piece, kv head).
-template <int TYPE, int D, bool PAGE>
+template <int TYPE, int D, bool PAGE, bool MASK>
 __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     using S = Shape<D>;
     __shared__ union {
@@ -395,7 +410,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     } shared;
     Lds<D>& lds = shared.lds;
     Work cut;
-    if (!find_work<D>(a, shared.plan, cut)) return;
+    if (!find_work<D, MASK>(a, shared.plan, cut)) return;
     __syncthreads();  // the plan has been read
     const int b = cut.b, row0 = cut.row0, piece = cut.piece, head = blockIdx.x % a.c.kv_heads;
     const Seq seq = a.seq_uniform(b);
@@ -403,14 +418,21 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, half = lane >> 5;
     const int row = row0 + 32 * wave + (lane & 31), token = row / a.group;
     const bool there = token < seq.n;
-    const int limit = there ? seq.seen(token, a.causal) : 0;
+    const int limit = MASK ? limit_of(a, seq, token) : there ? seq.seen(token, a.causal) : 0;
     const uint16_t* qp = a.q + static_cast<int64_t>(seq.at + token) * a.q_token_stride +
                          static_cast<int64_t>(head * a.group + row % a.group) * a.q_head_stride + 8 * half;
-    const int most = __builtin_amdgcn_readlane(limit, 31) > 0 ? __builtin_amdgcn_readlane(limit, 31) : seq.length;
+    const int most = MASK && a.mask.tree                            ? seq.length
+                     : __builtin_amdgcn_readlane(limit, 31) > 0 ? __builtin_amdgcn_readlane(limit, 31)
+                                                                : seq.length;
+    const Span span = MASK ? span_at<MASK>(a, seq, row0, S::kTokens) : Span{0, 0, 0};
+    auto base_of = [&](int t) { return span.tile(t) * S::kTokens; };
+    // the tokens between the sinks and the first row's window, of the workgroup's rows (counted from the sequence's end) and of the wavefront's
+    const int hidden_from = MASK ? a.mask.sinks - seq.length : 0, hidden_to = MASK ? window_begin(a, seq, row0 / a.group) - seq.length : 0;
+    const int window_at = MASK ? window_begin(a, seq, __builtin_amdgcn_readfirstlane(token)) : 0;
 
-    Stage<TYPE, D, PAGE> st;
-    st.find(a, b, cut.t0 * S::kTokens);
-    st.load(a, head, cut.t0 * S::kTokens, seq.length);
+    Stage<TYPE, D, PAGE, MASK> st;
+    st.find(a, b, base_of(cut.t0));
+    st.load(a, head, base_of(cut.t0), seq.length);
     Wave<D> w;
 #pragma unroll
     for (int i = 0; i < S::kSteps; i++) {
@@ -427,28 +449,39 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     w.l = 0.0f;
     const bool idle = !__any(there);
 
-    st.store(a, lds, 0);
+    st.store(a, lds, 0, hidden_from, hidden_to);
     if (cut.t0 + 1 < cut.t1) {
-        st.find(a, b, (cut.t0 + 1) * S::kTokens);
-        st.load(a, head, (cut.t0 + 1) * S::kTokens, seq.length);
-        st.store(a, lds, 1);
+        st.find(a, b, base_of(cut.t0 + 1));
+        st.load(a, head, base_of(cut.t0 + 1), seq.length);
+        st.store(a, lds, 1, hidden_from, hidden_to);
     }
     // q is here before the loop: were it still on its way, the first product of every round would wait for that round's loads
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
-    st.find(a, b, (cut.t0 + 2) * S::kTokens);
+    st.find(a, b, base_of(cut.t0 + 2));
     __syncthreads();
     for (int t = cut.t0; t < cut.t1; t++) {
-        const int buffer = (t - cut.t0) & (kRing - 1), base = t * S::kTokens;
+        const int buffer = (t - cut.t0) & (kRing - 1), base = base_of(t);
         if (t + 2 < cut.t1) {
-            st.load(a, head, base + 2 * S::kTokens, seq.length);
-            st.find(a, b, base + 3 * S::kTokens);
+            st.load(a, head, base_of(t + 2), seq.length);
+            st.find(a, b, base_of(t + 3));
         }
 #pragma unroll
         for (int u = 0; u < S::kSubs; u++) {
             if (idle || base + 32 * u >= most) break;
-            w.add(lds, buffer, u, limit - base - 32 * u - 16 * half);
+            const int at = base + 32 * u + 16 * half;
+            if constexpr (MASK) {
+                if (base + 32 * u + 32 <= window_at && base + 32 * u >= a.mask.sinks) continue;
+                uint32_t drafted = 0;
+                if (a.mask.tree && base + 32 * u + 32 > seq.begin) {  // a few tiles: the row is worked out again, as below
+                    const int r = row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero());
+                    drafted = tree_bits(a, seq, r / a.group, at);
+                }
+                w.template add<MASK>(lds, buffer, u, seen_bits(a, seq, limit, at, 16, drafted));
+            } else {
+                w.template add<MASK>(lds, buffer, u, limit - at);
+            }
         }
-        if (t + 2 < cut.t1) st.store(a, lds, (buffer + 2) & (kRing - 1));
+        if (t + 2 < cut.t1) st.store(a, lds, (buffer + 2) & (kRing - 1), hidden_from, hidden_to);
         if (buffer & 1) __syncthreads();
     }
     const float m = w.m, l = other_half(w.l, true);
@@ -486,14 +519,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
 // four: 15 and 7). blockIdx: (16 rows, kv head), sequence.
 constexpr int kMergeWaves = 4, kWaveRows = 4, kMergeRows = kMergeWaves * kWaveRows;
 static_assert(64 / kWaveRows == kMaxPieces && kGroupRows % kMergeRows == 0, "a lane for each piece of each row");
-template <int D>
+template <int D, bool MASK>
 __global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge(RowsArgs a) {
     const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, lane = threadIdx.x & 63;
     const int first = __builtin_amdgcn_readfirstlane(blockIdx.x / a.c.kv_heads * kMergeRows + (threadIdx.x >> 6) * kWaveRows);
     const Seq seq = a.seq_uniform(b);
     const int rows = seq.n * a.group;
     if (first >= rows) return;
-    const int pieces = cut_of(tiles_of(a, seq, first / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
+    const int pieces = cut_of(tiles_of<MASK>(a, seq, first / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
     if (pieces < 2) return;
     constexpr int V = D / 64;
     typedef float Lane __attribute__((ext_vector_type(V)));
@@ -553,9 +586,10 @@ struct RowsPlan {
     bool few_tiles;
 };
 constexpr int kLong = 64;  // tiles: about 80 us for one workgroup
-RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
+RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
     const int64_t tokens = 8192 / c->head_dim, group = q_heads / c->kv_heads;
-    const int64_t longest = std::max<int64_t>(1, std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens));
+    const int64_t rows = mask && mask->tree ? b->max_count : std::min<int64_t>(b->max_count, (kGroupRows + group - 2) / group + 1);
+    const int64_t longest = longest_span(c, b, max_length, mask, rows, tokens);  // that a row tile goes through
     const int64_t row_tiles = (b->max_count * group + kGroupRows - 1) / kGroupRows;
     // (row tile, kv head)s: as many as the sequences' most rows have room for, and no more than all rows together fill
     const int64_t items = std::min(row_tiles * b->seqs, b->tokens * group / kGroupRows + b->seqs) * c->kv_heads;
@@ -571,8 +605,8 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
 
 }  // namespace
 
-size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
-    const RowsPlan p = rows_plan(c, q_heads, b, max_length);
+size_t attend_rows_workspace(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
+    const RowsPlan p = rows_plan(c, q_heads, b, max_length, mask);
     if (p.pieces == 1) return 0;
     return 16 + static_cast<size_t>(p.pieces * b->tokens * q_heads) * (c->head_dim * sizeof(float) + sizeof(float2));
 }
@@ -581,15 +615,15 @@ static int64_t merge_groups(const WlKvCache* c, int64_t group, const WlKvBatch* 
     return (b->max_count * group + kMergeRows - 1) / kMergeRows * c->kv_heads;
 }
 
-bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length) {
-    const RowsPlan p = rows_plan(c, q_heads, b, max_length);
+bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
+    const RowsPlan p = rows_plan(c, q_heads, b, max_length, mask);
     return p.row_tiles * b->seqs < (int64_t{1} << 31) && fits_a_launch(p.groups, kThreads) &&
            fits_a_launch(merge_groups(c, q_heads / c->kv_heads, b), kMergeWaves * 64);
 }
 
-int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBatch* b, int64_t max_length, void* workspace,
-                       hipStream_t stream) {
-    const RowsPlan p = rows_plan(c, call.q_heads, b, max_length);
+int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask,
+                       void* workspace, hipStream_t stream) {
+    const RowsPlan p = rows_plan(c, call.q_heads, b, max_length, mask);
     RowsArgs a;
     static_cast<AttendArgs&>(a) = call;
     a.each = static_cast<int32_t*>(workspace);
@@ -600,15 +634,19 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
     a.few_tiles = p.few_tiles;
     const dim3 grid(static_cast<uint32_t>(p.groups));
     const dim3 merge(static_cast<uint32_t>(merge_groups(c, call.group, b)), b->seqs);
-    auto run = [&](auto type, auto dim) {
+    auto with_mask = [&](auto type, auto dim, auto masked) {
         constexpr int T = decltype(type)::value, D = decltype(dim)::value;
+        constexpr bool MASK = decltype(masked)::value;
         if (c->page_tokens >= Shape<D>::kTokens)
-            k_attend_rows<T, D, true><<<grid, kThreads, 0, stream>>>(a);
+            k_attend_rows<T, D, true, MASK><<<grid, kThreads, 0, stream>>>(a);
         else
-            k_attend_rows<T, D, false><<<grid, kThreads, 0, stream>>>(a);
+            k_attend_rows<T, D, false, MASK><<<grid, kThreads, 0, stream>>>(a);
         if (const int rc = launch_status()) return rc;
-        if (p.pieces > 1) k_attend_merge<D><<<merge, kMergeWaves * 64, 0, stream>>>(a);
+        if (p.pieces > 1) k_attend_merge<D, MASK><<<merge, kMergeWaves * 64, 0, stream>>>(a);
         return launch_status();
+    };
+    auto run = [&](auto type, auto dim) {
+        return mask ? with_mask(type, dim, std::true_type()) : with_mask(type, dim, std::false_type());
     };
     auto with_dim = [&](auto type) {
         if (c->head_dim == 64) return run(type, std::integral_constant<int, 64>());

@@ -1,0 +1,185 @@
+// Trees of drafted tokens (wl_kv_tree) and moving the accepted ones up in the paged 8-bit cache (wl_kv_keep).
+#include <algorithm>
+
+#include "wl_kv.h"
+
+namespace wl {
+namespace {
+
+constexpr int kTreeThreads = 256;
+constexpr int kTreeKept = 4096;  // parents of a sequence that fit in LDS
+
+// A workgroup takes a sequence, a thread a row: it walks from the row to its root. Parents stand before their children, so the
+// walk ends, and meets the words of the row's mask from the last to the first. The workgroup behind the last sequence
+// clears the rows before the first and behind the last one.
+__global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_t* __restrict__ parents,
+                                                          const int32_t* __restrict__ start, uint64_t* __restrict__ tree,
+                                                          int64_t words, int64_t* __restrict__ positions) {
+    __shared__ int32_t kept[kTreeKept];
+    const int b = blockIdx.x;
+    auto clear = [&](int from, int to) {
+        for (int64_t i = from * words + threadIdx.x; i < to * words; i += kTreeThreads) tree[i] = 0;
+        for (int i = from + static_cast<int>(threadIdx.x); i < to; i += kTreeThreads) positions[i] = 0;
+    };
+    if (b == s.seqs) {
+        clear(0, s.first(0));
+        clear(s.first(s.seqs), s.tokens);
+        return;
+    }
+    const int at = s.first(b), n = s.count(b, at);
+    clear(at + n, min(max(s.cu[b + 1], at), s.tokens));  // rows behind max_count
+    const int32_t* mine = parents + at;
+    for (int i = threadIdx.x; i < min(n, kTreeKept); i += kTreeThreads) kept[i] = mine[i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < n; i += kTreeThreads) {
+        uint64_t* row = tree + (at + i) * words;
+        int word = static_cast<int>(words) - 1, seen = 0;
+        for (; word > i >> 6; word--) row[word] = 0;
+        uint64_t bits = 0;
+        for (int j = i;;) {
+            bits |= uint64_t{1} << (j & 63);
+            seen++;
+            const int p = j < kTreeKept ? kept[j] : mine[j];
+            if (p < 0 || p >= j) break;
+            for (; word > p >> 6; word--) {
+                row[word] = bits;
+                bits = 0;
+            }
+            j = p;
+        }
+        for (; word >= 0; word--) {
+            row[word] = bits;
+            bits = 0;
+        }
+        positions[at + i] = static_cast<int64_t>(start[b]) + seen - 1;
+    }
+}
+
+constexpr int kKeepThreads = 256;
+
+// One workgroup takes one kv head's K or V of a sequence on one layer, and goes through the pages that receive tokens from the
+// first to the last. A token only ever moves towards the front, so what a page receives still stands where it stood when the
+// page's turn comes; within a page, tokens are read before a barrier and written behind it, as many at a time as there are threads.
+// Of each page first the largest value, which says whether its scale holds them.
+template <int TYPE, int D>
+__global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t layer_bytes, int64_t layer_blocks, KvSeqs s,
+                                                          const int32_t* __restrict__ start, const int32_t* __restrict__ keep) {
+    __shared__ uint32_t tops[kKeepThreads / 64];
+    const int b = blockIdx.z, head = blockIdx.x >> 1;
+    const bool is_v = blockIdx.x & 1;
+    const int at = s.first(b), n = s.count(b, at);
+    const int64_t from = max(start[b], 0);
+    const int P = c.page_tokens;
+    uint8_t* data = (is_v ? c.v : c.k) + blockIdx.y * layer_bytes;
+    float* scales = (is_v ? c.v_scale : c.k_scale) + blockIdx.y * layer_blocks;
+    auto page_at = [&](int64_t pos) {
+        const int64_t col = pos >> c.page_shift;
+        return col < s.table_width ? s.page(b, static_cast<int>(col), c.pages) : -1;
+    };
+    // a value's place: block, token in the page, dimension
+    auto byte_at = [&](int64_t block, int t, int d) { return data + block * P * D + (is_v ? d * P + t : t * D + d); };
+    struct Unit {
+        uint32_t byte;
+        float scale;
+        int token;  // in the target page; below 0: none
+    };
+    for (int64_t col = from >> c.page_shift; n > 0 && col <= (from + n - 1) >> c.page_shift; col++) {
+        const int64_t page0 = col * P;
+        const int page = page_at(page0);
+        if (page < 0) continue;  // the same for all threads
+        const int held = static_cast<int>(max(from - page0, int64_t{0}));
+        const int e0 = static_cast<int>(max(page0 - from, int64_t{0})), e1 = static_cast<int>(min(page0 + P - from, static_cast<int64_t>(n)));
+        const int64_t block = c.block(page, head);
+        const float old = scales[block];
+        const int units = (e1 - e0) * D;
+        auto read = [&](int u) -> Unit {  // u: token, then dimension
+            if (u >= units) return {0, 0.0f, -1};
+            const int e = e0 + u / D;
+            const int64_t source = from + max(keep[at + e], e);
+            const int spage = page_at(source);
+            if (spage < 0) return {0, 0.0f, -1};
+            const int64_t sblock = c.block(spage, head);
+            return {*byte_at(sblock, static_cast<int>(source & (P - 1)), u % D), spage == page ? old : scales[sblock],
+                    static_cast<int>(from + e - page0)};
+        };
+        uint32_t top = 0;  // magnitudes order as their bits do; infinities and NaN come out largest
+        for (int u = threadIdx.x; u < units; u += kKeepThreads) {
+            const Unit x = read(u);
+            if (x.token >= 0) top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(x.byte) * x.scale) & 0x7FFFFFFFu);
+        }
+#pragma unroll
+        for (int d = 32; d; d >>= 1) top = max(top, __shfl_xor(top, d));
+        if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
+        __syncthreads();
+        top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+        int shrink = 0;
+        const float now = top < 0x7F800000u ? block_scale<TYPE>(__builtin_bit_cast(float, top), true, old, shrink) : __builtin_nanf("");
+        const float by = now > 0.0f ? now : 1.0f;
+        if (shrink)
+            for (int u = threadIdx.x; u < held * D; u += kKeepThreads) {
+                uint8_t* p = byte_at(block, u / D, u % D);
+                *p = static_cast<uint8_t>(to_byte<TYPE>(ldexpf(from_byte<TYPE>(*p), -shrink)));
+            }
+        for (int u0 = 0; u0 < units; u0 += kKeepThreads) {
+            const Unit x = read(u0 + threadIdx.x);
+            __syncthreads();  // all has been read, the scale too
+            if (x.token >= 0)
+                *byte_at(block, x.token, (u0 + threadIdx.x) % D) =
+                    static_cast<uint8_t>(now > 0.0f ? to_byte<TYPE>(from_byte<TYPE>(x.byte) * x.scale / by) : 0);
+        }
+        if (threadIdx.x == 0) scales[block] = now;
+        __syncthreads();  // the next page's sums, and its reading of what was not moved
+    }
+}
+
+}  // namespace
+}  // namespace wl
+
+using namespace wl;
+
+extern "C" {
+
+int wl_kv_tree(const WlKvBatch* batch, const int32_t* parents, const int32_t* start, uint64_t* tree, int64_t words,
+               int64_t* positions, void* stream) {
+    if (!batch || !batch->cu || !parents || !start || !tree || !positions) return WL_EINVAL_NULL;
+    WlKvBatch b = *batch;  // without a table, of which nothing is read
+    b.table = b.cu;
+    b.table_width = 1;
+    b.table_stride = 1;
+    if (const int rc = check_batch(&b)) return rc;
+    if (words < (b.max_count + 63) / 64 || words >= (int64_t{1} << 31) / 64 || words * b.tokens >= (int64_t{1} << 40)) return WL_EINVAL_SHAPE;
+    if (reinterpret_cast<uintptr_t>(parents) % 4 || reinterpret_cast<uintptr_t>(start) % 4 || reinterpret_cast<uintptr_t>(tree) % 8 ||
+        reinterpret_cast<uintptr_t>(positions) % 8)
+        return WL_EINVAL_ALIGN;
+    k_kv_tree<<<b.seqs + 1, kTreeThreads, 0, static_cast<hipStream_t>(stream)>>>(seqs_of(&b), parents, start, tree, words, positions);
+    return launch_status();
+}
+
+int wl_kv_keep(const WlKvCache* cache, const WlKvBatch* batch, const int32_t* start, const int32_t* keep, void* stream) {
+    if (const int rc = check_cache(cache)) return rc;
+    if (const int rc = check_batch(batch)) return rc;
+    if (!start || !keep) return WL_EINVAL_NULL;
+    if (reinterpret_cast<uintptr_t>(start) % 4 || reinterpret_cast<uintptr_t>(keep) % 4) return WL_EINVAL_ALIGN;
+    const dim3 grid(2 * cache->kv_heads, cache->layers, batch->seqs);
+    const KvLayer c = layer_of(cache, 0);
+    const int64_t blocks = cache->pages * cache->kv_heads, bytes = blocks * cache->page_tokens * cache->head_dim;
+    auto run = [&](auto type, auto dim) {
+        k_kv_keep<decltype(type)::value, decltype(dim)::value>
+            <<<grid, kKeepThreads, 0, static_cast<hipStream_t>(stream)>>>(c, bytes, blocks, seqs_of(batch), start, keep);
+    };
+    auto with_dim = [&](auto type) {
+        if (cache->head_dim == 64)
+            run(type, std::integral_constant<int, 64>());
+        else if (cache->head_dim == 128)
+            run(type, std::integral_constant<int, 128>());
+        else
+            run(type, std::integral_constant<int, 256>());
+    };
+    if (cache->type == WL_KV_INT8)
+        with_dim(std::integral_constant<int, WL_KV_INT8>());
+    else
+        with_dim(std::integral_constant<int, WL_KV_E4M3>());
+    return launch_status();
+}
+
+}  // extern "C"

@@ -121,6 +121,54 @@ struct KvSeqs {
     __device__ __forceinline__ int page(int b, int col, int pages) const { return page_of(entry(b, col), pages); }
 };
 
+// Bytes and scales, for what writes into the cache.
+
+template <int TYPE>
+constexpr float kLargest = TYPE == WL_KV_INT8 ? 127.0f : 448.0f;
+
+// x (a value already divided by its scale, |x| <= kLargest) as a byte, rounded to nearest even.
+template <int TYPE>
+__device__ __forceinline__ uint32_t to_byte(float x) {
+    if constexpr (TYPE == WL_KV_INT8)
+        return static_cast<uint32_t>(static_cast<int>(__builtin_rintf(x))) & 0xFFu;
+    else
+        return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_fp8_f32(x, x, 0, false)) & 0xFFu;
+}
+
+template <int TYPE>
+__device__ __forceinline__ float from_byte(uint32_t b) {
+    if constexpr (TYPE == WL_KV_INT8)
+        return static_cast<float>(static_cast<int8_t>(b));
+    else
+        return __builtin_amdgcn_cvt_f32_fp8(static_cast<int>(b), 0);
+}
+
+__device__ __forceinline__ float bf16_to_float(uint32_t bits) { return __builtin_bit_cast(float, bits << 16); }
+
+// The smallest bf16 value not below x (x >= 0, finite).
+__device__ __forceinline__ float round_up_bf16(float x) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) + 0xFFFFu) & 0xFFFF0000u);
+}
+
+// The scale of a block whose new rows reach `top`, and the power of two by which its older bytes shrink. `held`: it has
+// older tokens, `old` their scale. Exact: top and old have 8 significant bits, so 127 old and 448 old fit fp32, and the
+// quotient top / 127 is a bf16 value or at least 2^-16 (relative) away from one, so its rounding up is not moved by fp32's.
+template <int TYPE>
+__device__ __forceinline__ float block_scale(float top, bool held, float old, int& shrink) {
+    shrink = 0;
+    if (!held || old == 0.0f) {
+        const float s = round_up_bf16(top / kLargest<TYPE>);
+        if (held && s > 0.0f) shrink = 32;  // older values are 0: so are their bytes from here on
+        return s;
+    }
+    const float reach = old * kLargest<TYPE>;
+    if (!(top > reach)) return old;  // a NaN scale stays
+    int n = max(0, ilogbf(top) - ilogbf(reach));
+    if (ldexpf(reach, n) < top) n++;
+    shrink = n;
+    return ldexpf(old, n);
+}
+
 inline KvSeqs seqs_of(const WlKvBatch* b) {
     return {b->table, b->cu, b->table_stride, static_cast<int32_t>(b->tokens), b->seqs, b->table_width, b->max_count};
 }

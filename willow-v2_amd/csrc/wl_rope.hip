@@ -1,4 +1,4 @@
-// Rotary positions with several axes (wl_rope).
+// Rotary positions with several axes (wl_rope), behind a norm of each head (wl_norm_rope).
 #include "wl_host.h"
 
 namespace wl {
@@ -28,6 +28,15 @@ __device__ __forceinline__ int axis_of(const RopeArgs& a, int j) {
         if (j >= end) axis = i + 1;
     }
     return axis;
+}
+
+// Cosine and sine of frequency j at a token's position, times the scale.
+__device__ __forceinline__ float2 turn_of(const RopeArgs& a, int j, int token) {
+    const double pos = static_cast<double>(a.positions[axis_of(a, j) * a.positions_stride + token]);
+    const double turns = pos * a.inv_freq[j] * 0.15915494309189533577;  // 1 / (2 pi)
+    float s, c;
+    sincospif(static_cast<float>(2.0 * (turns - __builtin_rint(turns))), &s, &c);
+    return make_float2(a.scale * c, a.scale * s);
 }
 
 template <typename T>
@@ -99,13 +108,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
         const int i = threadIdx.x / 32 + r * kRows;
         if (i < heads && lane < units) load(head_at(i), lane, lo[r], hi[r]);
     }
-    for (int j = threadIdx.x; j < a.half; j += kRopeThreads) {
-        const double pos = static_cast<double>(a.positions[axis_of(a, j) * a.positions_stride + token]);
-        const double turns = pos * a.inv_freq[j] * 0.15915494309189533577;  // 1 / (2 pi)
-        float s, c;
-        sincospif(static_cast<float>(2.0 * (turns - __builtin_rint(turns))), &s, &c);
-        turn[j] = make_float2(a.scale * c, a.scale * s);
-    }
+    for (int j = threadIdx.x; j < a.half; j += kRopeThreads) turn[j] = turn_of(a, j, token);
     __syncthreads();
 #pragma unroll
     for (int r = 0; r < kEarly; r++) {
@@ -118,6 +121,111 @@ __global__ __launch_bounds__(kRopeThreads) void k_rope(RopeArgs a) {
             load(head_at(i), u, x, y);
             finish(head_at(i), u, x, y);
         }
+}
+
+// The norm of each head before it turns. Weights: fp32 or bf16, null: all 1.
+struct NormArgs {
+    const void *q_weight, *k_weight;
+    float eps, offset;  // offset: 1 where weights are zero-centred
+    int32_t bf16;
+};
+
+// As k_rope, a workgroup a token and 32 lanes a head, with a head's sum of squares over its lanes between reading and turning; the
+// first run of values stays in registers meanwhile (all of a head up to 32 runs: 256 values of bf16, 128 of fp32), the others
+// are read again. Both weights go into LDS beside the cosines.
+template <typename T, int VEC>
+__global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs n) {
+    extern __shared__ float2 turn[];  // [half]: cos, sin; then the weights of q and of k [head_dim]
+    float* weight = reinterpret_cast<float*>(turn + a.half);
+    struct alignas(sizeof(T) * VEC) Run {
+        T v[VEC];
+    };
+    constexpr int kRows = kRopeThreads / 32;
+    const int token = blockIdx.x, lane = threadIdx.x % 32;
+    const int pairs = a.half / VEC, units = pairs + (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
+    struct Head {
+        const T* in;
+        T* out;
+        const float* w;
+    };
+    auto head_at = [&](int i) -> Head {
+        const bool is_k = i >= a.q.heads;
+        const WlRopeTensor& x = is_k ? a.k : a.q;
+        const int h = is_k ? i - a.q.heads : i;
+        return {static_cast<const T*>(x.in) + token * x.in_token_stride + h * x.in_head_stride,
+                static_cast<T*>(x.out) + token * x.out_token_stride + h * x.out_head_stride, weight + (is_k ? a.head_dim : 0)};
+    };
+    // unit u: run u of each half of what turns, then the rest
+    auto load = [&](const Head& x, int u, Run& lo, Run& hi) {
+        lo = *reinterpret_cast<const Run*>(x.in + (u < pairs ? u : u + pairs) * VEC);
+        if (u < pairs) hi = *reinterpret_cast<const Run*>(x.in + a.half + u * VEC);
+    };
+    auto squares = [&](int u, const Run& lo, const Run& hi) {
+        float s = 0.0f;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float p = load_value(lo.v + e);
+            s = __builtin_fmaf(p, p, s);
+        }
+        if (u < pairs)
+#pragma unroll
+            for (int e = 0; e < VEC; e++) {
+                const float p = load_value(hi.v + e);
+                s = __builtin_fmaf(p, p, s);
+            }
+        return s;
+    };
+    auto finish = [&](const Head& x, int u, Run lo, Run hi, float inv) {
+        const int at = (u < pairs ? u : u + pairs) * VEC;
+#pragma unroll
+        for (int e = 0; e < VEC; e++) {
+            const float p = load_value(lo.v + e) * inv * x.w[at + e];
+            if (u < pairs) {
+                const float2 cs = turn[u * VEC + e];
+                const float q = load_value(hi.v + e) * inv * x.w[a.half + at + e];
+                store_value(lo.v + e, p * cs.x - q * cs.y);
+                store_value(hi.v + e, q * cs.x + p * cs.y);
+            } else {
+                store_value(lo.v + e, p);
+            }
+        }
+        *reinterpret_cast<Run*>(x.out + at) = lo;
+        if (u < pairs) *reinterpret_cast<Run*>(x.out + a.half + at) = hi;
+    };
+    Run lo = {}, hi = {};
+    if (static_cast<int>(threadIdx.x) / 32 < heads && lane < units) load(head_at(threadIdx.x / 32), lane, lo, hi);
+    for (int j = threadIdx.x; j < 2 * a.head_dim; j += kRopeThreads) {
+        const bool is_k = j >= a.head_dim;
+        const void* w = is_k ? n.k_weight : n.q_weight;
+        const int d = is_k ? j - a.head_dim : j;
+        weight[j] = !w ? 1.0f : n.offset + (n.bf16 ? load_value(static_cast<const uint16_t*>(w) + d) : static_cast<const float*>(w)[d]);
+    }
+    for (int j = threadIdx.x; j < a.half; j += kRopeThreads) turn[j] = turn_of(a, j, token);
+    __syncthreads();
+    for (int i = threadIdx.x / 32; i < heads; i += kRows) {
+        const Head x = head_at(i);
+        if (i >= kRows && lane < units) load(x, lane, lo, hi);
+        float sum = lane < units ? squares(lane, lo, hi) : 0.0f;
+        for (int u = lane + 32; u < units; u += 32) {
+            Run y, z = {};
+            load(x, u, y, z);
+            sum += squares(u, y, z);
+        }
+#pragma unroll
+        for (int d = 16; d; d >>= 1) sum += __shfl_xor(sum, d);
+        const float inv = 1.0f / sqrtf(sum / a.head_dim + n.eps);
+        if (lane < units) finish(x, lane, lo, hi, inv);
+        for (int u = lane + 32; u < units; u += 32) {
+            Run y, z = {};
+            load(x, u, y, z);
+            finish(x, u, y, z, inv);
+        }
+    }
+}
+
+template <typename T, int VEC>
+void launch_norm_rope(const RopeArgs& a, const NormArgs& n, hipStream_t stream) {
+    k_norm_rope<T, VEC><<<a.tokens, kRopeThreads, sizeof(float2) * a.half + 2 * sizeof(float) * a.head_dim, stream>>>(a, n);
 }
 
 template <typename T, int VEC>
@@ -156,14 +264,10 @@ bool aligned16(const WlRopeTensor* x, int size) {
            x->out_head_stride % n == 0;
 }
 
-}  // namespace
-}  // namespace wl
-
-using namespace wl;
-
-extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
-                       const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
-                       const int32_t* sections_host, int interleaved, float scale, void* stream) {
+// Checks a call's arguments and fills in the kernels' (a: all zeros); wide: 16 bytes may be moved at once.
+int rope_args(RopeArgs& a, bool& wide, const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim,
+              int rotary_dim, const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
+              const int32_t* sections_host, int interleaved, float scale) {
     if (!q || !positions || !inv_freq || !sections_host) return WL_EINVAL_NULL;
     if (dtype != WL_DTYPE_F32 && dtype != WL_DTYPE_BF16) return WL_EINVAL_DTYPE;
     const int size = dtype == WL_DTYPE_F32 ? 4 : 2;
@@ -178,7 +282,6 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
     // one tensor's result where the other is read or written
     if (k && (q->out == k->out || q->out == k->in || k->out == q->in)) return WL_EINVAL_OVERLAP;
     if (reinterpret_cast<uintptr_t>(positions) % 8 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return WL_EINVAL_ALIGN;
-    RopeArgs a = {};
     a.half = rotary_dim / 2;
     int64_t sum = 0;
     for (int i = 0; i < axes; i++) {
@@ -200,7 +303,25 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
     a.interleaved = interleaved != 0;
     a.scale = scale;
     const int vec = 16 / size;
-    const bool wide = a.half % vec == 0 && head_dim % vec == 0 && aligned16(q, size) && (!k || aligned16(k, size));
+    wide = a.half % vec == 0 && head_dim % vec == 0 && aligned16(q, size) && (!k || aligned16(k, size));
+    return WL_OK;
+}
+
+}  // namespace
+}  // namespace wl
+
+using namespace wl;
+
+extern "C" {
+
+int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
+            const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes, const int32_t* sections_host,
+            int interleaved, float scale, void* stream) {
+    RopeArgs a = {};
+    bool wide;
+    if (const int rc = rope_args(a, wide, q, k, dtype, tokens, head_dim, rotary_dim, positions, positions_stride, inv_freq, axes,
+                                 sections_host, interleaved, scale))
+        return rc;
     const hipStream_t st = static_cast<hipStream_t>(stream);
     if (dtype == WL_DTYPE_F32)
         wide ? launch_rope<float, 4>(a, st) : launch_rope<float, 1>(a, st);
@@ -208,3 +329,27 @@ extern "C" int wl_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, 
         wide ? launch_rope<uint16_t, 8>(a, st) : launch_rope<uint16_t, 1>(a, st);
     return launch_status();
 }
+
+int wl_norm_rope(const WlRopeTensor* q, const WlRopeTensor* k, int dtype, int64_t tokens, int head_dim, int rotary_dim,
+                 const int64_t* positions, int64_t positions_stride, const double* inv_freq, int axes,
+                 const int32_t* sections_host, int interleaved, float scale, const void* q_weight, const void* k_weight,
+                 int weight_dtype, float eps, int zero_centered, void* stream) {
+    RopeArgs a = {};
+    bool wide;
+    if (const int rc = rope_args(a, wide, q, k, dtype, tokens, head_dim, rotary_dim, positions, positions_stride, inv_freq, axes,
+                                 sections_host, interleaved, scale))
+        return rc;
+    if (weight_dtype != WL_DTYPE_F32 && weight_dtype != WL_DTYPE_BF16) return WL_EINVAL_DTYPE;
+    const int size = weight_dtype == WL_DTYPE_F32 ? 4 : 2;
+    if (reinterpret_cast<uintptr_t>(q_weight) % size || reinterpret_cast<uintptr_t>(k_weight) % size) return WL_EINVAL_ALIGN;
+    if (!(eps >= 0.0f && eps < __builtin_inff())) return WL_EINVAL_SHAPE;
+    const NormArgs n = {q_weight, k_weight, eps, zero_centered ? 1.0f : 0.0f, weight_dtype == WL_DTYPE_BF16};
+    const hipStream_t st = static_cast<hipStream_t>(stream);
+    if (dtype == WL_DTYPE_F32)
+        wide ? launch_norm_rope<float, 4>(a, n, st) : launch_norm_rope<float, 1>(a, n, st);
+    else
+        wide ? launch_norm_rope<uint16_t, 8>(a, n, st) : launch_norm_rope<uint16_t, 1>(a, n, st);
+    return launch_status();
+}
+
+}  // extern "C"

@@ -16,7 +16,7 @@ of twice the heads' width holds each head's query and, behind it, its output gat
 import torch
 import torch.nn.functional as F
 
-from gguf.hip import rope
+from gguf.hip import norm_rope, rope
 
 
 class Rotary:
@@ -48,6 +48,14 @@ class Rotary:
     def __call__(self, q, k, positions):
         return rope(q, k, positions, self.inv_freq, sections=self.sections, interleaved=self.interleaved, scale=self.scale)
 
+    def normed(self, q, k, positions, q_weight, k_weight, eps: float):
+        """The same of queries and keys that are normed first (head_norm), in one pass and rounded once."""
+        q_weight, k_weight = (w.to(q.device) for w in (q_weight, k_weight))
+        if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (torch.float32, torch.bfloat16):
+            q_weight, k_weight = q_weight.float(), k_weight.float()
+        return norm_rope(q, k, positions, self.inv_freq, q_weight.contiguous(), k_weight.contiguous(), eps=eps, sections=self.sections,
+                         interleaved=self.interleaved, scale=self.scale)
+
 
 def head_norm(x: torch.Tensor, weight, eps: float) -> torch.Tensor:
     """The zero-centered RMSNorm of the last dimension (engines/base.py:27-31) in fp32, rounded to x's dtype; x itself
@@ -65,10 +73,12 @@ class HipAttention:
     attention_eps = 1e-6
 
     def hip_attention(self, x: torch.Tensor, layer: int, cache_layer: int, step, positions: torch.Tensor,
-                      causal: bool = True) -> torch.Tensor:
+                      causal: bool = True, window: int = None, sinks: int = 0, tree: torch.Tensor = None) -> torch.Tensor:
         """x [tokens, hidden], the step's rows in its sequences' order -> [tokens, hidden] in x's dtype. layer: the layer's
         number in the weights' names; cache_layer: in the cache (which holds the attention layers alone); positions int64
-        [axes, tokens] (Rotary.positions). The step's keys and values are written into the cache, then attended."""
+        [axes, tokens] (Rotary.positions). The step's keys and values are written into the cache, then attended; window and sinks:
+        of a layer that sees the last tokens and the first alone; tree: the step's tokens are drafts, with the masks and the positions
+        that the cache's tree() gave. Norms and positions are one call where both norms have weights and self.rotary can (Rotary)."""
         cache, p = self.kv_cache, f"{self.prefix}layers.{layer}.self_attn"
         dim, kv_heads = cache.pages.head_dim, cache.pages.kv_heads
         flat = x.reshape(-1, x.shape[-1]).to(device=cache.device, dtype=torch.bfloat16)
@@ -89,11 +99,14 @@ class HipAttention:
         else:
             raise ValueError(f"{p}.q_proj: {wide.shape[1]} rows for {heads} heads of {dim}")
         k, v = (project(n, kv_heads).view(-1, kv_heads, dim) for n in ("k_proj", "v_proj"))
-        q = head_norm(q, self.weights.get(f"{p}.q_norm.weight"), self.attention_eps)
-        k = head_norm(k, self.weights.get(f"{p}.k_norm.weight"), self.attention_eps)
-        q, k = self.rotary(q, k, positions)
+        q_norm, k_norm = (self.weights.get(f"{p}.{n}_norm.weight") for n in "qk")
+        if q_norm is not None and k_norm is not None and hasattr(self.rotary, "normed"):
+            q, k = self.rotary.normed(q, k, positions, q_norm, k_norm, self.attention_eps)
+        else:
+            q, k = head_norm(q, q_norm, self.attention_eps), head_norm(k, k_norm, self.attention_eps)
+            q, k = self.rotary(q, k, positions)
         cache.append(cache_layer, step, k, v)
-        o = cache.attend(cache_layer, step, q, causal=causal)
+        o = cache.attend(cache_layer, step, q, causal=causal, window=window, sinks=sinks, tree=tree)
         if gate is not None:
             o = (o.float() * torch.sigmoid(gate.float())).to(torch.bfloat16)
         y = F.linear(o.view(o.shape[0], -1), self.weights[f"{p}.o_proj.weight"])

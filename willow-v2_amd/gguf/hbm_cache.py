@@ -13,6 +13,9 @@ what is live to the lowest page numbers. The lowest free page is always taken fi
         cache.append(layer, step, k, v)                       # k, v bf16 [tokens, kv_heads, head_dim]
         out = cache.attend(layer, step, q)                    # q bf16 [tokens, heads, head_dim]
 
+A step whose tokens are a tree of drafts: tree, positions = cache.tree(step, parents), then attend(.., tree=tree) on every layer,
+and keep(seqs, counts, accepted) when the model has said which of them stay.
+
 Calls may come on any streams: the cache orders its work as its calls are (_StreamOrder). A captured graph's replays it does
 not see: replay on the stream on which refresh() was called for it.
 """
@@ -23,7 +26,7 @@ from dataclasses import dataclass, field
 import numpy as np
 import torch
 
-from .hip import KVPages, kv_append, kv_attend, kv_copy
+from .hip import KVPages, kv_append, kv_attend, kv_copy, kv_keep, kv_tree
 
 
 class OutOfPages(RuntimeError):
@@ -131,6 +134,31 @@ class PageBook:
                 s[1].append(self._take())
             s[0] += n
         return src, dst
+
+    def moves(self, seqs, counts, kept):
+        """What keeping just the tokens at kept[i] of the last counts[i] of seqs[i] moves, with nothing changed -> a list of (pages
+        from the one on that the first of the last tokens is in, where in it, kept) of the sequences that it moves tokens of.
+        Raises KeyError or ValueError for unknown or repeated sequences, counts beyond their lengths, tokens out of range or out
+        of order, and where tokens would move into a page that another sequence has too."""
+        if not len(seqs) == len(counts) == len(kept) or len(set(seqs)) != len(seqs):
+            raise ValueError("seqs must be different sequences, one count and one list of kept tokens for each")
+        out = []
+        for seq, n, keep in zip(seqs, counts, kept):
+            length, pages = self._sequence(seq)
+            n, keep = _whole(n), [_whole(i) for i in keep]
+            if not 0 <= n <= length:
+                raise ValueError(f"sequence {seq} has {length} tokens, not {n} to keep some of")
+            if any(not a < b for a, b in zip([-1] + keep, keep + [n])):
+                raise ValueError(f"sequence {seq}: {keep} are not increasing numbers of {n} tokens")
+            still = next((i for i, j in enumerate(keep) if i != j), len(keep))
+            if still == len(keep):
+                continue
+            first, stop = length - n, length - n + len(keep)
+            for page in pages[first // self.page_tokens:-(-stop // self.page_tokens)]:
+                if self.uses[page] != 1:
+                    raise ValueError(f"sequence {seq}: tokens would move into page {page}, which another sequence has too")
+            out.append((pages[first // self.page_tokens:], first % self.page_tokens, keep))
+        return out
 
     def compact(self):
         """Moves the live pages to the lowest numbers -> (source pages, target pages) to copy. No page is both."""
@@ -324,13 +352,44 @@ class HBMKVCache:
         kv_append(self.pages, layer, k, v, step.table, step.start, step.cu, max_count=step.max_count or 1)
 
     def attend(self, layer: int, step: KVStep, q: torch.Tensor, scale: float = None, causal: bool = True,
-               out: torch.Tensor = None) -> torch.Tensor:
+               out: torch.Tensor = None, window: int = None, sinks: int = 0, tree: torch.Tensor = None) -> torch.Tensor:
         """The step's rows' attention over one layer of their sequences, bf16 [tokens, heads, head_dim]; kv_attend. Rows of q behind
-        the step's tokens (padding) come out as zeros, or stay as they are in `out`."""
+        the step's tokens (padding) come out as zeros, or stay as they are in `out`. window, sinks: a layer that sees the last
+        `window` tokens and the first `sinks`. tree: the step's tokens are drafts, masks as tree() gives them (a row for each of q's)."""
         step.check(q, "q")
         if out is None and q.shape[0] > step.tokens:
             out = torch.empty_like(q, memory_format=torch.contiguous_format)
             out[step.tokens:].zero_()
         self._order(False, step)
         return kv_attend(self.pages, layer, q, step.table, step.length, step.cu, max_count=step.max_count or 1,
-                         max_length=step.max_length, scale=scale, causal=causal, out=out)
+                         max_length=step.max_length, scale=scale, causal=causal, out=out, window=window, sinks=sinks, tree=tree)
+
+    # -- drafted tokens -------------------------------------------------------------------------------------------
+
+    def tree(self, step: KVStep, parents: torch.Tensor):
+        """The step's tokens as trees of drafts -> (masks for attend, int64 [tokens] positions); kv_tree. parents int32 [tokens] on the
+        GPU, each row's parent among its sequence's rows (-1: a root). For all layers of the step."""
+        step.check(parents, "parents")
+        self._order(False, step)
+        return kv_tree(parents, step.start, step.cu, max_count=step.max_count or 1)
+
+    def keep(self, seqs, counts, kept):
+        """Of the last counts[i] tokens of seqs[i] just those at kept[i] stay (numbers below counts[i], in order), on every layer, and
+        move up behind the tokens before them; kv_keep. The sequences are that much shorter afterwards: steps made before hold lengths
+        that are no longer theirs. Not under capture."""
+        self._not_captured()
+        seqs, counts, kept = list(seqs), [_whole(n) for n in counts], [[_whole(i) for i in k] for k in kept]
+        moves = self.book.moves(seqs, counts, kept)
+        if moves:
+            width, n = max(len(pages) for pages, _, _ in moves), len(moves)
+            table = np.full((n, width), -1, dtype=np.int32)
+            for row, (pages, _, _) in zip(table, moves):
+                row[:len(pages)] = pages
+            parts = [table.ravel(), [at for _, at, _ in moves], np.cumsum([0] + [len(k) for _, _, k in moves]),
+                     [i for _, _, k in moves for i in k]]
+            self._order(True)
+            up = torch.from_numpy(np.concatenate(parts).astype(np.int32)).to(self.device)
+            table, start, cu, keep = up.split([len(p) for p in parts])
+            kv_keep(self.pages, table.view(n, width), start, keep, cu, max_count=max(len(k) for _, _, k in moves))
+        for seq, n, keep in zip(seqs, counts, kept):
+            self.book.truncate(seq, self.book.length(seq) - n + len(keep))

@@ -6,8 +6,10 @@ gemv_batch, gemv_combine, dequantize_gpu, GGMLWeight; gguf/metal.py:20,295,320-4
 Metal kernels round to bf16. It adds the fused MoE layer (moe_layer / MoELayer), which replaces Engine.moe's
 router -> host sync -> per-expert launches (engines/base.py:445-591) with device-side routing.
 
-Beside it the attention half's operators (gguf.hip.kv): rope (rotary positions with several axes), KVPages, kv_append,
-kv_attend and kv_copy (a paged 8-bit key/value cache, its writer, the attention that reads it, its page copies).
+Beside it the attention half's operators (gguf.hip.kv): rope and norm_rope (rotary positions with several axes, behind a norm of
+each head), KVPages, kv_append, kv_attend and kv_copy (a paged 8-bit key/value cache, its writer, the attention that reads it,
+with a sliding window or a tree of drafted tokens too, its page copies), kv_tree and kv_keep (such a tree's masks and
+positions, and moving its accepted tokens up in the cache).
 
 There is no CPU fallback: without the built library (or without a GPU) every compute call raises.
 """
@@ -87,6 +89,13 @@ class WlRopeTensor(ctypes.Structure):
     ]
 
 
+class WlKvMask(ctypes.Structure):
+    """Mirror of the C struct WlKvMask (include/willow_hip.h)."""
+    _fields_ = [
+        ("tree", ctypes.c_void_p), ("tree_stride", ctypes.c_int64), ("window", ctypes.c_int64), ("sinks", ctypes.c_int64),
+    ]
+
+
 def library() -> ctypes.CDLL:
     """libwillow_hip.so, loaded once. torch is imported first so the library binds to torch's HIP runtime."""
     global _lib
@@ -132,7 +141,16 @@ def library() -> ctypes.CDLL:
                                  ctypes.c_size_t, vp]
     lib.wl_kv_copy.argtypes = [cache_p, vp, vp, i64, vp]
     lib.wl_rope.argtypes = [rope_p, rope_p, c_int, i64, c_int, c_int, vp, i64, vp, c_int, i32p, c_int, ctypes.c_float, vp]
-    for name in ("wl_kv_check", "wl_kv_append", "wl_kv_attend", "wl_kv_copy", "wl_rope"):
+    mask_p = ctypes.POINTER(WlKvMask)
+    lib.wl_kv_attend_masked_workspace_bytes.argtypes = [cache_p, c_int, batch_p, i64, mask_p]
+    lib.wl_kv_attend_masked_workspace_bytes.restype = ctypes.c_size_t
+    lib.wl_kv_attend_masked.argtypes = [cache_p, c_int, vp, i64, i64, c_int, batch_p, vp, i64, ctypes.c_float, mask_p, vp, vp,
+                                        ctypes.c_size_t, vp]
+    lib.wl_kv_tree.argtypes = [batch_p, vp, vp, vp, i64, vp, vp]
+    lib.wl_kv_keep.argtypes = [cache_p, batch_p, vp, vp, vp]
+    lib.wl_norm_rope.argtypes = [*lib.wl_rope.argtypes[:-1], vp, vp, c_int, ctypes.c_float, c_int, vp]
+    for name in ("wl_kv_check", "wl_kv_append", "wl_kv_attend", "wl_kv_copy", "wl_rope", "wl_kv_attend_masked", "wl_kv_tree",
+                 "wl_kv_keep", "wl_norm_rope"):
         getattr(lib, name).restype = c_int
     for name in ("wl_dequant", "wl_gemv", "wl_gemv_dtype", "wl_linear", "wl_gemv_batch", "wl_gemv_combine",
                  "wl_moe_check", "wl_moe_route", "wl_moe_layer", "wl_moe_layer_profile"):
@@ -371,4 +389,4 @@ class GGMLWeight:
 
 
 from .moe import MoELayer, moe_layer  # noqa: E402  (needs the names above)
-from .kv import KVPages, kv_append, kv_attend, kv_copy, rope  # noqa: E402
+from .kv import KVPages, kv_append, kv_attend, kv_copy, kv_keep, kv_tree, norm_rope, rope  # noqa: E402

@@ -1,4 +1,5 @@
-"""The attention half's operators: rotary positions, the paged 8-bit key/value cache and attention over it.
+"""The attention half's operators: rotary positions, the paged 8-bit key/value cache and attention over it, trees of drafted
+tokens in it.
 
 The reference keeps keys and values in a bf16 tensor per layer that grows in blocks of 256 positions and runs torch's
 attention on it (engines/base.py:213-216,328-367). Here the cache is pages of bytes with one scale for each page and kv
@@ -12,7 +13,7 @@ import functools
 import numpy as np
 import torch
 
-from . import DTYPE_BF16, DTYPE_F32, KV_E4M3, KV_INT8, WlKvBatch, WlKvCache, WlRopeTensor, check, library
+from . import DTYPE_BF16, DTYPE_F32, KV_E4M3, KV_INT8, WlKvBatch, WlKvCache, WlKvMask, WlRopeTensor, check, library
 
 TYPES = {torch.int8: KV_INT8, torch.float8_e4m3fn: KV_E4M3}
 
@@ -148,9 +149,35 @@ def kv_append(pages: KVPages, layer: int, k: torch.Tensor, v: torch.Tensor, tabl
             b, start.data_ptr())
 
 
+def _mask(n, index, b, causal, window, sinks, tree):
+    """The WlKvMask of one call, or None."""
+    if window is None and tree is None:
+        if sinks:
+            raise ValueError("sinks are what stays visible in front of a window")
+        return None
+    if not causal:
+        raise ValueError("a window or a tree goes with causal=True")
+    if window is not None and (window < 1 or sinks < 0):
+        raise ValueError(f"window {window} with {sinks} sinks")
+    if window is None and sinks:
+        raise ValueError("sinks are what stays visible in front of a window")
+    m = WlKvMask(None, 0, 0 if window is None else min(window, 1 << 31), min(sinks, 1 << 31))
+    if tree is not None:
+        _need(tree, "tree", index, torch.int64, (n, "words"))
+        rows, words = tree.shape
+        if rows != n or words * 64 < b.max_count or (words > 1 and tree.stride(1) != 1) or (n > 1 and tree.stride(0) < words):
+            raise ValueError(f"tree must be [{n}, {-(-b.max_count // 64)} words or more] with contiguous rows that lie apart (got "
+                             f"{list(tree.shape)}, strides {list(tree.stride())})")
+        if window is not None and window < b.max_count:
+            raise ValueError(f"a window of {window} would begin inside a tree of up to {b.max_count} tokens")
+        m.tree, m.tree_stride = tree.data_ptr(), max(tree.stride(0), words)
+    return m
+
+
 def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, length: torch.Tensor, cu: torch.Tensor,
               max_count: int = None, max_length: int = None, scale: float = None, causal: bool = True,
-              out: torch.Tensor = None, workspace: torch.Tensor = None) -> torch.Tensor:
+              out: torch.Tensor = None, workspace: torch.Tensor = None, window: int = None, sinks: int = 0,
+              tree: torch.Tensor = None) -> torch.Tensor:
     """Grouped-query attention of one layer: q bf16 [tokens, q_heads, head_dim] (any strides over tokens and heads) -> bf16
     [tokens, q_heads, head_dim]. Sequence b's rows are cu[b] .. cu[b + 1], the last of its length[b] tokens in the cache (so
     append them first); query head i reads kv head i / (q_heads / kv_heads). causal: a row sees the positions up to its own;
@@ -159,8 +186,12 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     sequences the form that is made for them); cu must not decrease; max_length: a bound of length that only steers how the
     work is split (default: what the table's width holds). Rows of no sequence stay as they are in `out` (which may not overlap
     q), and hold anything without it.
-    workspace: a uint8 tensor that is large enough (wl_kv_attend_workspace_bytes), for calls that do not overlap in time; by
-    default it comes from torch's allocator, for this call and stream."""
+    workspace: a uint8 tensor that is large enough (wl_kv_attend_workspace_bytes; wl_kv_attend_masked_workspace_bytes with a
+    window or a tree), for calls that do not overlap in time; by default it comes from torch's allocator, for this call and stream.
+    window: a row sees the last `window` tokens up to its own alone, and the sequence's first `sinks`; only their pages are read.
+    tree: int64 [tokens, words], words >= max_count / 64: the rows are drafted tokens, and of its sequence's own rows a row sees
+    those whose bits are set (bit j % 64 of word j // 64 for row j; kv_tree makes them), all tokens before the rows as without it.
+    With both, a row's position is its first row's plus the drafted tokens that it sees less one; the window has to hold a whole tree."""
     _in_cache(pages, layer)
     n, heads, token_stride, head_stride = _rows(q, "q", pages.index, torch.bfloat16, None, pages.head_dim)
     if heads == 0 or heads % pages.kv_heads:
@@ -179,7 +210,11 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
             raise ValueError(f"max_length {max_length}")
         longest = max_length
     lib = library()
-    need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, b, longest)
+    mask = _mask(n, pages.index, b, causal, window, sinks, tree)
+    if mask is None:
+        need = lib.wl_kv_attend_workspace_bytes(pages.ref, heads, b, longest)
+    else:
+        need = lib.wl_kv_attend_masked_workspace_bytes(pages.ref, heads, b, longest, mask)
     space = None
     if workspace is not None:
         if workspace.dtype is not torch.uint8 or workspace.get_device() != pages.index or not workspace.is_contiguous():
@@ -188,9 +223,56 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     elif need:
         workspace = torch.empty(need, dtype=torch.uint8, device=pages.device)
         space = workspace.data_ptr()
-    _launch(pages.index, lib.wl_kv_attend, pages.ref, layer, q.data_ptr(), token_stride, head_stride, heads, b,
-            length.data_ptr(), longest, pages.head_dim ** -0.5 if scale is None else scale, causal, out.data_ptr(), space, need)
+    _launch(pages.index, lib.wl_kv_attend if mask is None else lib.wl_kv_attend_masked, pages.ref, layer, q.data_ptr(), token_stride,
+            head_stride, heads, b, length.data_ptr(), longest, pages.head_dim ** -0.5 if scale is None else scale,
+            causal if mask is None else mask, out.data_ptr(), space, need)
     return out
+
+
+def kv_tree(parents: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, max_count: int = None):
+    """A tree of drafted tokens for each sequence -> (tree, positions): int64 [tokens, words] masks as kv_attend takes them (a row's
+    ancestors and itself) and int64 [tokens] positions, start[b] plus the number of a row's ancestors. parents: int32 [tokens], each
+    row's parent among its sequence's rows cu[b] .. cu[b + 1], counted from 0, and before the row itself; anything else (-1) is a
+    root, behind the last token before the draft. start, cu int32 [seqs], [seqs + 1]; max_count: the most rows any sequence has
+    (words = max_count / 64 rounded up; rows beyond it are dropped; default: all rows). Rows of no sequence get no bits and
+    position 0. Once a step: every layer takes the same masks."""
+    index = parents.get_device() if isinstance(parents, torch.Tensor) else -1
+    _need(parents, "parents", index, torch.int32, ("tokens",))
+    _need(start, "start", index, torch.int32, ("sequences",))
+    n, seqs = parents.shape[0], start.shape[0]
+    _need(cu, "cu", index, torch.int32, (seqs + 1,))
+    if cu.shape[0] != seqs + 1 or not (parents.is_contiguous() and start.is_contiguous() and cu.is_contiguous()):
+        raise ValueError(f"parents, start and cu must be contiguous, cu [{seqs + 1}] (got {list(cu.shape)})")
+    if max_count is None or max_count > n:
+        max_count = n
+    if (seqs | n | max_count) >> 31:
+        raise ValueError(f"max_count {max_count} with {seqs} sequences and {n} rows")
+    words = max(1, -(-max_count // 64))
+    tree = torch.empty(n, words, dtype=torch.int64, device=parents.device)
+    positions = torch.empty(n, dtype=torch.int64, device=parents.device)
+    if n == 0 or seqs == 0:
+        return tree.zero_(), positions.zero_()
+    _launch(index, library().wl_kv_tree, WlKvBatch(None, cu.data_ptr(), 1, n, seqs, 1, max_count, 0), parents.data_ptr(),
+            start.data_ptr(), tree.data_ptr(), words, positions.data_ptr())
+    return tree, positions
+
+
+def kv_keep(pages: KVPages, table: torch.Tensor, start: torch.Tensor, keep: torch.Tensor, cu: torch.Tensor, max_count: int = None):
+    """Moves accepted tokens up in the cache, on every layer: for the i-th of keep's entries cu[b] .. cu[b + 1] (int32), the token at
+    position start[b] + keep[..] of sequence b goes to position start[b] + i, as if all were read before any is written. Entries
+    have to be at least i (less is taken as i: the token stays); increasing ones are the accepted tokens in order. What lies behind
+    the last of them is no longer the sequence's (shorten its length), and stays as it is. A page that receives tokens keeps its
+    scale, times the smallest power of two with which it covers the tokens kept in it; bytes that stay in a page whose scale stays
+    move as they are. Tokens whose page is not there are not moved. Pages written in one call must be distinct over its sequences."""
+    index = pages.index
+    _need(keep, "keep", index, torch.int32, ("rows",))
+    n = keep.shape[0]
+    if not keep.is_contiguous():
+        raise ValueError("keep must be contiguous")
+    b = _batch(pages, table, cu, start, "start", n, max_count)
+    if n == 0 or b.seqs == 0:
+        return
+    _launch(index, library().wl_kv_keep, pages.ref, b, start.data_ptr(), keep.data_ptr())
 
 
 def _page_numbers(x, name):
@@ -238,6 +320,35 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
     0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2) turn by positions[axis(j)] * inv_freq[j], taken in
     64 bits; cosine and sine are multiplied by `scale`; the rest of each head
     is copied. (engines/base.py:16-89 has the one-axis form.)"""
+    return _rotate(library().wl_rope, q, k, positions, inv_freq, sections, interleaved, scale, out, lambda dim: ())
+
+
+def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_weight: torch.Tensor = None,
+              k_weight: torch.Tensor = None, eps: float = 1e-6, zero_centered: bool = True, sections=None,
+              interleaved: bool = True, scale: float = 1.0, out=None):
+    """rope() on queries and keys that are normed first, each head by itself: x / sqrt(mean(x^2) + eps) * w, in fp32 up to the one
+    rounding of the rotated values. w: 1 + weight with zero_centered (the reference's RMSNorm, engines/base.py:27-31), else weight;
+    q_weight and k_weight [head_dim], both fp32 or both bf16, None: w = 1. The rest as in rope."""
+    weights = [w for w in (q_weight, k_weight) if w is not None]
+    if not 0 <= eps < float("inf"):
+        raise ValueError(f"eps {eps}")
+
+    def norm(dim):
+        kind = torch.float32 if not weights else weights[0].dtype
+        if kind is not torch.float32 and kind is not torch.bfloat16:
+            raise ValueError(f"the weights must be fp32 or bf16 (got {kind})")
+        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+            if w is not None:
+                _need(w, name, q.get_device(), kind, (dim,))
+                if w.shape[0] != dim or not w.is_contiguous():
+                    raise ValueError(f"{name} must be [{dim}], contiguous (got {list(w.shape)})")
+        return (None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+                DTYPE_F32 if kind is torch.float32 else DTYPE_BF16, eps, zero_centered)
+    return _rotate(library().wl_norm_rope, q, k, positions, inv_freq, sections, interleaved, scale, out, norm)
+
+
+def _rotate(call, q, k, positions, inv_freq, sections, interleaved, scale, out, more):
+    """One call of wl_rope or wl_norm_rope; more(head_dim): its arguments behind the scale."""
     dtype, index = q.dtype, q.get_device()
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError(f"q must be bf16 or fp32 (got {dtype})")
@@ -263,6 +374,7 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
         q_out, to = torch.empty_like(q, memory_format=torch.contiguous_format), (heads * dim, dim)
     else:
         to = _rotated_into(q_out, q, index, dim)
+    extra = more(dim)
     q_arg = WlRopeTensor(q.data_ptr(), q_out.data_ptr(), token, head, *to, heads, 0)
     k_arg = None
     if k is not None:
@@ -275,6 +387,6 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
             to = _rotated_into(k_out, k, index, dim)
         k_arg = WlRopeTensor(k.data_ptr(), k_out.data_ptr(), token, head, *to, heads, 0)
     if n:
-        _launch(index, library().wl_rope, q_arg, k_arg, DTYPE_BF16 if dtype is torch.bfloat16 else DTYPE_F32, n, dim, 2 * half,
-                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, _sections(sections), interleaved, scale)
+        _launch(index, call, q_arg, k_arg, DTYPE_BF16 if dtype is torch.bfloat16 else DTYPE_F32, n, dim, 2 * half,
+                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, _sections(sections), interleaved, scale, *extra)
     return q_out, k_out
