@@ -18,6 +18,7 @@ namespace {
 constexpr int kRows = 16;
 constexpr int kFewWaves = 4;
 constexpr int kFewGroups = 512;  // workgroups: two a CU
+constexpr int64_t kBlockTiles = 4096;
 
 // Where the partial results of a (sequence, kv head) lie: slot first, then two slots further for each of the other pieces,
 // from `next` on. pieces is 0 where there are none.
@@ -28,12 +29,13 @@ struct Pieces {
 struct FewArgs : AttendArgs {
     float* partial;      // [2 * workgroups][rows][D]
     float2* partial_ml;  // [2 * workgroups][rows]: maximum (in log2) and sum
-    Pieces* pieces;      // [seqs][kv heads]
-    int32_t rows;        // rows of a (sequence, kv head), at most
+    Pieces* pieces;      // [seqs][kv heads][blocks]
+    int32_t rows;        // rows of a block, at most
+    int32_t blocks;      // of 16 rows, of a (sequence, kv head), at most; 1 without MASK
     int32_t whole, groups;  // how the call is cut: not at all, or over how many workgroups
 };
 
-// One wavefront's share of the rows of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
+// One wavefront's share of a block of rows of (sequence b, kv head): its running maximum, its lanes' sums and O^T.
 // PAGE: a page holds whole tiles (64 tokens or more), so a tile has one page, one address and one pair of scales.
 // MASK: rows see what their window, the sinks and a tree leave them.
 template <int TYPE, int D, bool PAGE, bool MASK>
@@ -45,15 +47,29 @@ struct Rows {
     f32x4 o[kDims];
     float m, l;
     int limit;  // tokens that this lane's row sees; of a masked call its position plus 1
-    uint32_t tree;  // the 16 rows' bits of the tree
+    uint64_t tree;  // this lane's row's bits of a tree of up to 64
 
-    __device__ __forceinline__ void begin(const AttendArgs& a, int head, Seq seq) {
-        const int lane = threadIdx.x & 63, g = lane >> 4, row = lane & 15, token = row / a.group;
+    static __device__ __forceinline__ int token_of(const AttendArgs& a, int row0) {
+        return (row0 + static_cast<int>(threadIdx.x & 15)) / a.group;
+    }
+    // the tree's bits of 16 tokens from `first` on
+    __device__ __forceinline__ uint32_t drafted(const AttendArgs& a, Seq seq, int row0, int first) const {
+        if (seq.n > 64) return tree_bits(a, seq, token_of(a, row0), first);
+        const int off = first - seq.begin;
+        return off >= 64 || off <= -16 ? 0 : static_cast<uint32_t>(off < 0 ? tree << -off : tree >> off);
+    }
+
+    __device__ __forceinline__ void begin(const AttendArgs& a, int head, Seq seq, int row0) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, row = row0 + (lane & 15), token = row / a.group;
         m = -__builtin_inff();
         l = 0.0f;
         if constexpr (MASK) {
             limit = limit_of(a, seq, token);
-            tree = a.mask.tree ? tree_bits(a, seq, token, seq.begin) : 0;
+            tree = 0;
+            if (a.mask.tree && token < seq.n && seq.n <= 64) {
+                tree = *reinterpret_cast<const uint64_t*>(a.mask.tree + (seq.at + token) * a.mask.tree_stride);
+                if (seq.n < 64) tree &= (uint64_t{1} << seq.n) - 1;
+            }
         } else {
             limit = token >= seq.n ? 0 : seq.seen(token, a.causal);
         }
@@ -120,7 +136,7 @@ struct Rows {
         x.more = v;
     }
 
-    __device__ __forceinline__ void add(const AttendArgs& a, Tile& x, int base, Seq seq) {
+    __device__ __forceinline__ void add(const AttendArgs& a, Tile& x, int base, Seq seq, int row0) {
         const int length = seq.length;
         f32x4 s[4];
 #pragma unroll
@@ -144,9 +160,8 @@ struct Rows {
         const int mine = x.page < 0 ? 0 : min(max(limit - first, 0), 16);
         uint32_t bits = 0;
         if constexpr (MASK) {
-            const int off = seq.begin - first;  // where the tree's first token lies
-            const uint32_t drafted = off >= 16 || off <= -16 ? 0 : off < 0 ? tree >> -off : tree << off;
-            bits = x.page < 0 ? 0 : seen_bits(a, seq, limit, first, length - first, drafted);
+            const bool in_tree = a.mask.tree && base + kTile > seq.begin;
+            bits = x.page < 0 ? 0 : seen_bits(a, seq, limit, first, length - first, in_tree ? drafted(a, seq, row0, first) : 0);
         }
         auto counts = [&](int i) { return MASK ? (bits >> i & 1) != 0 : i < mine; };
         float top = m;
@@ -216,13 +231,14 @@ struct Rows {
     }
 
     // Tiles t0 (which has been found), t0 + step, .. below t1, as `span` numbers them.
-    __device__ __forceinline__ void tiles(const AttendArgs& a, int b, int head, Span span, int t0, int t1, int step, Seq seq) {
+    __device__ __forceinline__ void tiles(const AttendArgs& a, int b, int head, Span span, int t0, int t1, int step, Seq seq,
+                                          int row0) {
         for (int t = t0; t < t1; t += step) {
             Tile x;
             const int base = span.tile(t) * kTile;
             load(a, x, head, base);
             if (t + step < t1) find(a, b, span.tile(t + step) * kTile);
-            add(a, x, base, seq);
+            add(a, x, base, seq, row0);
         }
     }
 };
@@ -236,16 +252,16 @@ struct JoinLds {
 // The workgroup's wavefronts over tiles [t0, t1) of the rows; the rows are finished into out, or, with
 // slot >= 0, left as a partial result.
 template <int TYPE, int D, bool PAGE, bool MASK>
-__device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, int b, Seq seq, int head, int t0,
+__device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, int b, Seq seq, int head, int row0, int t0,
                                             int t1, int slot) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, m16 = lane & 15;
     const int at = seq.at, n = seq.n;
-    const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group, static_cast<int64_t>(kRows)));
+    const int rows = static_cast<int>(min(static_cast<int64_t>(n) * a.group - row0, static_cast<int64_t>(kRows)));
     Rows<TYPE, D, PAGE, MASK> r;
     const Span span = MASK ? span_of<MASK>(a, seq, 0, seq.length, kTile) : Span{0, 0, 0};
     if (t0 + wave < t1) r.find(a, b, span.tile(t0 + wave) * kTile);
-    r.begin(a, head, seq);
-    r.tiles(a, b, head, span, t0 + wave, t1, kFewWaves, seq);
+    r.begin(a, head, seq, row0);
+    r.tiles(a, b, head, span, t0 + wave, t1, kFewWaves, seq, row0);
     r.l = sum_over_groups(r.l);
     if (lane < kRows) {
         lds.m[wave][lane] = r.m;
@@ -281,22 +297,21 @@ __device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, i
             if (d == 0) a.partial_ml[slot * a.rows + row] = make_float2(m, l);
         } else {
             const float inv = l == 0.0f ? 0.0f : 1.0f / l;
-            const int token = row / a.group, h = head * a.group + row % a.group;
+            const int token = (row0 + row) / a.group, h = head * a.group + (row0 + row) % a.group;
             *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(at + token) * a.q_heads + h) * D + d) =
                 make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
         }
     }
 }
 
-// Calls of at most 16 rows a sequence are bound by reading the cache, so the cache is what is shared out: the tiles of all
-// sequences and kv heads stand in one line, and every workgroup takes the same number of them in a row, wherever sequences
-// begin and end. A (sequence, head) that lies in one share is finished there; of one that is cut, each share leaves a
+// Calls of few rows a sequence are bound by reading the cache, so the cache is what is shared out: the tiles of all
+// sequences, kv heads and blocks of 16 rows (one, but of a masked call) stand in one line, and every workgroup takes the same number of them in a row, wherever sequences
+// begin and end. A block that lies in one share is finished there; of one that is cut, each share leaves a
 // partial result, which k_attend_join adds up in order. A share has at most two such ends, its first and its last.
 // Where every sequence's last share may stay partly empty without more workgroups than the CUs hold at once, it does
 // (`pad`): a workgroup that holds an end and a beginning runs them one after the other.
 struct Line {
-    uint32_t each, pad;  // tiles of a share; a (sequence, head) takes a multiple of pad tiles of the line
-    uint32_t heads;
+    uint32_t each, pad;  // tiles of a share; a block takes a multiple of pad tiles of the line
 
     __device__ __forceinline__ uint32_t padded(uint32_t tiles) const { return (tiles + pad - 1) / pad * pad; }
 };
@@ -305,45 +320,54 @@ template <bool MASK>
 __device__ __forceinline__ uint32_t tiles_of(const FewArgs& a, Seq s) {
     return s.n == 0 ? 0 : max(span_of<MASK>(a, s, 0, s.length, kTile).tiles, 1);  // without a token there are still rows to write
 }
+// The blocks of a sequence, of all its kv heads
+template <bool MASK>
+__device__ __forceinline__ uint32_t blocks_of(const FewArgs& a, Seq s) {
+    return MASK ? max((s.n * a.group + kRows - 1) / kRows, 1) * a.c.kv_heads : a.c.kv_heads;
+}
 __device__ __forceinline__ Seq seq_or_none(const FewArgs& a, int b) { return b < a.s.seqs ? a.seq(b) : Seq{0, 0, 0, 0}; }
 
-// Every wavefront works the division out for itself; `mine`: tiles of sequence `lane`. Shares and (sequence, head)s are whole
+// Every wavefront works the division out for itself; `mine`: sequence `lane`. Shares and blocks are whole
 // rounds of a workgroup (a tile for each wavefront), so that only the last round of each leaves wavefronts idle.
 template <bool MASK>
-__device__ __forceinline__ Line line_of(const FewArgs& a, uint32_t mine) {
+__device__ __forceinline__ Line line_of(const FewArgs& a, Seq mine) {
     constexpr uint32_t W = kFewWaves;
-    const uint32_t heads = a.c.kv_heads, groups = a.groups;
+    const uint32_t groups = a.groups;
     const int lane = threadIdx.x & 63;
-    uint32_t rounds = (mine + W - 1) / W;
-    for (int b = lane + 64; b < a.s.seqs; b += 64) rounds += (tiles_of<MASK>(a, a.seq(b)) + W - 1) / W;
-    rounds = wave_sum(rounds) * heads;
+    auto rounds_of = [&](Seq s) { return (tiles_of<MASK>(a, s) + W - 1) / W * blocks_of<MASK>(a, s); };
+    uint32_t rounds = rounds_of(mine);
+    for (int b = lane + 64; b < a.s.seqs; b += 64) rounds += rounds_of(a.seq(b));
+    rounds = wave_sum(rounds);
     const uint32_t each = __builtin_amdgcn_readfirstlane(max((rounds + groups - 1) / groups, 1u) * W);
-    uint32_t shares = (mine + each - 1) / each;
-    for (int b = lane + 64; b < a.s.seqs; b += 64) shares += (tiles_of<MASK>(a, a.seq(b)) + each - 1) / each;
-    return {each, wave_sum(shares) * heads <= groups ? each : W, heads};
+    auto shares_of = [&](Seq s) { return (tiles_of<MASK>(a, s) + each - 1) / each * blocks_of<MASK>(a, s); };
+    uint32_t shares = shares_of(mine);
+    for (int b = lane + 64; b < a.s.seqs; b += 64) shares += shares_of(a.seq(b));
+    return {each, wave_sum(shares) <= groups ? each : W};
 }
 
 template <int TYPE, int D, bool PAGE, bool MASK>
 __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
     __shared__ JoinLds<D> lds;
     const int lane = threadIdx.x & 63;
-    Line line = {1, 1, static_cast<uint32_t>(a.c.kv_heads)};
+    Line line = {1, 1};
     uint32_t at, end, before = 0;  // the share, and the line before sequence b
     int b = 0;
     Seq seq;
-    if (a.whole) {  // a workgroup for each (sequence, head)
-        b = blockIdx.x / line.heads;
+    if (a.whole) {  // a workgroup for each block
+        const uint32_t blocks = MASK ? a.blocks * a.c.kv_heads : a.c.kv_heads;
+        b = blockIdx.x / blocks;
         seq = a.seq_uniform(b);
-        const uint32_t tiles = tiles_of<MASK>(a, seq);
-        at = blockIdx.x % line.heads * tiles;
+        const uint32_t tiles = tiles_of<MASK>(a, seq), block = blockIdx.x % blocks;
+        if (MASK && block >= blocks_of<MASK>(a, seq)) return;
+        at = block * tiles;
         end = at + tiles;
     } else {
         Seq mine = seq_or_none(a, lane);
-        line = line_of<MASK>(a, tiles_of<MASK>(a, mine));
+        line = line_of<MASK>(a, mine);
         at = blockIdx.x * line.each;
         end = at + line.each;
         for (;;) {
-            const uint32_t own = line.padded(tiles_of<MASK>(a, mine)) * line.heads, sum = wave_scan(own);
+            const uint32_t own = line.padded(tiles_of<MASK>(a, mine)) * blocks_of<MASK>(a, mine), sum = wave_scan(own);
             const uint64_t past = __ballot(before + sum > at);
             if (past) {
                 const int i = __builtin_amdgcn_readfirstlane(__builtin_ctzll(past));
@@ -365,38 +389,43 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
     while (at < end) {
         const uint32_t tiles = tiles_of<MASK>(a, seq), length = __builtin_amdgcn_readfirstlane(line.padded(tiles));
         if (tiles) {
-            const uint32_t head = __builtin_amdgcn_readfirstlane((at - before) / length), t0 = at - before - head * length;
+            const uint32_t blocks = blocks_of<MASK>(a, seq), block = __builtin_amdgcn_readfirstlane((at - before) / length),
+                           t0 = at - before - block * length;
+            // a head's blocks one after the other: they read the same keys and values
+            const uint32_t each = blocks / a.c.kv_heads, head = MASK ? block / each : block, row0 = MASK ? block % each * kRows : 0;
             const uint32_t t1 = min(t0 + (end - at), length), stop = min(t1, tiles);
             const bool whole = t0 == 0 && stop == tiles;
             if (t0 < stop) {
                 if (slot & 1) __syncthreads();  // the piece before still reads the LDS
-                attend_rows<TYPE, D, PAGE, MASK>(a, lds, b, seq, head, t0, stop, whole ? -1 : slot);
+                attend_rows<TYPE, D, PAGE, MASK>(a, lds, b, seq, head, row0, t0, stop, whole ? -1 : slot);
             }
             if (t0 == 0 && !a.whole && threadIdx.x == 0) {
                 const int rest = whole ? 0 : (tiles - stop + line.each - 1) / line.each;
-                a.pieces[b * line.heads + head] = {rest ? 1 + rest : 0, slot, 2 * (static_cast<int>(blockIdx.x) + 1), 0};
+                a.pieces[(b * a.c.kv_heads + head) * (MASK ? a.blocks : 1) + row0 / kRows] = {rest ? 1 + rest : 0, slot,
+                                                                                              2 * (static_cast<int>(blockIdx.x) + 1), 0};
             }
             slot |= 1;
             at += t1 - t0;
-            if (t1 < length || head < line.heads - 1) continue;
-            before += length * line.heads;
+            if (t1 < length || block < blocks - 1) continue;
+            before += length * blocks;
         }
         if (at >= end || ++b >= a.s.seqs) break;
         seq = a.seq_uniform(b);
     }
 }
 
-// One row of one (sequence, kv head) that was cut: its pieces' results, added up in the order of its tokens over eight
-// wavefronts, then those. blockIdx: (sequence and head, row).
+// One row of one block that was cut: its pieces' results, added up in the order of its tokens over eight
+// wavefronts, then those. blockIdx: (sequence, head and block, row).
 constexpr int kJoinWaves = 8;
 template <int D>
 __global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(FewArgs a) {
     __shared__ float weight[kFewGroups];
     __shared__ float red[2][kJoinWaves];
     __shared__ float o[kJoinWaves][D];
-    const int b = blockIdx.x / a.c.kv_heads, head = blockIdx.x % a.c.kv_heads, row = blockIdx.y;
+    const int unit = blockIdx.x / a.blocks, b = unit / a.c.kv_heads, head = unit % a.c.kv_heads, row = blockIdx.y,
+              row_of_all = blockIdx.x % a.blocks * kRows + row;
     const Seq seq = a.seq(b);
-    if (row >= seq.n * a.group) return;
+    if (row_of_all >= seq.n * a.group) return;
     const Pieces cut = a.pieces[blockIdx.x];
     const int pieces = cut.pieces;
     if (pieces == 0) return;
@@ -442,7 +471,7 @@ __global__ __launch_bounds__(kJoinWaves * 64) void k_attend_join(FewArgs a) {
         sum += red[1][w];
         x += o[w][threadIdx.x];
     }
-    const int token = row / a.group, h = head * a.group + row % a.group;
+    const int token = row_of_all / a.group, h = head * a.group + row_of_all % a.group;
     const float y = sum == 0.0f ? 0.0f : x / sum;
     a.out[(static_cast<int64_t>(seq.at + token) * a.q_heads + h) * D + threadIdx.x] =
         __builtin_bit_cast(uint16_t, static_cast<__bf16>(y));
@@ -454,13 +483,24 @@ struct FewPlan {
     bool whole;
 };
 
-bool is_few(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
-    return static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads) <= kRows;
+// Blocks of 16 rows that a (sequence, kv head) has at most, where the call takes this form; else 0. Without a mask it takes
+// one block. With one, each block converts the cache's bytes for itself, where the form for many rows does that once for 256
+// rows, but starts slower: two blocks are always faster here (trees over 300 to 32000 tokens of 1 to 64 sequences: 1.1 to 2.1
+// times), more of them up to about 4096 tiles over all blocks (up to 2000: 1.1 to 2.4 times, around 4000: 0.8 to 1.7, around
+// 8000: 0.8 to 1.3, from 16000 on mostly below 0.9; heads of 64, 128 and 256).
+int64_t few_blocks(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
+    const int64_t blocks = (static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads) + kRows - 1) / kRows;
+    if (blocks == 1 || !mask) return blocks == 1;
+    const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads * blocks;
+    const int64_t tiles = (longest_span(c, b, max_length, mask, b->max_count, kTile) + kTile - 1) / kTile;
+    if (blocks > 2 && items * tiles > kBlockTiles) return 0;
+    const int64_t line = (int64_t{b->table_width} * c->page_tokens + kTile) / kTile * items;  // counted in 31 bits
+    return line < (int64_t{1} << 31) && fits_a_launch(items, kJoinWaves * 64) ? blocks : 0;
 }
 
-FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
+FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask, int64_t blocks) {
     const int64_t longest = longest_span(c, b, max_length, mask, b->max_count, kTile);
-    const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads;
+    const int64_t items = static_cast<int64_t>(b->seqs) * c->kv_heads * blocks;
     // Two rounds of a workgroup cost less than one and the join: 500 tokens of 1 to 256 sequences on 8 kv heads of 128 9.2 to 45.6
     // against 10.1 to 61.5 us in a graph, on 8 of 64 5.8 to 24.1 against 8.3 to 32.8, of 32 to 256 on 2 of 256 15.3 to 28.0 against
     // 16.1 to 35.0; 300 tokens of 1 to 256 of those 12.6 to 21.5 against 13.2 to 28.5. Only where 256 dimensions, more than about
@@ -472,15 +512,19 @@ FewPlan few_plan(const WlKvCache* c, const WlKvBatch* b, int64_t max_length, con
     return {std::min<int64_t>(kFewGroups, items * each), false};
 }
 
+int32_t block_rows(const WlKvCache* c, int q_heads, const WlKvBatch* b) {
+    return static_cast<int32_t>(std::min<int64_t>(static_cast<int64_t>(b->max_count) * (q_heads / c->kv_heads), kRows));
+}
+
 // The workspace of a call of few rows: two slots of partial results a workgroup, then where they are.
 struct FewSpace {
     size_t ml, pieces, bytes;  // offsets, total
 };
-FewSpace few_space(const WlKvCache* c, int q_heads, const WlKvBatch* b, const FewPlan& p) {
+FewSpace few_space(const WlKvCache* c, int64_t rows_of_block, const WlKvBatch* b, const FewPlan& p, int64_t blocks) {
     if (p.whole) return {0, 0, 0};
-    const size_t rows = static_cast<size_t>(2 * p.groups) * b->max_count * (q_heads / c->kv_heads);
+    const size_t rows = static_cast<size_t>(2 * p.groups * rows_of_block);
     const size_t ml = rows * c->head_dim * sizeof(float), pieces = ml + rows * sizeof(float2);
-    return {ml, (pieces + 15) / 16 * 16, (pieces + 15) / 16 * 16 + static_cast<size_t>(b->seqs) * c->kv_heads * sizeof(Pieces)};
+    return {ml, (pieces + 15) / 16 * 16, (pieces + 15) / 16 * 16 + static_cast<size_t>(b->seqs) * c->kv_heads * blocks * sizeof(Pieces)};
 }
 
 int check_attend(const WlKvCache* cache, int q_heads, const WlKvBatch* batch, int64_t max_length) {
@@ -545,8 +589,8 @@ int attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token
     if (qb % 2 || reinterpret_cast<uintptr_t>(out) % 16 || reinterpret_cast<uintptr_t>(length) % 4) return WL_EINVAL_ALIGN;
     const size_t need = wl_kv_attend_masked_workspace_bytes(cache, q_heads, batch, max_length, mask);
     if (need && (!workspace || workspace_bytes < need || reinterpret_cast<uintptr_t>(workspace) % 16)) return WL_EINVAL_WORKSPACE;
-    const bool few = is_few(cache, q_heads, batch);
-    if (!few && !attend_rows_fit(cache, q_heads, batch, max_length, mask)) return WL_EINVAL_SHAPE;
+    const int64_t blocks = few_blocks(cache, q_heads, batch, max_length, mask);
+    if (!blocks && !attend_rows_fit(cache, q_heads, batch, max_length, mask)) return WL_EINVAL_SHAPE;
     if (out_meets_q(out, q, q_token_stride, q_head_stride, batch->tokens, q_heads, cache->head_dim)) return WL_EINVAL_OVERLAP;
     FewArgs a = {};
     a.c = layer_of(cache, layer);
@@ -563,13 +607,14 @@ int attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token
     if (mask) a.mask = device_mask(mask);
     a.wide_q = qb % 16 == 0 && q_token_stride % 8 == 0 && q_head_stride % 8 == 0;
     const hipStream_t st = static_cast<hipStream_t>(stream);
-    if (!few) return launch_attend_rows(cache, a, batch, max_length, mask, workspace, st);
-    const FewPlan plan = few_plan(cache, batch, max_length, mask);
-    const FewSpace space = few_space(cache, q_heads, batch, plan);
+    if (!blocks) return launch_attend_rows(cache, a, batch, max_length, mask, workspace, st);
+    const FewPlan plan = few_plan(cache, batch, max_length, mask, blocks);
+    a.rows = block_rows(cache, q_heads, batch);
+    a.blocks = static_cast<int32_t>(blocks);
+    const FewSpace space = few_space(cache, a.rows, batch, plan, blocks);
     a.partial = static_cast<float*>(workspace);
     a.partial_ml = reinterpret_cast<float2*>(static_cast<char*>(workspace) + space.ml);
     a.pieces = reinterpret_cast<Pieces*>(static_cast<char*>(workspace) + space.pieces);
-    a.rows = batch->max_count * a.group;
     a.whole = plan.whole;
     a.groups = static_cast<int32_t>(std::min<int64_t>(plan.groups, kFewGroups));
     auto run = [&](auto type, auto dim, auto page) {
@@ -582,7 +627,7 @@ int attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token
             k_attend_few<T, D, P, false><<<groups, kFewWaves * 64, 0, st>>>(a);
         if (const int rc = launch_status()) return rc;
         if (!plan.whole)
-            k_attend_join<D><<<dim3(batch->seqs * cache->kv_heads, a.rows), kJoinWaves * 64, 0, st>>>(a);
+            k_attend_join<D><<<dim3(static_cast<uint32_t>(batch->seqs * cache->kv_heads * blocks), a.rows), kJoinWaves * 64, 0, st>>>(a);
         return launch_status();
     };
     auto with_page = [&](auto type, auto dim) {
@@ -612,8 +657,9 @@ size_t wl_kv_attend_masked_workspace_bytes(const WlKvCache* cache, int q_heads, 
                                            const WlKvMask* mask) {
     if (check_attend(cache, q_heads, batch, max_length) || check_mask(mask, batch)) return 0;
     if (hides_nothing(mask)) mask = nullptr;
-    if (!is_few(cache, q_heads, batch)) return attend_rows_workspace(cache, q_heads, batch, max_length, mask);
-    return few_space(cache, q_heads, batch, few_plan(cache, batch, max_length, mask)).bytes;
+    const int64_t blocks = few_blocks(cache, q_heads, batch, max_length, mask);
+    if (!blocks) return attend_rows_workspace(cache, q_heads, batch, max_length, mask);
+    return few_space(cache, block_rows(cache, q_heads, batch), batch, few_plan(cache, batch, max_length, mask, blocks), blocks).bytes;
 }
 
 int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q_token_stride, int64_t q_head_stride,

@@ -32,6 +32,7 @@ constexpr int kThreads = kWaves * 64;
 constexpr int kGroupRows = kWaves * 32;
 constexpr int kRing = 4;  // tiles in LDS: two are multiplied between barriers, two are filled
 constexpr int kMaxPieces = 16;
+constexpr int kMaxMaskedPieces = 64;  // of a masked call: a tree's few rows may stand behind a long cache
 constexpr int kCus = 256;
 constexpr int64_t kPartialBytes = 256 << 20;  // for partial results, at most
 constexpr float kSlack = 8.0f;  // log2: how far a score may lie above the running maximum
@@ -283,7 +284,8 @@ struct Work {
     int b, row0, piece, pieces, t0, t1;
 };
 constexpr int kClasses = 64;
-constexpr int kLeast = 4;  // tiles that are worth a piece
+template <bool MASK>
+constexpr int kLeast = MASK ? 2 : 4;  // tiles that are worth a piece
 struct PlanLds {
     uint32_t classes[kClasses];
     uint32_t sums[kWaves];
@@ -324,7 +326,7 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
     __syncthreads();
     total = 0;
     for (int i = 0; i < kWaves; i++) total += lds.sums[i];
-    int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast);
+    int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast<MASK>);
     if (a.pieces > 1 && !a.few_tiles) {
         each += each / 2;  // more than a CU's share alone, see rows_plan
     } else if (a.pieces > 1) {
@@ -428,7 +430,14 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     auto base_of = [&](int t) { return span.tile(t) * S::kTokens; };
     // the tokens between the sinks and the first row's window, of the workgroup's rows (counted from the sequence's end) and of the wavefront's
     const int hidden_from = MASK ? a.mask.sinks - seq.length : 0, hidden_to = MASK ? window_begin(a, seq, row0 / a.group) - seq.length : 0;
+    // tokens that some row of the wavefront sees begin there; that every row sees (in front of a tree), from whole_from to whole_to
     const int window_at = MASK ? window_begin(a, seq, __builtin_amdgcn_readfirstlane(token)) : 0;
+    int whole_from = 0, whole_to = 0;
+    if constexpr (MASK) {
+        const int last = min((row0 + 32 * __builtin_amdgcn_readfirstlane(wave) + 31) / a.group, seq.n - 1);
+        whole_from = max(max(seq.begin + (a.mask.tree ? seq.n : last + 1), 0) - a.mask.window, 0);
+        whole_to = a.mask.tree ? seq.begin : __builtin_amdgcn_readfirstlane(limit);
+    }
 
     Stage<TYPE, D, PAGE, MASK> st;
     st.find(a, b, base_of(cut.t0));
@@ -471,12 +480,16 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
             const int at = base + 32 * u + 16 * half;
             if constexpr (MASK) {
                 if (base + 32 * u + 32 <= window_at && base + 32 * u >= a.mask.sinks) continue;
-                uint32_t drafted = 0;
-                if (a.mask.tree && base + 32 * u + 32 > seq.begin) {  // a few tiles: the row is worked out again, as below
-                    const int r = row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero());
-                    drafted = tree_bits(a, seq, r / a.group, at);
+                int seen = 0xFFFF;
+                if (base + 32 * u < whole_from || base + 32 * u + 32 > whole_to) {
+                    uint32_t drafted = 0;
+                    if (a.mask.tree && base + 32 * u + 32 > seq.begin) {  // a few tiles: the row is worked out again, as below
+                        const int r = row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero());
+                        drafted = tree_bits(a, seq, r / a.group, at);
+                    }
+                    seen = seen_bits(a, seq, limit, at, 16, drafted);
                 }
-                w.template add<MASK>(lds, buffer, u, seen_bits(a, seq, limit, at, 16, drafted));
+                w.template add<MASK>(lds, buffer, u, seen);
             } else {
                 w.template add<MASK>(lds, buffer, u, limit - at);
             }
@@ -574,6 +587,50 @@ __global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge(RowsArgs a) {
     }
 }
 
+// The same for more than kMaxPieces of them, which few rows have: a workgroup a row, its pieces in turn over the wavefronts.
+// blockIdx: (row, kv head), sequence.
+template <int D>
+__global__ __launch_bounds__(kMergeWaves * 64) void k_attend_merge_row(RowsArgs a) {
+    __shared__ float part[kMergeWaves][D];
+    const int b = blockIdx.y, head = blockIdx.x % a.c.kv_heads, row = blockIdx.x / a.c.kv_heads, wave = threadIdx.x >> 6,
+              lane = threadIdx.x & 63;
+    const Seq seq = a.seq_uniform(b);
+    if (row >= seq.n * a.group) return;
+    const int pieces = cut_of(tiles_of<true>(a, seq, row / kGroupRows * kGroupRows, Shape<D>::kTokens), *a.each, a.pieces).pieces;
+    if (pieces < 2) return;
+    constexpr int V = D / 64;
+    typedef float Lane __attribute__((ext_vector_type(V)));
+    const int64_t stride = static_cast<int64_t>(a.s.tokens) * a.q_heads;
+    const int64_t place = static_cast<int64_t>(seq.at + row / a.group) * a.q_heads + head * a.group + row % a.group;
+    auto values = [&](int i) { return *reinterpret_cast<const Lane*>(a.partial + (i * stride + place) * D + lane * V); };
+    constexpr int kMost = kMaxMaskedPieces / kMergeWaves;
+    Lane x[kMost];
+#pragma unroll
+    for (int i = 0; i < kMost; i++) x[i] = values(min(wave + kMergeWaves * i, pieces - 1));
+    const float2 ml = lane < pieces ? a.partial_ml[lane * stride + place] : make_float2(-__builtin_inff(), 0.0f);
+    float top = ml.x;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) top = fmaxf(top, __shfl_xor(top, d));
+    const float own = exp2_fast(ml.x - (top == -__builtin_inff() ? 0.0f : top));  // 0 behind the last piece
+    float l = ml.y * own;
+#pragma unroll
+    for (int d = 32; d; d >>= 1) l += __shfl_xor(l, d);
+    Lane sum = {};
+#pragma unroll
+    for (int i = 0; i < kMost; i++) {
+        const int piece = wave + kMergeWaves * i;
+        if (piece < pieces) sum += x[i] * __shfl(own, piece);
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) part[wave][lane * V + e] = sum[e];
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    float y = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kMergeWaves; w++) y += part[w][threadIdx.x];
+    a.out[place * D + threadIdx.x] = __builtin_bit_cast(uint16_t, static_cast<__bf16>(l == 0.0f ? 0.0f : y / l));
+}
+
 // How the row tiles' caches are cut. Calls of few row tiles would leave CUs idle, and a causal prompt's last row tiles would
 // run on alone: a cache is cut into pieces of a CU's share of the whole where that is less. From twice as many row tiles as
 // CUs on, taking the large ones first is enough while none is more than a CU's share: so for the rows of one sequence, which see
@@ -598,7 +655,8 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
     const bool few_tiles = items < 2 * kCus;
     if (!few_tiles && (b->seqs == 1 || most < kLong || room < 4)) return {row_tiles, 1, items, false};
-    const int64_t pieces = std::max<int64_t>(1, std::min({int64_t{kMaxPieces}, (most + kLeast - 1) / kLeast, room}));
+    const int64_t least = mask ? kLeast<true> : kLeast<false>, limit = mask && items < kCus / kMaxPieces ? kMaxMaskedPieces : kMaxPieces;
+    const int64_t pieces = std::max<int64_t>(1, std::min({limit, (most + least - 1) / least, room}));
     // the pieces of n tiles are less than n / each + 1, those of all (row tile, kv head)s less than kCus + items
     return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus), few_tiles};
 }
@@ -618,7 +676,8 @@ static int64_t merge_groups(const WlKvCache* c, int64_t group, const WlKvBatch* 
 bool attend_rows_fit(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask) {
     const RowsPlan p = rows_plan(c, q_heads, b, max_length, mask);
     return p.row_tiles * b->seqs < (int64_t{1} << 31) && fits_a_launch(p.groups, kThreads) &&
-           fits_a_launch(merge_groups(c, q_heads / c->kv_heads, b), kMergeWaves * 64);
+           fits_a_launch(p.pieces > kMaxPieces ? int64_t{b->max_count} * q_heads : merge_groups(c, q_heads / c->kv_heads, b),
+                         kMergeWaves * 64);
 }
 
 int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBatch* b, int64_t max_length, const WlKvMask* mask,
@@ -642,6 +701,13 @@ int launch_attend_rows(const WlKvCache* c, const AttendArgs& call, const WlKvBat
         else
             k_attend_rows<T, D, false, MASK><<<grid, kThreads, 0, stream>>>(a);
         if (const int rc = launch_status()) return rc;
+        if constexpr (MASK) {
+            if (p.pieces > kMaxPieces) {
+                k_attend_merge_row<D><<<dim3(static_cast<uint32_t>(b->max_count * call.group * c->kv_heads), b->seqs), kMergeWaves * 64, 0,
+                                        stream>>>(a);
+                return launch_status();
+            }
+        }
         if (p.pieces > 1) k_attend_merge<D, MASK><<<merge, kMergeWaves * 64, 0, stream>>>(a);
         return launch_status();
     };

@@ -56,19 +56,26 @@ __global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_
 }
 
 constexpr int kKeepThreads = 256;
+constexpr int kKeepChunk = 32;  // tokens that the threads hold at a time
 
 // One workgroup takes one kv head's K or V of a sequence on one layer, and goes through the pages that receive tokens from the
 // first to the last. A token only ever moves towards the front, so what a page receives still stands where it stood when the
-// page's turn comes; within a page, tokens are read before a barrier and written behind it, as many at a time as there are threads.
-// Of each page first the largest value, which says whether its scale holds them.
+// page's turn comes; within a page, a chunk of tokens is read before a barrier and written behind it. Of each page first the
+// largest value, which says whether its scale holds them. K: a thread holds 16 values of a token; V, whose tokens lie innermost: a
+// dimension of some of the chunk's tokens, byte by byte.
+// Bound by latency: where each token comes from (offset, row number, page, scale: a chain of four loads) is looked up once for a
+// chunk, by as many threads as it has tokens, and the bytes of a chunk are asked for at once and kept, so that a page of up to 32
+// tokens is read once.
 template <int TYPE, int D>
 __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t layer_bytes, int64_t layer_blocks, KvSeqs s,
                                                           const int32_t* __restrict__ start, const int32_t* __restrict__ keep) {
     __shared__ uint32_t tops[kKeepThreads / 64];
+    __shared__ const uint8_t* source[kKeepChunk];  // null: not moved
+    __shared__ float source_scale[kKeepChunk];
     const int b = blockIdx.z, head = blockIdx.x >> 1;
     const bool is_v = blockIdx.x & 1;
-    const int at = s.first(b), n = s.count(b, at);
     const int64_t from = max(start[b], 0);
+    const int at = s.first(b), n = s.count(b, at);
     const int P = c.page_tokens;
     uint8_t* data = (is_v ? c.v : c.k) + blockIdx.y * layer_bytes;
     float* scales = (is_v ? c.v_scale : c.k_scale) + blockIdx.y * layer_blocks;
@@ -76,13 +83,12 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         const int64_t col = pos >> c.page_shift;
         return col < s.table_width ? s.page(b, static_cast<int>(col), c.pages) : -1;
     };
-    // a value's place: block, token in the page, dimension
-    auto byte_at = [&](int64_t block, int t, int d) { return data + block * P * D + (is_v ? d * P + t : t * D + d); };
-    struct Unit {
-        uint32_t byte;
-        float scale;
-        int token;  // in the target page; below 0: none
-    };
+    auto token_at = [&](int64_t block, int t) { return data + block * P * D + (is_v ? t : t * D); };
+    // thread's unit of a chunk. K: run r is values 16 k_part .. of token k_token + r * kTokens; V: dimension v_dim of the kPer tokens
+    // from v_token on
+    constexpr int kTokens = kKeepThreads / (D / 16), kRuns = (kKeepChunk + kTokens - 1) / kTokens;
+    constexpr int kPer = kKeepChunk * D / kKeepThreads;
+    const int k_part = threadIdx.x % (D / 16), k_token = threadIdx.x / (D / 16), v_dim = threadIdx.x % D, v_token = threadIdx.x / D * kPer;
     for (int64_t col = from >> c.page_shift; n > 0 && col <= (from + n - 1) >> c.page_shift; col++) {
         const int64_t page0 = col * P;
         const int page = page_at(page0);
@@ -91,44 +97,104 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         const int e0 = static_cast<int>(max(page0 - from, int64_t{0})), e1 = static_cast<int>(min(page0 + P - from, static_cast<int64_t>(n)));
         const int64_t block = c.block(page, head);
         const float old = scales[block];
-        const int units = (e1 - e0) * D;
-        auto read = [&](int u) -> Unit {  // u: token, then dimension
-            if (u >= units) return {0, 0.0f, -1};
-            const int e = e0 + u / D;
-            const int64_t source = from + max(keep[at + e], e);
-            const int spage = page_at(source);
-            if (spage < 0) return {0, 0.0f, -1};
-            const int64_t sblock = c.block(spage, head);
-            return {*byte_at(sblock, static_cast<int>(source & (P - 1)), u % D), spage == page ? old : scales[sblock],
-                    static_cast<int>(from + e - page0)};
+        uint4 k[kRuns];
+        uint32_t v[kPer];
+        // tokens [e, e + 32) of the sequence's rows, as they stand
+        auto read = [&](int e) {
+            __syncthreads();  // the chunk before has been worked on
+            if (threadIdx.x < kKeepChunk) {
+                const int i = e + threadIdx.x;
+                const uint8_t* p = nullptr;
+                if (i < e1) {
+                    const int64_t pos = from + max(keep[at + i], i);
+                    const int spage = page_at(pos);
+                    if (spage >= 0) {
+                        const int64_t sblock = c.block(spage, head);
+                        p = token_at(sblock, static_cast<int>(pos & (P - 1)));
+                        source_scale[threadIdx.x] = spage == page ? old : scales[sblock];
+                    }
+                }
+                source[threadIdx.x] = p;
+            }
+            __syncthreads();
+            if (!is_v) {
+#pragma unroll
+                for (int r = 0; r < kRuns; r++) {
+                    const uint8_t* p = k_token + r * kTokens < kKeepChunk ? source[k_token + r * kTokens] : nullptr;
+                    if (p) k[r] = *reinterpret_cast<const uint4*>(p + 16 * k_part);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < kPer; r++) {
+                    const uint8_t* p = source[v_token + r];
+                    if (p) v[r] = p[v_dim * P];
+                }
+            }
         };
         uint32_t top = 0;  // magnitudes order as their bits do; infinities and NaN come out largest
-        for (int u = threadIdx.x; u < units; u += kKeepThreads) {
-            const Unit x = read(u);
-            if (x.token >= 0) top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(x.byte) * x.scale) & 0x7FFFFFFFu);
+        auto measure = [&](uint32_t byte, float scale) {
+            top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(byte & 0xFFu) * scale) & 0x7FFFFFFFu);
+        };
+        for (int e = e0; e < e1; e += kKeepChunk) {
+            read(e);
+            if (!is_v) {
+#pragma unroll
+                for (int r = 0; r < kRuns; r++) {
+                    const int i = k_token + r * kTokens;
+                    if (i >= kKeepChunk || !source[i]) continue;
+                    const uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
+#pragma unroll
+                    for (int j = 0; j < 16; j++) measure(w[j / 4] >> (8 * (j % 4)), source_scale[i]);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < kPer; r++)
+                    if (source[v_token + r]) measure(v[r], source_scale[v_token + r]);
+            }
         }
 #pragma unroll
         for (int d = 32; d; d >>= 1) top = max(top, __shfl_xor(top, d));
         if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
-        __syncthreads();
+        __syncthreads();  // all of a page of one chunk has been read, and every thread has the old scale
         top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
         int shrink = 0;
         const float now = top < 0x7F800000u ? block_scale<TYPE>(__builtin_bit_cast(float, top), true, old, shrink) : __builtin_nanf("");
-        const float by = now > 0.0f ? now : 1.0f;
+        const bool dead = !(now > 0.0f);  // zeros, or a NaN scale
+        auto moved = [&](uint32_t byte, float scale) {
+            return dead ? 0u : to_byte<TYPE>(from_byte<TYPE>(byte & 0xFFu) * scale / now);
+        };
+        auto older = [&](uint32_t byte) { return to_byte<TYPE>(ldexpf(from_byte<TYPE>(byte & 0xFFu), -shrink)); };
         if (shrink)
             for (int u = threadIdx.x; u < held * D; u += kKeepThreads) {
-                uint8_t* p = byte_at(block, u / D, u % D);
-                *p = static_cast<uint8_t>(to_byte<TYPE>(ldexpf(from_byte<TYPE>(*p), -shrink)));
+                uint8_t* p = token_at(block, u / D) + (is_v ? u % D * P : u % D);
+                *p = static_cast<uint8_t>(older(*p));
             }
-        for (int u0 = 0; u0 < units; u0 += kKeepThreads) {
-            const Unit x = read(u0 + threadIdx.x);
-            __syncthreads();  // all has been read, the scale too
-            if (x.token >= 0)
-                *byte_at(block, x.token, (u0 + threadIdx.x) % D) =
-                    static_cast<uint8_t>(now > 0.0f ? to_byte<TYPE>(from_byte<TYPE>(x.byte) * x.scale / by) : 0);
+        for (int e = e0; e < e1; e += kKeepChunk) {
+            if (e1 - e0 > kKeepChunk) {
+                read(e);
+                __syncthreads();
+            }
+            const int t = static_cast<int>(from + e - page0);  // the chunk's place in the page
+            if (!is_v) {
+#pragma unroll
+                for (int r = 0; r < kRuns; r++) {
+                    const int i = k_token + r * kTokens;
+                    if (i >= kKeepChunk || !source[i]) continue;
+                    const float scale = source_scale[i];
+                    uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        w[j] = moved(w[j], scale) | moved(w[j] >> 8, scale) << 8 | moved(w[j] >> 16, scale) << 16 | moved(w[j] >> 24, scale) << 24;
+                    *reinterpret_cast<uint4*>(token_at(block, t + i) + 16 * k_part) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
+            } else {
+#pragma unroll
+                for (int r = 0; r < kPer; r++)
+                    if (source[v_token + r])
+                        token_at(block, t + v_token + r)[v_dim * P] = static_cast<uint8_t>(moved(v[r], source_scale[v_token + r]));
+            }
         }
         if (threadIdx.x == 0) scales[block] = now;
-        __syncthreads();  // the next page's sums, and its reading of what was not moved
     }
 }
 

@@ -140,7 +140,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
     struct alignas(sizeof(T) * VEC) Run {
         T v[VEC];
     };
-    constexpr int kRows = kRopeThreads / 32;
+    constexpr int kRows = kRopeThreads / 32, kEarly = 3;
     const int token = blockIdx.x, lane = threadIdx.x % 32;
     const int pairs = a.half / VEC, units = pairs + (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
     struct Head {
@@ -192,8 +192,13 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
         *reinterpret_cast<Run*>(x.out + at) = lo;
         if (u < pairs) *reinterpret_cast<Run*>(x.out + a.half + at) = hi;
     };
-    Run lo = {}, hi = {};
-    if (static_cast<int>(threadIdx.x) / 32 < heads && lane < units) load(head_at(threadIdx.x / 32), lane, lo, hi);
+    Run lo[kEarly], hi[kEarly];
+#pragma unroll
+    for (int r = 0; r < kEarly; r++) {
+        const int i = threadIdx.x / 32 + r * kRows;
+        lo[r] = hi[r] = {};
+        if (i < heads && lane < units) load(head_at(i), lane, lo[r], hi[r]);
+    }
     for (int j = threadIdx.x; j < 2 * a.head_dim; j += kRopeThreads) {
         const bool is_k = j >= a.head_dim;
         const void* w = is_k ? n.k_weight : n.q_weight;
@@ -202,10 +207,9 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
     }
     for (int j = threadIdx.x; j < a.half; j += kRopeThreads) turn[j] = turn_of(a, j, token);
     __syncthreads();
-    for (int i = threadIdx.x / 32; i < heads; i += kRows) {
+    auto whole = [&](int i, const Run& first, const Run& second) {  // the head, of which the lanes hold 32 units
         const Head x = head_at(i);
-        if (i >= kRows && lane < units) load(x, lane, lo, hi);
-        float sum = lane < units ? squares(lane, lo, hi) : 0.0f;
+        float sum = lane < units ? squares(lane, first, second) : 0.0f;
         for (int u = lane + 32; u < units; u += 32) {
             Run y, z = {};
             load(x, u, y, z);
@@ -214,12 +218,22 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
 #pragma unroll
         for (int d = 16; d; d >>= 1) sum += __shfl_xor(sum, d);
         const float inv = 1.0f / sqrtf(sum / a.head_dim + n.eps);
-        if (lane < units) finish(x, lane, lo, hi, inv);
+        if (lane < units) finish(x, lane, first, second, inv);
         for (int u = lane + 32; u < units; u += 32) {
             Run y, z = {};
             load(x, u, y, z);
             finish(x, u, y, z, inv);
         }
+    };
+#pragma unroll
+    for (int r = 0; r < kEarly; r++) {
+        const int i = threadIdx.x / 32 + r * kRows;
+        if (i < heads) whole(i, lo[r], hi[r]);
+    }
+    for (int i = threadIdx.x / 32 + kEarly * kRows; i < heads; i += kRows) {
+        Run y = {}, z = {};
+        if (lane < units) load(head_at(i), lane, y, z);
+        whole(i, y, z);
     }
 }
 
