@@ -56,22 +56,32 @@ __global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_
 }
 
 constexpr int kKeepThreads = 256;
-constexpr int kKeepChunk = 32;  // tokens that the threads hold at a time
+constexpr int kKeepChunk = 32;  // tokens that the threads hold at a time, at most
+constexpr int kKeepGroups = 4;  // of V also not more than come from so many groups of 16 tokens
 
 // One workgroup takes one kv head's K or V of a sequence on one layer, and goes through the pages that receive tokens from the
 // first to the last. A token only ever moves towards the front, so what a page receives still stands where it stood when the
 // page's turn comes; within a page, a chunk of tokens is read before a barrier and written behind it. Of each page first the
-// largest value, which says whether its scale holds them. K: a thread holds 16 values of a token; V, whose tokens lie innermost: a
-// dimension of some of the chunk's tokens, byte by byte.
-// Bound by latency: where each token comes from (offset, row number, page, scale: a chain of four loads) is looked up once for a
-// chunk, by as many threads as it has tokens, and the bytes of a chunk are asked for at once and kept, so that a page of up to 32
-// tokens is read once.
+// largest value, which says whether its scale holds them.
+// K: a thread holds 16 values of a token. V lies with the tokens innermost: the groups of 16 tokens that the chunk's tokens come
+// from are read as they lie, 16 bytes a thread, and put into LDS, where a dimension's bytes stand together; a thread picks from
+// there what its dimension's next 16 tokens are, and writes them with the bytes around them (moving byte by byte, every line would
+// be asked for once a token, on both sides).
+// Bound by latency: a token's source (offset, row number, page, scale: a chain of four loads) is looked up once a chunk, by as many
+// threads as it has tokens, and a page of one chunk is read once.
 template <int TYPE, int D>
 __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t layer_bytes, int64_t layer_blocks, KvSeqs s,
                                                           const int32_t* __restrict__ start, const int32_t* __restrict__ keep) {
+    struct Entry {
+        const uint8_t* from;  // the token's first byte; null: not moved
+        float scale;
+        int32_t place;  // of V: in its row of `rows`
+    };
+    __shared__ Entry entries[kKeepChunk];
+    __shared__ const uint8_t* groups[kKeepGroups];
+    __shared__ int32_t chunk;  // how many entries it has
     __shared__ uint32_t tops[kKeepThreads / 64];
-    __shared__ const uint8_t* source[kKeepChunk];  // null: not moved
-    __shared__ float source_scale[kKeepChunk];
+    __shared__ uint32_t rows[D][4 * kKeepGroups + 1];  // a word more: dimensions on different banks
     const int b = blockIdx.z, head = blockIdx.x >> 1;
     const bool is_v = blockIdx.x & 1;
     const int64_t from = max(start[b], 0);
@@ -84,11 +94,10 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         return col < s.table_width ? s.page(b, static_cast<int>(col), c.pages) : -1;
     };
     auto token_at = [&](int64_t block, int t) { return data + block * P * D + (is_v ? t : t * D); };
-    // thread's unit of a chunk. K: run r is values 16 k_part .. of token k_token + r * kTokens; V: dimension v_dim of the kPer tokens
-    // from v_token on
+    // a thread's share of a chunk. K: values 16 k_part .. of tokens k_token + r * kTokens; V: dimension d, every kParts-th 16 tokens
     constexpr int kTokens = kKeepThreads / (D / 16), kRuns = (kKeepChunk + kTokens - 1) / kTokens;
-    constexpr int kPer = kKeepChunk * D / kKeepThreads;
-    const int k_part = threadIdx.x % (D / 16), k_token = threadIdx.x / (D / 16), v_dim = threadIdx.x % D, v_token = threadIdx.x / D * kPer;
+    constexpr int kParts = kKeepThreads / D, kTargets = (kKeepChunk / 16 + 1 + kParts - 1) / kParts;
+    const int k_part = threadIdx.x % (D / 16), k_token = threadIdx.x / (D / 16), d = threadIdx.x % D, part = threadIdx.x / D;
     for (int64_t col = from >> c.page_shift; n > 0 && col <= (from + n - 1) >> c.page_shift; col++) {
         const int64_t page0 = col * P;
         const int page = page_at(page0);
@@ -97,81 +106,120 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         const int e0 = static_cast<int>(max(page0 - from, int64_t{0})), e1 = static_cast<int>(min(page0 + P - from, static_cast<int64_t>(n)));
         const int64_t block = c.block(page, head);
         const float old = scales[block];
-        uint4 k[kRuns];
-        uint32_t v[kPer];
-        // tokens [e, e + 32) of the sequence's rows, as they stand
+        uint4 k[kRuns], before[kTargets];
+        // the tokens from row e on, as they stand -> how many
         auto read = [&](int e) {
-            __syncthreads();  // the chunk before has been worked on
-            if (threadIdx.x < kKeepChunk) {
+            __syncthreads();  // the chunk before has been worked on, and written
+            if (threadIdx.x < 64) {
                 const int i = e + threadIdx.x;
-                const uint8_t* p = nullptr;
-                if (i < e1) {
+                const bool some = threadIdx.x < kKeepChunk && i < e1;
+                Entry x = {nullptr, 0.0f, 0};
+                if (some) {
                     const int64_t pos = from + max(keep[at + i], i);
-                    const int spage = page_at(pos);
+                    const int spage = page_at(pos), t = static_cast<int>(pos & (P - 1));
                     if (spage >= 0) {
                         const int64_t sblock = c.block(spage, head);
-                        p = token_at(sblock, static_cast<int>(pos & (P - 1)));
-                        source_scale[threadIdx.x] = spage == page ? old : scales[sblock];
+                        x = {token_at(sblock, t), spage == page ? old : scales[sblock], t & 15};
                     }
                 }
-                source[threadIdx.x] = p;
+                // V: tokens of one group of 16 as the one before follow it in its place
+                const uint64_t group = reinterpret_cast<uint64_t>(x.from - x.place);
+                const uint32_t lo = __shfl_up(static_cast<uint32_t>(group), 1), hi = __shfl_up(static_cast<uint32_t>(group >> 32), 1);
+                const bool first = threadIdx.x == 0 || (static_cast<uint64_t>(hi) << 32 | lo) != group;
+                const uint64_t firsts = __ballot(first);
+                const int number = __popcll(firsts & ((uint64_t{2} << threadIdx.x) - 1)) - 1;
+                const int count = __popcll(__ballot(some && (!is_v || number < kKeepGroups)));
+                if (threadIdx.x == 0) {
+                    chunk = count;
+                    for (int g = 0; g < kKeepGroups; g++) groups[g] = nullptr;
+                }
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wavefront's writes to LDS are in order
+                if (x.from && first && number < kKeepGroups) groups[number] = x.from - x.place;
+                x.place += 16 * number;
+                if (threadIdx.x < kKeepChunk) entries[threadIdx.x] = x;
             }
             __syncthreads();
-            if (!is_v) {
-#pragma unroll
-                for (int r = 0; r < kRuns; r++) {
-                    const uint8_t* p = k_token + r * kTokens < kKeepChunk ? source[k_token + r * kTokens] : nullptr;
-                    if (p) k[r] = *reinterpret_cast<const uint4*>(p + 16 * k_part);
-                }
-            } else {
-#pragma unroll
-                for (int r = 0; r < kPer; r++) {
-                    const uint8_t* p = source[v_token + r];
-                    if (p) v[r] = p[v_dim * P];
-                }
-            }
-        };
-        uint32_t top = 0;  // magnitudes order as their bits do; infinities and NaN come out largest
-        auto measure = [&](uint32_t byte, float scale) {
-            top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(byte & 0xFFu) * scale) & 0x7FFFFFFFu);
-        };
-        for (int e = e0; e < e1; e += kKeepChunk) {
-            read(e);
+            const int count = chunk;
             if (!is_v) {
 #pragma unroll
                 for (int r = 0; r < kRuns; r++) {
                     const int i = k_token + r * kTokens;
-                    if (i >= kKeepChunk || !source[i]) continue;
-                    const uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
-#pragma unroll
-                    for (int j = 0; j < 16; j++) measure(w[j / 4] >> (8 * (j % 4)), source_scale[i]);
+                    const uint8_t* p = i < count ? entries[i].from : nullptr;
+                    k[r] = p ? *reinterpret_cast<const uint4*>(p + 16 * k_part) : make_uint4(0, 0, 0, 0);
                 }
             } else {
+                uint4 w[D * kKeepGroups / kKeepThreads];
 #pragma unroll
-                for (int r = 0; r < kPer; r++)
-                    if (source[v_token + r]) measure(v[r], source_scale[v_token + r]);
+                for (int r = 0; r < D * kKeepGroups / kKeepThreads; r++) {
+                    const int u = threadIdx.x + r * kKeepThreads, g = u % kKeepGroups;
+                    const uint8_t* p = groups[g];
+                    w[r] = p ? *reinterpret_cast<const uint4*>(p + u / kKeepGroups * P) : make_uint4(0, 0, 0, 0);
+                }
+                const int first = static_cast<int>(from + e - page0) >> 4, last = static_cast<int>(from + e + count - 1 - page0) >> 4;
+#pragma unroll
+                for (int r = 0; r < kTargets; r++)
+                    if (first + part + r * kParts <= last)
+                        before[r] = *reinterpret_cast<const uint4*>(token_at(block, 16 * (first + part + r * kParts)) + d * P);
+#pragma unroll
+                for (int r = 0; r < D * kKeepGroups / kKeepThreads; r++) {
+                    const int u = threadIdx.x + r * kKeepThreads;
+                    uint32_t* to = &rows[u / kKeepGroups][u % kKeepGroups * 4];
+                    to[0] = w[r].x, to[1] = w[r].y, to[2] = w[r].z, to[3] = w[r].w;
+                }
+                __syncthreads();
+            }
+            return count;
+        };
+        auto byte_of = [&](int i) { return reinterpret_cast<const uint8_t*>(rows[d])[entries[i].place]; };
+        uint32_t top = 0;  // magnitudes order as their bits do; infinities and NaN come out largest
+        auto measure = [&](uint32_t byte, float scale) {
+            top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(byte & 0xFFu) * scale) & 0x7FFFFFFFu);
+        };
+        int count = 0;
+        for (int e = e0; e < e1; e += count) {
+            count = read(e);
+            if (!is_v) {
+#pragma unroll
+                for (int r = 0; r < kRuns; r++) {
+                    const int i = k_token + r * kTokens;
+                    if (i >= count || !entries[i].from) continue;
+                    const uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
+#pragma unroll
+                    for (int j = 0; j < 16; j++) measure(w[j / 4] >> (8 * (j % 4)), entries[i].scale);
+                }
+            } else {
+                for (int i = part; i < count; i += kParts)
+                    if (entries[i].from) measure(byte_of(i), entries[i].scale);
             }
         }
+        const bool once = count == e1 - e0;  // the page's tokens are one chunk
 #pragma unroll
-        for (int d = 32; d; d >>= 1) top = max(top, __shfl_xor(top, d));
+        for (int x = 32; x; x >>= 1) top = max(top, __shfl_xor(top, x));
         if (threadIdx.x % 64 == 0) tops[threadIdx.x / 64] = top;
-        __syncthreads();  // all of a page of one chunk has been read, and every thread has the old scale
+        __syncthreads();  // a page of one chunk has been read, and every thread has the old scale
         top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
         int shrink = 0;
         const float now = top < 0x7F800000u ? block_scale<TYPE>(__builtin_bit_cast(float, top), true, old, shrink) : __builtin_nanf("");
         const bool dead = !(now > 0.0f);  // zeros, or a NaN scale
         auto moved = [&](uint32_t byte, float scale) {
-            return dead ? 0u : to_byte<TYPE>(from_byte<TYPE>(byte & 0xFFu) * scale / now);
+            byte &= 0xFFu;
+            if (dead) return 0u;
+            if (scale == now && now > 1.0e-30f) return byte;  // what byte * scale / scale rounds to
+            return to_byte<TYPE>(from_byte<TYPE>(byte) * scale / now);
         };
         auto older = [&](uint32_t byte) { return to_byte<TYPE>(ldexpf(from_byte<TYPE>(byte & 0xFFu), -shrink)); };
-        if (shrink)
-            for (int u = threadIdx.x; u < held * D; u += kKeepThreads) {
-                uint8_t* p = token_at(block, u / D) + (is_v ? u % D * P : u % D);
-                *p = static_cast<uint8_t>(older(*p));
+        auto older4 = [&](uint32_t w) { return older(w) | older(w >> 8) << 8 | older(w >> 16) << 16 | older(w >> 24) << 24; };
+        if (shrink) {  // of K all tokens before, of V those of whole groups before the first that changes
+            const int units = is_v ? D * (held / 16) : held * (D / 16), per = max(held / 16, 1);
+            for (int u = threadIdx.x; u < units; u += kKeepThreads) {
+                uint4* p = reinterpret_cast<uint4*>(token_at(block, 0) + (is_v ? u / per * P + u % per * 16 : 16 * u));
+                const uint4 w = *p;
+                *p = make_uint4(older4(w.x), older4(w.y), older4(w.z), older4(w.w));
             }
-        for (int e = e0; e < e1; e += kKeepChunk) {
-            if (e1 - e0 > kKeepChunk) {
-                read(e);
+        }
+        for (int e = e0; e < e1; e += count) {
+            if (!once) {
+                count = read(e);
                 __syncthreads();
             }
             const int t = static_cast<int>(from + e - page0);  // the chunk's place in the page
@@ -179,8 +227,8 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
 #pragma unroll
                 for (int r = 0; r < kRuns; r++) {
                     const int i = k_token + r * kTokens;
-                    if (i >= kKeepChunk || !source[i]) continue;
-                    const float scale = source_scale[i];
+                    if (i >= count || !entries[i].from) continue;
+                    const float scale = entries[i].scale;
                     uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
 #pragma unroll
                     for (int j = 0; j < 4; j++)
@@ -188,10 +236,24 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
                     *reinterpret_cast<uint4*>(token_at(block, t + i) + 16 * k_part) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             } else {
+                const int first = t >> 4, last = (t + count - 1) >> 4;
 #pragma unroll
-                for (int r = 0; r < kPer; r++)
-                    if (source[v_token + r])
-                        token_at(block, t + v_token + r)[v_dim * P] = static_cast<uint8_t>(moved(v[r], source_scale[v_token + r]));
+                for (int r = 0; r < kTargets; r++) {
+                    const int group = first + part + r * kParts;
+                    if (group > last) continue;
+                    uint32_t w[4] = {before[r].x, before[r].y, before[r].z, before[r].w};
+#pragma unroll
+                    for (int j = 0; j < 16; j++) {
+                        const int i = 16 * group + j - t, shift = 8 * (j % 4);
+                        uint32_t byte = w[j / 4] >> shift & 0xFFu;
+                        if (i >= 0 && i < count && entries[i].from)
+                            byte = moved(byte_of(i), entries[i].scale);
+                        else if (i < 0 && e == e0 && shrink)
+                            byte = older(byte);
+                        w[j / 4] = (w[j / 4] & ~(0xFFu << shift)) | byte << shift;
+                    }
+                    *reinterpret_cast<uint4*>(token_at(block, 16 * group) + d * P) = make_uint4(w[0], w[1], w[2], w[3]);
+                }
             }
         }
         if (threadIdx.x == 0) scales[block] = now;

@@ -1,4 +1,6 @@
 // Rotary positions with several axes (wl_rope), behind a norm of each head (wl_norm_rope).
+#include <type_traits>
+
 #include "wl_host.h"
 
 namespace wl {
@@ -140,7 +142,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
     struct alignas(sizeof(T) * VEC) Run {
         T v[VEC];
     };
-    constexpr int kRows = kRopeThreads / 32, kEarly = 3;
+    constexpr int kRows = kRopeThreads / 32, kEarly = 1;
     const int token = blockIdx.x, lane = threadIdx.x % 32;
     const int pairs = a.half / VEC, units = pairs + (a.head_dim - 2 * a.half) / VEC, heads = a.q.heads + a.k.heads;
     struct Head {
@@ -237,8 +239,145 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs
     }
 }
 
+// 16 bytes of a head as fp32, and back.
+template <typename T>
+constexpr int kVec = 16 / sizeof(T);
+template <typename T>
+__device__ __forceinline__ void unpack(uint4 w, float (&x)[kVec<T>]) {
+    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4) {
+            x[i] = __builtin_bit_cast(float, v[i]);
+        } else {
+            x[2 * i] = __builtin_bit_cast(float, v[i] << 16);
+            x[2 * i + 1] = __builtin_bit_cast(float, v[i] & 0xFFFF0000u);
+        }
+    }
+}
+template <typename T>
+__device__ __forceinline__ uint4 pack(const float (&x)[kVec<T>]) {
+    typedef __bf16 Pair __attribute__((ext_vector_type(2)));
+    typedef float Floats __attribute__((ext_vector_type(2)));
+    uint32_t v[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        if constexpr (sizeof(T) == 4)
+            v[i] = __builtin_bit_cast(uint32_t, x[i]);
+        else
+            v[i] = __builtin_bit_cast(uint32_t, __builtin_convertvector((Floats){x[2 * i], x[2 * i + 1]}, Pair));
+    }
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+// The sum over a head's lanes, 8 to 64 of them side by side.
+template <int LANES>
+__device__ __forceinline__ float sum_over(float x) {
+    auto dpp = [](float v, auto control) {
+        return v + __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), decltype(control)::value, 0xf, 0xf, true));
+    };
+    x = dpp(x, std::integral_constant<int, 0xB1>());   // neighbours
+    x = dpp(x, std::integral_constant<int, 0x4E>());   // pairs
+    x = dpp(x, std::integral_constant<int, 0x141>());  // four and four, mirrored
+    if constexpr (LANES >= 16) x = dpp(x, std::integral_constant<int, 0x140>());  // eight and eight
+    if constexpr (LANES >= 32) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const uint32_t r0 = r[0], r1 = r[1];
+        x = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
+    if constexpr (LANES >= 64) {
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+        const uint32_t r0 = r[0], r1 = r[1];
+        x = __builtin_bit_cast(float, r0) + __builtin_bit_cast(float, r1);
+    }
+    return x;
+}
+
+// Heads of 16 bytes for each of 8 to 64 lanes, everything aligned: a lane has the same dimensions of every head, and its
+// partner's, in another lane, the ones that they turn with: out = (x a + partner's x b) / rms with a = weight cos and b = -+ the
+// partner's weight sin (weight and 0 where nothing turns). These factors are worked out once for a token, into LDS, and a head
+// costs a load, a sum over its lanes, its partner's 16 bytes, three operations a value and a store.
+template <typename T, int LANES>
+__global__ __launch_bounds__(kRopeThreads) void k_norm_rope_lanes(RopeArgs a, NormArgs n, int per) {
+    constexpr int V = kVec<T>, D = V * LANES, kGroups = kRopeThreads / LANES;
+    extern __shared__ float4 tables[];  // factors a of q [per][D], of k, factors b of q, of k; then cosines and sines [per][half]
+    float* fa = reinterpret_cast<float*>(tables);
+    float* fb = fa + 2 * per * D;
+    float2* turn = reinterpret_cast<float2*>(fb + 2 * per * D);
+    const int first = blockIdx.x * per, tokens = min(per, a.tokens - first);
+    const int unit = threadIdx.x % LANES, heads = a.q.heads + a.k.heads, pairs = a.half / V;
+    const int other = unit < pairs ? unit + pairs : unit < 2 * pairs ? unit - pairs : unit;
+    int token = 0, head = threadIdx.x / LANES;  // of this group
+    auto forward = [&] {
+        for (; head >= heads && token < tokens; head -= heads) token++;
+    };
+    auto load = [&] {
+        const bool is_k = head >= a.q.heads;
+        const T* p = static_cast<const T*>(is_k ? a.k.in : a.q.in) + (first + token) * (is_k ? a.k.in_token_stride : a.q.in_token_stride) +
+                     (is_k ? head - a.q.heads : head) * (is_k ? a.k.in_head_stride : a.q.in_head_stride);
+        return *reinterpret_cast<const uint4*>(p + unit * V);
+    };
+    forward();
+    uint4 next = make_uint4(0, 0, 0, 0);
+    if (token < tokens) next = load();
+    for (int j = threadIdx.x; j < tokens * a.half; j += kRopeThreads) turn[j] = turn_of(a, j % a.half, first + j / a.half);
+    __syncthreads();
+    for (int i = threadIdx.x; i < 2 * D; i += kRopeThreads) {
+        const void* w = i < D ? n.q_weight : n.k_weight;
+        const int d = i % D, j = d < a.half ? d : d - a.half, e = d < a.half ? d + a.half : j;
+        const bool turns = d < 2 * a.half;
+        auto weight = [&](int at) {
+            return !w ? 1.0f : n.offset + (n.bf16 ? load_value(static_cast<const uint16_t*>(w) + at) : static_cast<const float*>(w)[at]);
+        };
+        const float own = weight(d), others = turns ? weight(e) : 0.0f;
+        for (int t = 0; t < tokens; t++) {
+            const float2 cs = turns ? turn[t * a.half + j] : make_float2(1.0f, 0.0f);
+            const int to = (i < D ? t : per + t) * D + d;
+            fa[to] = own * cs.x;
+            fb[to] = d < a.half ? -others * cs.y : others * cs.y;
+        }
+    }
+    __syncthreads();
+    while (token < tokens) {
+        const bool is_k = head >= a.q.heads;
+        const uint4 w = next;
+        const int at = (is_k ? per + token : token) * D + unit * V;
+        T* out = static_cast<T*>(is_k ? a.k.out : a.q.out) + (first + token) * (is_k ? a.k.out_token_stride : a.q.out_token_stride) +
+                 (is_k ? head - a.q.heads : head) * (is_k ? a.k.out_head_stride : a.q.out_head_stride);
+        head += kGroups;
+        forward();
+        if (token < tokens) next = load();
+        const uint4 p = make_uint4(__shfl(w.x, other, LANES), __shfl(w.y, other, LANES), __shfl(w.z, other, LANES), __shfl(w.w, other, LANES));
+        float x[V], y[V], z[V];
+        unpack<T>(w, x);
+        unpack<T>(p, y);
+        float sum = 0.0f;
+#pragma unroll
+        for (int e = 0; e < V; e++) sum = __builtin_fmaf(x[e], x[e], sum);
+        const float mean = sum_over<LANES>(sum) * (1.0f / D) + n.eps;
+        float inv = __builtin_amdgcn_rsqf(mean);
+        if (__any(!(mean > 1.0e-30f))) inv = 1.0f / sqrtf(mean);
+#pragma unroll
+        for (int e = 0; e < V; e++) z[e] = inv * __builtin_fmaf(x[e], fa[at + e], y[e] * fb[at + e]);
+        *reinterpret_cast<uint4*>(out + unit * V) = pack<T>(z);
+    }
+}
+
 template <typename T, int VEC>
 void launch_norm_rope(const RopeArgs& a, const NormArgs& n, hipStream_t stream) {
+    auto lanes = [&](auto count) {
+        const int per = sizeof(T) == 2 && a.tokens > 2048 ? 2 : 1;
+        const size_t lds = (4 * sizeof(float) * a.head_dim + sizeof(float2) * a.half) * per;
+        k_norm_rope_lanes<T, decltype(count)::value><<<(a.tokens + per - 1) / per, kRopeThreads, lds, stream>>>(a, n, per);
+    };
+    if constexpr (VEC > 1) {
+        if (a.head_dim == 8 * VEC) return lanes(std::integral_constant<int, 8>());
+        if (a.head_dim == 16 * VEC) return lanes(std::integral_constant<int, 16>());
+        if (a.head_dim == 32 * VEC) return lanes(std::integral_constant<int, 32>());
+        if (a.head_dim == 64 * VEC) return lanes(std::integral_constant<int, 64>());
+    }
     k_norm_rope<T, VEC><<<a.tokens, kRopeThreads, sizeof(float2) * a.half + 2 * sizeof(float) * a.head_dim, stream>>>(a, n);
 }
 
