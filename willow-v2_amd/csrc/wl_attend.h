@@ -80,9 +80,6 @@ struct AttendArgs {
 // The lowest n of 16 bits
 __device__ __forceinline__ uint32_t low_bits(int n) { return (1u << min(max(n, 0), 16)) - 1u; }
 
-// All bits of the four bytes whose bits (the lowest four) are set
-__device__ __forceinline__ uint32_t bytes_of(uint32_t bits) { return ((bits & 15u) * 0x00204081u & 0x01010101u) * 0xFFu; }
-
 // One row of a masked call: `limit` is its position plus 1 (0: it is not there).
 // Which of the 16 tokens from position p on it sees, as bits. `count` of them are there, counting from the first; `drafted`: the
 // bits of the tree that fall on them.

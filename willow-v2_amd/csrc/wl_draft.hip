@@ -98,6 +98,7 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
     constexpr int kTokens = kKeepThreads / (D / 16), kRuns = (kKeepChunk + kTokens - 1) / kTokens;
     constexpr int kParts = kKeepThreads / D, kTargets = (kKeepChunk / 16 + 1 + kParts - 1) / kParts;
     const int k_part = threadIdx.x % (D / 16), k_token = threadIdx.x / (D / 16), d = threadIdx.x % D, part = threadIdx.x / D;
+    const int first_entry = __builtin_amdgcn_readfirstlane(part);  // the same for a wavefront
     for (int64_t col = from >> c.page_shift; n > 0 && col <= (from + n - 1) >> c.page_shift; col++) {
         const int64_t page0 = col * P;
         const int page = page_at(page0);
@@ -107,6 +108,10 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         const int64_t block = c.block(page, head);
         const float old = scales[block];
         uint4 k[kRuns], before[kTargets];
+        // of V, entry lane % 32: what a loop over entries reads by readlane, and which are moved
+        int place = 0;
+        float scale = 0.0f;
+        uint32_t some = 0;
         // the tokens from row e on, as they stand -> how many
         auto read = [&](int e) {
             __syncthreads();  // the chunk before has been worked on, and written
@@ -135,7 +140,7 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wavefront's writes to LDS are in order
                 if (x.from && first && number < kKeepGroups) groups[number] = x.from - x.place;
-                x.place += 16 * number;
+                x.place = is_v && number < kKeepGroups ? x.place + 16 * number : 0;  // within `rows`, moved or not
                 if (threadIdx.x < kKeepChunk) entries[threadIdx.x] = x;
             }
             __syncthreads();
@@ -166,11 +171,16 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
                     uint32_t* to = &rows[u / kKeepGroups][u % kKeepGroups * 4];
                     to[0] = w[r].x, to[1] = w[r].y, to[2] = w[r].z, to[3] = w[r].w;
                 }
+                const Entry x = entries[threadIdx.x % kKeepChunk];
+                place = x.place;
+                scale = x.scale;
+                some = static_cast<uint32_t>(__ballot(x.from != nullptr)) & (count < 32 ? (1u << count) - 1u : ~0u);
                 __syncthreads();
             }
-            return count;
+            return __builtin_amdgcn_readfirstlane(count);
         };
-        auto byte_of = [&](int i) { return reinterpret_cast<const uint8_t*>(rows[d])[entries[i].place]; };
+        auto byte_of = [&](int i) { return static_cast<uint32_t>(reinterpret_cast<const uint8_t*>(rows[d])[__builtin_amdgcn_readlane(place, i)]); };
+        auto scale_of = [&](int i) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, scale), i)); };
         uint32_t top = 0;  // magnitudes order as their bits do; infinities and NaN come out largest
         auto measure = [&](uint32_t byte, float scale) {
             top = max(top, __builtin_bit_cast(uint32_t, from_byte<TYPE>(byte & 0xFFu) * scale) & 0x7FFFFFFFu);
@@ -188,8 +198,16 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
                     for (int j = 0; j < 16; j++) measure(w[j / 4] >> (8 * (j % 4)), entries[i].scale);
                 }
             } else {
-                for (int i = part; i < count; i += kParts)
-                    if (entries[i].from) measure(byte_of(i), entries[i].scale);
+                for (int i0 = 0; i0 < count; i0 += 8 * kParts) {
+                    uint32_t bytes[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) bytes[j] = byte_of(min(i0 + first_entry + j * kParts, 31));
+#pragma unroll
+                    for (int j = 0; j < 8; j++) {
+                        const int i = min(i0 + first_entry + j * kParts, 31);
+                        if (some >> i & 1) measure(bytes[j], scale_of(i));
+                    }
+                }
             }
         }
         const bool once = count == e1 - e0;  // the page's tokens are one chunk
@@ -201,12 +219,9 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
         int shrink = 0;
         const float now = top < 0x7F800000u ? block_scale<TYPE>(__builtin_bit_cast(float, top), true, old, shrink) : __builtin_nanf("");
         const bool dead = !(now > 0.0f);  // zeros, or a NaN scale
-        auto moved = [&](uint32_t byte, float scale) {
-            byte &= 0xFFu;
-            if (dead) return 0u;
-            if (scale == now && now > 1.0e-30f) return byte;  // what byte * scale / scale rounds to
-            return to_byte<TYPE>(from_byte<TYPE>(byte) * scale / now);
-        };
+        // byte * scale / scale rounds to the byte
+        auto stays = [&](float scale) { return scale == now && now > 1.0e-30f; };
+        auto moved = [&](uint32_t byte, float scale) { return dead ? 0u : to_byte<TYPE>(from_byte<TYPE>(byte & 0xFFu) * scale / now); };
         auto older = [&](uint32_t byte) { return to_byte<TYPE>(ldexpf(from_byte<TYPE>(byte & 0xFFu), -shrink)); };
         auto older4 = [&](uint32_t w) { return older(w) | older(w >> 8) << 8 | older(w >> 16) << 16 | older(w >> 24) << 24; };
         if (shrink) {  // of K all tokens before, of V those of whole groups before the first that changes
@@ -230,27 +245,43 @@ __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t lay
                     if (i >= count || !entries[i].from) continue;
                     const float scale = entries[i].scale;
                     uint32_t w[4] = {k[r].x, k[r].y, k[r].z, k[r].w};
+                    if (!stays(scale)) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        w[j] = moved(w[j], scale) | moved(w[j] >> 8, scale) << 8 | moved(w[j] >> 16, scale) << 16 | moved(w[j] >> 24, scale) << 24;
+                        for (int j = 0; j < 4; j++)
+                            w[j] = moved(w[j], scale) | moved(w[j] >> 8, scale) << 8 | moved(w[j] >> 16, scale) << 16 | moved(w[j] >> 24, scale) << 24;
+                    }
                     *reinterpret_cast<uint4*>(token_at(block, t + i) + 16 * k_part) = make_uint4(w[0], w[1], w[2], w[3]);
                 }
             } else {
                 const int first = t >> 4, last = (t + count - 1) >> 4;
+                const bool plain = __all(stays(scale) || !(some >> (threadIdx.x % kKeepChunk) & 1));
 #pragma unroll
                 for (int r = 0; r < kTargets; r++) {
-                    const int group = first + part + r * kParts;
+                    const int group = first + first_entry + r * kParts;
                     if (group > last) continue;
-                    uint32_t w[4] = {before[r].x, before[r].y, before[r].z, before[r].w};
+                    uint32_t w[4] = {before[r].x, before[r].y, before[r].z, before[r].w}, bytes[16];
+                    if (e == e0 && shrink && 16 * group < t) {
+                        // of the words' bytes those before the first kept token
 #pragma unroll
-                    for (int j = 0; j < 16; j++) {
-                        const int i = 16 * group + j - t, shift = 8 * (j % 4);
-                        uint32_t byte = w[j / 4] >> shift & 0xFFu;
-                        if (i >= 0 && i < count && entries[i].from)
-                            byte = moved(byte_of(i), entries[i].scale);
-                        else if (i < 0 && e == e0 && shrink)
-                            byte = older(byte);
-                        w[j / 4] = (w[j / 4] & ~(0xFFu << shift)) | byte << shift;
+                        for (int j = 0; j < 4; j++) {
+                            const uint32_t mask = byte_mask(t - 16 * group - 4 * j);
+                            w[j] = (older4(w[j]) & mask) | (w[j] & ~mask);
+                        }
+                    }
+                    const int i0 = 16 * group - t;  // the entry that the group's first byte is for
+#pragma unroll
+                    for (int j = 0; j < 16; j++) bytes[j] = byte_of(min(max(i0 + j, 0), 31));
+                    const uint32_t which = (i0 < 0 ? some << -i0 : some >> i0) & 0xFFFFu;
+                    if (!plain) {
+#pragma unroll
+                        for (int j = 0; j < 16; j++)
+                            if (which >> j & 1) bytes[j] = moved(bytes[j], scale_of(min(max(i0 + j, 0), 31)));
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const uint32_t mask = bytes_of(which >> 4 * j),
+                                       y = bytes[4 * j] | bytes[4 * j + 1] << 8 | bytes[4 * j + 2] << 16 | bytes[4 * j + 3] << 24;
+                        w[j] = (w[j] & ~mask) | (y & mask);
                     }
                     *reinterpret_cast<uint4*>(token_at(block, 16 * group) + d * P) = make_uint4(w[0], w[1], w[2], w[3]);
                 }

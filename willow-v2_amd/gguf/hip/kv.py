@@ -237,12 +237,12 @@ def kv_tree(parents: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, max_co
     (words = max_count / 64 rounded up; rows beyond it are dropped; default: all rows). Rows of no sequence get no bits and
     position 0. Once a step: every layer takes the same masks."""
     index = parents.get_device() if isinstance(parents, torch.Tensor) else -1
-    _need(parents, "parents", index, torch.int32, ("tokens",))
-    _need(start, "start", index, torch.int32, ("sequences",))
+    for t, name, dim in ((parents, "parents", "tokens"), (start, "start", "sequences"), (cu, "cu", "sequences + 1")):
+        if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1 and t.is_contiguous()):
+            _refuse(t, name, f"cuda:{index}", torch.int32, f"[{dim}], contiguous")
     n, seqs = parents.shape[0], start.shape[0]
-    _need(cu, "cu", index, torch.int32, (seqs + 1,))
-    if cu.shape[0] != seqs + 1 or not (parents.is_contiguous() and start.is_contiguous() and cu.is_contiguous()):
-        raise ValueError(f"parents, start and cu must be contiguous, cu [{seqs + 1}] (got {list(cu.shape)})")
+    if cu.shape[0] != seqs + 1:
+        raise ValueError(f"cu must be [{seqs + 1}] for {seqs} sequences (got {list(cu.shape)})")
     if max_count is None or max_count > n:
         max_count = n
     if (seqs | n | max_count) >> 31:
@@ -320,7 +320,7 @@ def rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: to
     0 the rest) or one axis after the other. Value pairs (j, j + rotary_dim / 2) turn by positions[axis(j)] * inv_freq[j], taken in
     64 bits; cosine and sine are multiplied by `scale`; the rest of each head
     is copied. (engines/base.py:16-89 has the one-axis form.)"""
-    return _rotate(library().wl_rope, q, k, positions, inv_freq, sections, interleaved, scale, out, lambda dim: ())
+    return _rotate(library().wl_rope, q, k, positions, inv_freq, sections, interleaved, scale, out, ())
 
 
 def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_freq: torch.Tensor, q_weight: torch.Tensor = None,
@@ -329,26 +329,25 @@ def norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, inv_fre
     """rope() on queries and keys that are normed first, each head by itself: x / sqrt(mean(x^2) + eps) * w, in fp32 up to the one
     rounding of the rotated values. w: 1 + weight with zero_centered (the reference's RMSNorm, engines/base.py:27-31), else weight;
     q_weight and k_weight [head_dim], both fp32 or both bf16, None: w = 1. The rest as in rope."""
-    weights = [w for w in (q_weight, k_weight) if w is not None]
     if not 0 <= eps < float("inf"):
         raise ValueError(f"eps {eps}")
-
-    def norm(dim):
-        kind = torch.float32 if not weights else weights[0].dtype
-        if kind is not torch.float32 and kind is not torch.bfloat16:
-            raise ValueError(f"the weights must be fp32 or bf16 (got {kind})")
-        for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-            if w is not None:
-                _need(w, name, q.get_device(), kind, (dim,))
-                if w.shape[0] != dim or not w.is_contiguous():
-                    raise ValueError(f"{name} must be [{dim}], contiguous (got {list(w.shape)})")
-        return (None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-                DTYPE_F32 if kind is torch.float32 else DTYPE_BF16, eps, zero_centered)
-    return _rotate(library().wl_norm_rope, q, k, positions, inv_freq, sections, interleaved, scale, out, norm)
+    index, dim, kind, at = q.get_device(), q.shape[-1], None, []
+    for w in (q_weight, k_weight):
+        if w is None:
+            at.append(None)
+            continue
+        kind = w.dtype if kind is None else kind
+        if not (w.dtype is kind and w.get_device() == index and w.dim() == 1 and w.shape[0] == dim and w.is_contiguous()):
+            _refuse(w, "q_weight" if not at else "k_weight", q.device, kind, f"[{dim}], contiguous,")
+        at.append(w.data_ptr())
+    if kind not in (None, torch.float32, torch.bfloat16):
+        raise ValueError(f"the weights must be fp32 or bf16 (got {kind})")
+    return _rotate(library().wl_norm_rope, q, k, positions, inv_freq, sections, interleaved, scale, out,
+                   (*at, DTYPE_BF16 if kind is torch.bfloat16 else DTYPE_F32, eps, zero_centered))
 
 
 def _rotate(call, q, k, positions, inv_freq, sections, interleaved, scale, out, more):
-    """One call of wl_rope or wl_norm_rope; more(head_dim): its arguments behind the scale."""
+    """One call of wl_rope or wl_norm_rope; more: its arguments behind the scale."""
     dtype, index = q.dtype, q.get_device()
     if dtype is not torch.bfloat16 and dtype is not torch.float32:
         raise ValueError(f"q must be bf16 or fp32 (got {dtype})")
@@ -374,7 +373,6 @@ def _rotate(call, q, k, positions, inv_freq, sections, interleaved, scale, out, 
         q_out, to = torch.empty_like(q, memory_format=torch.contiguous_format), (heads * dim, dim)
     else:
         to = _rotated_into(q_out, q, index, dim)
-    extra = more(dim)
     q_arg = WlRopeTensor(q.data_ptr(), q_out.data_ptr(), token, head, *to, heads, 0)
     k_arg = None
     if k is not None:
@@ -388,5 +386,5 @@ def _rotate(call, q, k, positions, inv_freq, sections, interleaved, scale, out, 
         k_arg = WlRopeTensor(k.data_ptr(), k_out.data_ptr(), token, head, *to, heads, 0)
     if n:
         _launch(index, call, q_arg, k_arg, DTYPE_BF16 if dtype is torch.bfloat16 else DTYPE_F32, n, dim, 2 * half,
-                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, _sections(sections), interleaved, scale, *extra)
+                positions.data_ptr(), axis_stride, inv_freq.data_ptr(), axes, _sections(sections), interleaved, scale, *more)
     return q_out, k_out
