@@ -654,6 +654,11 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     // how many pieces come of it is known on the device alone: room for as many as the partial results may take
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
     const bool few_tiles = items < 2 * kCus;
+    // With a window the row tiles of one sequence go through as many tiles each, from the window's length on: where they fill the CUs
+    // to nine tenths nothing is cut (4096 tokens in a window of 1024 102 -> XX us with the second kernel left out).
+    if (mask && longest < max_length && longest < int64_t{b->table_width} * c->page_tokens && b->seqs == 1 && few_tiles &&
+        10 * items >= 9 * ((items + kCus - 1) / kCus * kCus))
+        return {row_tiles, 1, items, true};
     if (!few_tiles && (b->seqs == 1 || most < kLong || room < 4)) return {row_tiles, 1, items, false};
     const int64_t least = mask ? kLeast<true> : kLeast<false>, limit = mask && items < kCus / kMaxPieces ? kMaxMaskedPieces : kMaxPieces;
     const int64_t pieces = std::max<int64_t>(1, std::min({limit, (most + least - 1) / least, room}));

@@ -9,9 +9,11 @@ namespace {
 constexpr int kTreeThreads = 256;
 constexpr int kTreeKept = 4096;  // parents of a sequence that fit in LDS
 
-// A workgroup takes a sequence, a thread a row: it walks from the row to its root. Parents stand before their children, so the
-// walk ends, and meets the words of the row's mask from the last to the first. The workgroup behind the last sequence
-// clears the rows before the first and behind the last one.
+// A workgroup takes a sequence, a thread a row. Up to 64 rows are a wavefront's: each takes over the mask and the parent of the
+// row that it has reached, which doubles its steps every time (walking them one by one took 5.0 us for a tree of 64, 2.3 for 16).
+// More rows are walked from the row to its root: parents stand before their children, so the walk ends, and meets the words
+// of the row's mask from the last to the first. The workgroup behind the last sequence clears the rows before the first and
+// behind the last one.
 __global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_t* __restrict__ parents,
                                                           const int32_t* __restrict__ start, uint64_t* __restrict__ tree,
                                                           int64_t words, int64_t* __restrict__ positions) {
@@ -29,6 +31,30 @@ __global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_
     const int at = s.first(b), n = s.count(b, at);
     clear(at + n, min(max(s.cu[b + 1], at), s.tokens));  // rows behind max_count
     const int32_t* mine = parents + at;
+    const int64_t before = start[b];
+    if (n <= 64) {  // the same for all threads
+        if (threadIdx.x >= 64) return;
+        const int i = threadIdx.x;
+        int up = i < n ? mine[i] : -1;
+        if (up >= i) up = -1;
+        uint32_t lo = i < 32 ? 1u << i : 0, hi = i < 32 ? 0 : 1u << (i - 32);
+        while (__any(up >= 0)) {  // up: the 2^r-th ancestor; lo, hi: the row and those before that one
+            const int from = max(up, 0);
+            const uint32_t more_lo = __shfl(lo, from), more_hi = __shfl(hi, from);
+            const int next = __shfl(up, from);
+            if (up >= 0) {
+                lo |= more_lo;
+                hi |= more_hi;
+                up = next;
+            }
+        }
+        if (i >= n) return;
+        uint64_t* row = tree + (at + i) * words;
+        row[0] = static_cast<uint64_t>(hi) << 32 | lo;
+        for (int64_t w = 1; w < words; w++) row[w] = 0;
+        positions[at + i] = before + __popc(lo) + __popc(hi) - 1;
+        return;
+    }
     for (int i = threadIdx.x; i < min(n, kTreeKept); i += kTreeThreads) kept[i] = mine[i];
     __syncthreads();
     for (int i = threadIdx.x; i < n; i += kTreeThreads) {
@@ -51,7 +77,7 @@ __global__ __launch_bounds__(kTreeThreads) void k_kv_tree(KvSeqs s, const int32_
             row[word] = bits;
             bits = 0;
         }
-        positions[at + i] = static_cast<int64_t>(start[b]) + seen - 1;
+        positions[at + i] = before + seen - 1;
     }
 }
 
