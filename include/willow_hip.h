@@ -371,7 +371,8 @@ int wl_kv_tree(const WlKvBatch* batch, const int32_t* parents, const int32_t* st
  * (s == 0: the smallest bf16 value that does); a value is its byte times its page's scale in fp32, divided by that and rounded to
  * nearest even, so bytes that stay in a page that keeps its scale are moved as they are. Bytes before start[b] are divided by 2^n
  * and rounded as wl_kv_append does. Tokens whose source or target page is not there are not moved. A NaN scale, or a value past
- * fp32's range, makes the target's scale NaN. Pages that a call writes must be distinct over its sequences. */
+ * fp32's range, makes the target's scale NaN. A page that receives tokens belongs to one sequence of the call alone. Meant for
+ * a step's drafts; any number of rows is taken, page after page by one workgroup for each head. */
 int wl_kv_keep(const WlKvCache* cache, const WlKvBatch* batch, const int32_t* start, const int32_t* keep, void* stream);
 
 /* Copies pages src_host[i] to dst_host[i], i < n, of every layer (bytes and scales). HOST arrays, passed by value to the

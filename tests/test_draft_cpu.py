@@ -31,6 +31,7 @@ def keep(cache=None, batch=None, start=FAKE, kept=FAKE):
 
 
 def test_struct_layout():
+    assert hip.library().wl_abi_version() & 0xFFFF >= 5
     assert ctypes.sizeof(hip.WlKvMask) == 32
 
 

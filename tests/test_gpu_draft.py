@@ -249,6 +249,34 @@ def test_tree_in_a_window(hip, dtype, count, group, window, sinks):
     check_masked(hip, pages, 0, q, table, i32(lengths), cu_of(counts), max_count=count, window=window, sinks=sinks, tree=tree)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("count,group", [(16, 1), (40, 1), (60, 4), (130, 4)])
+def test_tree_keeps_out_what_it_hides(hip, dtype, count, group):
+    """A page of drafted tokens whose scales are NaN reaches exactly the rows that see one of its tokens; pages that are not there
+    nobody; a row's own page among them leaves it what is in the others."""
+    g, rng = gen(45), random.Random(45)
+    start = 48
+    pages = random_pages(hip, g, 1, 14, 2, 16, 64, dtype)
+    table = table_of(g, (start + count,), 16, 14)
+    # two trees side by side: rows of one see nothing of the other
+    half = count // 2
+    parents = [max(i - 1 - rng.randrange(3), -1) if i < half else -1 if i == half else max(i - 1 - rng.randrange(2), half) for i in range(count)]
+    tree, _ = hip.kv_tree(i32(parents), i32([start]), i32([0, count]))
+    q = torch.randn(count, 2 * group, 64, generator=g).to(torch.bfloat16).to(DEV)
+    args = (q, table, i32([start + count]), i32([0, count]))
+    page = int(table[0, (start + half) // 16 if half % 16 == 0 else (start + half) // 16 + 1]) if half >= 16 else int(table[0, start // 16])
+    for scale, head in ((pages.k_scale, 0), (pages.v_scale, 1)):
+        was = float(scale[0, page, head])
+        scale[0, page, head] = math.nan
+        out = check_masked(hip, pages, 0, *args, tree=tree)
+        if half >= 16:
+            assert torch.isfinite(out[:8].float()).all() and torch.isnan(out[-1, head * group].float()).all()
+        scale[0, page, head] = was
+    missing = table.clone()
+    missing[0, (start + count - 1) // 16], missing[0, 1] = -1, 2 ** 31 - 1
+    check_masked(hip, pages, 0, q, missing, *args[2:], tree=tree)
+
+
 def test_tree_of_one_chain_is_causal(hip):
     g = gen(43)
     pages = random_pages(hip, g, 1, 20, 2, 64, 256, torch.int8)

@@ -134,7 +134,7 @@ struct Stage {
         to[(32 + row) ^ sw] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(k.z, k.w));
         uint4 w = v;
         const int n = min(max(count - 16 * v_part(), 0), 16);  // tokens that are there, of this thread's part
-        if (MASK && count > 0) {  // see below
+        if (MASK && count > 0 && -count < hidden_to) {  // the tile begins before the window; see below
             const int behind = 16 * v_part() - count;  // where this part begins, counted as well
             const uint32_t kept = low_bits(count - 16 * v_part()) & (~low_bits(hidden_to - behind) | low_bits(hidden_from - behind));
             w.x &= bytes_of(kept);
@@ -655,7 +655,7 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
     const bool few_tiles = items < 2 * kCus;
     // With a window the row tiles of one sequence go through as many tiles each, from the window's length on: where they fill the CUs
-    // to nine tenths nothing is cut (4096 tokens in a window of 1024 102 -> XX us with the second kernel left out).
+    // to nine tenths nothing is cut, and the second kernel (5 us of 102 for 4096 tokens in a window of 1024) is left out.
     if (mask && longest < max_length && longest < int64_t{b->table_width} * c->page_tokens && b->seqs == 1 && few_tiles &&
         10 * items >= 9 * ((items + kCus - 1) / kCus * kCus))
         return {row_tiles, 1, items, true};

@@ -1766,7 +1766,7 @@ const char* wl_error_string(int code) {
     return "unknown error";
 }
 
-int wl_abi_version(void) { return (1 << 16) | 4; }  // 1.4: rope, cache; 1.3: min_expert_weight (was reserved2, 0); 1.2: next, noalloc
+int wl_abi_version(void) { return (1 << 16) | 5; }  // 1.5: masks, drafts, norm_rope; 1.4: rope, cache; 1.3: min_expert_weight (was reserved2, 0); 1.2: next, noalloc
 
 int wl_moe_check(const WlMoeLayer* layer) { return check_layer(layer); }
 

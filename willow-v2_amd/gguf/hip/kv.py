@@ -263,7 +263,8 @@ def kv_keep(pages: KVPages, table: torch.Tensor, start: torch.Tensor, keep: torc
     have to be at least i (less is taken as i: the token stays); increasing ones are the accepted tokens in order. What lies behind
     the last of them is no longer the sequence's (shorten its length), and stays as it is. A page that receives tokens keeps its
     scale, times the smallest power of two with which it covers the tokens kept in it; bytes that stay in a page whose scale stays
-    move as they are. Tokens whose page is not there are not moved. Pages written in one call must be distinct over its sequences."""
+    move as they are. Tokens whose page is not there are not moved. A page that receives tokens belongs to one of the call's sequences
+    alone."""
     index = pages.index
     _need(keep, "keep", index, torch.int32, ("rows",))
     n = keep.shape[0]
