@@ -74,7 +74,7 @@ struct Lds {
     uint4 k[kRing][Shape<D>::kSubs * Shape<D>::kSteps][64];
     uint4 v[kRing][Shape<D>::kBlocks * Shape<D>::kSubs * 2][64];
     Part part[kRing][Shape<D>::kParts];
-    int count[kRing][Shape<D>::kParts];  // tokens that are there
+    int count[kRing][Shape<D>::kParts];  // tokens that are there; with MASK as bits
 };
 
 // One thread's share of a tile on its way: 16 values of one token of K, 16 tokens of one dimension of V. PAGE: a page holds
@@ -152,12 +152,19 @@ struct Stage {
         pair[0][slot] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(w.x, w.y));
         pair[1][slot] = __builtin_bit_cast(uint4, eight_bf16<TYPE>(w.z, w.w));
         if (threadIdx.x < S::kParts) {
+            int id = threadIdx.x;
+            if constexpr (MASK && D == 256) {
+                // asked for again for every tile: kept, what is addressed with it would be spilled, and come back from memory between
+                // the loads and the barrier
+                id = __builtin_amdgcn_mbcnt_lo(~0u, 0);
+                __asm__ volatile("" : "+v"(id));
+            }
             // never 0: a masked score is -inf, and times the scale it has to stay that (a block of zeros scores 0 all the same)
             const float scaled = ks * a.scale_log2;
             const bool fold = vs >= 8.6736174e-19f && vs <= 1.1529215e18f;  // 2^-60 .. 2^60
-            lds.part[buffer][threadIdx.x] = {scaled == 0.0f ? 1.17549435e-38f : scaled, fold ? __builtin_amdgcn_logf(vs) : 0.0f,
+            lds.part[buffer][id] = {scaled == 0.0f ? 1.17549435e-38f : scaled, fold ? __builtin_amdgcn_logf(vs) : 0.0f,
                                              fold ? 1.0f / vs : 1.0f, fold ? 1.0f : vs};
-            lds.count[buffer][threadIdx.x] = n;
+            lds.count[buffer][id] = MASK ? low_bits(n) : n;
         }
     }
 };
@@ -204,7 +211,7 @@ struct Wave {
         __builtin_amdgcn_s_setprio(0);
         const Part part = lds.part[buffer][2 * u + half];
         const int there = lds.count[buffer][2 * u + half];
-        const int mine = MASK ? seen & low_bits(there) : min(there, seen);
+        const int mine = MASK ? seen & there : min(there, seen);
         // a lane that sees no token of its block is not to meet the block's scales: they may be NaN
         const float ks = mine > 0 ? part.ks : 1.0f, rest = mine > 0 ? part.rest : 1.0f;
         const int slot = lane ^ S::v_swizzle(2 * u + half);
@@ -481,13 +488,10 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
             if constexpr (MASK) {
                 if (base + 32 * u + 32 <= window_at && base + 32 * u >= a.mask.sinks) continue;
                 int seen = 0xFFFF;
-                if (base + 32 * u < whole_from || base + 32 * u + 32 > whole_to) {
-                    uint32_t drafted = 0;
-                    if (a.mask.tree && base + 32 * u + 32 > seq.begin) {  // a few tiles: the row is worked out again, as below
-                        const int r = row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero());
-                        drafted = tree_bits(a, seq, r / a.group, at);
-                    }
-                    seen = seen_bits(a, seq, limit, at, 16, drafted);
+                if (base + 32 * u < whole_from || base + 32 * u + 32 > whole_to) {  // a few tiles: the row is worked out again, as below
+                    const int r = (row0 + static_cast<int>((threadIdx.x >> 6) * 32 + (threadIdx.x & 31) + lane_zero())) / a.group;
+                    const uint32_t drafted = a.mask.tree && base + 32 * u + 32 > seq.begin ? tree_bits(a, seq, r, at) : 0;
+                    seen = seen_bits(a, seq, limit_of(a, seq, r), at, 16, drafted);
                 }
                 w.template add<MASK>(lds, buffer, u, seen);
             } else {
