@@ -6,6 +6,9 @@
 // converted by one of eight wavefronts and used by all. LDS holds a ring of four tiles: while one is multiplied, the
 // bytes of the tile two ahead are on their way in registers, and are converted into its place; a barrier stands behind every
 // second tile (behind every one: 2% slower).
+// With a window, sinks or a tree of drafts (MASK) a row tile goes through the tiles that some row of it sees, a wavefront through the
+// parts that some row of its own sees, and of these just those that not all rows see whole are masked (4096 tokens behind as many in a
+// window of 1024, 16 heads of 256: 87 to 91 us, 790 to 760 TFLOP/s of what the rows see).
 // Token 16 h + i of a 32-token part is row 8 (i / 4) + 4 h + i % 4 of the first product, so a lane of half h holds the
 // scores of tokens 16 h .. 16 h + 15 of row lane % 32, which is how the second product takes the weights.
 // The running maximum is moved only when a score exceeds it by 2^8 (the weights stay below 2^8, fp32 sums hold them): the
@@ -32,7 +35,10 @@ constexpr int kThreads = kWaves * 64;
 constexpr int kGroupRows = kWaves * 32;
 constexpr int kRing = 4;  // tiles in LDS: two are multiplied between barriers, two are filled
 constexpr int kMaxPieces = 16;
-constexpr int kMaxMaskedPieces = 64;  // of a masked call: a tree's few rows may stand behind a long cache
+// Of a masked call with so few (row tile, kv head)s that 16 pieces of each leave CUs idle, as a drafted tree behind a long cache
+// (64 drafted tokens of 16 heads of 256 behind 32000: 160 us with 16 pieces, 77 with 64, where each of 256 workgroups multiplies for
+// 35 us and then writes its partial results, 67 MB together, that the second kernel reads again: 13 and 17 us).
+constexpr int kMaxMaskedPieces = 64;
 constexpr int kCus = 256;
 constexpr int64_t kPartialBytes = 256 << 20;  // for partial results, at most
 constexpr float kSlack = 8.0f;  // log2: how far a score may lie above the running maximum
@@ -291,8 +297,7 @@ struct Work {
     int b, row0, piece, pieces, t0, t1;
 };
 constexpr int kClasses = 64;
-template <bool MASK>
-constexpr int kLeast = MASK ? 2 : 4;  // tiles that are worth a piece
+constexpr int kLeast = 4;  // tiles that are worth a piece
 struct PlanLds {
     uint32_t classes[kClasses];
     uint32_t sums[kWaves];
@@ -333,7 +338,7 @@ __device__ __forceinline__ bool find_work(const RowsArgs& a, PlanLds& lds, Work&
     __syncthreads();
     total = 0;
     for (int i = 0; i < kWaves; i++) total += lds.sums[i];
-    int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast<MASK>);
+    int each = max(static_cast<int>((static_cast<uint64_t>(total) * a.c.kv_heads + kCus - 1) / kCus), kLeast);
     if (a.pieces > 1 && !a.few_tiles) {
         each += each / 2;  // more than a CU's share alone, see rows_plan
     } else if (a.pieces > 1) {
@@ -531,7 +536,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     if (half == 0) a.partial_ml[slot] = make_float2(m, l);
 }
 
-// Adds up the pieces of the row tiles that were cut: a wavefront takes four rows, so that a row's chain of loads is shared
+// Adds up the pieces of the row tiles that were cut, up to kMaxPieces of them: a wavefront takes four rows, so that a row's chain of loads is shared
 // (one row each: 21 us for a prompt of 4096 tokens, of which it adds up half, 12 us for the five ragged ones of up to 300;
 // four: 15 and 7). blockIdx: (16 rows, kv head), sequence.
 constexpr int kMergeWaves = 4, kWaveRows = 4, kMergeRows = kMergeWaves * kWaveRows;
@@ -664,8 +669,8 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
         10 * items >= 9 * ((items + kCus - 1) / kCus * kCus))
         return {row_tiles, 1, items, true};
     if (!few_tiles && (b->seqs == 1 || most < kLong || room < 4)) return {row_tiles, 1, items, false};
-    const int64_t least = mask ? kLeast<true> : kLeast<false>, limit = mask && items < kCus / kMaxPieces ? kMaxMaskedPieces : kMaxPieces;
-    const int64_t pieces = std::max<int64_t>(1, std::min({limit, (most + least - 1) / least, room}));
+    const int64_t limit = mask && items < kCus / kMaxPieces ? kMaxMaskedPieces : kMaxPieces;
+    const int64_t pieces = std::max<int64_t>(1, std::min({limit, (most + kLeast - 1) / kLeast, room}));
     // the pieces of n tiles are less than n / each + 1, those of all (row tile, kv head)s less than kCus + items
     return {row_tiles, pieces, pieces == 1 ? items : std::min(items * pieces, items + kCus), few_tiles};
 }

@@ -94,7 +94,10 @@ constexpr int kKeepGroups = 4;  // of V also not more than come from so many gro
 // there what its dimension's next 16 tokens are, and writes them with the bytes around them (moving byte by byte, every line would
 // be asked for once a token, on both sides).
 // Bound by latency: a token's source (offset, row number, page, scale: a chain of four loads) is looked up once a chunk, by as many
-// threads as it has tokens, and a page of one chunk is read once.
+// threads as it has tokens, and a page of one chunk is read once. 5 of 16 tokens of one sequence, 10 layers of 2 heads of 256: 5.0 us
+// in a graph; up to 12 of 64 of each of 64 sequences: 20 us for 8.3 MB that move, of which V's make 28 MB read and 14 written, since a
+// dimension's next 64 tokens are all that lies side by side (with every byte moved for itself, its source looked up for it and older
+// bytes rescaled one by one: 47 us).
 template <int TYPE, int D>
 __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t layer_bytes, int64_t layer_blocks, KvSeqs s,
                                                           const int32_t* __restrict__ start, const int32_t* __restrict__ keep) {
