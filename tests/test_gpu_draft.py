@@ -364,6 +364,20 @@ def test_keep(hip, dtype, dim, page, counts, starts, kept):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("dim,page,count,start,every", [(256, 256, 400, 37, 3), (64, 1024, 1500, 900, 5), (128, 512, 700, 500, 17), (256, 16, 150, 9, 1)])
+def test_keep_many(hip, dtype, dim, page, count, start, every):
+    """More tokens of a page than are held at a time, from few or many groups of 16: pages whose scale grows, and that do not."""
+    g, rng = gen(dim + page + 51), random.Random(every)
+    lengths = (start + count, start + count // 2)
+    need = sum(-(-n // page) for n in lengths)
+    pages = random_pages(hip, g, 1, need + 1, 2, page, dim, dtype)
+    pages.k_scale.mul_(torch.pow(2.0, torch.randint(-4, 5, pages.k_scale.shape, generator=g)).to(DEV))
+    table = table_of(g, lengths, page, need + 1)
+    kept = [sorted(rng.sample(range(n), max(n // every - 1, 1))) for n in (count, count // 2)]
+    check_keep(hip, pages, table, i32([start] * 2), i32([j for k in kept for j in k]), cu_of([len(k) for k in kept]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 def test_keep_moves_bytes_inside_a_page(hip, dtype):
     """What stays in its page keeps its bytes, whatever its scale, one of more bits than bf16's among them; nothing else changes."""
     g = gen(51)
@@ -478,6 +492,21 @@ def test_norm_rope(hip, dtype, tokens, heads, kv_heads, dim, half, sections, int
     assert none is None and iq is q and torch.equal(q, rq)  # in place, alone: the same bits
 
 
+@pytest.mark.parametrize("tokens,heads,kv_heads,dim,half", [(2051, 3, 1, 256, 32), (4099, 1, 2, 64, 32), (2049, 2, 1, 512, 64)])
+def test_norm_rope_many_tokens(hip, tokens, heads, kv_heads, dim, half):
+    """More tokens than a workgroup each holds at once, an odd number of them; against the oracle, and the same bits as in smaller calls."""
+    g = gen(tokens)
+    q, k = (torch.randn(tokens, h, dim, generator=g).to(torch.bfloat16).to(DEV) for h in (heads, kv_heads))
+    w = [torch.randn(dim, generator=g).to(DEV) for _ in range(2)]
+    p, f = torch.arange(tokens, device=DEV) * 7, torch.pow(1e6, -torch.arange(half, dtype=torch.float64, device=DEV) / half)
+    rq, rk = hip.norm_rope(q, k, p, f, *w)
+    check_norm_rope(q, rq, w[0], 1e-6, True, p[None], f, (half,), True)
+    check_norm_rope(k, rk, w[1], 1e-6, True, p[None], f, (half,), True)
+    for part in (slice(0, 1), slice(1000, 2000), slice(tokens - 3, tokens)):
+        sq, sk = hip.norm_rope(q[part], k[part], p[part], f, *w)
+        assert torch.equal(sq, rq[part]) and torch.equal(sk, rk[part])
+
+
 def test_norm_rope_small_and_large_values(hip):
     """Rows of zeros, of values whose squares leave eps nothing to do, and of values that are nothing beside it; NaN and infinities
     stay in their head."""
@@ -508,6 +537,32 @@ def test_norm_rope_refusals(hip):
     for bad in (q.half(), q.cpu(), q[..., :8]):
         with pytest.raises(ValueError):
             hip.norm_rope(bad, None, p, f)
+
+
+# -- workspaces -------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("count,window", [(1, 900), (8, None), (64, None), (300, 500)])
+def test_masked_workspaces(hip, count, window):
+    """A workspace of the size that is asked for, whatever it holds, gives the bits of one from the allocator; a smaller one is refused."""
+    import ctypes
+    g, rng = gen(72), random.Random(72)
+    pages = random_pages(hip, g, 1, 150, 2, 64, 128, torch.int8)
+    table = table_of(g, (4000, 3000), 64, 150)
+    length, cu = i32([4000, 3000]), cu_of((count, count))
+    q = torch.randn(2 * count, 8, 128, generator=g).to(torch.bfloat16).to(DEV)
+    kw = dict(window=window, sinks=3) if window else dict(tree=hip.kv_tree(i32(random_tree(rng, count) * 2), length - count, cu, max_count=count)[0])
+    want = hip.kv_attend(pages, 0, q, table, length, cu, max_count=count, **kw)
+    tree = kw.get("tree")
+    mask = hip.WlKvMask(tree.data_ptr() if tree is not None else None, tree.shape[1] if tree is not None else 0, window or 0, 3 if window else 0)
+    batch = hip.WlKvBatch(table.data_ptr(), cu.data_ptr(), table.stride(0), 2 * count, 2, table.shape[1], count, 0)
+    need = hip.library().wl_kv_attend_masked_workspace_bytes(pages.ref, 8, ctypes.byref(batch), table.shape[1] * 64, ctypes.byref(mask))
+    assert need > 0
+    space = torch.full((need + 64,), 255, dtype=torch.uint8, device=DEV)
+    assert torch.equal(want, hip.kv_attend(pages, 0, q, table, length, cu, max_count=count, workspace=space[:need], **kw))
+    assert (space[need:] == 255).all()
+    with pytest.raises(ValueError):
+        hip.kv_attend(pages, 0, q, table, length, cu, max_count=count, workspace=space[:need - 16], **kw)
 
 
 # -- captured ---------------------------------------------------------------------------------------------------------
