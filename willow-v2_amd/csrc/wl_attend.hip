@@ -251,6 +251,7 @@ template <int D>
 struct JoinLds {
     float o[kFewWaves][kRows][D + 4];
     float m[kFewWaves][kRows], l[kFewWaves][kRows];
+    float2 row[kRows];  // maximum and sum over the wavefronts
 };
 
 // The workgroup's wavefronts over tiles [t0, t1) of the rows; the rows are finished into out, or, with
@@ -282,25 +283,23 @@ __device__ __forceinline__ void attend_rows(const FewArgs& a, JoinLds<D>& lds, i
         for (int i = 0; i < D / 16; i++)
             *reinterpret_cast<f32x4*>(&lds.o[wave][m16][16 * i + 4 * g]) = r.o[i] * f;
     }
+    if (wave == 0 && lane < kRows) {
+        float l = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kFewWaves; w++) l += lds.l[w][lane] * exp2_fast(lds.m[w][lane] - safe);
+        lds.row[lane] = make_float2(top, l);
+    }
     __syncthreads();
+    if (slot >= 0 && static_cast<int>(threadIdx.x) < rows) a.partial_ml[slot * a.rows + threadIdx.x] = lds.row[threadIdx.x];
     for (int i = threadIdx.x; i < rows * (D / 4); i += kFewWaves * 64) {
         const int row = i / (D / 4), d = i % (D / 4) * 4;
-        float m = lds.m[0][row];
-#pragma unroll
-        for (int w = 1; w < kFewWaves; w++) m = fmaxf(m, lds.m[w][row]);
-        const float ms = m == -__builtin_inff() ? 0.0f : m;
-        float l = 0.0f;
         f32x4 o = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int w = 0; w < kFewWaves; w++) {
-            l += lds.l[w][row] * exp2_fast(lds.m[w][row] - ms);
-            o += *reinterpret_cast<const f32x4*>(&lds.o[w][row][d]);
-        }
+        for (int w = 0; w < kFewWaves; w++) o += *reinterpret_cast<const f32x4*>(&lds.o[w][row][d]);
         if (slot >= 0) {
             *reinterpret_cast<f32x4*>(a.partial + static_cast<int64_t>(slot * a.rows + row) * D + d) = o;
-            if (d == 0) a.partial_ml[slot * a.rows + row] = make_float2(m, l);
         } else {
-            const float inv = l == 0.0f ? 0.0f : 1.0f / l;
+            const float l = lds.row[row].y, inv = l == 0.0f ? 0.0f : 1.0f / l;
             const int token = (row0 + row) / a.group, h = head * a.group + (row0 + row) % a.group;
             *reinterpret_cast<uint2*>(a.out + (static_cast<int64_t>(at + token) * a.q_heads + h) * D + d) =
                 make_uint2(pack_bf16(o[0] * inv, o[1] * inv), pack_bf16(o[2] * inv, o[3] * inv));
@@ -396,7 +395,9 @@ __global__ __launch_bounds__(kFewWaves * 64, 2) void k_attend_few(FewArgs a) {
             const uint32_t blocks = blocks_of<MASK>(a, seq), block = __builtin_amdgcn_readfirstlane((at - before) / length),
                            t0 = at - before - block * length;
             // a head's blocks one after the other: they read the same keys and values
-            const uint32_t each = blocks / a.c.kv_heads, head = MASK ? block / each : block, row0 = MASK ? block % each * kRows : 0;
+            const bool some = MASK && a.blocks > 1;
+            const uint32_t each = some ? max((seq.n * a.group + kRows - 1) / kRows, 1) : 1, head = some ? block / each : block,
+                           row0 = (block - head * each) * kRows;
             const uint32_t t1 = min(t0 + (end - at), length), stop = min(t1, tiles);
             const bool whole = t0 == 0 && stop == tiles;
             if (t0 < stop) {
