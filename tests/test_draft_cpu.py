@@ -8,6 +8,7 @@ import pytest
 import torch
 
 from engines.qwen36 import Rotary
+from engines.qwen36.attention_hip import head_norm
 from gguf import hip
 from gguf.hbm_cache import HBMKVCache, PageBook
 from oracle import kv_ref
@@ -307,3 +308,16 @@ def test_oracle_keep_and_norm():
 
 def test_rotary_has_normed():
     assert callable(Rotary(64, device="cpu").normed)
+
+
+def test_a_rotary_of_its_own_turns_behind_the_norms():
+    class Reversed(Rotary):
+        def __call__(self, q, k, positions):
+            return q.flip(-1), k.flip(-1)
+
+    gen = torch.Generator().manual_seed(5)
+    q, k = (torch.randn(3, n, 64, generator=gen).bfloat16() for n in (4, 2))
+    wq, wk = (torch.randn(64, generator=gen) for _ in range(2))
+    got = Reversed(64, device="cpu").normed(q, k, torch.arange(3), wq, wk, 1e-6)
+    for g, x, w in zip(got, (q, k), (wq, wk)):
+        assert torch.equal(g, head_norm(x, w, 1e-6).flip(-1))

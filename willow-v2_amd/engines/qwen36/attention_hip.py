@@ -49,7 +49,10 @@ class Rotary:
         return rope(q, k, positions, self.inv_freq, sections=self.sections, interleaved=self.interleaved, scale=self.scale)
 
     def normed(self, q, k, positions, q_weight, k_weight, eps: float):
-        """The same of queries and keys that are normed first (head_norm), in one pass and rounded once."""
+        """The same of queries and keys that are normed first (head_norm), in one pass and rounded once. A subclass that turns in a way
+        of its own (__call__) gets the norms in front of that."""
+        if type(self).__call__ is not Rotary.__call__:
+            return self(head_norm(q, q_weight, eps), head_norm(k, k_weight, eps), positions)
         q_weight, k_weight = (w.to(q.device) for w in (q_weight, k_weight))
         if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (torch.float32, torch.bfloat16):
             q_weight, k_weight = q_weight.float(), k_weight.float()

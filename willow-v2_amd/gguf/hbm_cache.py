@@ -368,7 +368,8 @@ class HBMKVCache:
 
     def tree(self, step: KVStep, parents: torch.Tensor):
         """The step's tokens as trees of drafts -> (masks for attend, int64 [tokens] positions); kv_tree. parents int32 [tokens] on the
-        GPU, each row's parent among its sequence's rows (-1: a root). For all layers of the step."""
+        GPU, each row's parent among its sequence's rows (-1: a root). For all layers of the step; like any result the tensors
+        are the current stream's, and another has to wait for them."""
         step.check(parents, "parents")
         self._order(False, step)
         return kv_tree(parents, step.start, step.cu, max_count=step.max_count or 1)
