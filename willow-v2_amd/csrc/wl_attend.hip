@@ -9,9 +9,9 @@
 // where this took 34 at that stage. 512 workgroups: 256, 768 and 1024 were 7, 11 and 6% slower. One short sequence is a
 // chain of loads: 777 tokens 12.7 us in a graph, of which the join takes 4.
 // With a window and sinks (MASK) the tiles between them are left out of the line, so the time goes by the window: 64 sequences of up to
-// 16000 tokens in a window of 4096, 130 MB, 33 us and 5 for the join (3.9 TB/s), one token of one in a window of 128 to 4096 9.8 to
-// 14.3 us in a graph, whatever lies before it. A masked call may have several blocks of 16 rows, each of which goes through the tiles
-// for itself: 16 drafted tokens of 16 heads on 2 of 256 behind 776, 8 blocks a head, 13 us and 4 for the join.
+// 16000 tokens in a window of 4096, 130 MB, 33 us and 5 for the join (3.9 TB/s), one token of one in a window of 128 to 4096 8.5 to
+// 13.9 us in a graph, whatever lies before it. A masked call may have several blocks of 16 rows, each of which goes through the tiles
+// for itself: 16 drafted tokens of 16 heads on 2 of 256 behind 776, 8 blocks a head, 12 us and 4 for the join.
 #include <algorithm>
 
 #include "wl_attend.h"
