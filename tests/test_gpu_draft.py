@@ -277,6 +277,40 @@ def test_tree_keeps_out_what_it_hides(hip, dtype, count, group):
     check_masked(hip, pages, 0, q, missing, *args[2:], tree=tree)
 
 
+@pytest.mark.parametrize("dim,page", [(64, 16), (128, 64), (256, 32), (256, 128)])
+@pytest.mark.parametrize("count,group,width", [(3, 4, None), (24, 1, None), (70, 2, None), (30, 8, 300), (130, 4, 300), (300, 1, 300)])
+@pytest.mark.parametrize("window", [None, 400])
+def test_tree_keeps_out_drafts_that_no_row_sees(hip, dim, page, count, group, width, window):
+    """NaN bytes of drafted tokens whose bits no row of their sequence has, as of slots that nobody wrote, reach no row, in the form for
+    few rows and in the one for many (a wide table makes the call look long)."""
+    g, rng = gen(46), random.Random(46)
+    counts, lengths = (count, count // 2 + 1, count), (count + 55, count // 2 + 1, count + 300)
+    need = sum(-(-n // page) for n in lengths)
+    pages = random_pages(hip, g, 1, need, 2, page, dim, torch.float8_e4m3fn)
+    table = table_of(g, lengths, page, need, width and width * 64 // page)
+    words = -(-count // 64)
+    bits = torch.randint(-2 ** 63, 2 ** 63 - 1, (sum(counts), words), generator=g)
+    hidden, at = [], 0
+    for n in counts:
+        hidden.append(sorted({0, n - 1, n // 2} | {j for j in range(n) if rng.random() < 0.3}) if n > 3 else [n - 1])
+        for j in hidden[-1]:
+            bits[at:at + n, j // 64] &= ~(1 << j % 64) if j % 64 < 63 else 2 ** 63 - 1
+        at += n
+    q = torch.randn(sum(counts), 2 * group, dim, generator=g).to(torch.bfloat16).to(DEV)
+    kw = dict(max_count=count, tree=bits.to(DEV))
+    if window:
+        kw.update(window=window, sinks=3)
+    want = hip.kv_attend(pages, 0, q, table, i32(lengths), cu_of(counts), **kw)
+    for b, n in enumerate(counts):
+        for j in hidden[b]:
+            pos = lengths[b] - n + j
+            p, t = int(table[b, pos // page]), pos % page
+            pages.k.view(torch.uint8)[0, p, :, t], pages.v.view(torch.uint8)[0, p, :, :, t] = 0x7F, 0xFF if j % 2 else 0x7F
+    assert torch.equal(want, hip.kv_attend(pages, 0, q, table, i32(lengths), cu_of(counts), **kw))
+    if count <= 70:
+        check_masked(hip, pages, 0, q, table, i32(lengths), cu_of(counts), **kw)
+
+
 def test_tree_of_one_chain_is_causal(hip):
     g = gen(43)
     pages = random_pages(hip, g, 1, 20, 2, 64, 256, torch.int8)

@@ -98,6 +98,13 @@ __device__ __forceinline__ uint32_t tree_bits(const AttendArgs& a, Seq seq, int 
     if (bit > 16 && 32 * (word + 1) < seq.n) two |= static_cast<uint64_t>(row[word + 1]) << 32;
     return static_cast<uint32_t>(two >> bit) & low_bits(seq.n - off);
 }
+// The bits of all rows, which are the lanes of a group of 16.
+__device__ __forceinline__ uint32_t any_of_16(uint32_t x) {
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x128, 0xf, 0xf, false);  // row_ror 8, 4, 2, 1
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x124, 0xf, 0xf, false);
+    x |= __builtin_amdgcn_update_dpp(0, x, 0x122, 0xf, 0xf, false);
+    return x | __builtin_amdgcn_update_dpp(0, x, 0x121, 0xf, 0xf, false);
+}
 // Row `token`'s limit. Of the tree's rows only a window asks for it.
 __device__ __forceinline__ int limit_of(const AttendArgs& a, Seq seq, int token) {
     if (token >= seq.n) return 0;

@@ -162,10 +162,11 @@ struct Rows {
         const int first = base + 16 * vgroup();
         // of this lane's 16 tokens, those that count: so many, or these
         const int mine = x.page < 0 ? 0 : min(max(limit - first, 0), 16);
-        uint32_t bits = 0;
+        uint32_t bits = 0, own = 0;
+        const bool in_tree = MASK && a.mask.tree && base + kTile > seq.begin;
         if constexpr (MASK) {
-            const bool in_tree = a.mask.tree && base + kTile > seq.begin;
-            bits = x.page < 0 ? 0 : seen_bits(a, seq, limit, first, length - first, in_tree ? drafted(a, seq, row0, first) : 0);
+            own = in_tree ? drafted(a, seq, row0, first) : 0;
+            bits = x.page < 0 ? 0 : seen_bits(a, seq, limit, first, length - first, own);
         }
         auto counts = [&](int i) { return MASK ? (bits >> i & 1) != 0 : i < mine; };
         float top = m;
@@ -200,10 +201,11 @@ struct Rows {
             p[2 * j + 1] = pack_bf16(e[2], e[3]);
         }
         if constexpr (MASK) {
-            // the same for tokens that no row sees, before the window
+            // the same for tokens that no row sees, before the window and in the tree (where a byte of int8 times 0 is 0)
             const int lowest = window_begin(a, seq, 0);
-            if (base + kTile > length || base < lowest || __any(x.page < 0)) {
-                const uint32_t kept = x.page < 0 ? 0 : low_bits(length - first) & (~low_bits(lowest - first) | low_bits(a.mask.sinks - first));
+            if (base + kTile > length || base < lowest || (TYPE == WL_KV_E4M3 && in_tree) || __any(x.page < 0)) {
+                uint32_t kept = x.page < 0 ? 0 : low_bits(length - first) & (~low_bits(lowest - first) | low_bits(a.mask.sinks - first));
+                if (TYPE == WL_KV_E4M3 && in_tree) kept &= low_bits(seq.begin - first) | any_of_16(own);
                 const uint32_t m0 = bytes_of(kept), m1 = bytes_of(kept >> 4), m2 = bytes_of(kept >> 8), m3 = bytes_of(kept >> 12);
 #pragma unroll
                 for (int i = 0; i < kDims; i++) {

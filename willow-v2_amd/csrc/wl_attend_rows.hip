@@ -130,8 +130,10 @@ struct Stage {
             }
         }
     }
-    // hidden_from, hidden_to: no row sees the tokens between, counted from the sequence's end
-    __device__ __forceinline__ void store(const AttendArgs& a, Lds<D>& lds, int buffer, int hidden_from, int hidden_to) const {
+    // The tile at `base`, of the workgroup's rows from row0 on. hidden_from, hidden_to: no row sees the tokens between, counted from the
+    // sequence's end
+    __device__ __forceinline__ void store(const AttendArgs& a, Lds<D>& lds, int buffer, int base, Seq seq, int row0, int hidden_from,
+                                          int hidden_to) const {
         const int t = k_token(), step = k_chunk(), i = t & 15;
         const int row = 8 * (i >> 2) + 4 * ((t >> 4) & 1) + (i & 3);
         uint4* to = lds.k[buffer][(t >> 5) * S::kSteps + step];
@@ -152,6 +154,18 @@ struct Stage {
             w.y &= byte_mask(n - 4);
             w.z &= byte_mask(n - 8);
             w.w &= byte_mask(n - 12);
+        }
+        // The same for drafted tokens that none of the rows sees; looked up just where there are such bytes, since they are what nobody wrote
+        if constexpr (MASK && TYPE == WL_KV_E4M3) {
+            if (a.mask.tree && base + S::kTokens > seq.begin && (has_nan(w.x) || has_nan(w.y) || has_nan(w.z) || has_nan(w.w))) {
+                const int at = base + 16 * v_part(), last = min((row0 + kGroupRows - 1) / a.group, seq.n - 1);
+                uint32_t kept = low_bits(seq.begin - at);
+                for (int token = row0 / a.group; token <= last; token++) kept |= tree_bits(a, seq, token, at);
+                w.x &= bytes_of(kept);
+                w.y &= bytes_of(kept >> 4);
+                w.z &= bytes_of(kept >> 8);
+                w.w &= bytes_of(kept >> 12);
+            }
         }
         const int d = v_dim(), x = v_part(), slot = ((x & 1) * 32 + (d & 31)) ^ S::v_swizzle(x);
         uint4(*pair)[64] = &lds.v[buffer][((d >> 5) * S::kSubs + (x >> 1)) * 2];
@@ -470,11 +484,11 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
     w.l = 0.0f;
     const bool idle = !__any(there);
 
-    st.store(a, lds, 0, hidden_from, hidden_to);
+    st.store(a, lds, 0, base_of(cut.t0), seq, row0, hidden_from, hidden_to);
     if (cut.t0 + 1 < cut.t1) {
         st.find(a, b, base_of(cut.t0 + 1));
         st.load(a, head, base_of(cut.t0 + 1), seq.length);
-        st.store(a, lds, 1, hidden_from, hidden_to);
+        st.store(a, lds, 1, base_of(cut.t0 + 1), seq, row0, hidden_from, hidden_to);
     }
     // q is here before the loop: were it still on its way, the first product of every round would wait for that round's loads
     __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
@@ -503,7 +517,7 @@ __global__ __launch_bounds__(kThreads, 2) void k_attend_rows(RowsArgs a) {
                 w.template add<MASK>(lds, buffer, u, limit - at);
             }
         }
-        if (t + 2 < cut.t1) st.store(a, lds, (buffer + 2) & (kRing - 1), hidden_from, hidden_to);
+        if (t + 2 < cut.t1) st.store(a, lds, (buffer + 2) & (kRing - 1), base_of(t + 2), seq, row0, hidden_from, hidden_to);
         if (buffer & 1) __syncthreads();
     }
     const float m = w.m, l = other_half(w.l, true);

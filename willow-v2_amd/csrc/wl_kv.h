@@ -41,6 +41,9 @@ __device__ __forceinline__ uint32_t byte_mask(int n) { return n >= 4 ? ~0u : n <
 // All bits of the four bytes whose bits (the lowest four) are set
 __device__ __forceinline__ uint32_t bytes_of(uint32_t bits) { return ((bits & 15u) * 0x00204081u & 0x01010101u) * 0xFFu; }
 
+// Whether one of four e4m3 bytes is a NaN (0x7F or 0xFF)
+__device__ __forceinline__ bool has_nan(uint32_t w) { return ((w & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u; }
+
 // 0 that the compiler takes for a lane's own: an address with it is read by a vector load. A scalar load shares its counter
 // with LDS reads and comes back out of order, so the next LDS operand would wait for it to come from memory.
 __device__ __forceinline__ uint32_t lane_zero() {
