@@ -321,3 +321,18 @@ def test_a_rotary_of_its_own_turns_behind_the_norms():
     got = Reversed(64, device="cpu").normed(q, k, torch.arange(3), wq, wk, 1e-6)
     for g, x, w in zip(got, (q, k), (wq, wk)):
         assert torch.equal(g, head_norm(x, w, 1e-6).flip(-1))
+
+
+@pytest.mark.parametrize("q_shape,k_shape", [((1, 64), (1, 64)), ((1,), (1,)), ((4, 64), (2, 64)), ((), (64,)), ((64,), (2, 64)), ((64,), (64,))])
+def test_norm_weights_of_any_shape(q_shape, k_shape, monkeypatch):
+    """Weights that head_norm takes are taken behind Rotary.normed too; [head_dim] alone in one pass."""
+    gen = torch.Generator().manual_seed(6)
+    q, k = (torch.randn(3, n, 64, generator=gen).bfloat16() for n in (4, 2))
+    wq, wk = (torch.randn(shape, generator=gen) for shape in (q_shape, k_shape))
+    monkeypatch.setattr("engines.qwen36.attention_hip.rope", lambda q, k, *args, **kw: (q.flip(-1), k.flip(-1)))
+    monkeypatch.setattr("engines.qwen36.attention_hip.norm_rope", lambda *args, **kw: "one pass")
+    got = Rotary(64, device="cpu").normed(q, k, torch.arange(3), wq, wk, 1e-6)
+    if q_shape == k_shape == (64,):
+        assert got == "one pass"
+    else:
+        assert all(torch.equal(g, head_norm(x, w, 1e-6).flip(-1)) for g, x, w in zip(got, (q, k), (wq, wk)))

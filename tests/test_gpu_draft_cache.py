@@ -238,3 +238,23 @@ def test_engine_drafts(hip, monkeypatch, gated, norm):
             assert worst(seen["o"], *oracle_attend(cache, 0, step, seen["q"])) > 4  # what no mask would give
             cache.keep(seqs, counts, [path_to(t, c - 1) for t, c in zip(trees, counts)])
             assert [cache.length(s) for s in seqs] == [a + len(path_to(t, c - 1)) for a, t, c in zip(starts, trees, counts)]
+
+
+@pytest.mark.parametrize("shapes", [((1, 64), (1, 64)), ((1,), (1,)), ((8, 64), (2, 64)), ((64,), (1, 64))])
+def test_engine_norm_weights_of_any_shape(hip, shapes):
+    """Norm weights that are not one vector for all heads go through HipAttention: the layer's result is that of the norms in front of
+    the rotary positions."""
+    outs = []
+    for own in (False, True):
+        g = torch.Generator().manual_seed(18)
+        eng, heads, dim = engine(g, True, False, True)
+        p = "model.layers.3.self_attn"
+        for name, shape, n in zip("qk", shapes, (heads, 2)):
+            shape = tuple(n if x == 8 else x for x in shape)
+            eng.weights[f"{p}.{name}_norm.weight"] = (0.3 * torch.randn(shape, generator=g)).to(DEV)
+        if own:  # a rotary that knows nothing of norms
+            inner = eng.rotary
+            eng.rotary = lambda q, k, positions: inner(q, k, positions)
+        step = eng.kv_cache.step([eng.kv_cache.new()], [21])
+        outs.append(eng.hip_attention(bf16(g, 21, 256), 3, 0, step, torch.arange(21, device=DEV).expand(3, -1).contiguous()))
+    assert torch.equal(*outs) and torch.isfinite(outs[0].float()).all()

@@ -50,8 +50,8 @@ class Rotary:
 
     def normed(self, q, k, positions, q_weight, k_weight, eps: float):
         """The same of queries and keys that are normed first (head_norm), in one pass and rounded once. A subclass that turns in a way
-        of its own (__call__) gets the norms in front of that."""
-        if type(self).__call__ is not Rotary.__call__:
+        of its own (__call__) gets the norms in front of that, and so do weights other than [head_dim] (of each head, say)."""
+        if type(self).__call__ is not Rotary.__call__ or not q_weight.shape == k_weight.shape == q.shape[-1:]:
             return self(head_norm(q, q_weight, eps), head_norm(k, k_weight, eps), positions)
         q_weight, k_weight = (w.to(q.device) for w in (q_weight, k_weight))
         if q_weight.dtype != k_weight.dtype or q_weight.dtype not in (torch.float32, torch.bfloat16):
