@@ -7,7 +7,7 @@ import random
 import pytest
 import torch
 
-from engines.qwen36 import Rotary
+from engines.qwen36 import HipAttention, Rotary
 from engines.qwen36.attention_hip import head_norm
 from gguf import hip
 from gguf.hbm_cache import HBMKVCache, PageBook
@@ -336,3 +336,34 @@ def test_norm_weights_of_any_shape(q_shape, k_shape, monkeypatch):
         assert got == "one pass"
     else:
         assert all(torch.equal(g, head_norm(x, w, 1e-6).flip(-1)) for g, x, w in zip(got, (q, k), (wq, wk)))
+
+
+def test_a_rotary_that_passes_attributes_on_turns_behind_the_norms(monkeypatch):
+    """A wrapper that looks every other attribute up in a Rotary has a `normed` by that, which knows nothing of the wrapper's rotation."""
+    class Shifted:
+        def __init__(self, inner):
+            self.inner = inner
+
+        def __getattr__(self, name):
+            return getattr(self.inner, name)
+
+        def __call__(self, q, k, positions):
+            return q + positions.sum(), k - positions.sum()
+
+    gen = torch.Generator().manual_seed(7)
+    p, dim = "layers.0.self_attn", 64
+    weights = {f"{p}.{n}_proj.weight": torch.randn(rows, 32, generator=gen).bfloat16() for n, rows in (("q", 4 * dim), ("k", 2 * dim), ("v", 2 * dim))}
+    weights[f"{p}.o_proj.weight"] = torch.randn(32, 4 * dim, generator=gen).bfloat16()
+    weights.update({f"{p}.{n}_norm.weight": torch.randn(dim, generator=gen) for n in "qk"})
+    eng = HipAttention()
+    eng.prefix, eng.weights, eng.rotary = "", weights, Shifted(Rotary(dim, device="cpu"))
+    cache = eng.kv_cache = HBMKVCache(1, 4, 2, dim, 16, device="cpu")
+    seen = {}
+    monkeypatch.setattr(cache, "append", lambda layer, step, k, v: seen.update(k=k))
+    monkeypatch.setattr(cache, "attend", lambda layer, step, q, **kw: seen.setdefault("q", q))
+    monkeypatch.setattr("engines.qwen36.attention_hip.norm_rope", lambda q, k, *args, **kw: (q, k))
+    x, positions = torch.randn(3, 32, generator=gen).bfloat16(), torch.tensor([[1, 2, 3]])
+    eng.hip_attention(x, 0, 0, cache.step([cache.new()], [3]), positions)
+    for name, heads, sign in (("q", 4, 1), ("k", 2, -1)):
+        y = torch.nn.functional.linear(x, weights[f"{p}.{name}_proj.weight"]).view(3, heads, dim)
+        assert torch.equal(seen[name], head_norm(y, weights[f"{p}.{name}_norm.weight"], 1e-6) + sign * 6)

@@ -103,7 +103,8 @@ class HipAttention:
             raise ValueError(f"{p}.q_proj: {wide.shape[1]} rows for {heads} heads of {dim}")
         k, v = (project(n, kv_heads).view(-1, kv_heads, dim) for n in ("k_proj", "v_proj"))
         q_norm, k_norm = (self.weights.get(f"{p}.{n}_norm.weight") for n in "qk")
-        if q_norm is not None and k_norm is not None and hasattr(self.rotary, "normed"):
+        # of its class: a wrapper that passes attributes on to a Rotary has a rotation of its own
+        if q_norm is not None and k_norm is not None and hasattr(type(self.rotary), "normed"):
             q, k = self.rotary.normed(q, k, positions, q_norm, k_norm, self.attention_eps)
         else:
             q, k = head_norm(q, q_norm, self.attention_eps), head_norm(k, k_norm, self.attention_eps)
