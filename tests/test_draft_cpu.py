@@ -367,3 +367,22 @@ def test_a_rotary_that_passes_attributes_on_turns_behind_the_norms(monkeypatch):
     for name, heads, sign in (("q", 4, 1), ("k", 2, -1)):
         y = torch.nn.functional.linear(x, weights[f"{p}.{name}_proj.weight"]).view(3, heads, dim)
         assert torch.equal(seen[name], head_norm(y, weights[f"{p}.{name}_norm.weight"], 1e-6) + sign * 6)
+
+
+def test_book_moves_past_a_shared_page():
+    """A page that another sequence has too, in which the first kept tokens just stay, is left out of what moves."""
+    book = PageBook(10, 16)
+    a = book.new()
+    book.grow([a], [8])
+    book.grow([a], [40])  # drafts, from the middle of page 0 to the end of page 2
+    f = book.fork(a)
+    book.truncate(f, 16)  # has page 0 alone
+    stay = list(range(8))
+    assert book.moves([a], [40], [stay + [10, 11, 39]]) == [([1, 2], 0, [2, 3, 31])]
+    assert book.moves([a], [40], [stay + [8, 11, 39]]) == [([1, 2], 0, [0, 3, 31])]
+    assert book.moves([a], [40], [list(range(24)) + [30]]) == [([2], 0, [6])]
+    for kept in ([0, 2], [1], stay[:7] + [8]):
+        with pytest.raises(ValueError, match="another"):
+            book.moves([a], [40], [kept])
+    book.truncate(f, 0)
+    assert book.moves([a], [40], [[0, 2]]) == [([0, 1, 2], 8, [0, 2])]

@@ -258,3 +258,29 @@ def test_engine_norm_weights_of_any_shape(hip, shapes):
         step = eng.kv_cache.step([eng.kv_cache.new()], [21])
         outs.append(eng.hip_attention(bf16(g, 21, 256), 3, 0, step, torch.arange(21, device=DEV).expand(3, -1).contiguous()))
     assert torch.equal(*outs) and torch.isfinite(outs[0].float()).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.int8, torch.float8_e4m3fn])
+def test_keep_past_a_shared_page(hip, dtype):
+    """A fork made behind the draft that shares just a page whose kept tokens stay in their places: keep() moves the others, and the
+    fork's tokens stay as they are."""
+    g = torch.Generator().manual_seed(6)
+    cache = HBMKVCache(2, 20, 2, 64, 16, dtype=dtype)
+    a = cache.new()
+    for n in (8, 40):
+        step = cache.step([a], [n])
+        for layer in range(2):
+            cache.append(layer, step, bf16(g, n, 2, 64), bf16(g, n, 2, 64))
+    f = cache.fork(a)
+    cache.truncate(f, 16)
+    drafted = [[x.clone() for x, _ in stored(cache, layer, a)] for layer in range(2)]
+    kept = list(range(8)) + [10, 11, 39]
+    cache.keep([a], [40], [kept])
+    assert cache.length(a) == 19 and cache.length(f) == 16
+    for layer in range(2):
+        for (x, step_size), (y, _), was in zip(stored(cache, layer, a), stored(cache, layer, f), drafted[layer]):
+            assert torch.equal(x[:16], was[:16]) and torch.equal(y, was[:16])
+            want = was[[8 + i for i in kept[8:]]]
+            # rounded once, to half a step, of a quotient in fp32
+            tol = 0.501 * step_size[16:] if dtype == torch.int8 else 1.001 * (2.0 ** -4 * want.abs() + 2.0 ** -10 * step_size[16:])
+            assert ((x[16:] - want).abs() <= tol).all()

@@ -137,7 +137,8 @@ class PageBook:
 
     def moves(self, seqs, counts, kept):
         """What keeping just the tokens at kept[i] of the last counts[i] of seqs[i] moves, with nothing changed -> a list of (pages
-        from the one on that the first of the last tokens is in, where in it, kept) of the sequences that it moves tokens of.
+        from the first one on that a token moves into, where in it the last tokens begin, kept from there on) of the sequences that
+        it moves tokens of.
         Raises KeyError or ValueError for unknown or repeated sequences, counts beyond their lengths, tokens out of range or out
         of order, and where tokens would move into a page that another sequence has too."""
         if not len(seqs) == len(counts) == len(kept) or len(set(seqs)) != len(seqs):
@@ -154,6 +155,9 @@ class PageBook:
             if still == len(keep):
                 continue
             first, stop = length - n, length - n + len(keep)
+            # pages in front of the first one that a token moves into are left out
+            stay = max((first + still) // self.page_tokens * self.page_tokens - first, 0)
+            first, keep = first + stay, [j - stay for j in keep[stay:]]
             for page in pages[first // self.page_tokens:-(-stop // self.page_tokens)]:
                 if self.uses[page] != 1:
                     raise ValueError(f"sequence {seq}: tokens would move into page {page}, which another sequence has too")
