@@ -284,3 +284,18 @@ def test_keep_past_a_shared_page(hip, dtype):
             # rounded once, to half a step, of a quotient in fp32
             tol = 0.501 * step_size[16:] if dtype == torch.int8 else 1.001 * (2.0 ** -4 * want.abs() + 2.0 ** -10 * step_size[16:])
             assert ((x[16:] - want).abs() <= tol).all()
+
+
+def test_what_is_refused_under_capture_is_named(hip):
+    cache = HBMKVCache(1, 4, 2, 64, 16)
+    a = cache.new()
+    cache.step([a], [10])
+    torch.cuda.synchronize()
+    graph, x = torch.cuda.CUDAGraph(), torch.zeros(4, device=DEV)
+    with torch.cuda.graph(graph):
+        x.add_(1)
+        for name, call in (("step", lambda: cache.step([a], [1])), ("compact", cache.compact), ("keep", lambda: cache.keep([a], [5], [[3]]))):
+            with pytest.raises(RuntimeError, match=rf"{name}\(\).* cannot be captured"):
+                call()
+    torch.cuda.synchronize()
+    assert cache.length(a) == 10

@@ -283,7 +283,7 @@ class HBMKVCache:
         if self.pages.index >= 0:
             with torch.cuda.device(self.pages.index):
                 if torch.cuda.is_current_stream_capturing():
-                    raise RuntimeError("a cache's step(), refresh() and compact() cannot be captured into a graph")
+                    raise RuntimeError("a cache's step(), refresh(), compact() and keep() cannot be captured into a graph")
 
     @contextlib.contextmanager
     def _given_back(self, seqs, counts):
