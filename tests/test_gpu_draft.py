@@ -559,6 +559,24 @@ def test_norm_rope_small_and_large_values(hip):
     assert torch.isfinite(got[4, 1].float()).all() and torch.isfinite(got[5, 0].float()).all()
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_norm_rope_of_one_head_knows_no_other(hip, dtype, dim):
+    """A head's bits are those of a call of its own, whatever stands beside it: zeros without eps, values whose squares all but vanish."""
+    g = gen(62)
+    x = torch.randn(40, 3, dim, generator=g)
+    x[:20, 1] *= 1e-17
+    x[20:, 2] = 0
+    q = x.to(dtype).to(DEV)
+    w, f, p = torch.randn(dim, generator=g).to(DEV), torch.ones(16, dtype=torch.float64, device=DEV), torch.arange(40, device=DEV)
+    for eps in (0.0, 1e-32, 1e-6):
+        got, _ = hip.norm_rope(q, None, p, f, w, eps=eps)
+        for i in range(40):
+            for h in range(3):
+                alone, _ = hip.norm_rope(q[i:i + 1, h:h + 1], None, p[i:i + 1], f, w, eps=eps)
+                assert torch.equal(alone[0, 0].view(torch.uint8), got[i, h].view(torch.uint8)), (eps, i, h)
+
+
 def test_norm_rope_refusals(hip):
     q = torch.zeros(2, 1, 64, device=DEV)
     f, p = torch.ones(8, dtype=torch.float64, device=DEV), torch.zeros(2, dtype=torch.int64, device=DEV)

@@ -364,7 +364,7 @@ __global__ __launch_bounds__(kRopeThreads) void k_norm_rope_lanes(RopeArgs a, No
         for (int e = 0; e < V; e++) sum = __builtin_fmaf(x[e], x[e], sum);
         const float mean = sum_over<LANES>(sum) * (1.0f / D) + n.eps;
         float inv = __builtin_amdgcn_rsqf(mean);
-        if (__any(!(mean > 1.0e-30f))) inv = 1.0f / sqrtf(mean);
+        if (__any(!(mean > 1.0e-30f))) inv = mean > 1.0e-30f ? inv : 1.0f / sqrtf(mean);  // each head by its own mean alone
 #pragma unroll
         for (int e = 0; e < V; e++) z[e] = inv * __builtin_fmaf(x[e], fa[at + e], y[e] * fb[at + e]);
         *reinterpret_cast<uint4*>(out + unit * V) = pack<T>(z);
