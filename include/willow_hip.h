@@ -340,7 +340,7 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
  * tree != NULL: the call's rows are a sequence's drafted tokens, and of these a row sees those whose bit is set: bit j % 64 of
  * word tree[row * tree_stride + j / 64] for the sequence's own row j (bits of rows that it does not have are ignored). All tokens
  * before the sequence's rows count as before, and its position (which the window starts from) is that of its first row plus the
- * number of drafted tokens that it sees, less one (wl_kv_tree makes these words). A window that begins inside a tree is refused
+ * number of drafted tokens that it sees, less one where it sees any (wl_kv_tree makes these words). A window that begins inside a tree is refused
  * (window < max_count). */
 typedef struct WlKvMask {
     const uint64_t* tree; /* or NULL; 8-byte aligned */
@@ -360,7 +360,8 @@ int wl_kv_attend_masked(const WlKvCache* cache, int layer, const uint16_t* q, in
 /* A tree of drafted tokens as wl_kv_attend_masked takes it. parents[row]: the row's parent among its sequence's rows, before it
  * (anything else: the row is a root, behind the last token before the draft). tree[row][words]: the row's ancestors' bits and its
  * own (words >= max_count / 64 rounded up); positions[row] = start[b] + how many ancestors it has. Rows that belong to no
- * sequence get no bits and position 0. batch: cu, tokens, seqs and max_count are read; table may be NULL. */
+ * sequence get no bits and position 0. batch: cu (which must not decrease), tokens, seqs and max_count are read; table may be
+ * NULL. Meant for drafts: with more than 64 rows a row walks its ancestors one by one. */
 int wl_kv_tree(const WlKvBatch* batch, const int32_t* parents, const int32_t* start, uint64_t* tree, int64_t words,
                int64_t* positions, void* stream);
 

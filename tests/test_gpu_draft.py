@@ -199,6 +199,30 @@ def test_tree_masks_out_of_range(hip, cu):
         assert torch.equal(tree.cpu(), want) and torch.equal(positions.cpu(), at)
 
 
+@pytest.mark.parametrize("cu,known", [((0, 9, 4), (0, 4)), ((6, 2, 3), (0, 0)), ((0, 70, 10), (0, 10)), ((3, 2 ** 31 - 1, -5), (0, 0))])
+def test_tree_masks_of_a_cu_that_decreases(hip, cu, known):
+    """cu must not decrease. Where it does all the same: rows that one part alone has a say in are right, those behind every sequence
+    zeros, and nothing is written outside."""
+    import ctypes
+    n, words, guard = 80, 2, 64
+    parents = [-1, 0, 1, -1, 0, 1, 1, 0, 2, 3] * 8
+    space = torch.full((2 * guard + n * words,), 0x5A5A5A5A, dtype=torch.int64, device=DEV)
+    at = torch.full((2 * guard + n,), 0x5A5A5A5A, dtype=torch.int64, device=DEV)
+    where, starts, up = i32(cu), i32([100, 200]), i32(parents)
+    batch = hip.WlKvBatch(None, where.data_ptr(), 1, n, 2, 1, n, 0)
+    assert hip.library().wl_kv_tree(ctypes.byref(batch), up.data_ptr(), starts.data_ptr(), space[guard:].data_ptr(), words,
+                                    at[guard:].data_ptr(), torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    for t, size in ((space, n * words), (at, n)):
+        assert (t[:guard] == 0x5A5A5A5A).all() and (t[guard + size:] == 0x5A5A5A5A).all()
+    tree, positions = space[guard:guard + n * words].view(n, words).cpu(), at[guard:guard + n].cpu()
+    want, places = kv_ref.tree(parents, [100, 200], cu, words)
+    rows = slice(*known)
+    assert torch.equal(tree[rows], want[rows]) and torch.equal(positions[rows], places[rows])
+    behind = min(max(max(cu), 0), n)
+    assert not tree[behind:].any() and not positions[behind:].any()
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("heads,kv_heads,dim,page", SHAPES)
 @pytest.mark.parametrize("counts,starts", [((1,), (0,)), ((2, 1, 2), (63, 0, 300)), ((5, 16, 1), (0, 100, 64)), ((17, 0, 33), (5, 9, 130)),

@@ -234,8 +234,9 @@ def kv_tree(parents: torch.Tensor, start: torch.Tensor, cu: torch.Tensor, max_co
     ancestors and itself) and int64 [tokens] positions, start[b] plus the number of a row's ancestors. parents: int32 [tokens], each
     row's parent among its sequence's rows cu[b] .. cu[b + 1], counted from 0, and before the row itself; anything else (-1) is a
     root, behind the last token before the draft. start, cu int32 [seqs], [seqs + 1]; max_count: the most rows any sequence has
-    (words = max_count / 64 rounded up; rows beyond it are dropped; default: all rows). Rows of no sequence get no bits and
-    position 0. Once a step: every layer takes the same masks."""
+    (words = max_count / 64 rounded up; rows beyond it are dropped; default: all rows); cu must not decrease (rows that two sequences
+    then claim hold what either writes). Rows of no sequence get no bits and position 0. Once a step: every layer takes the same
+    masks. Meant for drafts: the time grows with a sequence's rows times their depth."""
     index = parents.get_device() if isinstance(parents, torch.Tensor) else -1
     for t, name, dim in ((parents, "parents", "tokens"), (start, "start", "sequences"), (cu, "cu", "sequences + 1")):
         if not (isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.get_device() == index and t.dim() == 1 and t.is_contiguous()):
