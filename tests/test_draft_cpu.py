@@ -76,6 +76,20 @@ def test_bad_masks():
     assert masked(batch=long, bound=1024, window=1000) == masked(batch=long, bound=1024, ws=FAKE + 4, n=1 << 30, window=1000) == -6
 
 
+@pytest.mark.parametrize("window,before,heads,cut", [
+    (1024, 4096, 16, False), (1024, 0, 16, False), (3072, 0, 16, False), (3072, 1024, 16, False), (3584, 0, 16, True), (3840, 0, 16, True),
+    (3840, 1024, 16, False), (3840, 10 ** 6, 16, False), (3840, 0, 32, False)])
+def test_windowed_prompts_that_are_cut(window, before, heads, cut):
+    """4096 tokens on two heads are one round of row tiles with 16 query heads: they are cut where the first rows' windows are so far from
+    full that the last row tile would run on alone."""
+    cache = cache_struct(kv_heads=2, head_dim=256, page_tokens=64, pages=1 << 20)
+    width = -(-(4096 + before) // 64)
+    batch = batch_struct(tokens=4096, max_count=4096, seqs=1, table_width=width, table_stride=width)
+    need = hip.library().wl_kv_attend_masked_workspace_bytes(ctypes.byref(cache), heads, ctypes.byref(batch), 4096 + before,
+                                                             ctypes.byref(hip.WlKvMask(None, 0, window, 4)))
+    assert (need > 0) == cut
+
+
 def test_bad_trees():
     assert tree(parents=None) == tree(start=None) == tree(out=None) == tree(positions=None) == tree(batch_struct(cu=None)) == -3
     assert tree(parents=FAKE + 2) == tree(start=FAKE + 2) == tree(out=FAKE + 4) == tree(positions=FAKE + 4) == -4

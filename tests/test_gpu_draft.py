@@ -140,6 +140,20 @@ def test_window_prompts(hip, heads, kv_heads, dim, counts, lengths, window, sink
                  window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("window", [3500, 3800])
+def test_windowed_prompt_without_history(hip, window):
+    """A first prompt whose row tiles fill the CUs once, in a window nearly as long: cut into pieces; rows of every part."""
+    g = gen(36)
+    n = 3900
+    pages = random_pages(hip, g, 1, 61, 2, 64, 64, torch.int8)
+    table = table_of(g, (n,), 64, 61)
+    q = torch.randn(n, 16, 64, generator=g).to(torch.bfloat16).to(DEV)
+    rows = [(0, i) for i in (0, 1, 255, 1000, window - 1, window, window + 4, n - 2, n - 1)]
+    args = (q, table, i32([n]), cu_of((n,)))
+    out = check_masked(hip, pages, 0, *args, rows, max_count=n, max_length=n, window=window, sinks=4)
+    assert torch.equal(out, hip.kv_attend(pages, 0, *args, max_count=n, max_length=n, window=window, sinks=4))
+
+
 def test_window_of_everything_is_attention(hip):
     g = gen(35)
     pages = random_pages(hip, g, 1, 20, 2, 32, 128, torch.int8)

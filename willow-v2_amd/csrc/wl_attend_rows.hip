@@ -678,10 +678,18 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
     const bool few_tiles = items < 2 * kCus;
     // With a window the row tiles of one sequence go through as many tiles each, from the window's length on: where they fill the CUs
-    // to nine tenths nothing is cut, and the second kernel (5 us of 102 for 4096 tokens in a window of 1024) is left out.
-    if (mask && longest < max_length && longest < int64_t{b->table_width} * c->page_tokens && b->seqs == 1 && few_tiles &&
-        10 * items >= 9 * ((items + kCus - 1) / kCus * kCus))
-        return {row_tiles, 1, items, true};
+    // to nine tenths nothing is cut, and the second kernel (5 us of 102 for 4096 tokens in a window of 1024) is left out. With fewer tokens
+    // than a window before them the first rows see less, and the longest row tile may be more than a CU's share and the three quarters of it by which
+    // the device lets a piece grow, where there is one round of row tiles: then they are cut (4096 tokens of 16 on 2 heads of 256 with nothing before, in
+    // a window of 3840: 225 us uncut, 195 cut; of 3584, where the two are nearly equal, 212 and 196, and 8192 of 8 on one of 64 in 7168 188 and
+    // 194; of 3072 186 and 193; two rounds, of 7680 tokens, in a window of 7200: 479 and 491).
+    const int64_t all = std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens);
+    if (mask && longest < all && b->seqs == 1 && few_tiles && 10 * items >= 9 * ((items + kCus - 1) / kCus * kCus)) {
+        const int64_t window = mask->window, rows_all = b->max_count,  // products below 2^60: one round has at most 2^16 rows
+            missing = mask->tree ? 0 : std::max<int64_t>(window - (all - rows_all), 0);  // of the first row's window
+        if (items > kCus || 7 * items * (2 * window * rows_all - missing * missing) >= 8 * kCus * window * rows_all)
+            return {row_tiles, 1, items, true};
+    }
     if (!few_tiles && (b->seqs == 1 || most < kLong || room < 4)) return {row_tiles, 1, items, false};
     const int64_t limit = mask && items < kCus / kMaxPieces ? kMaxMaskedPieces : kMaxPieces;
     const int64_t pieces = std::max<int64_t>(1, std::min({limit, (most + kLeast - 1) / kLeast, room}));
