@@ -143,6 +143,21 @@ def test_attend_mask_checks(monkeypatch):
     assert len(got) == 2
 
 
+def test_a_window_over_several_trees_goes_by_max_count(monkeypatch):
+    z, i = torch.zeros, dict(dtype=torch.int32)
+    p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")
+    args = (p, 0, z(128, 4, 64, dtype=torch.bfloat16), z(2, 2, **i), z(2, **i), z(3, **i))
+    launched = []
+    monkeypatch.setattr("gguf.hip.kv._launch", lambda *a: launched.append(a))
+    with pytest.raises(ValueError, match="128 tokens.*max_count"):
+        hip.kv_attend(*args, tree=z(128, 2, dtype=torch.int64), window=100)
+    with pytest.raises(ValueError, match="2 words.*max_count 128"):
+        hip.kv_attend(*args, tree=z(128, 1, dtype=torch.int64), window=100)
+    assert not launched
+    hip.kv_attend(*args, tree=z(128, 1, dtype=torch.int64), window=100, max_count=64)
+    assert len(launched) == 1
+
+
 def test_tree_and_keep_checks():
     z, i = torch.zeros, dict(dtype=torch.int32)
     p = hip.KVPages.empty(1, 4, 2, 64, 16, device="cpu")

@@ -166,10 +166,11 @@ def _mask(n, index, b, causal, window, sinks, tree):
         _need(tree, "tree", index, torch.int64, (n, "words"))
         rows, words = tree.shape
         if rows != n or words * 64 < b.max_count or (words > 1 and tree.stride(1) != 1) or (n > 1 and tree.stride(0) < words):
-            raise ValueError(f"tree must be [{n}, {-(-b.max_count // 64)} words or more] with contiguous rows that lie apart (got "
-                             f"{list(tree.shape)}, strides {list(tree.stride())})")
+            raise ValueError(f"tree must be [{n}, {-(-b.max_count // 64)} words or more] (max_count {b.max_count}) with contiguous rows "
+                             f"that lie apart (got {list(tree.shape)}, strides {list(tree.stride())})")
         if window is not None and window < b.max_count:
-            raise ValueError(f"a window of {window} would begin inside a tree of up to {b.max_count} tokens")
+            raise ValueError(f"a window of {window} would begin inside a tree of up to {b.max_count} tokens (max_count; without it all rows "
+                             "of the call)")
         m.tree, m.tree_stride = tree.data_ptr(), max(tree.stride(0), words)
     return m
 
@@ -191,7 +192,8 @@ def kv_attend(pages: KVPages, layer: int, q: torch.Tensor, table: torch.Tensor, 
     window: a row sees the last `window` tokens up to its own alone, and the sequence's first `sinks`; only their pages are read.
     tree: int64 [tokens, words], words >= max_count / 64: the rows are drafted tokens, and of its sequence's own rows a row sees
     those whose bits are set (bit j % 64 of word j // 64 for row j; kv_tree makes them), all tokens before the rows as without it.
-    With both, a row's position is its first row's plus the drafted tokens that it sees less one; the window has to hold a whole tree."""
+    With both, a row's position is its first row's plus the drafted tokens that it sees less one; the window has to hold a whole tree,
+    max_count tokens: name that where a call has several sequences, since without it any of them may have all rows."""
     _in_cache(pages, layer)
     n, heads, token_stride, head_stride = _rows(q, "q", pages.index, torch.bfloat16, None, pages.head_dim)
     if heads == 0 or heads % pages.kv_heads:
