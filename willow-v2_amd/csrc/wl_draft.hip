@@ -10,7 +10,8 @@ constexpr int kTreeThreads = 256;
 constexpr int kTreeKept = 4096;  // parents of a sequence that fit in LDS
 
 // A workgroup takes a sequence, a thread a row. Up to 64 rows are a wavefront's: each takes over the mask and the parent of the
-// row that it has reached, which doubles its steps every time (walking them one by one took 5.0 us for a tree of 64, 2.3 for 16).
+// row that it has reached, which doubles its steps every time: 2.4 to 2.6 us in a graph, whatever the tree (walked one by one, chains of 16
+// and 64 take 3.8 and 8.5, trees of 64 2.9 to 3.2); behind kernels that leave nothing of its inputs in the caches it takes up to 5.
 // More rows are walked from the row to its root: parents stand before their children, so the walk ends, and meets the words
 // of the row's mask from the last to the first. The workgroup behind the last sequence clears the rows before the first and
 // behind the last one.
@@ -95,9 +96,10 @@ constexpr int kKeepGroups = 4;  // of V also not more than come from so many gro
 // be asked for once a token, on both sides).
 // Bound by latency: a token's source (offset, row number, page, scale: a chain of four loads) is looked up once a chunk, by as many
 // threads as it has tokens, and a page of one chunk is read once. 5 of 16 tokens of one sequence, 10 layers of 2 heads of 256: 5.0 us
-// in a graph; up to 12 of 64 of each of 64 sequences: 20 us for 8.3 MB that move, of which V's make 28 MB read and 14 written, since a
+// in a graph; up to 12 of 64 of each of 64 sequences: 21 us for 8.3 MB that move, 28 MB read and 14 written of K and V together, since of V a
 // dimension's next 64 tokens are all that lies side by side (with every byte moved for itself, its source looked up for it and older
-// bytes rescaled one by one: 47 us).
+// bytes rescaled one by one: 47 us). That is on pages whose scales have grown already, and bytes that are still cached: with
+// 281 blocks that grow 24 us against 22 in the same run, with a cache that was written anew before 27.
 template <int TYPE, int D>
 __global__ __launch_bounds__(kKeepThreads) void k_kv_keep(KvLayer c, int64_t layer_bytes, int64_t layer_blocks, KvSeqs s,
                                                           const int32_t* __restrict__ start, const int32_t* __restrict__ keep) {

@@ -134,8 +134,10 @@ struct NormArgs {
 
 // Heads of any size and alignment: as k_rope, a workgroup a token and 32 lanes a head, with a head's sum of squares over its lanes between reading and turning; the
 // first run of values stays in registers meanwhile (all of a head up to 32 runs: 256 values of bf16, 128 of fp32), the others
-// are read again. Both weights go into LDS beside the cosines. Bound by its instructions (4096 tokens of 16 + 2 heads of 256 in bf16:
-// 32 us; further runs of values asked for ahead of their turn: 32 to 36), which is why aligned heads have k_norm_rope_lanes.
+// are read again. Both weights go into LDS beside the cosines. Bound by its instructions: every value takes its weight, cosine and sine
+// from LDS, and rows that are not 16-byte aligned move value by value (4096 tokens of 16 + 2 heads of 256 in bf16 at odd strides 42 us;
+// aligned heads of 320, 94 MB, 35; further runs of values asked for ahead of their turn: none the faster), which is why aligned heads of the
+// usual sizes have k_norm_rope_lanes.
 template <typename T, int VEC>
 __global__ __launch_bounds__(kRopeThreads) void k_norm_rope(RopeArgs a, NormArgs n) {
     extern __shared__ float2 turn[];  // [half]: cos, sin; then the weights of q and of k [head_dim]
@@ -300,11 +302,12 @@ __device__ __forceinline__ float sum_over(float x) {
 // partner's, in another lane, the ones that they turn with: out = (x a + partner's x b) / rms with a = weight cos and b = -+ the
 // partner's weight sin (weight and 0 where nothing turns). These factors are worked out once for a token, into LDS, and a head
 // costs a load, a sum over its lanes, its partner's 16 bytes, three operations a value and a store.
-// Bound by reading and writing: 4096 tokens of 16 + 2 heads of 256 in bf16, 75 MB, 16.5 us (4.6 TB/s); 64 tokens 5.0 us in a graph, a
-// chain of loads and the cosines.
+// Bound by reading and writing: 4096 tokens of 16 + 2 heads of 256 in bf16, 75 MB, 16 to 17 us (4.4 to 4.7 TB/s); 64 tokens 5.1 us in a
+// graph, a chain of loads and the cosines.
 // per: tokens of a workgroup, two of them in bf16 from 2049 tokens on, where one each would be more workgroups than the CUs hold at
-// once (4096 tokens in a graph 19.2 us with two, 21.6 with one, 22.2 with four; 16384 71, 79 and 72; 1024 8.8, 8.1 and 10.9; fp32
-// keeps one: 4096 tokens 37.8 with two, 36.9 with one).
+// once (in a graph of ten calls on the same tensors, with one, two, four: 1024 tokens 7.4, 8.3, 10.1 us; 2048 10.6, 11.3, 12.6; 2300 13.1,
+// 12.4, 14.2; 4096 18.3, 15.8, 17.1; 16384 81.6, 71.0, 69.2). fp32 keeps one: with one and two 2048 tokens take 15.9 and 16.4, 4096 27.2 and
+// 26.5, 16384 127 and 124, from memory 4096 took 36.9 and 37.8.
 template <typename T, int LANES>
 __global__ __launch_bounds__(kRopeThreads) void k_norm_rope_lanes(RopeArgs a, NormArgs n, int per) {
     constexpr int V = kVec<T>, D = V * LANES, kGroups = kRopeThreads / LANES;
