@@ -340,8 +340,8 @@ int wl_kv_attend(const WlKvCache* cache, int layer, const uint16_t* q, int64_t q
  * tree != NULL: the call's rows are a sequence's drafted tokens, and of these a row sees those whose bit is set: bit j % 64 of
  * word tree[row * tree_stride + j / 64] for the sequence's own row j (bits of rows that it does not have are ignored). All tokens
  * before the sequence's rows count as before, and its position (which the window starts from) is that of its first row plus the
- * number of drafted tokens that it sees, less one where it sees any (wl_kv_tree makes these words). A window that begins inside a tree is refused
- * (window < max_count). */
+ * number of drafted tokens that it sees, less one where it sees any (wl_kv_tree makes these words). A window that begins inside a
+ * tree is refused (window < max_count). */
 typedef struct WlKvMask {
     const uint64_t* tree; /* or NULL; 8-byte aligned */
     int64_t tree_stride;  /* words from row to row, at least max_count / 64 rounded up */

@@ -678,11 +678,11 @@ RowsPlan rows_plan(const WlKvCache* c, int q_heads, const WlKvBatch* b, int64_t 
     const int64_t room = kPartialBytes / (b->tokens * q_heads * c->head_dim * static_cast<int64_t>(sizeof(float)));
     const bool few_tiles = items < 2 * kCus;
     // With a window the row tiles of one sequence go through as many tiles each, from the window's length on: where they fill the CUs
-    // to nine tenths nothing is cut, and the second kernel (5 us of 102 for 4096 tokens in a window of 1024) is left out. With fewer tokens
-    // than a window before them the first rows see less, and the longest row tile may be more than a CU's share and the three quarters of it by which
-    // the device lets a piece grow, where there is one round of row tiles: then they are cut (4096 tokens of 16 on 2 heads of 256 with nothing before, in
-    // a window of 3840: 225 us uncut, 195 cut; of 3584, where the two are nearly equal, 212 and 196, and 8192 of 8 on one of 64 in 7168 188 and
-    // 194; of 3000 183 and 189; two rounds, of 7680 tokens, in a window of 7200: 479 and 491).
+    // to nine tenths nothing is cut, and the second kernel (5 us of 102 for 4096 tokens in a window of 1024) is left out. With fewer
+    // tokens than a window before them the first rows see less. Where there is one round of row tiles, and the longest is more than a
+    // CU's share and the three quarters of it by which the device lets a piece grow, they are cut (4096 tokens of 16 on 2 heads of 256
+    // with nothing before, in a window of 3840: 225 us uncut, 195 cut; of 3584, where the two are nearly equal, 212 and 196, and 8192
+    // of 8 on one of 64 in 7168 188 and 194; of 3000 183 and 189; two rounds, of 7680 tokens, in a window of 7200: 479 and 491).
     const int64_t all = std::min<int64_t>(max_length, int64_t{b->table_width} * c->page_tokens);
     if (mask && longest < all && b->seqs == 1 && few_tiles && 10 * items >= 9 * ((items + kCus - 1) / kCus * kCus)) {
         const int64_t window = mask->window, rows_all = b->max_count,  // products below 2^60: one round has at most 2^16 rows
